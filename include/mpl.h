@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-enum { MPL_F32 = 0, MPL_F16 = 1 };
+enum { MPL_F32 = 0, MPL_F16 = 1, MPL_BF16 = 2 };
 enum { MPL_OK = 0, MPL_EINVAL = 1, MPL_EHIP = 2, MPL_EWORKSPACE = 3, MPL_EUNSUPPORTED = 4 };
 
 /* query_mode of mpl_score_select */
@@ -731,6 +731,41 @@ int mpl_lookup_bwd_dense_queries(const float* q_hat, const float* queries, const
                                  const float* sub_keys, const float* g_diversity, void* div_workspace,
                                  size_t div_workspace_bytes, float* diversity_loss, float* d_sub_keys, int phase,
                                  void* stream);
+
+/*
+ * Softmax cross entropy of tokens over a vocabulary, from hidden rows and the
+ * embedding table, without the logits in memory (model.py:125-126, embed.attend,
+ * and the loss a trainer takes of its logits):
+ *   z = hidden . embedding^T,  lse = log sum_v exp(z_v),
+ *   loss = lse - z[target]  (0 where target == ignore_index, NaN for any other
+ *   target outside [0, vocab)),
+ * loss and lse fp32 [rows].  hidden [rows, d] and embedding [vocab, d] are of
+ * dtype MPL_F32, MPL_F16 or MPL_BF16, their rows hidden_pitch and
+ * embedding_pitch elements apart (>= d); 16-bit arrays of d % 64 == 0 are read
+ * as they lie and must have 16-byte aligned rows.  Sums are fp32; fp32 operands
+ * are held to 2^-23 of each (hi + lo fp16 under a power of two), and rows that
+ * meet one that is not finite give NaN.  target int64 [rows].  Deterministic.
+ *
+ * mpl_vocab_cross_entropy_bwd writes d_hidden [rows, d] and d_embedding [vocab,
+ * d] (dense, of dtype; either may be NULL) from the forward's lse and the
+ * gradients g_loss and g_lse of loss and lse (fp32 [rows]; either may be NULL,
+ * for zeros): dz = (g_loss + g_lse) exp(z - lse) - g_loss [v = target], with
+ * g_loss 0 where ignored, rounded to dtype (fp32: held to 2^-23 of each) between
+ * the products.  rows > 0.  A row of an invalid target makes both gradients NaN.
+ *
+ * The workspace (256-byte aligned) takes mpl_vocab_cross_entropy_workspace_bytes
+ * (0 for sizes out of range); calls that may run at the same time need one each.
+ */
+size_t mpl_vocab_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int d, int dtype, int backward);
+int mpl_vocab_cross_entropy(const void* hidden, int64_t hidden_pitch, const void* embedding, int64_t embedding_pitch,
+                            int dtype, const int64_t* target, int64_t rows, int64_t vocab, int d,
+                            int64_t ignore_index, void* workspace, size_t workspace_bytes, float* loss, float* lse,
+                            void* stream);
+int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pitch, const void* embedding,
+                                int64_t embedding_pitch, int dtype, const int64_t* target, int64_t rows,
+                                int64_t vocab, int d, int64_t ignore_index, const float* lse, const float* g_loss,
+                                const float* g_lse, void* workspace, size_t workspace_bytes, void* d_hidden,
+                                void* d_embedding, void* stream);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmpl.so")
 
-MPL_F32, MPL_F16 = 0, 1
+MPL_F32, MPL_F16, MPL_BF16 = 0, 1, 2
 MPL_OK, MPL_EINVAL, MPL_EHIP, MPL_EWORKSPACE, MPL_EUNSUPPORTED = 0, 1, 2, 3, 4  # include/mpl.h status codes
 MPL_Q_NORMALIZED, MPL_Q_RAW, MPL_Q_RAW_SCALED = 0, 1, 2
 MPL_ACT_NONE, MPL_ACT_GELU_TANH, MPL_ACT_SILU = 0, 1, 2
@@ -85,6 +85,10 @@ SIGNATURES = {
     "mpl_rows_linear": (_I, [_P, _P, _P, _P, _F, _P, _I, _P, _I, _P, _I64, _I, _I, _P, _P]),
     "mpl_dense_layers": (_I, [_P, _P, _P, _P, _F, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I64, _I, _P]),
     "mpl_causal_attention": (_I, [_P, _I64, _I, _I, _I, _F, _P, _P]),
+    "mpl_vocab_cross_entropy_workspace_bytes": (_SZ, [_I64, _I64, _I, _I, _I]),
+    "mpl_vocab_cross_entropy": (_I, [_P, _I64, _P, _I64, _I, _P, _I64, _I64, _I, _I64, _P, _SZ, _P, _P, _P]),
+    "mpl_vocab_cross_entropy_bwd": (_I, [_P, _I64, _P, _I64, _I, _P, _I64, _I64, _I, _I64, _P, _P, _P, _P, _SZ, _P,
+                                         _P, _P]),
     "mpl_vocab_logits": (_I, [_P, _P, _P, _F, _P, _I64, _I, _I64, _P, _P]),
     "mpl_rows_linear_pair": (_I, [_P, _P, _P, _F, _P, _P, _I, _I, _I64, _I, _I, _I, _P, _P, _P]),
     "mpl_balance_state_bytes": (_SZ, [_I64, _I]),
@@ -149,3 +153,30 @@ def stream_ptr(device) -> int:
     if type(device) is torch.device and device.index is not None:
         _stream_index[device] = device.index
     return stream
+
+
+class on_device:
+    """Makes ``device`` the current one inside a with block, where it is not
+    already: a launch goes to a stream of the current device."""
+
+    __slots__ = ("to", "back")
+
+    def __init__(self, device):
+        import torch
+
+        now = torch._C._cuda_getDevice()
+        self.to = now if device.index is None else device.index
+        self.back = now
+
+    def __enter__(self):
+        if self.to != self.back:
+            import torch
+
+            torch._C._cuda_setDevice(self.to)
+
+    def __exit__(self, *exc):
+        if self.to != self.back:
+            import torch
+
+            torch._C._cuda_setDevice(self.back)
+        return False

@@ -1,0 +1,740 @@
+// Softmax cross entropy of tokens over a vocabulary, from the hidden rows and
+// the embedding table, without the logits in memory, and its gradients:
+//
+//   z_rv   = hidden_r . embedding_v
+//   lse_r  = log sum_v exp(z_rv),      loss_r = lse_r - z_r,target (0 where ignored)
+//   dz_rv  = (g_r + gl_r) exp(z_rv - lse_r) - g_r [v = target_r]
+//   d hidden = dz . embedding,         d embedding = dz^T . hidden
+//
+// with g_r the loss's gradient (0 where ignored) and gl_r the logsumexp's.
+//
+// Forward: tiles of z (tile_mma.h: the vocabulary down, tokens across, so a
+// lane's accumulators are one token's and its maximum and sum stay in
+// registers) end in one (maximum, sum of exp) pair a token and vocabulary
+// tile; a second launch joins the pairs in a fixed order.
+//
+// Backward: the vocabulary goes in pieces.  A piece's tiles of z are formed
+// again with the same instructions, so z has the forward's bits, and written
+// as dz in 16 bits (fp32 calls: hi and lo); two products read it from there.
+// A piece's dz is small enough to stay in the Infinity Cache.
+#include <math.h>
+
+#include "common.h"
+#include "tile_mma.h"
+
+namespace mpl {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Device scalars of a call (floats): powers of two that fp32 and fp16 operands
+// were multiplied by, and their inverses.
+enum { kScaleE = 0, kInvE, kScaleH, kInvH, kScaleP, kInvP, kScalars = 16 };
+
+// 2^(top - exponent of the largest magnitude), given by its bits; 1 for 0.
+__device__ __forceinline__ float scale_for(uint32_t bits, int top) {
+  const int e = (int)(bits >> 23) - 127;
+  const int s = bits == 0 ? 0 : max(-126, min(126, top - e));
+  return __uint_as_float((uint32_t)(127 + s) << 23);
+}
+// Magnitude bits of x, 0 if it is not finite.
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+  const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
+  return b < 0x7F800000u ? b : 0u;
+}
+
+// ---------------------------------------------------------------- operands
+// One array.  The fields that kernels choose by array stand in one struct of a
+// size and alignment that scalar loads take whole: with bool vec[2] beside
+// pointer arrays the compiler split the index of a scalar load into parts that
+// are no multiples of 4, which those loads ignore the low bits of.
+struct PackOne {
+  const void* src;
+  char* dst;
+  int64_t rows, pitch;  // pitch in elements
+  int64_t blocks;
+  int64_t vec;  // rows are 16-byte aligned
+};
+struct PackArgs {
+  PackOne e, h;  // embedding, hidden
+  int d, dpad;
+  float* scal;
+  uint32_t* part;  // [kAmaxBlocks] maxima of each array
+};
+constexpr int kAmaxBlocks = 512;
+
+// Largest finite magnitudes of both arrays, one partial maximum a workgroup.
+__global__ __launch_bounds__(256) void amax_kernel(PackArgs p) {
+  const int a = blockIdx.y;
+  const PackOne o = a ? p.h : p.e;
+  const float* x = (const float*)o.src;
+  const int vecs = p.d / 4;
+  uint32_t m = 0;
+  if (o.vec) {
+    const int64_t n = o.rows * vecs;
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += 256 * (int64_t)gridDim.x) {
+      const int64_t r = i / vecs;
+      const float4 v = *(const float4*)(x + r * o.pitch + 4 * (i - r * vecs));
+      m = max(max(max(m, finite_bits(v.x)), max(finite_bits(v.y), finite_bits(v.z))), finite_bits(v.w));
+    }
+  }
+  const int c0 = o.vec ? 4 * vecs : 0, tail = p.d - c0;
+  if (tail) {
+    const int64_t n = o.rows * tail;
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += 256 * (int64_t)gridDim.x) {
+      const int64_t r = i / tail;
+      m = max(m, finite_bits(x[r * o.pitch + c0 + (i - r * tail)]));
+    }
+  }
+  __shared__ uint32_t s[256];
+  s[threadIdx.x] = m;
+  __syncthreads();
+  for (int h = 128; h; h >>= 1) {
+    if (threadIdx.x < h) s[threadIdx.x] = max(s[threadIdx.x], s[threadIdx.x + h]);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) p.part[a * kAmaxBlocks + blockIdx.x] = s[0];
+}
+
+// Rows of an array as a tile product's operand: 16-bit rows zero-filled to
+// whole stages, or fp32 rows as hi and lo.  A thread writes 8 elements.
+template <bool SPLIT>
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
+  const int a = blockIdx.x < p.e.blocks ? 0 : 1;
+  const PackOne o = a ? p.h : p.e;
+  float scale = 1.f;
+  if (SPLIT) {
+    __shared__ uint32_t s[4];
+    uint32_t m = max(p.part[a * kAmaxBlocks + threadIdx.x], p.part[a * kAmaxBlocks + 256 + threadIdx.x]);
+    for (int h = 32; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+    __syncthreads();
+    scale = scale_for(max(max(s[0], s[1]), max(s[2], s[3])), 14);
+    if (threadIdx.x == 0 && (blockIdx.x == 0 || blockIdx.x == p.e.blocks)) {
+      p.scal[a == 0 ? kScaleE : kScaleH] = scale;
+      p.scal[a == 0 ? kInvE : kInvH] = 1.f / scale;
+    }
+  }
+  const int per = p.dpad / 8;
+  const int64_t i = (int64_t)(blockIdx.x - (a ? p.e.blocks : 0)) * 256 + threadIdx.x;
+  if (i >= o.rows * per) return;
+  const int64_t r = i / per;
+  const int c = 8 * (int)(i - r * per);
+  if (SPLIT) {
+    const float* x = (const float*)o.src + r * o.pitch + c;
+    float v[8];
+    if (o.vec && c + 8 <= p.d) {
+      *(float4*)v = *(const float4*)x;
+      *(float4*)(v + 4) = *(const float4*)(x + 4);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < p.d ? x[j] : 0.f;
+    }
+    half8 hi, lo;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = v[j] * scale;
+      hi[j] = (_Float16)y;
+      lo[j] = (_Float16)(y - (float)hi[j]);
+    }
+    char* q = o.dst + (r * p.dpad + c / 32 * 32) * 4 + (c % 32) * 2;
+    *(half8*)q = hi;
+    *(half8*)(q + 64) = lo;
+  } else {
+    const uint16_t* x = (const uint16_t*)o.src + r * o.pitch + c;
+    uint16_t v[8] __attribute__((aligned(16)));
+    if (o.vec && c + 8 <= p.d) {
+      *(uint4*)v = *(const uint4*)x;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < p.d ? x[j] : (uint16_t)0;
+    }
+    *(uint4*)(o.dst + (r * p.dpad + c) * 2) = *(const uint4*)v;
+  }
+}
+
+// ------------------------------------------------------------------ forward
+struct LogitArgs {
+  TileOperand E, H;
+  int64_t R, V;
+  int iters;
+  uint32_t tiles_v, tiles_t;
+  const float* scal;
+  const int64_t* target;
+  // forward
+  float2* part;  // [tiles_v][R]
+  float* z_target;
+  // backward: the piece starts at row v0 of the table
+  int64_t v0, rows_p, pitch_p;  // rows_p: rows of dz that exist (zero past R); pitch in bytes
+  const float* coef;            // [3][rows_p]: g + gl, g, lse
+  char* P;
+};
+
+#define MPL_TILE_LDS(C)                                      \
+  __shared__ __attribute__((aligned(1024))) char a0[C::kStageA]; \
+  __shared__ __attribute__((aligned(1024))) char b0[C::kStageB]; \
+  __shared__ __attribute__((aligned(1024))) char a1[C::kStageA]; \
+  __shared__ __attribute__((aligned(1024))) char b1[C::kStageB];
+
+template <class C>
+__global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
+  MPL_TILE_LDS(C)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / C::WN, wn = wave % C::WN;
+  uint32_t tv, tt;
+  tile_of(blockIdx.x, gridDim.x, p.tiles_v, p.tiles_t, 8, tv, tt);
+  const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
+  f32x16 acc[C::TM][C::TN];
+  C::run(p.E, p.H, v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
+  float u0 = 1.f, u1 = 1.f;
+  if (C::S == 2) u0 = p.scal[kInvE], u1 = p.scal[kInvH];
+  const int64_t vw = v0 + wm * C::TM * 32 + 4 * (lane >> 5);  // of acc[0][.][0]
+  __syncthreads();  // every wave is done with the stages: they hold the waves' pairs from here
+  float2* pair = (float2*)a0;  // [WM][BN]
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j) {
+    const int64_t tok = t0 + (wn * C::TN + j) * 32 + (lane & 31);
+    if (C::S == 2) {
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = acc[i][j][r] * u0 * u1;
+    }
+    const int64_t at = tok < p.R ? p.target[tok] - vw : -1;  // place of the target among the lane's, if it is there
+    const int place = at >= 0 && at < C::TM * 32 && !(at & 4) ? (int)at : -1;
+    if (__any(place >= 0)) {
+      float z = 0.f;
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z = place == 32 * i + 8 * (r >> 2) + (r & 3) ? acc[i][j][r] : z;
+      if (place >= 0) p.z_target[tok] = z;
+    }
+    if (v0 + C::BM > p.V) {
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (vw + 32 * i + 8 * (r >> 2) + (r & 3) >= p.V) acc[i][j][r] = -INFINITY;
+    }
+    float m = acc[0][j][0];
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+    float x = m, y = m;
+    half_swap(x, y);
+    m = fmaxf(x, y);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2e);
+    x = s, y = s;
+    half_swap(x, y);
+    if (lane < 32) pair[wm * C::BN + (wn * C::TN + j) * 32 + lane] = make_float2(m, x + y);
+  }
+  __syncthreads();
+  for (int t = tid; t < C::BN; t += C::kThreads) {
+    if (t0 + t >= p.R) continue;
+    float m = pair[t].x;
+#pragma unroll
+    for (int w = 1; w < C::WM; ++w) m = fmaxf(m, pair[w * C::BN + t].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < C::WM; ++w)
+      s += pair[w * C::BN + t].y * __builtin_amdgcn_exp2f((pair[w * C::BN + t].x - ref) * kLog2e);
+    p.part[(int64_t)tv * p.R + t0 + t] = make_float2(m, s);
+  }
+}
+
+// Joins a token's pairs: a workgroup takes 32 tokens, 8 threads a token, each
+// every eighth pair in order, then the eight in order.
+__global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict__ part, int tiles, int64_t R, int64_t V,
+                                                        const int64_t* __restrict__ target, int64_t ignore,
+                                                        const float* __restrict__ z_target, float* __restrict__ loss,
+                                                        float* __restrict__ lse) {
+  __shared__ float2 s[8][32];
+  const int t = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int64_t tok = (int64_t)blockIdx.x * 32 + t;
+  float m = -INFINITY, l = 0.f;
+  if (tok < R)
+    for (int i = g; i < tiles; i += 8) {
+      const float2 v = part[(int64_t)i * R + tok];
+      const float n = fmaxf(m, v.x), ref = n == -INFINITY ? 0.f : n;
+      l = l * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + v.y * __builtin_amdgcn_exp2f((v.x - ref) * kLog2e);
+      m = n;
+    }
+  s[g][t] = make_float2(m, l);
+  __syncthreads();
+  if (g || tok >= R) return;
+  for (int i = 1; i < 8; ++i) {
+    const float2 v = s[i][t];
+    const float n = fmaxf(m, v.x), ref = n == -INFINITY ? 0.f : n;
+    l = l * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + v.y * __builtin_amdgcn_exp2f((v.x - ref) * kLog2e);
+    m = n;
+  }
+  const float out = m + logf(l);
+  const int64_t at = target[tok];
+  lse[tok] = out;
+  loss[tok] = at == ignore ? 0.f : (at < 0 || at >= V) ? NAN : out - z_target[tok];
+}
+
+// ----------------------------------------------------------------- backward
+// Coefficients of each row, zero for the rows that only fill dz up, and the
+// power of two that dz is held under (fp32 and fp16 calls; |dz| <= |g + gl| +
+// |g|, below 2^15 after it).  One workgroup: rows are few against the products.
+__global__ __launch_bounds__(1024) void xent_coef_kernel(const int64_t* __restrict__ target, int64_t R, int64_t rows_p,
+                                                         int64_t V, int64_t ignore, const float* __restrict__ g_loss,
+                                                         const float* __restrict__ g_lse,
+                                                         const float* __restrict__ lse, bool scaled,
+                                                         float* __restrict__ coef, float* __restrict__ scal) {
+  uint32_t m = 0;
+  for (int64_t i = threadIdx.x; i < rows_p; i += 1024) {
+    float all = 0.f, g = 0.f, l = 0.f;
+    if (i < R) {
+      const int64_t at = target[i];
+      g = at == ignore || g_loss == nullptr ? 0.f : g_loss[i];
+      if (at != ignore && (at < 0 || at >= V)) g = NAN;
+      all = g_lse ? g + g_lse[i] : g;
+      l = lse[i];
+    }
+    coef[i] = all;
+    coef[rows_p + i] = g;
+    coef[2 * rows_p + i] = l;
+    m = max(m, max(finite_bits(all), finite_bits(g)));
+  }
+  for (int h = 32; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
+  __shared__ uint32_t s[16];
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) m = max(m, s[i]);
+    const float scale = scaled ? scale_for(m, 13) : 1.f;
+    scal[kScaleP] = scale;
+    scal[kInvP] = 1.f / scale;
+  }
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (BF) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    b2 v;
+    v[0] = (__bf16)x;
+    v[1] = (__bf16)y;
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    h2 v;
+    v[0] = (_Float16)x;
+    v[1] = (_Float16)y;
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+template <class C>
+__global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
+  MPL_TILE_LDS(C)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / C::WN, wn = wave % C::WN;
+  uint32_t tv, tt;
+  tile_of(blockIdx.x, gridDim.x, p.tiles_v, p.tiles_t, 8, tv, tt);
+  const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
+  f32x16 acc[C::TM][C::TN];
+  C::run(p.E, p.H, p.v0 + v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
+  float u0 = 1.f, u1 = 1.f;
+  if (C::S == 2) u0 = p.scal[kInvE], u1 = p.scal[kInvH];
+  const float up = p.scal[kScaleP];
+  const int half = lane >> 5;
+  const int64_t vw = v0 + wm * C::TM * 32;  // the wave's first column of the piece
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j) {
+    const int64_t tok = t0 + (wn * C::TN + j) * 32 + (lane & 31);
+    const bool there = tok < p.R;
+    const int64_t row = min(tok, p.rows_p - 1);
+    const float ga = p.coef[row] * up, gb = p.coef[p.rows_p + row] * up, lse = p.coef[2 * p.rows_p + row];
+    const int64_t at = (there ? p.target[tok] - p.v0 : -1) - (vw + 4 * half);
+    const int place = at >= 0 && at < C::TM * 32 ? (int)at : -1;
+    const bool hit = __any(place >= 0);
+    const bool edge = p.v0 + v0 + C::BM > p.V;
+    char* out = p.P + row * p.pitch_p;
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) {
+      float x[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float z = acc[i][j][r];
+        if (C::S == 2) z = z * u0 * u1;
+        x[r] = ga * __builtin_amdgcn_exp2f((z - lse) * kLog2e);
+      }
+      if (hit) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          x[r] -= place == 32 * i + 8 * (r >> 2) + (r & 3) ? gb : 0.f;
+      }
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (p.v0 + vw + 4 * half + 32 * i + 8 * (r >> 2) + (r & 3) >= p.V) x[r] = 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = there ? x[r] : 0.f;
+      // 4 neighbours a group of registers; the lane's other half holds the next 4:
+      // after the exchange a lane has 8 neighbours, 16 bytes
+#pragma unroll
+      for (int pl = 0; pl < C::S; ++pl) {
+        uint32_t u[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) u[r] = pack2<C::BF>(x[2 * r], x[2 * r + 1]);
+        if (C::S == 2 && pl == 0) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            const h2 v = __builtin_bit_cast(h2, u[r]);
+            x[2 * r] -= (float)v[0];
+            x[2 * r + 1] -= (float)v[1];
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const auto sw = __builtin_amdgcn_permlane32_swap(u[4 * q + e], u[4 * q + 2 + e], false, false);
+            w[e] = sw[0];
+            w[2 + e] = sw[1];
+          }
+          if (tok < p.rows_p)
+            *(uint4*)(out + (vw + 32 * i) * (2 * C::S) + 64 * pl + 32 * q + 16 * half) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+  }
+}
+
+// The two products with dz.  Output rows below `rows` and columns below `cols`.
+struct GradArgs {
+  TileOperand A, B;
+  int64_t rows;
+  int cols, iters, splits;
+  uint32_t tiles_m, tiles_n;
+  const float* u0;  // device scalars that undo the operands' scaling
+  const float* u1;
+  float* part;  // [splits][rows][cols] sums, or null: the result goes to out
+  bool add;     // onto what part holds
+  void* out;
+  int dtype;
+};
+
+__device__ __forceinline__ void store_as(void* out, int64_t i, float x, int dtype) {
+  if (dtype == MPL_F32) ((float*)out)[i] = x;
+  else if (dtype == MPL_F16) ((_Float16*)out)[i] = (_Float16)x;
+  else ((__bf16*)out)[i] = (__bf16)x;
+}
+
+template <class C>
+__global__ __launch_bounds__(C::kThreads) void xent_grad_kernel(GradArgs p) {
+  MPL_TILE_LDS(C)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / C::WN, wn = wave % C::WN;
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, gridDim.x, p.tiles_m, p.tiles_n, 8, tm, tn);
+  const int64_t m0 = (int64_t)tm * C::BM;
+  const int n0 = (int)tn * C::BN;
+  const int split = blockIdx.y;
+  const int it0 = (int)((int64_t)p.iters * split / p.splits), it1 = (int)((int64_t)p.iters * (split + 1) / p.splits);
+  f32x16 acc[C::TM][C::TN];
+  C::run(p.A, p.B, m0, n0, it0, it1, a0, b0, a1, b1, acc);
+  const float u0 = *p.u0, u1 = C::S == 2 ? *p.u1 : 1.f;
+  float* part = p.part ? p.part + (int64_t)split * p.rows * p.cols : nullptr;
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      const int col = n0 + (wn * C::TN + j) * 32 + (lane & 31);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int64_t row = m0 + (wm * C::TM + i) * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+        if (row >= p.rows || col >= p.cols) continue;
+        const float x = acc[i][j][r] * u0 * u1;
+        if (part) part[row * p.cols + col] = p.add ? part[row * p.cols + col] + x : x;
+        else store_as(p.out, row * p.cols + col, x, p.dtype);
+      }
+    }
+}
+
+__global__ __launch_bounds__(256) void xent_sum_kernel(const float* __restrict__ part, int splits, int64_t n,
+                                                       void* __restrict__ out, int dtype) {
+  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += 256 * (int64_t)gridDim.x) {
+    float s = part[i];
+    for (int k = 1; k < splits; ++k) s += part[k * n + i];
+    store_as(out, i, s, dtype);
+  }
+}
+
+// --------------------------------------------------------------------- host
+template <int S, bool BF, bool AST, bool BST> using Big = TileMma<S, BF, AST, BST, 2, 4, 4, 2>;    // 256 x 256
+template <int S, bool BF, bool AST, bool BST> using Mid = TileMma<S, BF, AST, BST, 2, 2, 2, 2>;    // 128 x 128
+
+struct Plan {
+  int64_t rows_p, v_piece, pieces;
+  int dpad;
+  bool pack, split;
+  bool big_z, big_h, big_e;
+  uint32_t tiles_v;  // of the forward
+  int splits_h, splits_e;
+  // offsets into the workspace
+  size_t scal, amax, e, h, part, zt, coef, P, ph, pe, bytes_fwd, bytes_bwd;
+};
+
+constexpr int64_t kPieceBytes = 256ll << 20;
+
+inline int64_t up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
+
+Plan make_plan(int64_t R, int64_t V, int d, int dtype) {
+  Plan p{};
+  p.split = dtype == MPL_F32;
+  const int S = p.split ? 2 : 1;
+  p.pack = p.split || d % 64;
+  p.dpad = (int)up(d, 64);
+  p.rows_p = up(R, 64);
+  p.big_z = cdiv(R, 256) * cdiv(V, 256) >= 512;
+  p.tiles_v = (uint32_t)cdiv(V, p.big_z ? 256 : 128);
+  const int64_t col = p.rows_p * 2 * S;
+  const int64_t most = kPieceBytes / col / 256 * 256;
+  p.pieces = cdiv(V, most < 256 ? 256 : most);
+  p.v_piece = up(cdiv(V, p.pieces), 256);
+  p.pieces = cdiv(V, p.v_piece);
+  auto pick = [&](int64_t M, int64_t N, int64_t K, bool& big, int& splits) {
+    big = cdiv(M, 256) * cdiv(N, 256) >= 256;
+    const int64_t tiles = big ? cdiv(M, 256) * cdiv(N, 256) : cdiv(M, 128) * cdiv(N, 128);
+    const int64_t iters = K * S / 64, want = cdiv(512, tiles);
+    splits = (int)(big ? 1 : want < 1 ? 1 : want > iters / 8 ? (iters / 8 > 0 ? iters / 8 : 1) : want);
+  };
+  pick(R, p.dpad, p.v_piece, p.big_h, p.splits_h);
+  pick(p.v_piece, p.dpad, p.rows_p, p.big_e, p.splits_e);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at = (at + bytes + 1023) / 1024 * 1024;
+    return o;
+  };
+  p.scal = take(kScalars * 4);
+  p.amax = take(2 * kAmaxBlocks * 4);
+  p.e = take(p.pack ? (size_t)V * p.dpad * 2 * S : 0);
+  p.h = take(p.pack ? (size_t)R * p.dpad * 2 * S : 0);
+  const size_t shared = at;
+  p.part = take((size_t)p.tiles_v * R * 8);
+  p.zt = take((size_t)R * 4);
+  p.bytes_fwd = at;
+  at = shared;
+  p.coef = take((size_t)p.rows_p * 12);
+  p.P = take((size_t)p.v_piece * col);
+  p.ph = take(p.splits_h > 1 || p.pieces > 1 ? (size_t)p.splits_h * R * d * 4 : 0);
+  p.pe = take(p.splits_e > 1 ? (size_t)p.splits_e * p.v_piece * d * 4 : 0);
+  p.bytes_bwd = at;
+  return p;
+}
+
+struct Call {
+  const void* hidden;
+  int64_t hidden_pitch;
+  const void* embedding;
+  int64_t embedding_pitch;
+  int dtype;
+  int64_t R, V;
+  int d;
+};
+
+bool sizes_ok(int64_t R, int64_t V, int d, int dtype) {
+  return R >= 0 && V > 0 && d > 0 && d <= 65536 && R <= (1ll << 31) && V <= (1ll << 31) &&
+         (dtype == MPL_F32 || dtype == MPL_F16 || dtype == MPL_BF16);
+}
+
+int check_call(const char* what, const Call& c, const void* ws, size_t ws_bytes, size_t need) {
+  MPL_REQUIRE(c.hidden && c.embedding, MPL_EINVAL, "%s: null buffer", what);
+  MPL_REQUIRE(c.hidden_pitch >= c.d && c.embedding_pitch >= c.d, MPL_EINVAL, "%s: a pitch is below d = %d", what, c.d);
+  const int size = c.dtype == MPL_F32 ? 4 : 2;
+  for (const void* q : {c.hidden, c.embedding})
+    MPL_REQUIRE(((uintptr_t)q & (size - 1)) == 0, MPL_EINVAL, "%s: an array is not aligned to its elements", what);
+  if (c.dtype != MPL_F32 && c.d % 64 == 0)  // read as they lie
+    MPL_REQUIRE(((uintptr_t)c.hidden & 15) == 0 && ((uintptr_t)c.embedding & 15) == 0 && c.hidden_pitch % 8 == 0 &&
+                    c.embedding_pitch % 8 == 0,
+                MPL_EINVAL, "%s: 16-bit rows of d %% 64 == 0 must be 16-byte aligned", what);
+  MPL_REQUIRE(ws && ((uintptr_t)ws & 255) == 0, MPL_EINVAL, "%s: the workspace must be 256-byte aligned", what);
+  MPL_REQUIRE(ws_bytes >= need, MPL_EWORKSPACE, "%s: workspace %zu < %zu bytes", what, ws_bytes, need);
+  return MPL_OK;
+}
+
+// Brings both arrays into operand form; E and H are the rows forms.
+void operands(const Call& c, const Plan& p, char* ws, hipStream_t s, TileOperand& E, TileOperand& H) {
+  const int64_t row = (int64_t)p.dpad * (p.split ? 4 : 2);
+  if (!p.pack) {
+    E = {(const char*)c.embedding, c.embedding_pitch * 2, c.V, row};
+    H = {(const char*)c.hidden, c.hidden_pitch * 2, c.R, row};
+    return;
+  }
+  auto one = [&](const void* src, char* dst, int64_t rows, int64_t pitch) {
+    const bool vec = ((uintptr_t)src & 15) == 0 && pitch % (p.split ? 4 : 8) == 0;
+    return PackOne{src, dst, rows, pitch, cdiv(rows * (p.dpad / 8), 256), vec};
+  };
+  PackArgs a{};
+  a.e = one(c.embedding, ws + p.e, c.V, c.embedding_pitch);
+  a.h = one(c.hidden, ws + p.h, c.R, c.hidden_pitch);
+  a.d = c.d, a.dpad = p.dpad;
+  a.scal = (float*)(ws + p.scal);
+  a.part = (uint32_t*)(ws + p.amax);
+  const unsigned grid = (unsigned)(a.e.blocks + a.h.blocks);
+  if (p.split) {
+    amax_kernel<<<dim3(kAmaxBlocks, 2), 256, 0, s>>>(a);
+    pack_kernel<true><<<grid, 256, 0, s>>>(a);
+  } else {
+    pack_kernel<false><<<grid, 256, 0, s>>>(a);
+  }
+  E = {ws + p.e, row, c.V, row};
+  H = {ws + p.h, row, c.R, row};
+}
+
+// The instantiation of one product for the call's type and tile.
+#define MPL_TILE_DISPATCH(KERNEL, AST, BST, big, grid, s, args)                                            \
+  do {                                                                                                     \
+    if (c.dtype == MPL_F32) {                                                                              \
+      if (big) KERNEL<Big<2, false, AST, BST>><<<grid, Big<2, false, AST, BST>::kThreads, 0, s>>>(args);   \
+      else KERNEL<Mid<2, false, AST, BST>><<<grid, Mid<2, false, AST, BST>::kThreads, 0, s>>>(args);       \
+    } else if (c.dtype == MPL_F16) {                                                                       \
+      if (big) KERNEL<Big<1, false, AST, BST>><<<grid, Big<1, false, AST, BST>::kThreads, 0, s>>>(args);   \
+      else KERNEL<Mid<1, false, AST, BST>><<<grid, Mid<1, false, AST, BST>::kThreads, 0, s>>>(args);       \
+    } else {                                                                                               \
+      if (big) KERNEL<Big<1, true, AST, BST>><<<grid, Big<1, true, AST, BST>::kThreads, 0, s>>>(args);     \
+      else KERNEL<Mid<1, true, AST, BST>><<<grid, Mid<1, true, AST, BST>::kThreads, 0, s>>>(args);         \
+    }                                                                                                      \
+  } while (0)
+
+}  // namespace
+}  // namespace mpl
+
+using namespace mpl;
+
+extern "C" size_t mpl_vocab_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int d, int dtype, int backward) {
+  if (!sizes_ok(rows, vocab, d, dtype)) return 0;
+  const Plan p = make_plan(rows, vocab, d, dtype);
+  return backward ? p.bytes_bwd : p.bytes_fwd;
+}
+
+extern "C" int mpl_vocab_cross_entropy(const void* hidden, int64_t hidden_pitch, const void* embedding,
+                                       int64_t embedding_pitch, int dtype, const int64_t* target, int64_t rows,
+                                       int64_t vocab, int d, int64_t ignore_index, void* workspace,
+                                       size_t workspace_bytes, float* loss, float* lse, void* stream) {
+  clear_error();
+  const char* what = "mpl_vocab_cross_entropy";
+  MPL_REQUIRE(sizes_ok(rows, vocab, d, dtype), MPL_EINVAL, "%s: bad sizes or type: rows=%lld vocab=%lld d=%d dtype=%d",
+              what, (long long)rows, (long long)vocab, d, dtype);
+  if (rows == 0) return MPL_OK;
+  const Call c{hidden, hidden_pitch, embedding, embedding_pitch, dtype, rows, vocab, d};
+  const Plan p = make_plan(rows, vocab, d, dtype);
+  if (const int rc = check_call(what, c, workspace, workspace_bytes, p.bytes_fwd)) return rc;
+  MPL_REQUIRE(target && loss && lse, MPL_EINVAL, "%s: null buffer", what);
+  char* ws = (char*)workspace;
+  hipStream_t s = (hipStream_t)stream;
+  LogitArgs a{};
+  operands(c, p, ws, s, a.E, a.H);
+  a.R = rows, a.V = vocab;
+  a.iters = p.dpad * (p.split ? 2 : 1) / 64;
+  a.tiles_v = p.tiles_v;
+  a.tiles_t = (uint32_t)cdiv(rows, p.big_z ? 256 : 128);
+  a.scal = (const float*)(ws + p.scal);
+  a.target = target;
+  a.part = (float2*)(ws + p.part);
+  a.z_target = (float*)(ws + p.zt);
+  MPL_TILE_DISPATCH(xent_lse_kernel, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
+  xent_join_kernel<<<(unsigned)cdiv(rows, 32), 256, 0, s>>>(a.part, (int)p.tiles_v, rows, vocab, target, ignore_index,
+                                                          a.z_target, loss, lse);
+  return check_launch(what);
+}
+
+extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pitch, const void* embedding,
+                                           int64_t embedding_pitch, int dtype, const int64_t* target, int64_t rows,
+                                           int64_t vocab, int d, int64_t ignore_index, const float* lse,
+                                           const float* g_loss, const float* g_lse, void* workspace,
+                                           size_t workspace_bytes, void* d_hidden, void* d_embedding, void* stream) {
+  clear_error();
+  const char* what = "mpl_vocab_cross_entropy_bwd";
+  MPL_REQUIRE(sizes_ok(rows, vocab, d, dtype) && rows > 0, MPL_EINVAL,
+              "%s: bad sizes or type: rows=%lld vocab=%lld d=%d dtype=%d", what, (long long)rows, (long long)vocab, d,
+              dtype);
+  const Call c{hidden, hidden_pitch, embedding, embedding_pitch, dtype, rows, vocab, d};
+  const Plan p = make_plan(rows, vocab, d, dtype);
+  if (const int rc = check_call(what, c, workspace, workspace_bytes, p.bytes_bwd)) return rc;
+  MPL_REQUIRE(target && lse && (g_loss || g_lse) && (d_hidden || d_embedding), MPL_EINVAL, "%s: null buffer", what);
+  char* ws = (char*)workspace;
+  hipStream_t s = (hipStream_t)stream;
+  const int S = p.split ? 2 : 1;
+  LogitArgs a{};
+  operands(c, p, ws, s, a.E, a.H);
+  float* scal = (float*)(ws + p.scal);
+  float* coef = (float*)(ws + p.coef);
+  xent_coef_kernel<<<1, 1024, 0, s>>>(target, rows, p.rows_p, vocab, ignore_index, g_loss, g_lse, lse,
+                                      dtype != MPL_BF16, coef, scal);
+  a.R = rows, a.V = vocab;
+  a.iters = p.dpad * S / 64;
+  const int bz = p.big_z ? 256 : 128;
+  a.tiles_t = (uint32_t)cdiv(rows, bz);
+  a.scal = scal;
+  a.target = target;
+  a.rows_p = p.rows_p;
+  a.pitch_p = p.v_piece * 2 * S;
+  a.coef = coef;
+  a.P = ws + p.P;
+  for (int64_t i = 0; i < p.pieces; ++i) {
+    a.v0 = i * p.v_piece;
+    const int64_t nv = p.v_piece < vocab - a.v0 ? p.v_piece : vocab - a.v0;  // rows of the table in the piece
+    const int64_t nvp = up(nv, 256);
+    a.tiles_v = (uint32_t)(nvp / bz);
+    MPL_TILE_DISPATCH(xent_dz_kernel, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
+    if (d_hidden) {
+      GradArgs g{};
+      g.A = {a.P, a.pitch_p, p.rows_p, a.pitch_p};
+      g.B = {a.E.base + a.v0 * a.E.pitch, a.E.pitch, nv, a.E.width};
+      g.rows = rows, g.cols = d;
+      g.iters = (int)(nvp * S / 64);
+      g.splits = p.splits_h;
+      const int b = p.big_h ? 256 : 128;
+      g.tiles_m = (uint32_t)cdiv(rows, b), g.tiles_n = (uint32_t)cdiv(d, b);
+      g.u0 = scal + kInvP, g.u1 = scal + kInvE;
+      g.part = p.splits_h > 1 || p.pieces > 1 ? (float*)(ws + p.ph) : nullptr;
+      g.add = i > 0;
+      g.out = d_hidden, g.dtype = dtype;
+      MPL_TILE_DISPATCH(xent_grad_kernel, false, true, p.big_h, dim3(g.tiles_m * g.tiles_n, g.splits), s, g);
+    }
+    if (d_embedding) {
+      GradArgs g{};
+      g.A = {a.P, a.pitch_p, p.rows_p, nvp * 2 * S};
+      g.B = {a.H.base, a.H.pitch, rows, a.H.width};
+      g.rows = nv, g.cols = d;
+      g.iters = (int)(p.rows_p * S / 64);
+      g.splits = p.splits_e;
+      const int b = p.big_e ? 256 : 128;
+      g.tiles_m = (uint32_t)cdiv(nv, b), g.tiles_n = (uint32_t)cdiv(d, b);
+      g.u0 = scal + kInvP, g.u1 = scal + kInvH;
+      g.part = p.splits_e > 1 ? (float*)(ws + p.pe) : nullptr;
+      g.out = (char*)d_embedding + a.v0 * d * (dtype == MPL_F32 ? 4 : 2);
+      g.dtype = dtype;
+      MPL_TILE_DISPATCH(xent_grad_kernel, true, true, p.big_e, dim3(g.tiles_m * g.tiles_n, g.splits), s, g);
+      if (g.part) {
+        const int64_t n = nv * d;
+        xent_sum_kernel<<<(unsigned)(cdiv(n, 256) < 4096 ? cdiv(n, 256) : 4096), 256, 0, s>>>(g.part, g.splits, n,
+                                                                                           g.out, dtype);
+      }
+    }
+  }
+  if (d_hidden && (p.splits_h > 1 || p.pieces > 1)) {
+    const int64_t n = rows * d;
+    xent_sum_kernel<<<(unsigned)(cdiv(n, 256) < 4096 ? cdiv(n, 256) : 4096), 256, 0, s>>>(
+        (const float*)(ws + p.ph), p.splits_h, n, d_hidden, dtype);
+  }
+  return check_launch(what);
+}
