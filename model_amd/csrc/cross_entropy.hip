@@ -412,6 +412,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
                 make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
@@ -427,13 +428,49 @@ struct GradArgs {
   float* part;  // [splits][rows][cols] sums, or null: the result goes to out
   bool add;     // onto what part holds
   void* out;
-  int dtype;
 };
 
 __device__ __forceinline__ void store_as(void* out, int64_t i, float x, int dtype) {
   if (dtype == MPL_F32) ((float*)out)[i] = x;
   else if (dtype == MPL_F16) ((_Float16*)out)[i] = (_Float16)x;
   else ((__bf16*)out)[i] = (__bf16)x;
+}
+
+template <class C, bool PART, bool ADD>
+__device__ __forceinline__ void grad_store(const GradArgs& p, const f32x16 (&acc)[C::TM][C::TN], int64_t m0, int n0,
+                                           int wm, int wn, int lane, float* part, bool whole) {
+  constexpr int dtype = C::S == 2 ? MPL_F32 : C::BF ? MPL_BF16 : MPL_F16;
+  constexpr int size = PART || C::S == 2 ? 4 : 2;
+  const float u0 = *p.u0, u1 = C::S == 2 ? *p.u1 : 1.f;
+  // the tile's rows from a scalar address, the lane's place in 32 bits
+  char* base = (PART ? (char*)part : (char*)p.out) + m0 * p.cols * size;
+  const int last = (int)min(p.rows - m0, (int64_t)C::BM);
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+      const int col = n0 + (wn * C::TN + j) * 32 + (lane & 31);
+      const int row0 = (wm * C::TM + i) * 32 + 4 * (lane >> 5);
+      const uint32_t at = (uint32_t)(row0 * p.cols + col) * size;
+      const int rows = col < p.cols ? last - row0 : 0;  // below it there are rows
+      float old[16];
+      if (ADD) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int step = 8 * (r >> 2) + (r & 3);
+          old[r] = whole || step < rows ? *(const float*)(base + (int64_t)step * p.cols * size + at) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int step = 8 * (r >> 2) + (r & 3);
+        float x = acc[i][j][r] * u0 * u1;
+        if (ADD) x += old[r];
+        char* q = base + (int64_t)step * p.cols * size + at;
+        if (whole || step < rows) store_as(q, 0, x, PART ? MPL_F32 : dtype);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 template <class C>
@@ -449,22 +486,17 @@ __global__ __launch_bounds__(C::kThreads) void xent_grad_kernel(GradArgs p) {
   const int it0 = (int)((int64_t)p.iters * split / p.splits), it1 = (int)((int64_t)p.iters * (split + 1) / p.splits);
   f32x16 acc[C::TM][C::TN];
   C::run(p.A, p.B, m0, n0, it0, it1, a0, b0, a1, b1, acc);
-  const float u0 = *p.u0, u1 = C::S == 2 ? *p.u1 : 1.f;
-  float* part = p.part ? p.part + (int64_t)split * p.rows * p.cols : nullptr;
-#pragma unroll
-  for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-    for (int j = 0; j < C::TN; ++j) {
-      const int col = n0 + (wn * C::TN + j) * 32 + (lane & 31);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t row = m0 + (wm * C::TM + i) * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-        if (row >= p.rows || col >= p.cols) continue;
-        const float x = acc[i][j][r] * u0 * u1;
-        if (part) part[row * p.cols + col] = p.add ? part[row * p.cols + col] + x : x;
-        else store_as(p.out, row * p.cols + col, x, p.dtype);
-      }
-    }
+  float* part = p.part + (int64_t)split * p.rows * p.cols;
+  const bool whole = m0 + C::BM <= p.rows && n0 + C::BN <= p.cols;
+#define MPL_STORE(PART, ADD)                                                             \
+  do {                                                                                   \
+    if (whole) grad_store<C, PART, ADD>(p, acc, m0, n0, wm, wn, lane, part, true);       \
+    else grad_store<C, PART, ADD>(p, acc, m0, n0, wm, wn, lane, part, false);            \
+  } while (0)
+  if (!p.part) MPL_STORE(false, false);
+  else if (p.add) MPL_STORE(true, true);
+  else MPL_STORE(true, false);
+#undef MPL_STORE
 }
 
 __global__ __launch_bounds__(256) void xent_sum_kernel(const float* __restrict__ part, int splits, int64_t n,
@@ -707,7 +739,7 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
       g.u0 = scal + kInvP, g.u1 = scal + kInvE;
       g.part = p.splits_h > 1 || p.pieces > 1 ? (float*)(ws + p.ph) : nullptr;
       g.add = i > 0;
-      g.out = d_hidden, g.dtype = dtype;
+      g.out = d_hidden;
       MPL_TILE_DISPATCH(xent_grad_kernel, false, true, p.big_h, dim3(g.tiles_m * g.tiles_n, g.splits), s, g);
     }
     if (d_embedding) {
@@ -722,7 +754,6 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
       g.u0 = scal + kInvP, g.u1 = scal + kInvH;
       g.part = p.splits_e > 1 ? (float*)(ws + p.pe) : nullptr;
       g.out = (char*)d_embedding + a.v0 * d * (dtype == MPL_F32 ? 4 : 2);
-      g.dtype = dtype;
       MPL_TILE_DISPATCH(xent_grad_kernel, true, true, p.big_e, dim3(g.tiles_m * g.tiles_n, g.splits), s, g);
       if (g.part) {
         const int64_t n = nv * d;
