@@ -733,6 +733,35 @@ int mpl_lookup_bwd_dense_queries(const float* q_hat, const float* queries, const
                                  void* stream);
 
 /*
+ * LayerNorm of rows (model.py:86-125, nn.LayerNorm) and its backward pass, with
+ * the residual add before it:
+ *   s = x (+ residual, rounded to dtype),  y = (s - mean) rstd scale + bias,
+ *   rstd = 1 / sqrt(mean((s - mean)^2) + eps),
+ * in fp32, rounded once.  x, residual, y and sum are of dtype (MPL_F32, MPL_F16
+ * or MPL_BF16), scale and bias [d] of param_dtype: MPL_F32 or dtype.  x and
+ * residual have rows x_pitch and residual_pitch elements apart (>= d), of any
+ * alignment of whole elements; y and sum are dense.  residual and sum may be
+ * NULL (sum needs residual), and mean and rstd, fp32 [rows], both; d is at most
+ * 16,384 (else MPL_EUNSUPPORTED).  Outputs may not overlap inputs.  A row's
+ * result does not depend on the others.
+ *
+ * mpl_layer_norm_bwd takes x = the forward's s, its mean and rstd and the
+ * gradient dy of y, and writes dx (g_residual, the gradient of s from
+ * elsewhere, is added if it is not NULL), d_scale and d_bias (of param_dtype);
+ * each may be NULL.  d_scale and d_bias are sums over the rows in fp32 in a
+ * fixed order; for them the workspace takes
+ * mpl_layer_norm_bwd_workspace_bytes (4-byte aligned).  rows > 0.
+ */
+int mpl_layer_norm(const void* x, int64_t x_pitch, const void* residual, int64_t residual_pitch, int dtype,
+                   const void* scale, const void* bias, int param_dtype, int64_t rows, int d, float eps, void* y,
+                   void* sum, float* mean, float* rstd, void* stream);
+size_t mpl_layer_norm_bwd_workspace_bytes(int64_t rows, int d, int dtype);
+int mpl_layer_norm_bwd(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, const void* g_residual,
+                       int64_t g_residual_pitch, int dtype, const void* scale, int param_dtype, const float* mean,
+                       const float* rstd, int64_t rows, int d, void* dx, void* d_scale, void* d_bias, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
  * Softmax cross entropy of tokens over a vocabulary, from hidden rows and the
  * embedding table, without the logits in memory (model.py:125-126, embed.attend,
  * and the loss a trainer takes of its logits):

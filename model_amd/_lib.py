@@ -85,6 +85,9 @@ SIGNATURES = {
     "mpl_rows_linear": (_I, [_P, _P, _P, _P, _F, _P, _I, _P, _I, _P, _I64, _I, _I, _P, _P]),
     "mpl_dense_layers": (_I, [_P, _P, _P, _P, _F, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I64, _I, _P]),
     "mpl_causal_attention": (_I, [_P, _I64, _I, _I, _I, _F, _P, _P]),
+    "mpl_layer_norm": (_I, [_P, _I64, _P, _I64, _I, _P, _P, _I, _I64, _I, _F, _P, _P, _P, _P, _P]),
+    "mpl_layer_norm_bwd_workspace_bytes": (_SZ, [_I64, _I, _I]),
+    "mpl_layer_norm_bwd": (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _P, _I, _P, _P, _I64, _I, _P, _P, _P, _P, _SZ, _P]),
     "mpl_vocab_cross_entropy_workspace_bytes": (_SZ, [_I64, _I64, _I, _I, _I]),
     "mpl_vocab_cross_entropy": (_I, [_P, _I64, _P, _I64, _I, _P, _I64, _I64, _I, _I64, _P, _SZ, _P, _P, _P]),
     "mpl_vocab_cross_entropy_bwd": (_I, [_P, _I64, _P, _I64, _I, _P, _I64, _I64, _I, _I64, _P, _P, _P, _P, _SZ, _P,
