@@ -779,8 +779,11 @@ int mpl_layer_norm_bwd(const void* dy, int64_t dy_pitch, const void* x, int64_t 
  * d] (dense, of dtype; either may be NULL) from the forward's lse and the
  * gradients g_loss and g_lse of loss and lse (fp32 [rows]; either may be NULL,
  * for zeros): dz = (g_loss + g_lse) exp(z - lse) - g_loss [v = target], with
- * g_loss 0 where ignored, rounded to dtype (fp32: held to 2^-23 of each) between
- * the products.  rows > 0.  A row of an invalid target makes both gradients NaN.
+ * g_loss 0 where ignored, held in fp16 between the products (fp32: hi + lo, 2^-23
+ * of each) under a power of two that leaves 2^-38 of the largest |g_loss| or
+ * |g_loss + g_lse|.  bf16 operands are read as fp16 under a power of two of each
+ * array there, exact above 2^-29 of its largest.  rows > 0.  A row of an invalid
+ * target makes both gradients NaN.
  *
  * The workspace (256-byte aligned) takes mpl_vocab_cross_entropy_workspace_bytes
  * (0 for sizes out of range); calls that may run at the same time need one each.

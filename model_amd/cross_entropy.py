@@ -20,21 +20,21 @@ from . import _lib
 _DTYPES = {torch.float32: _lib.MPL_F32, torch.float16: _lib.MPL_F16, torch.bfloat16: _lib.MPL_BF16}
 
 
-def _rows(name: str, t: torch.Tensor, d: int) -> torch.Tensor:
-    """``t`` as [rows, d] that the library reads: elements of a row next to
-    each other, rows apart by any pitch.  Copied only where it does not lie
-    so, or where 16-bit rows that are read by tiles as they lie (d a multiple
-    of 64) do not start at 16 bytes."""
-    t = t.reshape(-1, d)
-    if t.shape[0] > 1 and (t.stride(0) < d or t.stride(1) != 1) or d > 1 and t.stride(1) != 1:
-        return t.contiguous()
-    if t.dtype != torch.float32 and d % 64 == 0 and (t.data_ptr() % 16 or t.shape[0] > 1 and t.stride(0) % 8):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _rows(t: torch.Tensor, d: int) -> Tuple[torch.Tensor, int]:
+    """``t`` [..., d] as rows that the library reads, elements of a row next to
+    each other, and the elements from row to row.  Copied only where it does
+    not lie so, or where 16-bit rows that are read by tiles as they lie (d a
+    multiple of 64) do not start at 16 bytes."""
+    pitch = d
+    if not t.is_contiguous():
+        t = t.reshape(-1, d)
+        if d > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < d:
+            t = t.contiguous()
+        elif t.shape[0] > 1:
+            pitch = t.stride(0)
+    if t.dtype != torch.float32 and d % 64 == 0 and (t.data_ptr() % 16 or pitch % 8):
+        return t.clone(memory_format=torch.contiguous_format), d
+    return t, pitch
 
 
 def _check(hidden: torch.Tensor, embedding: torch.Tensor, targets: torch.Tensor, what: str) -> None:
@@ -62,38 +62,42 @@ def _workspace(rows: int, vocab: int, d: int, code: int, backward: int, device) 
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-def _forward(h, e, t, ignore_index: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    """h [rows, d], e [vocab, d], t [rows] int64, as _rows gives them."""
-    R, d = h.shape
-    loss = torch.empty(R, dtype=torch.float32, device=h.device)
-    lse = torch.empty(R, dtype=torch.float32, device=h.device)
+def _ids(targets: torch.Tensor) -> torch.Tensor:
+    return (targets if targets.dtype == torch.int64 else targets.to(torch.int64)).contiguous()
+
+
+def _forward(hidden, embedding, ids, ignore_index: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(loss, lse) of ids' shape; ids contiguous int64."""
+    dev, (V, d), R = hidden.device, embedding.shape, ids.numel()
+    loss = torch.empty(ids.shape, dtype=torch.float32, device=dev)
+    lse = torch.empty(ids.shape, dtype=torch.float32, device=dev)
     if R:
+        (h, h_pitch), (e, e_pitch) = _rows(hidden, d), _rows(embedding, d)
         code = _DTYPES[h.dtype]
-        with _lib.on_device(h.device):
-            ws = _workspace(R, e.shape[0], d, code, 0, h.device)
+        with _lib.on_device(dev):
+            ws = _workspace(R, V, d, code, 0, dev)
             _lib.check(_lib.lib().mpl_vocab_cross_entropy(
-                h.data_ptr(), _pitch(h), e.data_ptr(), _pitch(e), code, t.data_ptr(), R, e.shape[0], d,
-                int(ignore_index), ws.data_ptr(), ws.numel(), loss.data_ptr(), lse.data_ptr(),
-                _lib.stream_ptr(h.device)), "mpl_vocab_cross_entropy")
+                h.data_ptr(), h_pitch, e.data_ptr(), e_pitch, code, ids.data_ptr(), R, V, d, ignore_index,
+                ws.data_ptr(), ws.numel(), loss.data_ptr(), lse.data_ptr(), _lib.stream_ptr(dev)),
+                "mpl_vocab_cross_entropy")
     return loss, lse
 
 
-def _backward(h, e, t, ignore_index: int, lse, g_loss, g_lse, want_h: bool, want_e: bool):
-    """Gradients of h and e (None where not wanted); g_loss and g_lse [rows] fp32 or None (not both)."""
-    R, d = h.shape
-    dh = torch.empty((R, d), dtype=h.dtype, device=h.device) if want_h else None
-    de = torch.empty(e.shape, dtype=e.dtype, device=h.device) if want_e else None
-    if R == 0:
-        return dh, None if de is None else de.zero_()
-    if want_h or want_e:
+def _backward(hidden, embedding, ids, ignore_index: int, lse, g_loss, g_lse, want_h: bool, want_e: bool):
+    """Gradients of hidden and embedding (None where not wanted); g_loss and g_lse fp32 or None (not both)."""
+    dev, (V, d), R = hidden.device, embedding.shape, ids.numel()
+    dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if want_h else None
+    de = (torch.empty if R else torch.zeros)((V, d), dtype=hidden.dtype, device=dev) if want_e else None
+    if R and (want_h or want_e):
+        (h, h_pitch), (e, e_pitch) = _rows(hidden, d), _rows(embedding, d)
         code = _DTYPES[h.dtype]
         P = _lib.ptr
-        with _lib.on_device(h.device):
-            ws = _workspace(R, e.shape[0], d, code, 1, h.device)
+        with _lib.on_device(dev):
+            ws = _workspace(R, V, d, code, 1, dev)
             _lib.check(_lib.lib().mpl_vocab_cross_entropy_bwd(
-                h.data_ptr(), _pitch(h), e.data_ptr(), _pitch(e), code, t.data_ptr(), R, e.shape[0], d,
-                int(ignore_index), lse.data_ptr(), P(g_loss), P(g_lse), ws.data_ptr(), ws.numel(), P(dh), P(de),
-                _lib.stream_ptr(h.device)), "mpl_vocab_cross_entropy_bwd")
+                h.data_ptr(), h_pitch, e.data_ptr(), e_pitch, code, ids.data_ptr(), R, V, d, ignore_index,
+                lse.data_ptr(), P(g_loss), P(g_lse), ws.data_ptr(), ws.numel(), P(dh), P(de), _lib.stream_ptr(dev)),
+                "mpl_vocab_cross_entropy_bwd")
     return dh, de
 
 
@@ -102,7 +106,7 @@ def _row_grad(g: Optional[torch.Tensor], shape, device, name: str) -> Optional[t
         return None
     if g.shape != shape or g.device != device or not g.is_floating_point():
         raise ValueError(f"{name} {tuple(g.shape)} {g.dtype} on {g.device}: must be floating, {tuple(shape)}, on {device}")
-    return g.detach().reshape(-1).to(torch.float32).contiguous()
+    return g.detach().to(torch.float32).contiguous()
 
 
 def _capturing() -> bool:
@@ -116,31 +120,26 @@ _NO_CAPTURE = ("torch autograd through vocab_cross_entropy is not supported unde
 class _CrossEntropyFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, embedding, targets, ignore_index):
-        d = hidden.shape[-1]
-        h, e = _rows("hidden", hidden, d), _rows("embedding", embedding, d)
-        t = targets.reshape(-1).to(torch.int64).contiguous()
-        loss, lse = _forward(h, e, t, ignore_index)
-        # the arguments themselves: autograd then sees them changed in place before the backward
-        ctx.save_for_backward(hidden, embedding, t, lse)
+        ids = _ids(targets)
+        loss, lse = _forward(hidden, embedding, ids, ignore_index)
+        ctx.save_for_backward(hidden, embedding, ids, lse)
         ctx.ignore_index = ignore_index
         ctx.set_materialize_grads(False)
-        return loss.reshape(targets.shape), lse.clone().reshape(targets.shape)
+        return loss, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, g_lse):
         if _capturing():
             raise RuntimeError(_NO_CAPTURE)
-        hidden, embedding, t, lse = ctx.saved_tensors
-        want_h, want_e = ctx.needs_input_grad[:2]
         if g_loss is None and g_lse is None:
             return None, None, None, None
-        d = hidden.shape[-1]
-        h, e = _rows("hidden", hidden, d), _rows("embedding", embedding, d)
-        shape = hidden.shape[:-1]
-        dh, de = _backward(h, e, t, ctx.ignore_index, lse, _row_grad(g_loss, shape, h.device, "the loss's gradient"),
-                           _row_grad(g_lse, shape, h.device, "the logsumexp's gradient"), want_h, want_e)
-        return None if dh is None else dh.reshape(hidden.shape), de, None, None
+        hidden, embedding, ids, lse = ctx.saved_tensors
+        want_h, want_e = ctx.needs_input_grad[:2]
+        dh, de = _backward(hidden, embedding, ids, ctx.ignore_index, lse,
+                           _row_grad(g_loss, ids.shape, hidden.device, "the loss's gradient"),
+                           _row_grad(g_lse, ids.shape, hidden.device, "the logsumexp's gradient"), want_h, want_e)
+        return dh, de, None, None
 
 
 def vocab_cross_entropy(hidden: torch.Tensor, embedding: torch.Tensor, targets: torch.Tensor, *,
@@ -159,7 +158,8 @@ def vocab_cross_entropy(hidden: torch.Tensor, embedding: torch.Tensor, targets: 
 
     Logits are sums in fp32 of the exact products (fp32 operands are held to
     2^-23 of each).  fp32 rows or table entries that are not finite give NaN.
-    The gradients take dz in the operands' type (fp32: to 2^-23).  For gradients
+    The gradients hold dz in fp16 under a power of two (fp32: hi and lo, to
+    2^-23), down to 2^-38 of the largest gradient of a token.  For gradients
     inside a captured HIP graph use vocab_cross_entropy_grads."""
     _check(hidden, embedding, targets, "vocab_cross_entropy")
     if torch.is_grad_enabled() and (hidden.requires_grad or embedding.requires_grad):
@@ -167,11 +167,8 @@ def vocab_cross_entropy(hidden: torch.Tensor, embedding: torch.Tensor, targets: 
             raise RuntimeError(_NO_CAPTURE)
         loss, lse = _CrossEntropyFunction.apply(hidden, embedding, targets, int(ignore_index))
         return (loss, lse) if return_lse else loss
-    d = hidden.shape[-1]
-    loss, lse = _forward(_rows("hidden", hidden, d), _rows("embedding", embedding, d),
-                         targets.reshape(-1).to(torch.int64).contiguous(), ignore_index)
-    loss = loss.reshape(targets.shape)
-    return (loss, lse.reshape(targets.shape)) if return_lse else loss
+    loss, lse = _forward(hidden, embedding, _ids(targets), int(ignore_index))
+    return (loss, lse) if return_lse else loss
 
 
 def vocab_cross_entropy_grads(hidden: torch.Tensor, embedding: torch.Tensor, targets: torch.Tensor,
@@ -183,14 +180,12 @@ def vocab_cross_entropy_grads(hidden: torch.Tensor, embedding: torch.Tensor, tar
     each token's loss and logsumexp (targets' shape; either may be None).  It
     may be captured in a HIP graph."""
     _check(hidden, embedding, targets, "vocab_cross_entropy_grads")
-    d = hidden.shape[-1]
     gl = _row_grad(g_loss, targets.shape, hidden.device, "g_loss")
     gs = _row_grad(g_lse, targets.shape, hidden.device, "g_lse")
     if gl is None and gs is None:
         raise ValueError("vocab_cross_entropy_grads: g_loss or g_lse is needed")
     with torch.no_grad():
-        h, e = _rows("hidden", hidden, d), _rows("embedding", embedding, d)
-        t = targets.reshape(-1).to(torch.int64).contiguous()
-        loss, lse = _forward(h, e, t, ignore_index)
-        dh, de = _backward(h, e, t, ignore_index, lse, gl, gs, True, True)
-    return loss.reshape(targets.shape), lse.reshape(targets.shape), dh.reshape(hidden.shape), de
+        ids = _ids(targets)
+        loss, lse = _forward(hidden, embedding, ids, int(ignore_index))
+        dh, de = _backward(hidden, embedding, ids, int(ignore_index), lse, gl, gs, True, True)
+    return loss, lse, dh, de

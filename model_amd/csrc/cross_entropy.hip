@@ -19,17 +19,19 @@
 // A piece's dz is small enough to stay in the Infinity Cache.
 #include <math.h>
 
+#include <algorithm>
+
 #include "common.h"
 #include "tile_mma.h"
 
 namespace mpl {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Device scalars of a call (floats): powers of two that fp32 and fp16 operands
-// were multiplied by, and their inverses.
-enum { kScaleE = 0, kInvE, kScaleH, kInvH, kScaleP, kInvP, kScalars = 16 };
+// Device scalars of a call (floats): the inverses of the powers of two that the
+// operands were multiplied by, and dz's with its inverse.
+enum { kInvE = 0, kInvH, kScaleP, kInvP, kScalars = 16 };
 
 // 2^(top - exponent of the largest magnitude), given by its bits; 1 for 0.
 __device__ __forceinline__ float scale_for(uint32_t bits, int top) {
@@ -63,73 +65,105 @@ struct PackArgs {
 };
 constexpr int kAmaxBlocks = 512;
 
-// Largest finite magnitudes of both arrays, one partial maximum a workgroup.
-__global__ __launch_bounds__(256) void amax_kernel(PackArgs p) {
-  const int a = blockIdx.y;
-  const PackOne o = a ? p.h : p.e;
-  const float* x = (const float*)o.src;
-  const int vecs = p.d / 4;
-  uint32_t m = 0;
-  if (o.vec) {
-    const int64_t n = o.rows * vecs;
-    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += 256 * (int64_t)gridDim.x) {
-      const int64_t r = i / vecs;
-      const float4 v = *(const float4*)(x + r * o.pitch + 4 * (i - r * vecs));
-      m = max(max(max(m, finite_bits(v.x)), max(finite_bits(v.y), finite_bits(v.z))), finite_bits(v.w));
-    }
-  }
-  const int c0 = o.vec ? 4 * vecs : 0, tail = p.d - c0;
-  if (tail) {
-    const int64_t n = o.rows * tail;
-    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += 256 * (int64_t)gridDim.x) {
-      const int64_t r = i / tail;
-      m = max(m, finite_bits(x[r * o.pitch + c0 + (i - r * tail)]));
-    }
-  }
-  __shared__ uint32_t s[256];
-  s[threadIdx.x] = m;
-  __syncthreads();
-  for (int h = 128; h; h >>= 1) {
-    if (threadIdx.x < h) s[threadIdx.x] = max(s[threadIdx.x], s[threadIdx.x + h]);
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) p.part[a * kAmaxBlocks + blockIdx.x] = s[0];
+// i / n in 32 bits where i allows it (wave-uniform branch mostly): a 64-bit
+// division is some hundred instructions.
+__device__ __forceinline__ int64_t divide(int64_t i, int n) {
+  return (uint64_t)i >> 32 ? i / n : (int64_t)((uint32_t)i / (uint32_t)n);
 }
 
-// Rows of an array as a tile product's operand: 16-bit rows zero-filled to
-// whole stages, or fp32 rows as hi and lo.  A thread writes 8 elements.
-template <bool SPLIT>
+// Source types of packed operands and what becomes of them: 16-bit rows that are
+// only filled up; bf16 rows as scaled fp16; fp32 rows as scaled hi and lo.
+enum { kCopy16 = 0, kBf16ToF16, kSplit };
+
+// 8 (fp32: 4) elements from element c of row r, zero past d.
+template <int MODE>
+struct Source {
+  static constexpr int VE = MODE == kSplit ? 4 : 8;
+  __device__ static void load(const PackOne& o, int64_t r, int64_t c, int64_t d, float (&v)[VE]) {
+    if constexpr (MODE == kSplit) {
+      const float* x = (const float*)o.src + r * o.pitch + c;
+      if (o.vec && c + VE <= d) {
+        *(float4*)v = *(const float4*)x;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) v[j] = c + j < d ? x[j] : 0.f;
+      }
+    } else {  // bf16
+      const uint16_t* x = (const uint16_t*)o.src + r * o.pitch + c;
+      uint16_t u[VE] __attribute__((aligned(16)));
+      if (o.vec && c + VE <= d) {
+        *(uint4*)u = *(const uint4*)x;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) u[j] = c + j < d ? x[j] : (uint16_t)0;
+      }
+#pragma unroll
+      for (int j = 0; j < VE; ++j) v[j] = __uint_as_float((uint32_t)u[j] << 16);
+    }
+  }
+};
+
+// Largest finite magnitudes of both arrays, one partial maximum a workgroup.
+template <int MODE>
+__global__ __launch_bounds__(256) void amax_kernel(PackArgs p) {
+  constexpr int VE = Source<MODE>::VE;
+  const int a = blockIdx.y;
+  const PackOne o = a ? p.h : p.e;
+  const int vecs = (p.d + VE - 1) / VE;
+  const int64_t n = o.rows * vecs, step = 256 * (int64_t)gridDim.x;
+  uint32_t m = 0;
+  auto take = [&](int64_t r, int64_t c, int64_t d) __attribute__((always_inline)) {
+    float v[VE];
+    Source<MODE>::load(o, r, c, d, v);
+#pragma unroll
+    for (int j = 0; j < VE; ++j) m = max(m, finite_bits(v[j]));
+  };
+  int64_t i = blockIdx.x * 256 + threadIdx.x;
+  if (o.vec && o.pitch == p.d && p.d % VE == 0) {  // one long row
+    for (; i + 3 * step < n; i += 4 * step) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) take(0, VE * (i + k * step), VE * n);
+    }
+    for (; i < n; i += step) take(0, VE * i, VE * n);
+  } else {
+    for (; i < n; i += step) {
+      const int64_t r = divide(i, vecs);
+      take(r, VE * (i - r * vecs), p.d);
+    }
+  }
+  __shared__ uint32_t s[4];
+  for (int h = 32; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) p.part[a * kAmaxBlocks + blockIdx.x] = max(max(s[0], s[1]), max(s[2], s[3]));
+}
+
+// Rows of an array as a tile product's operand, zero-filled to whole stages.  A
+// thread writes 8 elements.
+template <int MODE>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   const int a = blockIdx.x < p.e.blocks ? 0 : 1;
   const PackOne o = a ? p.h : p.e;
   float scale = 1.f;
-  if (SPLIT) {
+  if constexpr (MODE != kCopy16) {
     __shared__ uint32_t s[4];
     uint32_t m = max(p.part[a * kAmaxBlocks + threadIdx.x], p.part[a * kAmaxBlocks + 256 + threadIdx.x]);
     for (int h = 32; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
     __syncthreads();
     scale = scale_for(max(max(s[0], s[1]), max(s[2], s[3])), 14);
-    if (threadIdx.x == 0 && (blockIdx.x == 0 || blockIdx.x == p.e.blocks)) {
-      p.scal[a == 0 ? kScaleE : kScaleH] = scale;
+    if (threadIdx.x == 0 && (blockIdx.x == 0 || blockIdx.x == p.e.blocks))
       p.scal[a == 0 ? kInvE : kInvH] = 1.f / scale;
-    }
   }
   const int per = p.dpad / 8;
   const int64_t i = (int64_t)(blockIdx.x - (a ? p.e.blocks : 0)) * 256 + threadIdx.x;
   if (i >= o.rows * per) return;
-  const int64_t r = i / per;
+  const int64_t r = divide(i, per);
   const int c = 8 * (int)(i - r * per);
-  if (SPLIT) {
-    const float* x = (const float*)o.src + r * o.pitch + c;
+  if constexpr (MODE == kSplit) {
     float v[8];
-    if (o.vec && c + 8 <= p.d) {
-      *(float4*)v = *(const float4*)x;
-      *(float4*)(v + 4) = *(const float4*)(x + 4);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < p.d ? x[j] : 0.f;
-    }
+    Source<MODE>::load(o, r, c, p.d, *(float(*)[4])v);
+    Source<MODE>::load(o, r, c + 4, p.d, *(float(*)[4])(v + 4));
     half8 hi, lo;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -140,6 +174,13 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
     char* q = o.dst + (r * p.dpad + c / 32 * 32) * 4 + (c % 32) * 2;
     *(half8*)q = hi;
     *(half8*)(q + 64) = lo;
+  } else if constexpr (MODE == kBf16ToF16) {
+    float v[8];
+    Source<MODE>::load(o, r, c, p.d, v);
+    half8 h;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = (_Float16)(v[j] * scale);
+    *(half8*)(o.dst + (r * p.dpad + c) * 2) = h;
   } else {
     const uint16_t* x = (const uint16_t*)o.src + r * o.pitch + c;
     uint16_t v[8] __attribute__((aligned(16)));
@@ -160,13 +201,14 @@ struct LogitArgs {
   int iters;
   uint32_t tiles_v, tiles_t;
   const float* scal;
+  bool scaled;  // the operands carry powers of two
   const int64_t* target;
   // forward
-  float2* part;  // [tiles_v][R]
+  float2* part;  // [tiles_v][R]: maximum of z log2(e), sum of 2^(z log2(e) - maximum)
   float* z_target;
   // backward: the piece starts at row v0 of the table
   int64_t v0, rows_p, pitch_p;  // rows_p: rows of dz that exist (zero past R); pitch in bytes
-  const float* coef;            // [3][rows_p]: g + gl, g, lse
+  const float* coef;            // [3][rows_p]: g + gl, g, lse log2(e)
   char* P;
 };
 
@@ -186,20 +228,13 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
   const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
   f32x16 acc[C::TM][C::TN];
   C::run(p.E, p.H, v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
-  float u0 = 1.f, u1 = 1.f;
-  if (C::S == 2) u0 = p.scal[kInvE], u1 = p.scal[kInvH];
+  // z log2(e) = acc * unit: one multiply and add before each exp2
+  const float unscale = p.scaled ? p.scal[kInvE] * p.scal[kInvH] : 1.f, unit = unscale * kLog2e;
   const int64_t vw = v0 + wm * C::TM * 32 + 4 * (lane >> 5);  // of acc[0][.][0]
-  __syncthreads();  // every wave is done with the stages: they hold the waves' pairs from here
-  float2* pair = (float2*)a0;  // [WM][BN]
+  float2* pair = (float2*)a0;  // [WM][BN]: the stages are free
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) {
     const int64_t tok = t0 + (wn * C::TN + j) * 32 + (lane & 31);
-    if (C::S == 2) {
-#pragma unroll
-      for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = acc[i][j][r] * u0 * u1;
-    }
     const int64_t at = tok < p.R ? p.target[tok] - vw : -1;  // place of the target among the lane's, if it is there
     const int place = at >= 0 && at < C::TM * 32 && !(at & 4) ? (int)at : -1;
     if (__any(place >= 0)) {
@@ -208,7 +243,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
       for (int i = 0; i < C::TM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) z = place == 32 * i + 8 * (r >> 2) + (r & 3) ? acc[i][j][r] : z;
-      if (place >= 0) p.z_target[tok] = z;
+      if (place >= 0) p.z_target[tok] = z * unscale;
     }
     if (v0 + C::BM > p.V) {
 #pragma unroll
@@ -225,12 +260,13 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
     float x = m, y = m;
     half_swap(x, y);
     m = fmaxf(x, y);
+    m *= unit;
     const float ref = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2e);
+      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], unit, -ref));
     x = s, y = s;
     half_swap(x, y);
     if (lane < 32) pair[wm * C::BN + (wn * C::TN + j) * 32 + lane] = make_float2(m, x + y);
@@ -245,7 +281,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < C::WM; ++w)
-      s += pair[w * C::BN + t].y * __builtin_amdgcn_exp2f((pair[w * C::BN + t].x - ref) * kLog2e);
+      s += pair[w * C::BN + t].y * __builtin_amdgcn_exp2f(pair[w * C::BN + t].x - ref);
     p.part[(int64_t)tv * p.R + t0 + t] = make_float2(m, s);
   }
 }
@@ -264,7 +300,7 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
     for (int i = g; i < tiles; i += 8) {
       const float2 v = part[(int64_t)i * R + tok];
       const float n = fmaxf(m, v.x), ref = n == -INFINITY ? 0.f : n;
-      l = l * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + v.y * __builtin_amdgcn_exp2f((v.x - ref) * kLog2e);
+      l = l * __builtin_amdgcn_exp2f(m - ref) + v.y * __builtin_amdgcn_exp2f(v.x - ref);
       m = n;
     }
   s[g][t] = make_float2(m, l);
@@ -273,10 +309,10 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
   for (int i = 1; i < 8; ++i) {
     const float2 v = s[i][t];
     const float n = fmaxf(m, v.x), ref = n == -INFINITY ? 0.f : n;
-    l = l * __builtin_amdgcn_exp2f((m - ref) * kLog2e) + v.y * __builtin_amdgcn_exp2f((v.x - ref) * kLog2e);
+    l = l * __builtin_amdgcn_exp2f(m - ref) + v.y * __builtin_amdgcn_exp2f(v.x - ref);
     m = n;
   }
-  const float out = m + logf(l);
+  const float out = (m + log2f(l)) * kLn2;
   const int64_t at = target[tok];
   lse[tok] = out;
   loss[tok] = at == ignore ? 0.f : (at < 0 || at >= V) ? NAN : out - z_target[tok];
@@ -284,22 +320,24 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
 
 // ----------------------------------------------------------------- backward
 // Coefficients of each row, zero for the rows that only fill dz up, and the
-// power of two that dz is held under (fp32 and fp16 calls; |dz| <= |g + gl| +
-// |g|, below 2^15 after it).  One workgroup: rows are few against the products.
+// power of two that dz is held under (|dz| <= |g + gl| + |g|, below 2^15 after
+// it).  One workgroup: rows are few against the products.
 __global__ __launch_bounds__(1024) void xent_coef_kernel(const int64_t* __restrict__ target, int64_t R, int64_t rows_p,
                                                          int64_t V, int64_t ignore, const float* __restrict__ g_loss,
                                                          const float* __restrict__ g_lse,
-                                                         const float* __restrict__ lse, bool scaled,
+                                                         const float* __restrict__ lse,
                                                          float* __restrict__ coef, float* __restrict__ scal) {
   uint32_t m = 0;
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < rows_p; i += 1024) {
     float all = 0.f, g = 0.f, l = 0.f;
+    const int64_t k = min(i, R - 1);  // loads without branches, so that they fly together
+    const int64_t at = target[k];
+    const float gk = g_loss ? g_loss[k] : 0.f, sk = g_lse ? g_lse[k] : 0.f, lk = lse[k];
     if (i < R) {
-      const int64_t at = target[i];
-      g = at == ignore || g_loss == nullptr ? 0.f : g_loss[i];
-      if (at != ignore && (at < 0 || at >= V)) g = NAN;
-      all = g_lse ? g + g_lse[i] : g;
-      l = lse[i];
+      g = at == ignore ? 0.f : at < 0 || at >= V ? NAN : gk;
+      all = g + sk;
+      l = lk * kLog2e;
     }
     coef[i] = all;
     coef[rows_p + i] = g;
@@ -312,28 +350,13 @@ __global__ __launch_bounds__(1024) void xent_coef_kernel(const int64_t* __restri
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) m = max(m, s[i]);
-    const float scale = scaled ? scale_for(m, 13) : 1.f;
+    const float scale = scale_for(m, 13);
     scal[kScaleP] = scale;
     scal[kInvP] = 1.f / scale;
   }
 }
 
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-  if constexpr (BF) {
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    b2 v;
-    v[0] = (__bf16)x;
-    v[1] = (__bf16)y;
-    return __builtin_bit_cast(uint32_t, v);
-  } else {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    h2 v;
-    v[0] = (_Float16)x;
-    v[1] = (_Float16)y;
-    return __builtin_bit_cast(uint32_t, v);
-  }
-}
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 template <class C>
 __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
@@ -345,8 +368,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
   const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
   f32x16 acc[C::TM][C::TN];
   C::run(p.E, p.H, p.v0 + v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
-  float u0 = 1.f, u1 = 1.f;
-  if (C::S == 2) u0 = p.scal[kInvE], u1 = p.scal[kInvH];
+  const float unit = (p.scaled ? p.scal[kInvE] * p.scal[kInvH] : 1.f) * kLog2e;
   const float up = p.scal[kScaleP];
   const int half = lane >> 5;
   const int64_t vw = v0 + wm * C::TM * 32;  // the wave's first column of the piece
@@ -365,11 +387,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
     for (int i = 0; i < C::TM; ++i) {
       float x[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float z = acc[i][j][r];
-        if (C::S == 2) z = z * u0 * u1;
-        x[r] = ga * __builtin_amdgcn_exp2f((z - lse) * kLog2e);
-      }
+      for (int r = 0; r < 16; ++r) x[r] = ga * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], unit, -lse));
       if (hit) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -388,12 +406,12 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
       for (int pl = 0; pl < C::S; ++pl) {
         uint32_t u[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) u[r] = pack2<C::BF>(x[2 * r], x[2 * r + 1]);
-        if (C::S == 2 && pl == 0) {
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-            const h2 v = __builtin_bit_cast(h2, u[r]);
+        for (int r = 0; r < 8; ++r) {
+          half2v v;
+          v[0] = (_Float16)x[2 * r];
+          v[1] = (_Float16)x[2 * r + 1];
+          u[r] = __builtin_bit_cast(uint32_t, v);
+          if (C::S == 2 && pl == 0) {
             x[2 * r] -= (float)v[0];
             x[2 * r + 1] -= (float)v[1];
           }
@@ -428,6 +446,7 @@ struct GradArgs {
   float* part;  // [splits][rows][cols] sums, or null: the result goes to out
   bool add;     // onto what part holds
   void* out;
+  int dtype;  // of out
 };
 
 __device__ __forceinline__ void store_as(void* out, int64_t i, float x, int dtype) {
@@ -436,14 +455,14 @@ __device__ __forceinline__ void store_as(void* out, int64_t i, float x, int dtyp
   else ((__bf16*)out)[i] = (__bf16)x;
 }
 
-template <class C, bool PART, bool ADD>
+// DTYPE: of what is stored, fp32 sums or the result; ADD: onto the sums there.
+template <class C, int DTYPE, bool ADD>
 __device__ __forceinline__ void grad_store(const GradArgs& p, const f32x16 (&acc)[C::TM][C::TN], int64_t m0, int n0,
-                                           int wm, int wn, int lane, float* part, bool whole) {
-  constexpr int dtype = C::S == 2 ? MPL_F32 : C::BF ? MPL_BF16 : MPL_F16;
-  constexpr int size = PART || C::S == 2 ? 4 : 2;
-  const float u0 = *p.u0, u1 = C::S == 2 ? *p.u1 : 1.f;
+                                           int wm, int wn, int lane, void* out, bool whole) {
+  constexpr int size = DTYPE == MPL_F32 ? 4 : 2;
+  const float u0 = *p.u0, u1 = p.u1 ? *p.u1 : 1.f;
   // the tile's rows from a scalar address, the lane's place in 32 bits
-  char* base = (PART ? (char*)part : (char*)p.out) + m0 * p.cols * size;
+  char* base = (char*)out + m0 * p.cols * size;
   const int last = (int)min(p.rows - m0, (int64_t)C::BM);
 #pragma unroll
   for (int i = 0; i < C::TM; ++i)
@@ -467,7 +486,7 @@ __device__ __forceinline__ void grad_store(const GradArgs& p, const f32x16 (&acc
         float x = acc[i][j][r] * u0 * u1;
         if (ADD) x += old[r];
         char* q = base + (int64_t)step * p.cols * size + at;
-        if (whole || step < rows) store_as(q, 0, x, PART ? MPL_F32 : dtype);
+        if (whole || step < rows) store_as(q, 0, x, DTYPE);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -488,23 +507,35 @@ __global__ __launch_bounds__(C::kThreads) void xent_grad_kernel(GradArgs p) {
   C::run(p.A, p.B, m0, n0, it0, it1, a0, b0, a1, b1, acc);
   float* part = p.part + (int64_t)split * p.rows * p.cols;
   const bool whole = m0 + C::BM <= p.rows && n0 + C::BN <= p.cols;
-#define MPL_STORE(PART, ADD)                                                             \
-  do {                                                                                   \
-    if (whole) grad_store<C, PART, ADD>(p, acc, m0, n0, wm, wn, lane, part, true);       \
-    else grad_store<C, PART, ADD>(p, acc, m0, n0, wm, wn, lane, part, false);            \
+#define MPL_STORE(DTYPE, ADD, out)                                                      \
+  do {                                                                                  \
+    if (whole) grad_store<C, DTYPE, ADD>(p, acc, m0, n0, wm, wn, lane, out, true);      \
+    else grad_store<C, DTYPE, ADD>(p, acc, m0, n0, wm, wn, lane, out, false);           \
   } while (0)
-  if (!p.part) MPL_STORE(false, false);
-  else if (p.add) MPL_STORE(true, true);
-  else MPL_STORE(true, false);
+  if (p.part && p.add) MPL_STORE(MPL_F32, true, part);
+  else if (p.part) MPL_STORE(MPL_F32, false, part);
+  else if (p.dtype == MPL_F32) MPL_STORE(MPL_F32, false, p.out);
+  else if (p.dtype == MPL_F16) MPL_STORE(MPL_F16, false, p.out);
+  else MPL_STORE(MPL_BF16, false, p.out);
 #undef MPL_STORE
 }
 
+// Adds the splits' sums in order; 4 values a thread.
 __global__ __launch_bounds__(256) void xent_sum_kernel(const float* __restrict__ part, int splits, int64_t n,
                                                        void* __restrict__ out, int dtype) {
-  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += 256 * (int64_t)gridDim.x) {
-    float s = part[i];
-    for (int k = 1; k < splits; ++k) s += part[k * n + i];
-    store_as(out, i, s, dtype);
+  const bool vec = n % 4 == 0;
+  for (int64_t i = 4 * (blockIdx.x * 256 + (int64_t)threadIdx.x); i < n; i += 1024 * (int64_t)gridDim.x) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const int m = (int)min(n - i, (int64_t)4);
+    for (int k = 0; k < splits; ++k) {
+      if (vec) {
+        const float4 v = *(const float4*)(part + k * n + i);
+        s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+      } else {
+        for (int e = 0; e < m; ++e) s[e] += part[k * n + i + e];
+      }
+    }
+    for (int e = 0; e < m; ++e) store_as(out, i + e, s[e], dtype);
   }
 }
 
@@ -514,41 +545,28 @@ template <int S, bool BF, bool AST, bool BST> using Mid = TileMma<S, BF, AST, BS
 
 struct Plan {
   int64_t rows_p, v_piece, pieces;
-  int dpad;
-  bool pack, split;
+  int dpad, mode;  // mode: what the operands need, -1 nothing
+  bool split;
   bool big_z, big_h, big_e;
   uint32_t tiles_v;  // of the forward
   int splits_h, splits_e;
   // offsets into the workspace
-  size_t scal, amax, e, h, part, zt, coef, P, ph, pe, bytes_fwd, bytes_bwd;
+  size_t scal, amax, e, h, part, zt, coef, P, ph, pe, bytes;
 };
 
-constexpr int64_t kPieceBytes = 256ll << 20;
+constexpr int64_t kPieceBytes = 512ll << 20;
 
 inline int64_t up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
 
-Plan make_plan(int64_t R, int64_t V, int d, int dtype) {
+Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
   Plan p{};
   p.split = dtype == MPL_F32;
   const int S = p.split ? 2 : 1;
-  p.pack = p.split || d % 64;
+  p.mode = p.split ? kSplit : backward && dtype == MPL_BF16 ? kBf16ToF16 : d % 64 ? kCopy16 : -1;
   p.dpad = (int)up(d, 64);
   p.rows_p = up(R, 64);
-  p.big_z = cdiv(R, 256) * cdiv(V, 256) >= 512;
+  p.big_z = cdiv(R, 256) * cdiv(V, 256) >= 256;
   p.tiles_v = (uint32_t)cdiv(V, p.big_z ? 256 : 128);
-  const int64_t col = p.rows_p * 2 * S;
-  const int64_t most = kPieceBytes / col / 256 * 256;
-  p.pieces = cdiv(V, most < 256 ? 256 : most);
-  p.v_piece = up(cdiv(V, p.pieces), 256);
-  p.pieces = cdiv(V, p.v_piece);
-  auto pick = [&](int64_t M, int64_t N, int64_t K, bool& big, int& splits) {
-    big = cdiv(M, 256) * cdiv(N, 256) >= 256;
-    const int64_t tiles = big ? cdiv(M, 256) * cdiv(N, 256) : cdiv(M, 128) * cdiv(N, 128);
-    const int64_t iters = K * S / 64, want = cdiv(512, tiles);
-    splits = (int)(big ? 1 : want < 1 ? 1 : want > iters / 8 ? (iters / 8 > 0 ? iters / 8 : 1) : want);
-  };
-  pick(R, p.dpad, p.v_piece, p.big_h, p.splits_h);
-  pick(p.v_piece, p.dpad, p.rows_p, p.big_e, p.splits_e);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -557,18 +575,37 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype) {
   };
   p.scal = take(kScalars * 4);
   p.amax = take(2 * kAmaxBlocks * 4);
-  p.e = take(p.pack ? (size_t)V * p.dpad * 2 * S : 0);
-  p.h = take(p.pack ? (size_t)R * p.dpad * 2 * S : 0);
-  const size_t shared = at;
-  p.part = take((size_t)p.tiles_v * R * 8);
-  p.zt = take((size_t)R * 4);
-  p.bytes_fwd = at;
-  at = shared;
+  p.e = take(p.mode >= 0 ? (size_t)V * p.dpad * 2 * S : 0);
+  p.h = take(p.mode >= 0 ? (size_t)R * p.dpad * 2 * S : 0);
+  if (!backward) {
+    p.part = take((size_t)p.tiles_v * R * 8);
+    p.zt = take((size_t)R * 4);
+    p.bytes = at;
+    return p;
+  }
+  // Pieces of the vocabulary: as few as their dz's bytes allow, and where the
+  // table's gradient has 256 tiles in a piece, whole multiples of that: each
+  // product of a piece then fills the 256 CUs evenly.
+  const int64_t col = p.rows_p * 2 * S, even = 256 * cdiv(256, cdiv(d, 256));
+  int64_t most = std::max<int64_t>(kPieceBytes / col / 256, 1) * 256;
+  if (most >= even && most < V) most = most / even * even;
+  p.pieces = cdiv(V, most);
+  p.v_piece = p.pieces == 1 ? up(V, 256) : most;
+  // Products with few tiles split their contraction, at least 16 stages a part.
+  auto pick = [&](int64_t M, int64_t K, bool& big, int& splits) {
+    const int64_t tiles = cdiv(M, 256) * cdiv(d, 256), iters = K * S / 64;
+    big = tiles * std::max<int64_t>(1, iters / 16) >= 256;
+    const int64_t n = big ? tiles : cdiv(M, 128) * cdiv(d, 128), want = big ? 256 : 512;
+    splits = (int)std::max<int64_t>(1, std::min(cdiv(want, n), iters / 16));
+    if (n * 4 >= want * 3) splits = 1;
+  };
+  pick(R, p.v_piece, p.big_h, p.splits_h);
+  pick(p.v_piece, p.rows_p, p.big_e, p.splits_e);
   p.coef = take((size_t)p.rows_p * 12);
   p.P = take((size_t)p.v_piece * col);
   p.ph = take(p.splits_h > 1 || p.pieces > 1 ? (size_t)p.splits_h * R * d * 4 : 0);
   p.pe = take(p.splits_e > 1 ? (size_t)p.splits_e * p.v_piece * d * 4 : 0);
-  p.bytes_bwd = at;
+  p.bytes = at;
   return p;
 }
 
@@ -605,7 +642,7 @@ int check_call(const char* what, const Call& c, const void* ws, size_t ws_bytes,
 // Brings both arrays into operand form; E and H are the rows forms.
 void operands(const Call& c, const Plan& p, char* ws, hipStream_t s, TileOperand& E, TileOperand& H) {
   const int64_t row = (int64_t)p.dpad * (p.split ? 4 : 2);
-  if (!p.pack) {
+  if (p.mode < 0) {
     E = {(const char*)c.embedding, c.embedding_pitch * 2, c.V, row};
     H = {(const char*)c.hidden, c.hidden_pitch * 2, c.R, row};
     return;
@@ -621,29 +658,24 @@ void operands(const Call& c, const Plan& p, char* ws, hipStream_t s, TileOperand
   a.scal = (float*)(ws + p.scal);
   a.part = (uint32_t*)(ws + p.amax);
   const unsigned grid = (unsigned)(a.e.blocks + a.h.blocks);
-  if (p.split) {
-    amax_kernel<<<dim3(kAmaxBlocks, 2), 256, 0, s>>>(a);
-    pack_kernel<true><<<grid, 256, 0, s>>>(a);
+  if (p.mode == kSplit) {
+    amax_kernel<kSplit><<<dim3(kAmaxBlocks, 2), 256, 0, s>>>(a);
+    pack_kernel<kSplit><<<grid, 256, 0, s>>>(a);
+  } else if (p.mode == kBf16ToF16) {
+    amax_kernel<kBf16ToF16><<<dim3(kAmaxBlocks, 2), 256, 0, s>>>(a);
+    pack_kernel<kBf16ToF16><<<grid, 256, 0, s>>>(a);
   } else {
-    pack_kernel<false><<<grid, 256, 0, s>>>(a);
+    pack_kernel<kCopy16><<<grid, 256, 0, s>>>(a);
   }
   E = {ws + p.e, row, c.V, row};
   H = {ws + p.h, row, c.R, row};
 }
 
-// The instantiation of one product for the call's type and tile.
-#define MPL_TILE_DISPATCH(KERNEL, AST, BST, big, grid, s, args)                                            \
-  do {                                                                                                     \
-    if (c.dtype == MPL_F32) {                                                                              \
-      if (big) KERNEL<Big<2, false, AST, BST>><<<grid, Big<2, false, AST, BST>::kThreads, 0, s>>>(args);   \
-      else KERNEL<Mid<2, false, AST, BST>><<<grid, Mid<2, false, AST, BST>::kThreads, 0, s>>>(args);       \
-    } else if (c.dtype == MPL_F16) {                                                                       \
-      if (big) KERNEL<Big<1, false, AST, BST>><<<grid, Big<1, false, AST, BST>::kThreads, 0, s>>>(args);   \
-      else KERNEL<Mid<1, false, AST, BST>><<<grid, Mid<1, false, AST, BST>::kThreads, 0, s>>>(args);       \
-    } else {                                                                                               \
-      if (big) KERNEL<Big<1, true, AST, BST>><<<grid, Big<1, true, AST, BST>::kThreads, 0, s>>>(args);     \
-      else KERNEL<Mid<1, true, AST, BST>><<<grid, Mid<1, true, AST, BST>::kThreads, 0, s>>>(args);         \
-    }                                                                                                      \
+// The instantiation of one product for the operands' type and the tile.
+#define MPL_TILE(KERNEL, S, BF, AST, BST, big, grid, s, args)                                           \
+  do {                                                                                                  \
+    if (big) KERNEL<Big<S, BF, AST, BST>><<<grid, Big<S, BF, AST, BST>::kThreads, 0, s>>>(args);        \
+    else KERNEL<Mid<S, BF, AST, BST>><<<grid, Mid<S, BF, AST, BST>::kThreads, 0, s>>>(args);            \
   } while (0)
 
 }  // namespace
@@ -653,8 +685,7 @@ using namespace mpl;
 
 extern "C" size_t mpl_vocab_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int d, int dtype, int backward) {
   if (!sizes_ok(rows, vocab, d, dtype)) return 0;
-  const Plan p = make_plan(rows, vocab, d, dtype);
-  return backward ? p.bytes_bwd : p.bytes_fwd;
+  return make_plan(rows, vocab, d, dtype, backward != 0).bytes;
 }
 
 extern "C" int mpl_vocab_cross_entropy(const void* hidden, int64_t hidden_pitch, const void* embedding,
@@ -667,8 +698,8 @@ extern "C" int mpl_vocab_cross_entropy(const void* hidden, int64_t hidden_pitch,
               what, (long long)rows, (long long)vocab, d, dtype);
   if (rows == 0) return MPL_OK;
   const Call c{hidden, hidden_pitch, embedding, embedding_pitch, dtype, rows, vocab, d};
-  const Plan p = make_plan(rows, vocab, d, dtype);
-  if (const int rc = check_call(what, c, workspace, workspace_bytes, p.bytes_fwd)) return rc;
+  const Plan p = make_plan(rows, vocab, d, dtype, false);
+  if (const int rc = check_call(what, c, workspace, workspace_bytes, p.bytes)) return rc;
   MPL_REQUIRE(target && loss && lse, MPL_EINVAL, "%s: null buffer", what);
   char* ws = (char*)workspace;
   hipStream_t s = (hipStream_t)stream;
@@ -679,10 +710,14 @@ extern "C" int mpl_vocab_cross_entropy(const void* hidden, int64_t hidden_pitch,
   a.tiles_v = p.tiles_v;
   a.tiles_t = (uint32_t)cdiv(rows, p.big_z ? 256 : 128);
   a.scal = (const float*)(ws + p.scal);
+  a.scaled = p.split;
   a.target = target;
   a.part = (float2*)(ws + p.part);
   a.z_target = (float*)(ws + p.zt);
-  MPL_TILE_DISPATCH(xent_lse_kernel, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
+  const unsigned grid = a.tiles_v * a.tiles_t;
+  if (dtype == MPL_F32) MPL_TILE(xent_lse_kernel, 2, false, false, false, p.big_z, grid, s, a);
+  else if (dtype == MPL_F16) MPL_TILE(xent_lse_kernel, 1, false, false, false, p.big_z, grid, s, a);
+  else MPL_TILE(xent_lse_kernel, 1, true, false, false, p.big_z, grid, s, a);
   xent_join_kernel<<<(unsigned)cdiv(rows, 32), 256, 0, s>>>(a.part, (int)p.tiles_v, rows, vocab, target, ignore_index,
                                                           a.z_target, loss, lse);
   return check_launch(what);
@@ -699,8 +734,8 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
               "%s: bad sizes or type: rows=%lld vocab=%lld d=%d dtype=%d", what, (long long)rows, (long long)vocab, d,
               dtype);
   const Call c{hidden, hidden_pitch, embedding, embedding_pitch, dtype, rows, vocab, d};
-  const Plan p = make_plan(rows, vocab, d, dtype);
-  if (const int rc = check_call(what, c, workspace, workspace_bytes, p.bytes_bwd)) return rc;
+  const Plan p = make_plan(rows, vocab, d, dtype, true);
+  if (const int rc = check_call(what, c, workspace, workspace_bytes, p.bytes)) return rc;
   MPL_REQUIRE(target && lse && (g_loss || g_lse) && (d_hidden || d_embedding), MPL_EINVAL, "%s: null buffer", what);
   char* ws = (char*)workspace;
   hipStream_t s = (hipStream_t)stream;
@@ -710,12 +745,13 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
   float* scal = (float*)(ws + p.scal);
   float* coef = (float*)(ws + p.coef);
   xent_coef_kernel<<<1, 1024, 0, s>>>(target, rows, p.rows_p, vocab, ignore_index, g_loss, g_lse, lse,
-                                      dtype != MPL_BF16, coef, scal);
+                                      coef, scal);
   a.R = rows, a.V = vocab;
   a.iters = p.dpad * S / 64;
   const int bz = p.big_z ? 256 : 128;
   a.tiles_t = (uint32_t)cdiv(rows, bz);
   a.scal = scal;
+  a.scaled = p.mode > kCopy16;
   a.target = target;
   a.rows_p = p.rows_p;
   a.pitch_p = p.v_piece * 2 * S;
@@ -726,7 +762,8 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
     const int64_t nv = p.v_piece < vocab - a.v0 ? p.v_piece : vocab - a.v0;  // rows of the table in the piece
     const int64_t nvp = up(nv, 256);
     a.tiles_v = (uint32_t)(nvp / bz);
-    MPL_TILE_DISPATCH(xent_dz_kernel, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
+    if (p.split) MPL_TILE(xent_dz_kernel, 2, false, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
+    else MPL_TILE(xent_dz_kernel, 1, false, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
     if (d_hidden) {
       GradArgs g{};
       g.A = {a.P, a.pitch_p, p.rows_p, a.pitch_p};
@@ -736,11 +773,13 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
       g.splits = p.splits_h;
       const int b = p.big_h ? 256 : 128;
       g.tiles_m = (uint32_t)cdiv(rows, b), g.tiles_n = (uint32_t)cdiv(d, b);
-      g.u0 = scal + kInvP, g.u1 = scal + kInvE;
+      g.u0 = scal + kInvP, g.u1 = a.scaled ? scal + kInvE : nullptr;
       g.part = p.splits_h > 1 || p.pieces > 1 ? (float*)(ws + p.ph) : nullptr;
       g.add = i > 0;
-      g.out = d_hidden;
-      MPL_TILE_DISPATCH(xent_grad_kernel, false, true, p.big_h, dim3(g.tiles_m * g.tiles_n, g.splits), s, g);
+      g.out = d_hidden, g.dtype = dtype;
+      const dim3 grid(g.tiles_m * g.tiles_n, g.splits);
+      if (p.split) MPL_TILE(xent_grad_kernel, 2, false, false, true, p.big_h, grid, s, g);
+      else MPL_TILE(xent_grad_kernel, 1, false, false, true, p.big_h, grid, s, g);
     }
     if (d_embedding) {
       GradArgs g{};
@@ -751,20 +790,23 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
       g.splits = p.splits_e;
       const int b = p.big_e ? 256 : 128;
       g.tiles_m = (uint32_t)cdiv(nv, b), g.tiles_n = (uint32_t)cdiv(d, b);
-      g.u0 = scal + kInvP, g.u1 = scal + kInvH;
+      g.u0 = scal + kInvP, g.u1 = a.scaled ? scal + kInvH : nullptr;
       g.part = p.splits_e > 1 ? (float*)(ws + p.pe) : nullptr;
       g.out = (char*)d_embedding + a.v0 * d * (dtype == MPL_F32 ? 4 : 2);
-      MPL_TILE_DISPATCH(xent_grad_kernel, true, true, p.big_e, dim3(g.tiles_m * g.tiles_n, g.splits), s, g);
+      g.dtype = dtype;
+      const dim3 grid(g.tiles_m * g.tiles_n, g.splits);
+      if (p.split) MPL_TILE(xent_grad_kernel, 2, false, true, true, p.big_e, grid, s, g);
+      else MPL_TILE(xent_grad_kernel, 1, false, true, true, p.big_e, grid, s, g);
       if (g.part) {
         const int64_t n = nv * d;
-        xent_sum_kernel<<<(unsigned)(cdiv(n, 256) < 4096 ? cdiv(n, 256) : 4096), 256, 0, s>>>(g.part, g.splits, n,
+        xent_sum_kernel<<<(unsigned)std::min<int64_t>(cdiv(n, 1024), 4096), 256, 0, s>>>(g.part, g.splits, n,
                                                                                            g.out, dtype);
       }
     }
   }
   if (d_hidden && (p.splits_h > 1 || p.pieces > 1)) {
     const int64_t n = rows * d;
-    xent_sum_kernel<<<(unsigned)(cdiv(n, 256) < 4096 ? cdiv(n, 256) : 4096), 256, 0, s>>>(
+    xent_sum_kernel<<<(unsigned)std::min<int64_t>(cdiv(n, 1024), 4096), 256, 0, s>>>(
         (const float*)(ws + p.ph), p.splits_h, n, d_hidden, dtype);
   }
   return check_launch(what);

@@ -64,11 +64,12 @@ struct TileMma {
   static constexpr int instrs() { return B * 128 / 1024 / NW; }
   static_assert(BM * 128 % (1024 * NW) == 0 && BN * 128 % (1024 * NW) == 0, "a stage splits evenly over the waves");
 
-  // Sends the loads of stage `it` (from contraction row it * KI) of one operand:
-  // a scalar address of the stage and 32-bit places of the lanes in it.
+  // Sends load i of the wave's instrs<B>() of stage `it` (from contraction row
+  // it * KI) of one operand: a scalar address of the stage and 32-bit places of
+  // the lanes in it.
   template <bool ST, int B>
   __device__ static __forceinline__ void issue(const TileOperand& o, int64_t origin, int it, char* lds, int wave,
-                                               int lane) {
+                                               int lane, int i) {
     const char* base;
     int last;
     // a tile or a stage that lies behind the array reads its last row
@@ -82,22 +83,19 @@ struct TileMma {
       last = (int)min(o.rows - 1 - first, (int64_t)(KI - 1));
     }
     const uint32_t pitch = (uint32_t)o.pitch;
-#pragma unroll
-    for (int i = 0; i < instrs<B>(); ++i) {
-      const int n = wave * instrs<B>() + i;
-      uint32_t at;
-      if constexpr (!ST) {
-        const int row = min(n * 8 + (lane >> 3), last);
-        at = row * pitch + (((lane & 7) ^ (lane >> 3)) << 4);
-      } else {
-        constexpr int L = B * 2 * S;  // bytes of a contraction row in the stage
-        static_assert(L <= 1024 && L >= 128, "");
-        const int k = (n * 1024 + lane * 16) / L;
-        const int piece = ((lane * 16 % L) >> 4) ^ ((4 * (k & 3)) & (L / 16 - 1));
-        at = min(k, last) * pitch + (uint32_t)min(piece * 16, (int)(o.width - 16 - origin * (2 * S)));
-      }
-      __builtin_amdgcn_global_load_lds((const void*)(base + at), (lds_void*)(lds + n * 1024), 16, 0, 0);
+    const int n = wave * instrs<B>() + i;
+    uint32_t at;
+    if constexpr (!ST) {
+      const int row = min(n * 8 + (lane >> 3), last);
+      at = row * pitch + (((lane & 7) ^ (lane >> 3)) << 4);
+    } else {
+      constexpr int L = B * 2 * S;  // bytes of a contraction row in the stage
+      static_assert(L <= 1024 && L >= 128, "");
+      const int k = (n * 1024 + lane * 16) / L;
+      const int piece = ((lane * 16 % L) >> 4) ^ ((4 * (k & 3)) & (L / 16 - 1));
+      at = min(k, last) * pitch + (uint32_t)min(piece * 16, (int)(o.width - 16 - origin * (2 * S)));
     }
+    __builtin_amdgcn_global_load_lds((const void*)(base + at), (lds_void*)(lds + n * 1024), 16, 0, 0);
   }
 
   // A lane's places in a stage of one operand: what differs between its
@@ -144,70 +142,101 @@ struct TileMma {
                                                     0, 0);
   }
 
-  template <int N>
-  __device__ static __forceinline__ void products(const short8v (&a)[TM], const short8v (&b)[N][TN],
-                                                  f32x16 (&acc)[TM][TN]) {
+  // The fragments of a step in registers: A's (fp32: hi, then lo), B's of this
+  // step and the next.
+  struct Frags {
+    short8v a[2][TM], b[2][S][TN];
+  };
+
+  // Products of all of a with N planes of b.  `slot(n)` comes after product n;
+  // the scheduler keeps what it sends there.
+  template <int N, class F>
+  __device__ static __forceinline__ void products(const short8v (&a)[TM], const short8v (&b)[S][TN],
+                                                  f32x16 (&acc)[TM][TN], F&& slot) {
 #pragma unroll
     for (int p = 0; p < N; ++p)
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mma(a[i], b[p][j], acc[i][j]);
+        for (int j = 0; j < TN; ++j) {
+          acc[i][j] = mma(a[i], b[p][j], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+          slot((p * TM + i) * TN + j);
+          __builtin_amdgcn_sched_barrier(0);
+        }
   }
 
-  // A stage's products.  The reads of the next fragments are sent before the
-  // products of these, and the scheduler is kept from sending more (it would
-  // spill).  fp32: a step is hi hi + hi lo, then lo hi.
-  __device__ static __forceinline__ void compute(const char* la, const char* lb, const PlacesA& pa, const PlacesB& pb,
-                                                 f32x16 (&acc)[TM][TN]) {
-    short8v b[2][S][TN];
-    auto read_b = [&](int s) __attribute__((always_inline)) {
-#pragma unroll
-      for (int p = 0; p < S; ++p)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) b[s & 1][p][j] = pb.read(lb, j, p, s);
+  // Loads of a stage that one wave sends, and how many of them in the last
+  // group of products of the stage before the one in flight.
+  static constexpr int kLoads = instrs<BM>() + instrs<BN>(), kEarly = kLoads / 2;
+  // A load after every kEvery products.
+  static constexpr int kEvery = TM * TN >= kLoads ? TM * TN / kEarly : 1;
+  static_assert(kEarly * kEvery <= TM * TN, "the loads must fit between the products");
+
+  // A stage's products, from the stage la, lb, whose first fragments are in
+  // registers.  Between any two products at most one fragment of the next step
+  // is read and every few products one load is sent: a wave issues in order, so
+  // a burst of either would hold its products up until the queues drain.  The
+  // barrier comes before the last group: by then the wave has read all of the
+  // stage, so behind it the loads of the stage after next go over it (`fresh`,
+  // the first kEarly; the next stage's first products send the rest, `old`), and
+  // the first fragments of the next stage, na and nb, are read.
+  template <class OLD, class NEW>
+  __device__ static __forceinline__ void stage(const char* la, const char* lb, const char* na, const char* nb,
+                                               const PlacesA& pa, const PlacesB& pb, Frags& f, f32x16 (&acc)[TM][TN],
+                                               OLD&& old, NEW&& fresh) {
+    int sent = kEarly;
+    auto turn = [&]() __attribute__((always_inline)) {
+      wait_vmcnt_le<0>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
     };
-    auto read_a = [&](short8v(&a)[TM], int p, int s) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i) a[i] = pa.read(la, i, p, s);
+    auto load = [&](int n, bool last) __attribute__((always_inline)) {
+      if (n % kEvery != kEvery - 1) return;
+      if (last) {
+        if (n / kEvery < kEarly) fresh(n / kEvery);
+      } else if (sent < kLoads) {
+        old(sent++);
+      }
     };
-    short8v a[2][TM];
-    read_b(0);
-    read_a(a[0], 0, 0);
+    // reads fragments [from, to) of step s + 1: B's planes, then A's first plane
+    auto read_next = [&](int s, int from, int to) __attribute__((always_inline)) {
+      const bool last = s + 1 == kSteps;
+#pragma unroll
+      for (int q = from; q < to; ++q) {
+        if (q < S * TN) f.b[(s + 1) & 1][q / TN % S][q % TN] = pb.read(last ? nb : lb, q % TN, q / TN % S, (s + 1) % kSteps);
+        else if (q < S * TN + TM)
+          f.a[S == 1 ? (s + 1) & 1 : 0][(q - S * TN) % TM] = pa.read(last ? na : la, (q - S * TN) % TM, 0, (s + 1) % kSteps);
+      }
+    };
+    constexpr int kRead = (S * TN + TM + TM * TN - 1) / (TM * TN);  // fragments after a product
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
+      const bool last = s + 1 == kSteps;
       if constexpr (S == 1) {
-        if (s + 1 < kSteps) {
-          read_b(s + 1);
-          read_a(a[(s + 1) & 1], 0, s + 1);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        products(a[s & 1], b[s & 1], acc);
-        __builtin_amdgcn_sched_barrier(0);
+        if (last) turn();
+        products<1>(f.a[s & 1], f.b[s & 1], acc, [&](int n) __attribute__((always_inline)) {
+          read_next(s, n * kRead, (n + 1) * kRead);
+          load(n, last);
+        });
       } else {
-        read_a(a[1], 1, s);
-        __builtin_amdgcn_sched_barrier(0);
-        products(a[0], b[s & 1], acc);
-        __builtin_amdgcn_sched_barrier(0);
-        if (s + 1 < kSteps) {
-          read_b(s + 1);
-          read_a(a[0], 0, s + 1);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        short8v hi[1][TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) hi[0][j] = b[s & 1][0][j];
-        products(a[1], hi, acc);
-        __builtin_amdgcn_sched_barrier(0);
+        products<2>(f.a[0], f.b[s & 1], acc, [&](int n) __attribute__((always_inline)) {
+          if (n < TM) f.a[1][n % TM] = pa.read(la, n % TM, 1, s);
+          load(n, false);
+        });
+        if (last) turn();
+        products<1>(f.a[1], f.b[s & 1], acc, [&](int n) __attribute__((always_inline)) {
+          read_next(s, n * kRead, (n + 1) * kRead);
+          load(n, last);
+        });
       }
     }
   }
 
   // The tile whose first row of A is m0 and of B n0, over the stages [it0, it1),
-  // it0 < it1.
-  // Between the barrier of a stage and the next one's, its operands are read
-  // and the next stage's loads fly; a wave passes a barrier only with its loads
-  // landed and its reads done.
+  // it0 < it1.  One exit of the loop, so that the accumulators are not copied at
+  // its edges; past the last stage it is sent again rather than under a branch.
   __device__ static __forceinline__ void run(const TileOperand& A, const TileOperand& B, int64_t m0, int64_t n0, int it0,
                                              int it1, char* a0, char* b0, char* a1, char* b1, f32x16 (&acc)[TM][TN]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -217,30 +246,37 @@ struct TileMma {
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
-    auto sync = [&]() __attribute__((always_inline)) {
-      wait_vmcnt_le<0>();
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
+    auto send = [&](int it, char* a, char* b, int n) __attribute__((always_inline)) {
+      it = min(it, it1 - 1);
+      if (n < instrs<BM>()) issue<AST, BM>(A, m0, it, a, wave, lane, n);
+      else issue<BST, BN>(B, n0, it, b, wave, lane, n - instrs<BM>());
     };
-    issue<AST, BM>(A, m0, it0, a0, wave, lane);
-    issue<BST, BN>(B, n0, it0, b0, wave, lane);
-    // One exit, so that the accumulators are not copied at its edges; the last
-    // stages are sent twice rather than under a branch.
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) send(it0, a0, b0, n);
+#pragma unroll
+    for (int n = 0; n < kEarly; ++n) send(it0 + 1, a1, b1, n);
+    wait_vmcnt_le<kEarly>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    Frags f;
+#pragma unroll
+    for (int p = 0; p < S; ++p)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) f.b[0][p][j] = pb.read(b0, j, p, 0);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) f.a[0][i] = pa.read(a0, i, 0, 0);
     int it = it0;
     for (; it + 1 < it1; it += 2) {
-      sync();
-      issue<AST, BM>(A, m0, it + 1, a1, wave, lane);
-      issue<BST, BN>(B, n0, it + 1, b1, wave, lane);
-      compute(a0, b0, pa, pb, acc);
-      sync();
-      const int next = min(it + 2, it1 - 1);
-      issue<AST, BM>(A, m0, next, a0, wave, lane);
-      issue<BST, BN>(B, n0, next, b0, wave, lane);
-      compute(a1, b1, pa, pb, acc);
+      stage(a0, b0, a1, b1, pa, pb, f, acc, [&](int n) __attribute__((always_inline)) { send(it + 1, a1, b1, n); },
+            [&](int n) __attribute__((always_inline)) { send(it + 2, a0, b0, n); });
+      stage(a1, b1, a0, b0, pa, pb, f, acc, [&](int n) __attribute__((always_inline)) { send(it + 2, a0, b0, n); },
+            [&](int n) __attribute__((always_inline)) { send(it + 3, a1, b1, n); });
     }
-    sync();
-    if (it < it1) compute(a0, b0, pa, pb, acc);
+    if (it < it1) stage(a0, b0, a1, b1, pa, pb, f, acc, [](int) {}, [](int) {});
+    wait_vmcnt_le<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   }
 };
 

@@ -20,17 +20,15 @@ _DTYPES = {torch.float32: _lib.MPL_F32, torch.float16: _lib.MPL_F16, torch.bfloa
 MAX_WIDTH = 16384
 
 
-def _rows(t: torch.Tensor, d: int) -> torch.Tensor:
-    """``t`` as [rows, d], elements of a row next to each other, rows apart by
-    any pitch of at least d; copied only where it does not lie so."""
+def _rows(t: torch.Tensor, d: int) -> Tuple[torch.Tensor, int]:
+    """``t`` as rows of d elements next to each other, and the elements from
+    row to row (at least d); copied only where it does not lie so."""
+    if t.is_contiguous():
+        return t, d
     t = t.reshape(-1, d)
     if d > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < d:
-        return t.contiguous()
-    return t
-
-
-def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+        return t.contiguous(), d
+    return t, t.stride(0) if t.shape[0] > 1 else d
 
 
 def _check(what: str, x: torch.Tensor, params, others) -> None:
@@ -56,50 +54,51 @@ def _check(what: str, x: torch.Tensor, params, others) -> None:
 
 
 def _forward(x, scale, bias, eps, residual, stats: bool):
-    """(y, sum or None, mean, rstd [rows]) of x [..., d] and its parameters, checked."""
-    d, shape = x.shape[-1], x.shape
-    x2 = _rows(x, d)
-    rows = x2.shape[0]
-    y = torch.empty((rows, d), dtype=x.dtype, device=x.device)
-    total = None if residual is None else torch.empty((rows, d), dtype=x.dtype, device=x.device)
-    st = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else None
-    mean, rstd = (st[0], st[1]) if stats else (None, None)
+    """(y, sum or None, statistics [2, rows] or None) of x [..., d] and its parameters, checked."""
+    d, dev = x.shape[-1], x.device
+    rows = x.numel() // d
+    x2, x_pitch = _rows(x, d)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    r2, r_pitch, total = None, 0, None
+    if residual is not None:
+        r2, r_pitch = _rows(residual, d)
+        total = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    st = torch.empty((2, rows), dtype=torch.float32, device=dev) if stats else None
     if rows:
-        r2 = None if residual is None else _rows(residual, d)
         scale, bias = scale.contiguous(), bias.contiguous()
         P = _lib.ptr
-        with _lib.on_device(x.device):
+        mean = P(st)
+        with _lib.on_device(dev):
             _lib.check(_lib.lib().mpl_layer_norm(
-                x2.data_ptr(), _pitch(x2), P(r2), 0 if r2 is None else _pitch(r2), _DTYPES[x.dtype], scale.data_ptr(),
-                bias.data_ptr(), _DTYPES[scale.dtype], rows, d, float(eps), y.data_ptr(), P(total), P(mean), P(rstd),
-                _lib.stream_ptr(x.device)), "mpl_layer_norm")
-    return y.view(shape), None if total is None else total.view(shape), mean, rstd
+                x2.data_ptr(), x_pitch, P(r2), r_pitch, _DTYPES[x.dtype], scale.data_ptr(), bias.data_ptr(),
+                _DTYPES[scale.dtype], rows, d, eps, y.data_ptr(), P(total), mean, mean and mean + 4 * rows,
+                _lib.stream_ptr(dev)), "mpl_layer_norm")
+    return y, total, st
 
 
-def _backward(g_y, s, scale, mean, rstd, g_residual, want_x: bool, want_params: bool):
-    """(dx, d_scale, d_bias), None where not wanted."""
-    d = s.shape[-1]
-    s2, g2 = _rows(s, d), _rows(g_y, d)
-    rows = s2.shape[0]
-    dx = torch.empty((rows, d), dtype=s.dtype, device=s.device) if want_x else None
-    dp = torch.empty((2, d), dtype=scale.dtype, device=s.device) if want_params else None
-    if rows == 0:
-        if want_params:
-            dp.zero_()
-    elif want_x or want_params:
-        r2 = None if g_residual is None else _rows(g_residual, d)
+def _backward(g_y, s, scale, mean: int, rstd: int, g_residual, want_x: bool, want_params: bool):
+    """(dx, d_scale, d_bias), None where not wanted; mean and rstd are the addresses of fp32 [rows]."""
+    d, dev = s.shape[-1], s.device
+    rows = s.numel() // d
+    dx = torch.empty(s.shape, dtype=s.dtype, device=dev) if want_x else None
+    ds = db = ws = None
+    if want_params:
+        new = torch.empty if rows else torch.zeros
+        ds, db = new(d, dtype=scale.dtype, device=dev), new(d, dtype=scale.dtype, device=dev)
+    if rows and (want_x or want_params):
+        (s2, s_pitch), (g2, g_pitch) = _rows(s, d), _rows(g_y, d)
+        r2, r_pitch = (None, 0) if g_residual is None else _rows(g_residual, d)
         scale = scale.contiguous()
-        L, P, code = _lib.lib(), _lib.ptr, _DTYPES[s.dtype]
-        with _lib.on_device(s.device):
-            ws = None
+        L, P, code, n = _lib.lib(), _lib.ptr, _DTYPES[s.dtype], 0
+        with _lib.on_device(dev):
             if want_params:
-                ws = torch.empty(L.mpl_layer_norm_bwd_workspace_bytes(rows, d, code), dtype=torch.uint8, device=s.device)
+                n = L.mpl_layer_norm_bwd_workspace_bytes(rows, d, code)
+                ws = torch.empty(n, dtype=torch.uint8, device=dev)
             _lib.check(L.mpl_layer_norm_bwd(
-                g2.data_ptr(), _pitch(g2), s2.data_ptr(), _pitch(s2), P(r2), 0 if r2 is None else _pitch(r2), code,
-                scale.data_ptr(), _DTYPES[scale.dtype], mean.data_ptr(), rstd.data_ptr(), rows, d, P(dx),
-                dp[0].data_ptr() if want_params else None, dp[1].data_ptr() if want_params else None, P(ws),
-                ws.numel() if want_params else 0, _lib.stream_ptr(s.device)), "mpl_layer_norm_bwd")
-    return (None if dx is None else dx.view(s.shape)), *((dp[0], dp[1]) if want_params else (None, None))
+                g2.data_ptr(), g_pitch, s2.data_ptr(), s_pitch, P(r2), r_pitch, code, scale.data_ptr(),
+                _DTYPES[scale.dtype], mean, rstd, rows, d, P(dx), P(ds), P(db), P(ws), n, _lib.stream_ptr(dev)),
+                "mpl_layer_norm_bwd")
+    return dx, ds, db
 
 
 def _capturing() -> bool:
@@ -113,9 +112,9 @@ _NO_CAPTURE = ("torch autograd through layer_norm is not supported under HIP gra
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, bias, eps, residual):
-        y, total, mean, rstd = _forward(x, scale, bias, eps, residual, True)
+        y, total, stats = _forward(x, scale, bias, eps, residual, True)
         # the sum is an output: saved as one, it keeps no cycle
-        ctx.save_for_backward(x if residual is None else total, scale, mean, rstd)
+        ctx.save_for_backward(x if residual is None else total, scale, stats)
         ctx.set_materialize_grads(False)
         return y if residual is None else (y, total)
 
@@ -124,11 +123,12 @@ class _LayerNormFunction(torch.autograd.Function):
     def backward(ctx, g_y, g_sum=None):
         if _capturing():
             raise RuntimeError(_NO_CAPTURE)
-        s, scale, mean, rstd = ctx.saved_tensors
+        s, scale, stats = ctx.saved_tensors
         nx, ns, nb, _, nr = ctx.needs_input_grad
         if g_y is None:  # only the sum was used
             return (g_sum if nx else None), None, None, None, (g_sum if nr else None)
-        dx, ds, db = _backward(g_y, s, scale, mean, rstd, g_sum, nx or nr, ns or nb)
+        mean = stats.data_ptr()
+        dx, ds, db = _backward(g_y, s, scale, mean, mean + 2 * stats.numel(), g_sum, nx or nr, ns or nb)
         return (dx if nx else None), (ds if ns else None), (db if nb else None), None, (dx if nr else None)
 
 
@@ -152,7 +152,7 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, eps: fl
         if _capturing():
             raise RuntimeError(_NO_CAPTURE)
         return _LayerNormFunction.apply(x, scale, bias, float(eps), residual)
-    y, total, _, _ = _forward(x, scale, bias, eps, residual, False)
+    y, total, _ = _forward(x, scale, bias, float(eps), residual, False)
     return y if residual is None else (y, total)
 
 
@@ -164,8 +164,8 @@ def layer_norm_forward(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor,
     others = () if residual is None else (("residual", residual),)
     _check("layer_norm_forward", x, (("scale", scale), ("bias", bias)), others)
     with torch.no_grad():
-        y, total, mean, rstd = _forward(x, scale, bias, eps, residual, True)
-    return y, (x if residual is None else total), mean, rstd
+        y, total, stats = _forward(x, scale, bias, float(eps), residual, True)
+    return y, (x if residual is None else total), *stats.unbind(0)
 
 
 def layer_norm_backward(g_y: torch.Tensor, s: torch.Tensor, scale: torch.Tensor, mean: torch.Tensor,
@@ -182,4 +182,4 @@ def layer_norm_backward(g_y: torch.Tensor, s: torch.Tensor, scale: torch.Tensor,
             raise ValueError(f"layer_norm_backward: {name} {tuple(t.shape)} {t.dtype} must be contiguous fp32 of {rows} "
                              f"rows on {s.device}")
     with torch.no_grad():
-        return _backward(g_y, s, scale, mean, rstd, g_residual, True, True)
+        return _backward(g_y, s, scale, mean.data_ptr(), rstd.data_ptr(), g_residual, True, True)

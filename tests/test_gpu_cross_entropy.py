@@ -4,17 +4,20 @@ Tolerances, elementwise, from the arithmetic (u = half a step of the type,
 torch.finfo(t).eps / 2):
 
   z       sums of d products in fp32: d 2^-24 of sum |h e|; fp32 operands are
-          held to 2^-23 each and lo lo (2^-22) is left out: 2^-21 more
+          held to 2^-23 each and lo lo (2^-22) is left out: 2^-21 more; where
+          operands are held in fp16 (fp32 calls, bf16's gradients), 2^-39 of
+          their array's largest, the end of fp16's range under its power of two
   lse     the largest z error, and 2^-20 (1 + |lse|): exp, log and the sums of the
           exps, relative to a sum whose error the log turns into an absolute one
-  dz      |z error| + |lse error| + 2^-20 relative (exp of both), one rounding u
-          (fp32: 2^-22), and where the type is fp16 or fp32 half of fp16's
-          smallest step under dz's scale, 2^-25 2^-13 of the largest
-          coefficient; below 2^-126, fp32's and bf16's smallest normal number,
-          exp gives 0, so 2^-126 of the largest coefficient (or of 1)
+  dz      |z error| + |lse error| + 2^-20 relative (exp of both), one rounding to
+          fp16, 2^-11 (fp32 calls: hi and lo, 2^-22), and half of fp16's smallest
+          step under dz's power of two, 2^-25 2^-13 of the largest coefficient;
+          below 2^-126, fp32's smallest normal number, exp gives 0, so 2^-126 of
+          the largest coefficient (or of 1)
   d h, d e   sum |dz error| |operand|, K 2^-24 of sum |dz| |operand| for sums of K
-          products (and 2^-21 for fp32 operands), one rounding u of the result;
-          products and sums below 2^-126 are 0 too: (K + 1) 2^-126
+          products (and 2^-21 for fp32 operands, 2^-39 of the array's largest as
+          above), one rounding u of the result; products and sums below 2^-126
+          are 0 too: (K + 1) 2^-126
 """
 
 import math
@@ -47,6 +50,8 @@ def _formula(h, e, t, gl, gs):
     H, E = h.double(), e.double()
     z = H @ E.t()
     z_tol = (d * 2.0 ** -24 + (2.0 ** -21 if fp32 else 0)) * (H.abs() @ E.abs().t())
+    end = 0 if dtype == torch.float16 else 2.0 ** -39
+    z_tol = z_tol + end * (E.abs().max() * H.abs().sum(1)[:, None] + H.abs().max() * E.abs().sum(1)[None])
     lse = torch.logsumexp(z, 1)
     lse_tol = z_tol.amax(1) + 2.0 ** -20 * (1 + lse.abs())
     keep = t != IGNORE
@@ -57,14 +62,15 @@ def _formula(h, e, t, gl, gs):
     p = torch.exp(z - lse[:, None]) * a[:, None]
     dz = p.clone().scatter_add_(1, at, -g[:, None])
     most = max(a.abs().max().item(), g.abs().max().item())
-    dz_tol = (p.abs() * (z_tol + lse_tol[:, None] + 2.0 ** -20) + dz.abs() * (2.0 ** -22 if fp32 else u)
-              + (0 if dtype == torch.bfloat16 else 2.0 ** -38 * most) + 2.0 ** -126 * max(1.0, most))
+    dz_tol = (p.abs() * (z_tol + lse_tol[:, None] + 2.0 ** -20) + dz.abs() * 2.0 ** (-22 if fp32 else -11)
+              + 2.0 ** -38 * most + 2.0 ** -126 * max(1.0, most))
 
     def product(x, x_tol, y, K):
         out = x @ y
         acc = K * 2.0 ** -24 + (2.0 ** -21 if fp32 else 0)
         floor = 2.0 ** -126 * (K + 1) + (2.0 ** -25 if dtype == torch.float16 else 0)
-        return out, (x_tol + acc * x.abs()) @ y.abs() + u * out.abs() + floor
+        tol = (x_tol + acc * x.abs()) @ y.abs() + end * y.abs().max() * x.abs().sum(1)[:, None]
+        return out, tol + u * out.abs() + floor
 
     dh, dh_tol = product(dz, dz_tol, E, V)
     de, de_tol = product(dz.t().contiguous(), dz_tol.t().contiguous(), H, R)
