@@ -61,7 +61,8 @@ struct PackArgs {
   PackOne e, h;  // embedding, hidden
   int d, dpad;
   float* scal;
-  uint32_t* part;  // [kAmaxBlocks] maxima of each array
+  uint32_t* part;  // [kAmaxBlocks] maxima of each array, and of the coefficients
+  bool coefs;
 };
 constexpr int kAmaxBlocks = 512;
 
@@ -103,11 +104,73 @@ struct Source {
   }
 };
 
-// Largest finite magnitudes of both arrays, one partial maximum a workgroup.
+// Coefficients of the rows [first, last) of dz (threads stride through them),
+// zero for those that only fill it up; their largest finite magnitude.
+struct CoefArgs {
+  const int64_t* target;
+  int64_t R, rows_p, V, ignore;
+  const float* g_loss;
+  const float* g_lse;
+  const float* lse;
+  float* coef;  // [3][rows_p]: g + gl, g, lse log2(e)
+};
+__device__ __forceinline__ uint32_t coefficients(const CoefArgs& p, int64_t first, int64_t step) {
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int64_t i = first; i < p.rows_p; i += step) {
+    float all = 0.f, g = 0.f, l = 0.f;
+    const int64_t k = min(i, p.R - 1);  // loads without branches, so that they fly together
+    const int64_t at = p.target[k];
+    const float gk = p.g_loss ? p.g_loss[k] : 0.f, sk = p.g_lse ? p.g_lse[k] : 0.f, lk = p.lse[k];
+    if (i < p.R) {
+      g = at == p.ignore ? 0.f : at < 0 || at >= p.V ? NAN : gk;
+      all = g + sk;
+      l = lk * kLog2e;
+    }
+    p.coef[i] = all;
+    p.coef[p.rows_p + i] = g;
+    p.coef[2 * p.rows_p + i] = l;
+    m = max(m, max(finite_bits(all), finite_bits(g)));
+  }
+  return m;
+}
+
+// The largest of a workgroup's THREADS values, in its first thread.
+template <int THREADS>
+__device__ __forceinline__ uint32_t block_max(uint32_t m) {
+  __shared__ uint32_t s[THREADS / 64];
+  for (int h = 32; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) m = max(m, s[i]);
+  return m;
+}
+
+// dz's power of two: |dz| <= |g + gl| + |g|, below 2^15 after it.
+__device__ __forceinline__ void write_scale_p(float* scal, uint32_t most) {
+  const float scale = scale_for(most, 13);
+  scal[kScaleP] = scale;
+  scal[kInvP] = 1.f / scale;
+}
+
+// The coefficients where the operands are read as they lie.  One workgroup.
+__global__ __launch_bounds__(1024) void xent_coef_kernel(CoefArgs p, float* __restrict__ scal) {
+  const uint32_t m = block_max<1024>(coefficients(p, threadIdx.x, 1024));
+  if (threadIdx.x == 0) write_scale_p(scal, m);
+}
+
+// Largest finite magnitudes of both arrays, one partial maximum a workgroup; in
+// the backward a third row of workgroups forms the coefficients.
 template <int MODE>
-__global__ __launch_bounds__(256) void amax_kernel(PackArgs p) {
+__global__ __launch_bounds__(256) void amax_kernel(PackArgs p, CoefArgs q) {
   constexpr int VE = Source<MODE>::VE;
   const int a = blockIdx.y;
+  if (a == 2) {
+    const uint32_t m = block_max<256>(coefficients(q, blockIdx.x * 256 + threadIdx.x, 256 * (int64_t)gridDim.x));
+    if (threadIdx.x == 0) p.part[2 * kAmaxBlocks + blockIdx.x] = m;
+    return;
+  }
   const PackOne o = a ? p.h : p.e;
   const int vecs = (p.d + VE - 1) / VE;
   const int64_t n = o.rows * vecs, step = 256 * (int64_t)gridDim.x;
@@ -131,11 +194,8 @@ __global__ __launch_bounds__(256) void amax_kernel(PackArgs p) {
       take(r, VE * (i - r * vecs), p.d);
     }
   }
-  __shared__ uint32_t s[4];
-  for (int h = 32; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) p.part[a * kAmaxBlocks + blockIdx.x] = max(max(s[0], s[1]), max(s[2], s[3]));
+  m = block_max<256>(m);
+  if (threadIdx.x == 0) p.part[a * kAmaxBlocks + blockIdx.x] = m;
 }
 
 // Rows of an array as a tile product's operand, zero-filled to whole stages.  A
@@ -146,14 +206,18 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   const PackOne o = a ? p.h : p.e;
   float scale = 1.f;
   if constexpr (MODE != kCopy16) {
-    __shared__ uint32_t s[4];
-    uint32_t m = max(p.part[a * kAmaxBlocks + threadIdx.x], p.part[a * kAmaxBlocks + 256 + threadIdx.x]);
-    for (int h = 32; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
-    __syncthreads();
-    scale = scale_for(max(max(s[0], s[1]), max(s[2], s[3])), 14);
+    auto most = [&](int k) __attribute__((always_inline)) {
+      const uint32_t* q = p.part + k * kAmaxBlocks + threadIdx.x;
+      return block_max<256>(max(q[0], q[256]));
+    };
+    scale = scale_for(most(a), 14);
     if (threadIdx.x == 0 && (blockIdx.x == 0 || blockIdx.x == p.e.blocks))
       p.scal[a == 0 ? kInvE : kInvH] = 1.f / scale;
+    if (p.coefs && blockIdx.x == 0) {
+      __syncthreads();  // block_max's words are used again
+      const uint32_t m = most(2);
+      if (threadIdx.x == 0) write_scale_p(p.scal, m);
+    }
   }
   const int per = p.dpad / 8;
   const int64_t i = (int64_t)(blockIdx.x - (a ? p.e.blocks : 0)) * 256 + threadIdx.x;
@@ -286,76 +350,149 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
   }
 }
 
-// Joins a token's pairs: a workgroup takes 32 tokens, 8 threads a token, each
-// every eighth pair in order, then the eight in order.
+// Joins a token's pairs: a workgroup takes TOK tokens, 256 / TOK threads a
+// token, each every so-manieth pair in order, then the threads in order.
+template <int TOK>
 __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict__ part, int tiles, int64_t R, int64_t V,
                                                         const int64_t* __restrict__ target, int64_t ignore,
                                                         const float* __restrict__ z_target, float* __restrict__ loss,
                                                         float* __restrict__ lse) {
-  __shared__ float2 s[8][32];
-  const int t = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t tok = (int64_t)blockIdx.x * 32 + t;
+  constexpr int N = 256 / TOK;
+  __shared__ float2 s[N][TOK];
+  const int t = threadIdx.x % TOK, g = threadIdx.x / TOK;
+  const int64_t tok = (int64_t)blockIdx.x * TOK + t, at = min(tok, R - 1);
   float m = -INFINITY, l = 0.f;
-  if (tok < R)
-    for (int i = g; i < tiles; i += 8) {
-      const float2 v = part[(int64_t)i * R + tok];
-      const float n = fmaxf(m, v.x), ref = n == -INFINITY ? 0.f : n;
-      l = l * __builtin_amdgcn_exp2f(m - ref) + v.y * __builtin_amdgcn_exp2f(v.x - ref);
-      m = n;
-    }
-  s[g][t] = make_float2(m, l);
-  __syncthreads();
-  if (g || tok >= R) return;
-  for (int i = 1; i < 8; ++i) {
-    const float2 v = s[i][t];
+  auto add = [&](float2 v) __attribute__((always_inline)) {
     const float n = fmaxf(m, v.x), ref = n == -INFINITY ? 0.f : n;
     l = l * __builtin_amdgcn_exp2f(m - ref) + v.y * __builtin_amdgcn_exp2f(v.x - ref);
     m = n;
+  };
+  int i = g;
+  for (; i + 7 * N < tiles; i += 8 * N) {
+    float2 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = part[(int64_t)(i + k * N) * R + at];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) add(v[k]);
   }
+  for (; i < tiles; i += N) add(part[(int64_t)i * R + at]);
+  s[g][t] = make_float2(m, l);
+  __syncthreads();
+  if (g || tok >= R) return;
+  for (int k = 1; k < N; ++k) add(s[k][t]);
   const float out = (m + log2f(l)) * kLn2;
-  const int64_t at = target[tok];
+  const int64_t to = target[tok];
   lse[tok] = out;
-  loss[tok] = at == ignore ? 0.f : (at < 0 || at >= V) ? NAN : out - z_target[tok];
+  loss[tok] = to == ignore ? 0.f : (to < 0 || to >= V) ? NAN : out - z_target[tok];
+}
+
+// Few tokens: the table is read once, straight into the operands (no copy of
+// it, no LDS), as rows of 16 bytes a lane.  A workgroup takes 32 words at a
+// time; its 4 waves split d, so that a wave's loads are all in flight, and
+// their sums of z meet in LDS, from where each wave keeps the running maximum
+// and sum of 8 of the words.  fp32 rows go to v_mfma_f32_32x32x2_f32 as they
+// are: 4 products a vector, for which lanes of half h take dims 4h .. 4h + 3 of
+// each 8.  Bound: the table's bytes, and the fp32 products from some 100 tokens
+// on.
+struct RowsArgs {
+  const void* E;
+  const void* H;
+  int64_t e_pitch, h_pitch, R, V;
+  int d;
+  const int64_t* target;
+  float2* part;  // [workgroups][R]
+  float* z_target;
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 row_vector(const T* row, int at, int d) {
+  constexpr int VE = 16 / sizeof(T);
+  typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
+  if (at + VE <= d) return __builtin_bit_cast(uint4, (any4)(*(const any4*)(row + at)));
+  T v[VE] __attribute__((aligned(16)));
+#pragma unroll
+  for (int e = 0; e < VE; ++e) v[e] = at + e < d ? row[at + e] : (T)0.f;
+  return *(const uint4*)v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs p) {
+  constexpr int VE = 16 / sizeof(T);
+  __shared__ float s[2][4][16][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int64_t tok = blockIdx.y * 32 + col;
+  const T* h = (const T*)p.H + min(tok, p.R - 1) * p.h_pitch;
+  const int64_t to = p.target[min(tok, p.R - 1)];
+  const int chunks = (p.d + 2 * VE - 1) / (2 * VE);
+  const int c0 = chunks * wave / 4, c1 = chunks * (wave + 1) / 4;
+  const int64_t groups = (p.V + 31) / 32;
+  float m = -INFINITY, l = 0.f;
+  int turn = 0;
+  for (int64_t g = blockIdx.x; g < groups; g += gridDim.x, turn ^= 1) {
+    const T* e = (const T*)p.E + min(32 * g + col, p.V - 1) * p.e_pitch;
+    f32x16 acc = f32x16{};
+    auto product = [&](uint4 a, uint4 b) __attribute__((always_inline)) {
+      if constexpr (sizeof(T) == 4) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), acc, 0, 0, 0);
+      } else if constexpr (__is_same(T, _Float16)) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), acc, 0,
+                                                     0, 0);
+      } else {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), acc,
+                                                      0, 0, 0);
+      }
+    };
+    int c = c0;
+    for (; c + 8 <= c1 && (c + 8) * 2 * VE <= p.d; c += 8) {
+      uint4 a[8], b[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[k] = row_vector(e, VE * (2 * (c + k) + half), 0x7FFFFFFF);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) b[k] = row_vector(h, VE * (2 * (c + k) + half), 0x7FFFFFFF);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) product(a[k], b[k]);
+    }
+    for (; c < c1; ++c) product(row_vector(e, VE * (2 * c + half), p.d), row_vector(h, VE * (2 * c + half), p.d));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[turn][wave][r][lane] = acc[r];
+    __syncthreads();  // the other half of s is written next: no second barrier
+    float z[4], n = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * wave + i;
+      z[i] = ((s[turn][0][r][lane] + s[turn][1][r][lane]) + s[turn][2][r][lane]) + s[turn][3][r][lane];
+      const int64_t v = 32 * g + 8 * wave + 4 * half + i;
+      if (v == to && tok < p.R) p.z_target[tok] = z[i];
+      z[i] = v < p.V ? z[i] * kLog2e : -INFINITY;
+      n = fmaxf(n, z[i]);
+    }
+    const float ref = n == -INFINITY ? 0.f : n;
+    l *= __builtin_amdgcn_exp2f(m - ref);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(z[i] - ref);
+    m = n;
+  }
+  // the token's 8 pairs: two halves of four waves
+  __shared__ float2 pair[4][64];
+  pair[wave][lane] = make_float2(m, l);
+  __syncthreads();
+  if (threadIdx.x >= 32 || tok >= p.R) return;
+  float n = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) n = fmaxf(n, fmaxf(pair[w][lane].x, pair[w][lane + 32].x));
+  const float ref = n == -INFINITY ? 0.f : n;
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    sum += pair[w][lane].y * __builtin_amdgcn_exp2f(pair[w][lane].x - ref) +
+           pair[w][lane + 32].y * __builtin_amdgcn_exp2f(pair[w][lane + 32].x - ref);
+  p.part[(int64_t)blockIdx.x * p.R + tok] = make_float2(n, sum);
 }
 
 // ----------------------------------------------------------------- backward
-// Coefficients of each row, zero for the rows that only fill dz up, and the
-// power of two that dz is held under (|dz| <= |g + gl| + |g|, below 2^15 after
-// it).  One workgroup: rows are few against the products.
-__global__ __launch_bounds__(1024) void xent_coef_kernel(const int64_t* __restrict__ target, int64_t R, int64_t rows_p,
-                                                         int64_t V, int64_t ignore, const float* __restrict__ g_loss,
-                                                         const float* __restrict__ g_lse,
-                                                         const float* __restrict__ lse,
-                                                         float* __restrict__ coef, float* __restrict__ scal) {
-  uint32_t m = 0;
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < rows_p; i += 1024) {
-    float all = 0.f, g = 0.f, l = 0.f;
-    const int64_t k = min(i, R - 1);  // loads without branches, so that they fly together
-    const int64_t at = target[k];
-    const float gk = g_loss ? g_loss[k] : 0.f, sk = g_lse ? g_lse[k] : 0.f, lk = lse[k];
-    if (i < R) {
-      g = at == ignore ? 0.f : at < 0 || at >= V ? NAN : gk;
-      all = g + sk;
-      l = lk * kLog2e;
-    }
-    coef[i] = all;
-    coef[rows_p + i] = g;
-    coef[2 * rows_p + i] = l;
-    m = max(m, max(finite_bits(all), finite_bits(g)));
-  }
-  for (int h = 32; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
-  __shared__ uint32_t s[16];
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; ++i) m = max(m, s[i]);
-    const float scale = scale_for(m, 13);
-    scal[kScaleP] = scale;
-    scal[kInvP] = 1.f / scale;
-  }
-}
-
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 template <class C>
@@ -548,13 +685,23 @@ struct Plan {
   int dpad, mode;  // mode: what the operands need, -1 nothing
   bool split;
   bool big_z, big_h, big_e;
-  uint32_t tiles_v;  // of the forward
+  uint32_t tiles_v;    // of the forward
+  uint32_t rows_grid;  // workgroups of the few-token forward, 0: tiles
   int splits_h, splits_e;
   // offsets into the workspace
   size_t scal, amax, e, h, part, zt, coef, P, ph, pe, bytes;
 };
 
 constexpr int64_t kPieceBytes = 512ll << 20;
+
+// Tokens up to which the forward reads the table into the operands: the tiles
+// read a copy of it that has to be made first (fp32, and 16-bit rows of d % 64
+// != 0), or go over it with mostly empty columns.  Measured, us, few tokens /
+// tiles, fp32: 1, 64, 96 tokens of 16,384 x 256: 9.9 / 27, 16 / 30, 20 / 30; of
+// 131,072 x 1,024: 142 / 524, 404 / 531, 602 / 536.  bf16: 1, 32 tokens of
+// 131,072 x 1,024: 53 / 62, 79 / 64; of 50,021 x 500: 22 / 44, 28 / 45, 64: 43 / 45.
+inline int64_t few_rows(int d, int dtype) { return dtype == MPL_F32 || d % 64 ? 64 : 16; }
+
 
 inline int64_t up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
 
@@ -573,8 +720,15 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
     at = (at + bytes + 1023) / 1024 * 1024;
     return o;
   };
+  if (!backward && R <= few_rows(d, dtype)) {
+    p.rows_grid = (uint32_t)std::min<int64_t>(cdiv(V, 32), 2048);
+    p.part = take((size_t)p.rows_grid * R * 8);
+    p.zt = take((size_t)R * 4);
+    p.bytes = at;
+    return p;
+  }
   p.scal = take(kScalars * 4);
-  p.amax = take(2 * kAmaxBlocks * 4);
+  p.amax = take(3 * kAmaxBlocks * 4);
   p.e = take(p.mode >= 0 ? (size_t)V * p.dpad * 2 * S : 0);
   p.h = take(p.mode >= 0 ? (size_t)R * p.dpad * 2 * S : 0);
   if (!backward) {
@@ -591,12 +745,13 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
   if (most >= even && most < V) most = most / even * even;
   p.pieces = cdiv(V, most);
   p.v_piece = p.pieces == 1 ? up(V, 256) : most;
-  // Products with few tiles split their contraction, at least 16 stages a part.
+  // Products with few tiles split their contraction, at least 16 stages a part
+  // (8 of the small tiles).
   auto pick = [&](int64_t M, int64_t K, bool& big, int& splits) {
     const int64_t tiles = cdiv(M, 256) * cdiv(d, 256), iters = K * S / 64;
     big = tiles * std::max<int64_t>(1, iters / 16) >= 256;
     const int64_t n = big ? tiles : cdiv(M, 128) * cdiv(d, 128), want = big ? 256 : 512;
-    splits = (int)std::max<int64_t>(1, std::min(cdiv(want, n), iters / 16));
+    splits = (int)std::max<int64_t>(1, std::min(cdiv(want, n), iters / (big ? 16 : 8)));
     if (n * 4 >= want * 3) splits = 1;
   };
   pick(R, p.v_piece, p.big_h, p.splits_h);
@@ -640,8 +795,11 @@ int check_call(const char* what, const Call& c, const void* ws, size_t ws_bytes,
 }
 
 // Brings both arrays into operand form; E and H are the rows forms.
-void operands(const Call& c, const Plan& p, char* ws, hipStream_t s, TileOperand& E, TileOperand& H) {
+// In the backward `q` also gets the coefficients formed.
+void operands(const Call& c, const Plan& p, char* ws, const CoefArgs* q, hipStream_t s, TileOperand& E, TileOperand& H) {
   const int64_t row = (int64_t)p.dpad * (p.split ? 4 : 2);
+  const bool apart = q && p.mode <= kCopy16;
+  if (apart) xent_coef_kernel<<<1, 1024, 0, s>>>(*q, (float*)(ws + p.scal));
   if (p.mode < 0) {
     E = {(const char*)c.embedding, c.embedding_pitch * 2, c.V, row};
     H = {(const char*)c.hidden, c.hidden_pitch * 2, c.R, row};
@@ -657,12 +815,15 @@ void operands(const Call& c, const Plan& p, char* ws, hipStream_t s, TileOperand
   a.d = c.d, a.dpad = p.dpad;
   a.scal = (float*)(ws + p.scal);
   a.part = (uint32_t*)(ws + p.amax);
+  a.coefs = q && !apart;
+  const dim3 maxima(kAmaxBlocks, a.coefs ? 3 : 2);
+  const CoefArgs coef = q ? *q : CoefArgs{};
   const unsigned grid = (unsigned)(a.e.blocks + a.h.blocks);
   if (p.mode == kSplit) {
-    amax_kernel<kSplit><<<dim3(kAmaxBlocks, 2), 256, 0, s>>>(a);
+    amax_kernel<kSplit><<<maxima, 256, 0, s>>>(a, coef);
     pack_kernel<kSplit><<<grid, 256, 0, s>>>(a);
   } else if (p.mode == kBf16ToF16) {
-    amax_kernel<kBf16ToF16><<<dim3(kAmaxBlocks, 2), 256, 0, s>>>(a);
+    amax_kernel<kBf16ToF16><<<maxima, 256, 0, s>>>(a, coef);
     pack_kernel<kBf16ToF16><<<grid, 256, 0, s>>>(a);
   } else {
     pack_kernel<kCopy16><<<grid, 256, 0, s>>>(a);
@@ -703,8 +864,27 @@ extern "C" int mpl_vocab_cross_entropy(const void* hidden, int64_t hidden_pitch,
   MPL_REQUIRE(target && loss && lse, MPL_EINVAL, "%s: null buffer", what);
   char* ws = (char*)workspace;
   hipStream_t s = (hipStream_t)stream;
+  float2* part = (float2*)(ws + p.part);
+  float* z_target = (float*)(ws + p.zt);
+  auto join = [&](int pairs) {
+    if (rows <= 2048)
+      xent_join_kernel<4><<<(unsigned)cdiv(rows, 4), 256, 0, s>>>(part, pairs, rows, vocab, target, ignore_index,
+                                                               z_target, loss, lse);
+    else
+      xent_join_kernel<32><<<(unsigned)cdiv(rows, 32), 256, 0, s>>>(part, pairs, rows, vocab, target, ignore_index,
+                                                                 z_target, loss, lse);
+    return check_launch(what);
+  };
+  if (p.rows_grid) {
+    const RowsArgs a{embedding, hidden, embedding_pitch, hidden_pitch, rows, vocab, d, target, part, z_target};
+    const dim3 grid(p.rows_grid, (unsigned)cdiv(rows, 32));
+    if (dtype == MPL_F32) xent_rows_kernel<float><<<grid, 256, 0, s>>>(a);
+    else if (dtype == MPL_F16) xent_rows_kernel<_Float16><<<grid, 256, 0, s>>>(a);
+    else xent_rows_kernel<__bf16><<<grid, 256, 0, s>>>(a);
+    return join((int)p.rows_grid);
+  }
   LogitArgs a{};
-  operands(c, p, ws, s, a.E, a.H);
+  operands(c, p, ws, nullptr, s, a.E, a.H);
   a.R = rows, a.V = vocab;
   a.iters = p.dpad * (p.split ? 2 : 1) / 64;
   a.tiles_v = p.tiles_v;
@@ -712,15 +892,13 @@ extern "C" int mpl_vocab_cross_entropy(const void* hidden, int64_t hidden_pitch,
   a.scal = (const float*)(ws + p.scal);
   a.scaled = p.split;
   a.target = target;
-  a.part = (float2*)(ws + p.part);
-  a.z_target = (float*)(ws + p.zt);
+  a.part = part;
+  a.z_target = z_target;
   const unsigned grid = a.tiles_v * a.tiles_t;
   if (dtype == MPL_F32) MPL_TILE(xent_lse_kernel, 2, false, false, false, p.big_z, grid, s, a);
   else if (dtype == MPL_F16) MPL_TILE(xent_lse_kernel, 1, false, false, false, p.big_z, grid, s, a);
   else MPL_TILE(xent_lse_kernel, 1, true, false, false, p.big_z, grid, s, a);
-  xent_join_kernel<<<(unsigned)cdiv(rows, 32), 256, 0, s>>>(a.part, (int)p.tiles_v, rows, vocab, target, ignore_index,
-                                                          a.z_target, loss, lse);
-  return check_launch(what);
+  return join((int)p.tiles_v);
 }
 
 extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pitch, const void* embedding,
@@ -741,11 +919,10 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
   hipStream_t s = (hipStream_t)stream;
   const int S = p.split ? 2 : 1;
   LogitArgs a{};
-  operands(c, p, ws, s, a.E, a.H);
   float* scal = (float*)(ws + p.scal);
   float* coef = (float*)(ws + p.coef);
-  xent_coef_kernel<<<1, 1024, 0, s>>>(target, rows, p.rows_p, vocab, ignore_index, g_loss, g_lse, lse,
-                                      coef, scal);
+  const CoefArgs q{target, rows, p.rows_p, vocab, ignore_index, g_loss, g_lse, lse, coef};
+  operands(c, p, ws, &q, s, a.E, a.H);
   a.R = rows, a.V = vocab;
   a.iters = p.dpad * S / 64;
   const int bz = p.big_z ? 256 : 128;
