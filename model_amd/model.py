@@ -5,7 +5,11 @@ The backbone (embedding, attention, layer norms, feed-forward blocks, router
 and gated memory write-back) is small dense work: plain torch ops in fp32 in
 training, fused dense layers and causal attention (mpl_dense_layers,
 mpl_causal_attention) under torch.no_grad on the GPU; every memory read is
-MemoryPool (libmpl.so).  Parameter names and shapes follow the Flax modules, so a checkpoint of the reference
+MemoryPool (libmpl.so).  MemoryPoolLM.token_loss gives each token's cross
+entropy without the logits in memory, for training and evaluation on the GPU:
+its layer norms (with the residual add before each) and its output layer with
+the loss are libmpl.so launches with their own backward passes
+(model_amd/layer_norm.py, model_amd/cross_entropy.py).  Parameter names and shapes follow the Flax modules, so a checkpoint of the reference
 (model_amd/checkpoint.py) loads into it:
 
   embed/embedding [vocab, d]            nn.Embed (logits use embed.attend)
@@ -38,9 +42,9 @@ from typing import Any, Dict, List, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from .cross_entropy import vocab_cross_entropy
+from .layer_norm import LN_EPS, layer_norm
 from .memory import MemoryPool
-
-LN_EPS = 1e-6  # flax.linen.LayerNorm default
 
 
 @dataclasses.dataclass(frozen=True)
@@ -317,6 +321,20 @@ def vocab_logits(x: torch.Tensor, ln_scale: torch.Tensor, ln_bias: torch.Tensor,
 
 def _ln(x, p):
     return F.layer_norm(x, (x.shape[-1],), p["scale"], p["bias"], LN_EPS)
+
+
+def _add_ln(x, y, p):
+    """(LayerNorm(x + y), x + y), y None for none, in torch ops."""
+    if y is not None:
+        x = x + y
+    return _ln(x, p), x
+
+
+def _add_layer_norm(x, y, p):
+    """_add_ln as one libmpl.so launch, with its backward pass."""
+    if y is None:
+        return layer_norm(x, p["scale"], p["bias"], LN_EPS), x
+    return layer_norm(x, p["scale"], p["bias"], LN_EPS, residual=y)
 
 
 def merge_layer_aux(layer_aux: List[Dict[str, Any]]) -> Dict[str, Any]:
@@ -620,6 +638,13 @@ class MemoryPoolLM:
         and residual adds inside the dense layers (mpl_dense_layers), and the
         attention one launch without score matrix, mask or transposed copies
         (mpl_causal_attention)."""
+        B, T = tokens.shape
+        x, layer_aux = self._trunk_gpu(p, tokens, pool_off, noise_scale, shuffle_pool, rngs)
+        logits = F.linear(_ln(x, p["ln_final"]), p["embed"]["embedding"])
+        return logits.reshape(B, T, -1), _LazyMerged(layer_aux)
+
+    def _trunk_gpu(self, p, tokens, pool_off, noise_scale, shuffle_pool, rngs):
+        """_forward_gpu up to ln_final's input: ([B * T, d], the layers' aux)."""
         cfg = self.cfg
         B, T = tokens.shape
         d, H = cfg.d_model, cfg.n_heads
@@ -647,8 +672,7 @@ class MemoryPoolLM:
                 x, = dense_layers(mem.reshape(B * T, cfg.d_value), [(mo["kernel"], mo["bias"], None)], x_mul=gate,
                                   residual=x)
                 layer_aux.append(aux)
-        logits = F.linear(_ln(x, p["ln_final"]), emb)
-        return logits.reshape(B, T, -1), _LazyMerged(layer_aux)
+        return x, layer_aux
 
     def _attention(self, p, h, layer_cache, positions, drop=None):
         cfg = self.cfg
@@ -699,6 +723,57 @@ class MemoryPoolLM:
         if (not self.decode and positions is None and not train and not route_through_pool and probes is None
                 and not sparse_grad and self._fused_forward_ok(p, tokens, pool_off)):
             return self._forward_gpu(p, tokens, pool_off, noise_scale, shuffle_pool, rngs)
+        x, layer_aux = self._trunk(p, tokens, _add_ln, train=train, pool_off=pool_off,
+                                   route_through_pool=route_through_pool, sparse_grad=sparse_grad, probes=probes,
+                                   positions=positions, noise_scale=noise_scale, shuffle_pool=shuffle_pool,
+                                   cache=cache, rngs=rngs)
+        logits = F.linear(x, p["embed"]["embedding"])  # x . emb^T as one product, no transposed copy of the table
+        return logits, _LazyMerged(layer_aux)
+
+    __call__ = apply
+
+    def token_loss(self, variables: Dict[str, Any], tokens: torch.Tensor, targets: torch.Tensor, *,
+                   ignore_index: int = -100, return_lse: bool = False, train: bool = False, pool_off: bool = False,
+                   route_through_pool: bool = False, sparse_grad: bool = False,
+                   probes: Optional[Dict[int, torch.Tensor]] = None, noise_scale: float = 1.0,
+                   shuffle_pool: bool = False, rngs=None):
+        """The cross entropy of each token's target under apply()'s logits,
+        without the logits in memory: (loss [B, T] fp32, aux), or (loss, lse,
+        aux) with ``return_lse``; on the GPU.  targets [B, T] int64 or int32,
+        ``ignore_index`` where there is none (vocab_cross_entropy).  The other
+        arguments are apply()'s.  Differentiable in all the parameters that
+        apply() is (the table's gradient through the output layer and through
+        the input rows); the layer norms run with the residual adds before
+        them (layer_norm).  Under torch.no_grad the blocks take the fused
+        launches that apply() takes there."""
+        if self.decode:
+            raise ValueError("token_loss takes whole sequences: build the model without decode=True")
+        if not tokens.is_cuda:
+            raise ValueError(f"token_loss runs on the GPU only (libmpl.so), tokens are on {tokens.device}")
+        if targets.shape != tokens.shape:
+            raise ValueError(f"token_loss: targets {tuple(targets.shape)} for tokens {tuple(tokens.shape)}")
+        p = variables["params"] if "params" in variables else variables
+        if (not train and not route_through_pool and probes is None and not sparse_grad
+                and self._fused_forward_ok(p, tokens, pool_off)):
+            x, layer_aux = self._trunk_gpu(p, tokens, pool_off, noise_scale, shuffle_pool, rngs)
+            lf = p["ln_final"]
+            x = layer_norm(x, lf["scale"], lf["bias"], LN_EPS).reshape(*tokens.shape, -1)
+        else:
+            x, layer_aux = self._trunk(p, tokens, _add_layer_norm, train=train, pool_off=pool_off,
+                                       route_through_pool=route_through_pool, sparse_grad=sparse_grad, probes=probes,
+                                       positions=None, noise_scale=noise_scale, shuffle_pool=shuffle_pool, cache=None,
+                                       rngs=rngs)
+        loss, lse = vocab_cross_entropy(x, p["embed"]["embedding"], targets, ignore_index=ignore_index, return_lse=True)
+        return (loss, lse, _LazyMerged(layer_aux)) if return_lse else (loss, _LazyMerged(layer_aux))
+
+    def _trunk(self, p, tokens, add_ln, *, train, pool_off, route_through_pool, sparse_grad, probes, positions,
+               noise_scale, shuffle_pool, cache, rngs):
+        """The backbone up to the output layer: (LayerNorm of the last layer's
+        output [B, T, d], the layers' aux).  ``add_ln`` adds a block's output to
+        the residual stream and normalises it for the next (_add_ln,
+        _add_layer_norm)."""
+        cfg = self.cfg
+        B, T = tokens.shape
         emb = p["embed"]["embedding"]
         if positions is None:
             x = emb[tokens] + p["pos_embed"][None, :T]
@@ -708,10 +783,11 @@ class MemoryPoolLM:
             raise ValueError("decode mode needs cache and positions")
         drop = _make_dropout(cfg.dropout, rngs, x.device) if (train and cfg.dropout > 0) else None
         layer_aux = []
+        y = None
         for i in range(cfg.n_layers):
-            h = _ln(x, p[f"ln_attn_{i}"])
-            x = x + self._attention(p[f"attn_{i}"], h, cache[i] if self.decode else None, positions, drop)
-            h = _ln(x, p[f"ln_ffn_{i}"])
+            h, x = add_ln(x, y, p[f"ln_attn_{i}"])
+            y = self._attention(p[f"attn_{i}"], h, cache[i] if self.decode else None, positions, drop)
+            h, x = add_ln(x, y, p[f"ln_ffn_{i}"])
             mem_layer = self.pool is not None and i in cfg.memory_layers
             y = torch.zeros_like(x)
             if not mem_layer or cfg.memory_ffn:
@@ -731,9 +807,4 @@ class MemoryPoolLM:
                     layer_aux.append(aux)
             if drop is not None:  # model.py:122: dropout on the layer's residual branch
                 y = drop(y)
-            x = x + y
-        x = _ln(x, p["ln_final"])
-        logits = F.linear(x, emb)  # x . emb^T as one product, no transposed copy of the table
-        return logits, _LazyMerged(layer_aux)
-
-    __call__ = apply
+        return add_ln(x, y, p["ln_final"])[0], layer_aux
