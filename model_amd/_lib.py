@@ -11,6 +11,7 @@ import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmpl.so")
+OPS_PATH = os.path.join(HERE, "_ops.so")
 
 MPL_F32, MPL_F16, MPL_BF16 = 0, 1, 2
 MPL_OK, MPL_EINVAL, MPL_EHIP, MPL_EWORKSPACE, MPL_EUNSUPPORTED = 0, 1, 2, 3, 4  # include/mpl.h status codes
@@ -125,6 +126,26 @@ def lib() -> C.CDLL:
     return _lib
 
 
+_ops = None
+
+
+def ops():
+    """The extension module of csrc/torch/ops.cpp: layer_norm's and
+    vocab_cross_entropy's calls and autograd nodes (raises MplError if it was
+    not built)."""
+    global _ops
+    if _ops is None:
+        lib()
+        try:
+            import torch  # noqa: F401  (its libraries, before the module that needs them)
+
+            from . import _ops as module
+        except ImportError as e:
+            raise MplError(f"{OPS_PATH} is missing or does not load ({e}): build it with `python -m model_amd.build`")
+        _ops = module
+    return _ops
+
+
 def check(rc: int, what: str = "") -> None:
     if rc != 0:
         msg = lib().mpl_last_error().decode(errors="replace")
@@ -157,29 +178,3 @@ def stream_ptr(device) -> int:
         _stream_index[device] = device.index
     return stream
 
-
-class on_device:
-    """Makes ``device`` the current one inside a with block, where it is not
-    already: a launch goes to a stream of the current device."""
-
-    __slots__ = ("to", "back")
-
-    def __init__(self, device):
-        import torch
-
-        now = torch._C._cuda_getDevice()
-        self.to = now if device.index is None else device.index
-        self.back = now
-
-    def __enter__(self):
-        if self.to != self.back:
-            import torch
-
-            torch._C._cuda_setDevice(self.to)
-
-    def __exit__(self, *exc):
-        if self.to != self.back:
-            import torch
-
-            torch._C._cuda_setDevice(self.back)
-        return False

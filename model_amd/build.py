@@ -3,7 +3,8 @@
 Usage: ``python -m model_amd.build`` (or ``__graft_entry__.build()``).  Each
 ``csrc/*.hip`` file (hipcc) and host-only ``csrc/*.cpp`` file (g++) is
 compiled to an object in ``_build/`` in parallel, then linked into
-``model_amd/libmpl.so`` (written atomically).
+``model_amd/libmpl.so`` (written atomically).  ``csrc/torch/ops.cpp`` (g++, torch's
+headers) becomes the extension module ``model_amd/_ops.so`` beside it.
 """
 
 from __future__ import annotations
@@ -20,6 +21,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(ROOT, "_build", "obj")
 LIB = os.path.join(HERE, "libmpl.so")
+OPS = os.path.join(HERE, "_ops.so")
 ARCH = "gfx950"
 
 # Packed fp32 VALU ops are disabled for every device compile.  MFMA results
@@ -71,20 +73,50 @@ def _compile(src: str, cc: str) -> str:
     return obj
 
 
+def _compile_ops() -> str:
+    """The object of csrc/torch/ops.cpp."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    src, obj = os.path.join(CSRC, "torch", "ops.cpp"), os.path.join(OBJ, "torch_ops.o")
+    rocm = os.path.dirname(os.path.dirname(hipcc()))
+    rocm = rocm if os.path.isdir(os.path.join(rocm, "include", "hip")) else "/opt/rocm"
+    inc = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(rocm, "include")]
+    cmd = [host_cxx(), "-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-D__HIP_PLATFORM_AMD__=1",
+           "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f for i in inc for f in ("-isystem", i)), "-c", src, "-o", obj]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed for {src}:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    return obj
+
+
+def _link(cmd, out: str) -> None:
+    tmp = out + f".tmp{os.getpid()}"
+    r = subprocess.run([*cmd, "-o", tmp], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, out)
+
+
 def build(verbose: bool = False, jobs: int = 8) -> str:
     cc = hipcc()
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")) + glob.glob(os.path.join(CSRC, "*.cpp")))
-    with cf.ThreadPoolExecutor(max_workers=max(1, min(jobs, len(srcs)))) as ex:
+    with cf.ThreadPoolExecutor(max_workers=max(1, min(jobs, len(srcs) + 1))) as ex:
+        ops = ex.submit(_compile_ops)
         objs = list(ex.map(lambda s: _compile(s, cc), srcs))
-    tmp = LIB + f".tmp{os.getpid()}"
-    cmd = [cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread", "-o", tmp, *objs]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, LIB)
+        ops = ops.result()
+    _link([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread", *objs], LIB)
+    from torch.utils import cpp_extension
+
+    libs = [f"-L{p}" for p in cpp_extension.library_paths()]
+    _link([host_cxx(), "-shared", "-fPIC", ops, f"-L{HERE}", "-lmpl", *libs, "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
+           "-ltorch_python", "-Wl,-rpath,$ORIGIN"], OPS)
     if verbose:
-        print(f"built {LIB} from {len(srcs)} sources")
+        print(f"built {LIB} from {len(srcs)} sources, and {OPS}")
     return LIB
 
 

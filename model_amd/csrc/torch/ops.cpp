@@ -1,0 +1,304 @@
+// The host path of layer_norm and vocab_cross_entropy (model_amd/layer_norm.py,
+// model_amd/cross_entropy.py check the arguments and document them): output and
+// workspace tensors, the calls into libmpl.so (include/mpl.h), and the autograd
+// nodes.  In C++ because a training step's small calls are bound by host time:
+// torch runs backward nodes on a thread of its own, where a Python node of these
+// two operators took 40 to 80 us a call, several times its kernels.
+//
+// Host code only: built by the host compiler against torch's headers and linked
+// to libmpl.so beside it.
+#include <ATen/ATen.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <optional>
+#include <tuple>
+
+#include "../../../include/mpl.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+int dtype_code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return MPL_F32;
+    case at::kHalf: return MPL_F16;
+    case at::kBFloat16: return MPL_BF16;
+    default: TORCH_CHECK(false, "unsupported dtype ", t.scalar_type());
+  }
+}
+
+void check(int rc, const char* what) { TORCH_CHECK(rc == MPL_OK, what, " failed (code ", rc, "): ", mpl_last_error()); }
+
+void* stream_of(const Tensor& t) {
+  return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream();
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// A captured backward of leaves that an eager graph holds ends the process, so
+// the nodes refuse to run under capture; tests set `pretend`.
+bool pretend_capturing = false;
+bool capturing() {
+  return pretend_capturing ||
+         c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+
+// First derivatives only: what a node returns under create_graph raises when it
+// is differentiated again.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", 1);
+    g = (*error)({g.detach().requires_grad_(true)})[0];
+  }
+  return grads;
+}
+
+// Rows of d elements next to each other and the elements from row to row (at
+// least d); copied only where they do not lie so.
+struct Rows {
+  Tensor t;
+  int64_t pitch = 0;
+  void* data() const { return t.defined() ? t.data_ptr() : nullptr; }
+};
+Rows rows_of(const Tensor& t, int64_t d) {
+  if (!t.defined()) return {};
+  if (t.is_contiguous()) return {t, d};
+  Tensor r = t.reshape({-1, d});
+  if ((d > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < d)) return {r.contiguous(), d};
+  return {r, r.size(0) > 1 ? r.stride(0) : d};
+}
+
+// ------------------------------------------------------------- layer norm
+// (y, sum or undefined, statistics [2, rows] or undefined)
+std::tuple<Tensor, Tensor, Tensor> ln_forward(const Tensor& x, const Tensor& scale, const Tensor& bias, double eps,
+                                              const Tensor& residual, bool stats) {
+  const c10::DeviceGuard guard(x.device());
+  const int64_t d = x.size(-1), rows = x.numel() / d;
+  Tensor y = at::empty(x.sizes(), x.options()), total, st;
+  if (residual.defined()) total = at::empty(x.sizes(), x.options());
+  if (stats) st = at::empty({2, rows}, x.options().dtype(at::kFloat));
+  if (rows) {
+    const Rows a = rows_of(x, d), r = rows_of(residual, d);
+    const Tensor w = scale.contiguous(), b = bias.contiguous();
+    float* mean = (float*)ptr(st);
+    check(mpl_layer_norm(a.data(), a.pitch, r.data(), r.pitch, dtype_code(x), w.data_ptr(), b.data_ptr(), dtype_code(w),
+                         rows, (int)d, (float)eps, y.data_ptr(), ptr(total), mean, mean ? mean + rows : nullptr,
+                         stream_of(x)),
+          "mpl_layer_norm");
+  }
+  return {y, total, st};
+}
+
+// (dx, d_scale, d_bias), undefined where not wanted
+std::tuple<Tensor, Tensor, Tensor> ln_backward(const Tensor& g_y, const Tensor& s, const Tensor& scale,
+                                               const float* mean, const float* rstd, const Tensor& g_residual,
+                                               bool want_x, bool want_params) {
+  const c10::DeviceGuard guard(s.device());
+  const int64_t d = s.size(-1), rows = s.numel() / d;
+  Tensor dx, ds, db;
+  if (want_x) dx = at::empty(s.sizes(), s.options());
+  if (want_params) {
+    ds = rows ? at::empty({d}, scale.options()) : at::zeros({d}, scale.options());
+    db = rows ? at::empty({d}, scale.options()) : at::zeros({d}, scale.options());
+  }
+  if (rows && (want_x || want_params)) {
+    const Rows a = rows_of(s, d), g = rows_of(g_y, d), r = rows_of(g_residual, d);
+    const Tensor w = scale.contiguous();
+    const int code = dtype_code(s);
+    const size_t n = want_params ? mpl_layer_norm_bwd_workspace_bytes(rows, (int)d, code) : 0;
+    Tensor ws;
+    if (n) ws = at::empty({(int64_t)n}, s.options().dtype(at::kByte));
+    check(mpl_layer_norm_bwd(g.data(), g.pitch, a.data(), a.pitch, r.data(), r.pitch, code, w.data_ptr(), dtype_code(w),
+                             mean, rstd, rows, (int)d, ptr(dx), ptr(ds), ptr(db), ptr(ws), n, stream_of(s)),
+          "mpl_layer_norm_bwd");
+  }
+  return {dx, ds, db};
+}
+
+Tensor or_none(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+
+struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& scale, const Tensor& bias, double eps,
+                               const std::optional<Tensor>& residual) {
+    auto [y, total, st] = ln_forward(x, scale, bias, eps, or_none(residual), true);
+    ctx->save_for_backward({total.defined() ? total : x, scale, st});
+    ctx->set_materialize_grads(false);
+    if (total.defined()) return {y, total};
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!capturing(), "torch autograd through layer_norm is not supported under HIP graph capture: use "
+                "layer_norm_forward and layer_norm_backward, which capture");
+    const bool added = grads.size() > 1;  // two outputs: there was a residual
+    const bool nx = ctx->needs_input_grad(0), ns = ctx->needs_input_grad(1), nb = ctx->needs_input_grad(2),
+               nr = added && ctx->needs_input_grad(3);
+    const Tensor g_sum = added ? grads[1] : Tensor();
+    variable_list out(5);
+    if (!grads[0].defined()) {  // only the sum was used
+      if (nx) out[0] = g_sum;
+      if (nr) out[4] = g_sum;
+      return out;
+    }
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &s = saved[0], &st = saved[2];
+    {
+      const at::AutoGradMode no_grad(false);
+      const float* mean = (const float*)st.data_ptr();
+      auto [dx, ds, db] = ln_backward(grads[0], s, saved[1], mean, mean + st.size(1), g_sum, nx || nr, ns || nb);
+      if (nx) out[0] = dx;
+      if (ns) out[1] = ds;
+      if (nb) out[2] = db;
+      if (nr) out[4] = dx;
+    }
+    return once(std::move(out), "layer_norm");
+  }
+};
+
+py::object layer_norm(const Tensor& x, const Tensor& scale, const Tensor& bias, double eps,
+                      const std::optional<Tensor>& residual, bool autograd) {
+  const Tensor r = or_none(residual);
+  if (autograd) {
+    const variable_list out = LayerNormFunction::apply(x, scale, bias, eps, residual);
+    return r.defined() ? py::cast(std::make_tuple(out[0], out[1])) : py::cast(out[0]);
+  }
+  auto [y, total, st] = ln_forward(x, scale, bias, eps, r, false);
+  return r.defined() ? py::cast(std::make_tuple(y, total)) : py::cast(y);
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> layer_norm_forward(const Tensor& x, const Tensor& scale, const Tensor& bias,
+                                                              double eps, const std::optional<Tensor>& residual) {
+  const at::AutoGradMode no_grad(false);
+  auto [y, total, st] = ln_forward(x, scale, bias, eps, or_none(residual), true);
+  return {y, total.defined() ? total : x, st.select(0, 0), st.select(0, 1)};
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& g_y, const Tensor& s, const Tensor& scale,
+                                                       const Tensor& mean, const Tensor& rstd,
+                                                       const std::optional<Tensor>& g_residual) {
+  const at::AutoGradMode no_grad(false);
+  return ln_backward(g_y, s, scale, (const float*)mean.data_ptr(), (const float*)rstd.data_ptr(), or_none(g_residual),
+                     true, true);
+}
+
+// ---------------------------------------------------------- cross entropy
+// 16-bit rows that the tiles read as they lie (d a multiple of 64) start at 16 bytes.
+Rows operand_of(const Tensor& t, int64_t d) {
+  Rows r = rows_of(t, d);
+  if (t.scalar_type() != at::kFloat && d % 64 == 0 && ((uintptr_t)r.data() % 16 || r.pitch % 8))
+    return {r.t.clone(at::MemoryFormat::Contiguous), d};
+  return r;
+}
+
+Tensor workspace(int64_t rows, int64_t vocab, int64_t d, const Tensor& like, bool backward) {
+  const size_t n = mpl_vocab_cross_entropy_workspace_bytes(rows, vocab, (int)d, dtype_code(like), backward);
+  TORCH_CHECK_VALUE(n, "vocab_cross_entropy: ", rows, " rows, a vocabulary of ", vocab, " and a width of ", d,
+                    " are out of range");
+  return at::empty({(int64_t)n}, like.options().dtype(at::kByte));
+}
+
+Tensor ids_of(const Tensor& targets) { return targets.to(at::kLong).contiguous(); }
+
+std::tuple<Tensor, Tensor> ce_forward(const Tensor& hidden, const Tensor& embedding, const Tensor& ids,
+                                      int64_t ignore_index) {
+  const c10::DeviceGuard guard(hidden.device());
+  const int64_t V = embedding.size(0), d = embedding.size(1), R = ids.numel();
+  const auto f32 = hidden.options().dtype(at::kFloat);
+  Tensor loss = at::empty(ids.sizes(), f32), lse = at::empty(ids.sizes(), f32);
+  if (R) {
+    const Rows h = operand_of(hidden, d), e = operand_of(embedding, d);
+    const Tensor ws = workspace(R, V, d, hidden, false);
+    check(mpl_vocab_cross_entropy(h.data(), h.pitch, e.data(), e.pitch, dtype_code(hidden), (const int64_t*)ids.data_ptr(),
+                                  R, V, (int)d, ignore_index, ws.data_ptr(), ws.numel(), (float*)loss.data_ptr(),
+                                  (float*)lse.data_ptr(), stream_of(hidden)),
+          "mpl_vocab_cross_entropy");
+  }
+  return {loss, lse};
+}
+
+std::tuple<Tensor, Tensor> ce_backward(const Tensor& hidden, const Tensor& embedding, const Tensor& ids,
+                                       int64_t ignore_index, const Tensor& lse, const Tensor& g_loss,
+                                       const Tensor& g_lse, bool want_h, bool want_e) {
+  const c10::DeviceGuard guard(hidden.device());
+  const int64_t V = embedding.size(0), d = embedding.size(1), R = ids.numel();
+  Tensor dh, de;
+  if (want_h) dh = at::empty(hidden.sizes(), hidden.options());
+  if (want_e) de = R ? at::empty({V, d}, hidden.options()) : at::zeros({V, d}, hidden.options());
+  if (R && (want_h || want_e)) {
+    auto row_grad = [](const Tensor& g) { return g.defined() ? g.to(at::kFloat).contiguous() : g; };
+    const Tensor gl = row_grad(g_loss), gs = row_grad(g_lse);
+    const Rows h = operand_of(hidden, d), e = operand_of(embedding, d);
+    const Tensor ws = workspace(R, V, d, hidden, true);
+    check(mpl_vocab_cross_entropy_bwd(h.data(), h.pitch, e.data(), e.pitch, dtype_code(hidden),
+                                      (const int64_t*)ids.data_ptr(), R, V, (int)d, ignore_index,
+                                      (const float*)lse.data_ptr(), (const float*)ptr(gl), (const float*)ptr(gs),
+                                      ws.data_ptr(), ws.numel(), ptr(dh), ptr(de), stream_of(hidden)),
+          "mpl_vocab_cross_entropy_bwd");
+  }
+  return {dh, de};
+}
+
+struct CrossEntropyFunction : torch::autograd::Function<CrossEntropyFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& embedding, const Tensor& ids,
+                               int64_t ignore_index) {
+    auto [loss, lse] = ce_forward(hidden, embedding, ids, ignore_index);
+    ctx->save_for_backward({hidden, embedding, ids, lse});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->set_materialize_grads(false);
+    return {loss, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!capturing(), "torch autograd through vocab_cross_entropy is not supported under HIP graph capture: use "
+                "vocab_cross_entropy_grads, which captures");
+    variable_list out(4);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    {
+      const at::AutoGradMode no_grad(false);
+      std::tie(out[0], out[1]) =
+          ce_backward(s[0], s[1], s[2], ctx->saved_data["ignore_index"].toInt(), s[3], grads[0], grads[1],
+                      ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    }
+    return once(std::move(out), "vocab_cross_entropy");
+  }
+};
+
+std::tuple<Tensor, Tensor> vocab_cross_entropy(const Tensor& hidden, const Tensor& embedding, const Tensor& targets,
+                                               int64_t ignore_index, bool autograd) {
+  const Tensor ids = ids_of(targets);
+  if (!autograd) return ce_forward(hidden, embedding, ids, ignore_index);
+  const variable_list out = CrossEntropyFunction::apply(hidden, embedding, ids, ignore_index);
+  return {out[0], out[1]};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> vocab_cross_entropy_grads(const Tensor& hidden, const Tensor& embedding,
+                                                                     const Tensor& targets,
+                                                                     const std::optional<Tensor>& g_loss,
+                                                                     const std::optional<Tensor>& g_lse,
+                                                                     int64_t ignore_index) {
+  const at::AutoGradMode no_grad(false);
+  const Tensor ids = ids_of(targets);
+  auto [loss, lse] = ce_forward(hidden, embedding, ids, ignore_index);
+  auto [dh, de] = ce_backward(hidden, embedding, ids, ignore_index, lse, or_none(g_loss), or_none(g_lse), true, true);
+  return {loss, lse, dh, de};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_ops, m) {
+  m.def("layer_norm", &layer_norm);
+  m.def("layer_norm_forward", &layer_norm_forward);
+  m.def("layer_norm_backward", &layer_norm_backward);
+  m.def("vocab_cross_entropy", &vocab_cross_entropy);
+  m.def("vocab_cross_entropy_grads", &vocab_cross_entropy_grads);
+  m.def("pretend_capturing", [](bool on) { pretend_capturing = on; });
+}

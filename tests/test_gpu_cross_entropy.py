@@ -339,16 +339,20 @@ def test_autograd_refused_under_capture(gpu_lib):
 
     h, e, t, _, _ = _inputs(8, 20, 64, torch.float32)
     h.requires_grad_(True)
+    from model_amd import _lib
+
     saved = ce._capturing
     try:
         loss = ce.vocab_cross_entropy(h, e, t)
         ce._capturing = lambda: True
         with pytest.raises(RuntimeError, match="vocab_cross_entropy_grads"):
             ce.vocab_cross_entropy(h, e, t)
+        _lib.ops().pretend_capturing(True)
         with pytest.raises(RuntimeError, match="vocab_cross_entropy_grads"):
             loss.sum().backward()
     finally:
         ce._capturing = saved
+        _lib.ops().pretend_capturing(False)
 
 
 def test_two_streams(gpu_lib):
@@ -379,3 +383,18 @@ def test_changed_in_place_is_refused(gpu_lib):
         x.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.sum().backward()
+
+
+def test_second_derivative_is_refused(gpu_lib):
+    """Under create_graph the gradients are there, and raise when they are
+    differentiated again."""
+    from model_amd.cross_entropy import vocab_cross_entropy
+
+    h, e, t, gl, _ = _inputs(8, 20, 64, torch.float32)
+    h.requires_grad_(True)
+    loss = (vocab_cross_entropy(h, e, t) * gl).sum()
+    g, = torch.autograd.grad(loss, h, create_graph=True)
+    plain, = torch.autograd.grad((vocab_cross_entropy(h, e, t) * gl).sum(), h)
+    assert torch.equal(g.detach(), plain)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        g.sum().backward()

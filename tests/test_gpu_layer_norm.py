@@ -296,13 +296,44 @@ def test_autograd_refused_under_capture(gpu_lib):
 
     x, w, b, _, _, _ = _inputs(4, 32, torch.float32)
     x.requires_grad_(True)
+    from model_amd import _lib
+
     saved = ln._capturing
     try:
         y = ln.layer_norm(x, w, b)
         ln._capturing = lambda: True
         with pytest.raises(RuntimeError, match="layer_norm_forward"):
             ln.layer_norm(x, w, b)
+        _lib.ops().pretend_capturing(True)
         with pytest.raises(RuntimeError, match="layer_norm_forward"):
             y.sum().backward()
     finally:
         ln._capturing = saved
+        _lib.ops().pretend_capturing(False)
+
+
+def test_second_derivative_is_refused(gpu_lib):
+    """Under create_graph the gradients are there, and raise when they are
+    differentiated again."""
+    from model_amd.layer_norm import layer_norm
+
+    x, w, b, _, gy, _ = _inputs(4, 32, torch.float32)
+    for t in (x, w, b):
+        t.requires_grad_(True)
+    grads = torch.autograd.grad(layer_norm(x, w, b), [x, w, b], gy, create_graph=True)
+    plain = torch.autograd.grad(layer_norm(x, w, b), [x, w, b], gy)
+    assert all(torch.equal(p.detach(), q) for p, q in zip(grads, plain))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        grads[0].sum().backward()
+
+
+def test_changed_in_place_is_refused(gpu_lib):
+    from model_amd.layer_norm import layer_norm
+
+    x, w, b, r, _, _ = _inputs(4, 32, torch.float32, add=True)
+    x.requires_grad_(True)
+    y, s = layer_norm(x, w, b, residual=r)
+    with torch.no_grad():
+        s.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
