@@ -679,23 +679,33 @@ __global__ __launch_bounds__(C::kThreads) void xent_grad_kernel(GradArgs p) {
 #undef MPL_STORE
 }
 
-// Adds the splits' sums in order; 4 values a thread.
+// Adds the splits' sums in order; VE values a thread (1 where n is no multiple
+// of 4, or small).
+template <int VE>
 __global__ __launch_bounds__(256) void xent_sum_kernel(const float* __restrict__ part, int splits, int64_t n,
                                                        void* __restrict__ out, int dtype) {
-  const bool vec = n % 4 == 0;
-  for (int64_t i = 4 * (blockIdx.x * 256 + (int64_t)threadIdx.x); i < n; i += 1024 * (int64_t)gridDim.x) {
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    const int m = (int)min(n - i, (int64_t)4);
-    for (int k = 0; k < splits; ++k) {
-      if (vec) {
-        const float4 v = *(const float4*)(part + k * n + i);
-        s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
-      } else {
-        for (int e = 0; e < m; ++e) s[e] += part[k * n + i + e];
-      }
-    }
-    for (int e = 0; e < m; ++e) store_as(out, i + e, s[e], dtype);
+  typedef float vec __attribute__((ext_vector_type(VE)));
+  const int64_t i = VE * (blockIdx.x * 256 + (int64_t)threadIdx.x);
+  if (i >= n) return;
+  vec s = 0.f;
+  int k = 0;
+  for (; k + 8 <= splits; k += 8) {  // 8 loads in flight
+    vec v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = *(const vec*)(part + (k + e) * n + i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += v[e];
   }
+  for (; k < splits; ++k) s += *(const vec*)(part + k * n + i);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) store_as(out, i + e, s[e], dtype);
+}
+
+void sum_splits(const float* part, int splits, int64_t n, void* out, int dtype, hipStream_t s) {
+  if (n % 4 == 0 && n >= (1 << 19))
+    xent_sum_kernel<4><<<(unsigned)cdiv(n, 1024), 256, 0, s>>>(part, splits, n, out, dtype);
+  else
+    xent_sum_kernel<1><<<(unsigned)cdiv(n, 256), 256, 0, s>>>(part, splits, n, out, dtype);
 }
 
 // --------------------------------------------------------------------- host
@@ -797,8 +807,10 @@ struct Call {
   int d;
 };
 
+// Grids are 32-bit: tiles of 128 x 128, and 2,048 elements a workgroup of a copy.
 bool sizes_ok(int64_t R, int64_t V, int d, int dtype) {
   return R >= 0 && V > 0 && d > 0 && d <= 65536 && R <= (1ll << 31) && V <= (1ll << 31) &&
+         cdiv(R, 128) * cdiv(V, 128) < (1ll << 31) && (R + V) * up(d, 64) / 2048 < (1ll << 31) - 2 &&
          (dtype == MPL_F32 || dtype == MPL_F16 || dtype == MPL_BF16);
 }
 
@@ -812,6 +824,9 @@ int check_call(const char* what, const Call& c, const void* ws, size_t ws_bytes,
     MPL_REQUIRE(((uintptr_t)c.hidden & 15) == 0 && ((uintptr_t)c.embedding & 15) == 0 && c.hidden_pitch % 8 == 0 &&
                     c.embedding_pitch % 8 == 0,
                 MPL_EINVAL, "%s: 16-bit rows of d %% 64 == 0 must be 16-byte aligned", what);
+  if (c.dtype != MPL_F32 && c.d % 64 == 0)  // 256 rows of a tile in 32 bits
+    MPL_REQUIRE(c.hidden_pitch < (1 << 23) && c.embedding_pitch < (1 << 23), MPL_EUNSUPPORTED,
+                "%s: 16-bit rows of d %% 64 == 0 must be less than 2^23 elements apart", what);
   MPL_REQUIRE(ws && ((uintptr_t)ws & 255) == 0, MPL_EINVAL, "%s: the workspace must be 256-byte aligned", what);
   MPL_REQUIRE(ws_bytes >= need, MPL_EWORKSPACE, "%s: workspace %zu < %zu bytes", what, ws_bytes, need);
   return MPL_OK;
@@ -1002,17 +1017,10 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
       const dim3 grid(g.tiles_m * g.tiles_n, g.splits);
       if (p.split) MPL_TILE(xent_grad_kernel, 2, false, true, true, p.big_e, grid, s, g);
       else MPL_TILE(xent_grad_kernel, 1, false, true, true, p.big_e, grid, s, g);
-      if (g.part) {
-        const int64_t n = nv * d;
-        xent_sum_kernel<<<(unsigned)std::min<int64_t>(cdiv(n, 1024), 4096), 256, 0, s>>>(g.part, g.splits, n,
-                                                                                           g.out, dtype);
-      }
+      if (g.part) sum_splits(g.part, g.splits, nv * d, g.out, dtype, s);
     }
   }
-  if (d_hidden && (p.splits_h > 1 || p.pieces > 1)) {
-    const int64_t n = rows * d;
-    xent_sum_kernel<<<(unsigned)std::min<int64_t>(cdiv(n, 1024), 4096), 256, 0, s>>>(
-        (const float*)(ws + p.ph), p.splits_h, n, d_hidden, dtype);
-  }
+  if (d_hidden && (p.splits_h > 1 || p.pieces > 1))
+    sum_splits((const float*)(ws + p.ph), p.splits_h, rows * d, d_hidden, dtype, s);
   return check_launch(what);
 }

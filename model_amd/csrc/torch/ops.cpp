@@ -191,10 +191,11 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& g_y, const 
 }
 
 // ---------------------------------------------------------- cross entropy
-// 16-bit rows that the tiles read as they lie (d a multiple of 64) start at 16 bytes.
+// 16-bit rows that the tiles read as they lie (d a multiple of 64) start at 16
+// bytes and are less than 2^23 elements apart.
 Rows operand_of(const Tensor& t, int64_t d) {
   Rows r = rows_of(t, d);
-  if (t.scalar_type() != at::kFloat && d % 64 == 0 && ((uintptr_t)r.data() % 16 || r.pitch % 8))
+  if (t.scalar_type() != at::kFloat && d % 64 == 0 && ((uintptr_t)r.data() % 16 || r.pitch % 8 || r.pitch >= (1 << 23)))
     return {r.t.clone(at::MemoryFormat::Contiguous), d};
   return r;
 }

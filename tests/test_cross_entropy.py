@@ -45,7 +45,7 @@ def test_workspace_bytes():
     big = L.mpl_vocab_cross_entropy_workspace_bytes(16384, 1 << 20, 1024, _lib.MPL_F16, 1)
     assert big < (1 << 30)
     for rows, vocab, d, dtype in ((-1, 4, 4, 0), (4, 0, 4, 0), (4, 4, 0, 0), (4, 4, 65537, 0), (4, 4, 4, 3),
-                                  ((1 << 31) + 1, 4, 4, 0)):
+                                  ((1 << 31) + 1, 4, 4, 0), (1 << 31, 1 << 20, 64, 0)):
         assert L.mpl_vocab_cross_entropy_workspace_bytes(rows, vocab, d, dtype, 0) == 0
 
 
@@ -71,6 +71,8 @@ def test_c_entries_validate_before_launch():
         assert f(h=None) == _lib.MPL_EINVAL and f(e=None) == _lib.MPL_EINVAL and f(t=None) == _lib.MPL_EINVAL
         assert f(hp=63) == _lib.MPL_EINVAL and b"pitch" in L.mpl_last_error()
         assert f(ep=68) == _lib.MPL_EINVAL and b"16-byte" in L.mpl_last_error()
+        assert f(hp=1 << 23) == _lib.MPL_EUNSUPPORTED and b"2^23" in L.mpl_last_error()
+        assert f(rows=1 << 31, vocab=1 << 31) == _lib.MPL_EINVAL
         assert f(h=ctypes.c_void_p(4098)) == _lib.MPL_EINVAL
         assert f(h=ctypes.c_void_p(4097), d=60) == _lib.MPL_EINVAL and b"elements" in L.mpl_last_error()
         assert f(ws=None) == _lib.MPL_EINVAL
