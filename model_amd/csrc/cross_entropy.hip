@@ -10,13 +10,29 @@
 //
 // Forward: tiles of z (tile_mma.h: the vocabulary down, tokens across, so a
 // lane's accumulators are one token's and its maximum and sum stay in
-// registers) end in one (maximum, sum of exp) pair a token and vocabulary
-// tile; a second launch joins the pairs in a fixed order.
+// registers) end in one (maximum, sum of 2^) pair a token and vocabulary tile;
+// a second launch joins the pairs in a fixed order.  Few tokens have a kernel of
+// their own (xent_rows_kernel).
 //
-// Backward: the vocabulary goes in pieces.  A piece's tiles of z are formed
-// again with the same instructions, so z has the forward's bits, and written
-// as dz in 16 bits (fp32 calls: hi and lo); two products read it from there.
-// A piece's dz is small enough to stay in the Infinity Cache.
+// Backward: the vocabulary goes in pieces of up to 512 MiB of dz.  A piece's
+// tiles of z are formed again from the same products and written as dz, fp16
+// under a power of two (fp32 calls: hi and lo); two products read it from there,
+// dz . embedding with its sums kept over the pieces, dz^T . hidden piece by
+// piece.  Forming z again is the fourth product of size rows x vocab x d where
+// three would do with the logits in memory.  dz is fp16 for bf16 calls too (their
+// operands go through fp16 under a power of two of their own, which holds bf16
+// exactly): 8 bits of dz would put an error of bf16's own rounding into the
+// gradients before they are rounded (2-norm error 1.45 times that of fp32 sums
+// rounded once; 1.0 so).
+//
+// Bound: the MFMAs.  At 16,384 x 131,072 x 1,024 bf16 the four products take 4.0,
+// 4.6, 3.6 and 3.4 ms (1,100, 955, 1,230 and 1,305 TFLOP/s; a library product
+// without the softmax reaches 1,210 there), 15.0 ms in all against 105 for the
+// formula in fp32 tensors.  What they lose is the epilogues at the end of each
+// tile, which no other wave of the CU covers (128 exp a lane, 3 us beside 26 us
+// of a tile at d = 1,024, and dz's bytes), and the copies of the operands
+// (0.2 ms).  fp32 calls run three fp16 products for one: 8,192 x 16,384 x 256 in
+// 0.86 ms (202, 284, 196 and 179 us the products), 2.70 in fp32 tensors.
 #include <math.h>
 
 #include <algorithm>
@@ -183,9 +199,9 @@ __global__ __launch_bounds__(256) void amax_kernel(PackArgs p, CoefArgs q) {
   };
   int64_t i = blockIdx.x * 256 + threadIdx.x;
   if (o.vec && o.pitch == p.d && p.d % VE == 0) {  // one long row
-    for (; i + 3 * step < n; i += 4 * step) {
+    for (; i + 7 * step < n; i += 8 * step) {  // 8 loads in flight
 #pragma unroll
-      for (int k = 0; k < 4; ++k) take(0, VE * (i + k * step), VE * n);
+      for (int k = 0; k < 8; ++k) take(0, VE * (i + k * step), VE * n);
     }
     for (; i < n; i += step) take(0, VE * i, VE * n);
   } else {
@@ -394,7 +410,8 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
 // and sum of 8 of the words.  fp32 rows go to v_mfma_f32_32x32x2_f32 as they
 // are: 4 products a vector, for which lanes of half h take dims 4h .. 4h + 3 of
 // each 8.  Bound: the table's bytes, and the fp32 products from some 100 tokens
-// on.
+// on.  One token of 16,384 x 256 fp32 6.6 us with 4.4 to join (tiles, with the
+// table's copy: 27); of 131,072 x 1,024 142 us, 3.8 TB/s of the table.
 struct RowsArgs {
   const void* E;
   const void* H;
