@@ -1007,7 +1007,8 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
       g.B = {a.E.base + a.v0 * a.E.pitch, a.E.pitch, nv, a.E.width};
       g.rows = rows, g.cols = d;
       g.iters = (int)(nvp * S / 64);
-      g.splits = p.splits_h;
+      // a short last piece has fewer stages than parts: the others' sums stand
+      g.splits = std::min(p.splits_h, g.iters);
       const int b = p.big_h ? 256 : 128;
       g.tiles_m = (uint32_t)cdiv(rows, b), g.tiles_n = (uint32_t)cdiv(d, b);
       g.u0 = scal + kInvP, g.u1 = a.scaled ? scal + kInvE : nullptr;

@@ -126,6 +126,22 @@ def test_many_tiles(gpu_lib, R, V, d, dtype):
         _near(name, got, want[name])
 
 
+@pytest.mark.parametrize("R,V,d,dtype", [(8192, 32768 + 100, 256, torch.bfloat16), (8192, 16384 + 37, 192, torch.float32),
+                                         (16384, 16384 + 300, 256, torch.float16)])
+def test_short_last_piece(gpu_lib, R, V, d, dtype):
+    """Two pieces of the vocabulary, the second with fewer stages than the
+    first's d hidden has parts."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    print(f"cross entropy, two pieces R={R} V={V} d={d} {dtype}", flush=True)
+    h, e, t, gl, _ = _inputs(R, V, d, dtype)
+    t[:50] = V - 1
+    want = _formula(h, e, t, gl, None)
+    loss, lse, dh, de = vocab_cross_entropy_grads(h, e, t, gl)
+    for name, got in (("loss", loss), ("lse", lse), ("dh", dh), ("de", de)):
+        _near(name, got, want[name])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_autograd_equals_direct(gpu_lib, dtype):
     from model_amd.cross_entropy import vocab_cross_entropy, vocab_cross_entropy_grads
