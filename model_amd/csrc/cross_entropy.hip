@@ -293,6 +293,13 @@ struct LogitArgs {
   bool stream;  // dz is written past the caches
 };
 
+// What accumulators are multiplied by to give z: finite and not 0, so that a
+// masked -inf and an exact 0 stay what they are where both arrays lie at an end
+// of fp32's range.
+__device__ __forceinline__ float unscale_z(const LogitArgs& p) {
+  return p.scaled ? fminf(fmaxf(p.scal[kInvE] * p.scal[kInvH], 1.17549435e-38f), 1e38f) : 1.f;
+}
+
 #define MPL_TILE_LDS(C)                                      \
   __shared__ __attribute__((aligned(1024))) char a0[C::kStageA]; \
   __shared__ __attribute__((aligned(1024))) char b0[C::kStageB]; \
@@ -310,7 +317,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
   f32x16 acc[C::TM][C::TN];
   C::run(p.E, p.H, v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
   // z log2(e) = acc * unit: one multiply and add before each exp2
-  const float unscale = p.scaled ? p.scal[kInvE] * p.scal[kInvH] : 1.f, unit = unscale * kLog2e;
+  const float unscale = unscale_z(p), unit = unscale * kLog2e;
   const int64_t vw = v0 + wm * C::TM * 32 + 4 * (lane >> 5);  // of acc[0][.][0]
   float2* pair = (float2*)a0;  // [WM][BN]: the stages are free
 #pragma unroll
@@ -524,7 +531,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
   const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
   f32x16 acc[C::TM][C::TN];
   C::run(p.E, p.H, p.v0 + v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
-  const float unit = (p.scaled ? p.scal[kInvE] * p.scal[kInvH] : 1.f) * kLog2e;
+  const float unit = unscale_z(p) * kLog2e;
   const float up = p.scal[kScaleP];
   const int half = lane >> 5;
   const int64_t vw = v0 + wm * C::TM * 32;  // the wave's first column of the piece
@@ -750,7 +757,6 @@ constexpr int64_t kPieceBytes = 512ll << 20;
 // 131,072 x 1,024: 142 / 524, 404 / 531, 602 / 536.  bf16: 1, 32 tokens of
 // 131,072 x 1,024: 53 / 62, 79 / 64; of 50,021 x 500: 22 / 44, 28 / 45, 64: 43 / 45.
 inline int64_t few_rows(int d, int dtype) { return dtype == MPL_F32 || d % 64 ? 64 : 16; }
-
 
 inline int64_t up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
 

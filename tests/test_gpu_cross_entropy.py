@@ -142,6 +142,23 @@ def test_short_last_piece(gpu_lib, R, V, d, dtype):
         _near(name, got, want[name])
 
 
+@pytest.mark.parametrize("h_size,e_size", [(1e-25, 1e-25), (0.0, 1e-25), (1e-30, 1e30), (0.0, 0.0)])
+@pytest.mark.parametrize("R", [5, 70, 300])
+def test_ends_of_fp32(gpu_lib, R, h_size, e_size):
+    """Arrays whose powers of two multiply to less than fp32 holds: logits of 0."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    h, e, t, gl, _ = _inputs(R, 300, 64, torch.float32)
+    h, e = h / h.abs().max() * h_size, e / e.abs().max() * e_size
+    if h_size * e_size < 1e-20:  # else ordinary logits
+        loss, lse, dh, de = vocab_cross_entropy_grads(h, e, t, gl)
+        assert (lse - math.log(300)).abs().max() <= 2 ** -20 * 7
+        assert torch.isfinite(dh).all() and torch.isfinite(de).all()
+    want = _formula(h, e, t, gl, None)
+    for name, got in zip(("loss", "lse", "dh", "de"), vocab_cross_entropy_grads(h, e, t, gl)):
+        _near(name, got, want[name])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_autograd_equals_direct(gpu_lib, dtype):
     from model_amd.cross_entropy import vocab_cross_entropy, vocab_cross_entropy_grads
