@@ -177,4 +177,3 @@ def stream_ptr(device) -> int:
     if type(device) is torch.device and device.index is not None:
         _stream_index[device] = device.index
     return stream
-

@@ -19,6 +19,7 @@ import torch
 from . import _lib
 
 _DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+MAX_WIDTH = 65536
 
 
 def _check(hidden: torch.Tensor, embedding: torch.Tensor, targets: torch.Tensor, what: str) -> None:
@@ -27,6 +28,8 @@ def _check(hidden: torch.Tensor, embedding: torch.Tensor, targets: torch.Tensor,
                          "([..., d] and [vocab, d])")
     if embedding.shape[0] == 0 or embedding.shape[1] == 0:
         raise ValueError(f"{what}: an empty embedding {tuple(embedding.shape)}")
+    if embedding.shape[1] > MAX_WIDTH:
+        raise ValueError(f"{what}: rows of {embedding.shape[1]} elements, at most {MAX_WIDTH}")
     if targets.shape != hidden.shape[:-1]:
         raise ValueError(f"{what}: targets {tuple(targets.shape)} for hidden {tuple(hidden.shape)}")
     if targets.dtype not in (torch.int64, torch.int32):
@@ -67,7 +70,9 @@ def vocab_cross_entropy(hidden: torch.Tensor, embedding: torch.Tensor, targets: 
     counted tokens is loss.sum() / (targets != ignore_index).sum().
 
     Logits are sums in fp32 of the exact products (fp32 operands are held to
-    2^-23 of each).  fp32 rows or table entries that are not finite give NaN.
+    2^-23 of each).  fp32 rows or table entries that are not finite may give NaN
+    where the formula has a logit of -inf.  Up to some 2^39 logits and 2^34
+    elements of both arrays.
     The gradients hold dz in fp16 under a power of two (fp32: hi and lo, to
     2^-23), down to 2^-38 of the largest gradient of a token.  For gradients
     inside a captured HIP graph use vocab_cross_entropy_grads."""

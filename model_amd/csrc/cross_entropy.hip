@@ -709,27 +709,27 @@ template <int VE>
 __global__ __launch_bounds__(256) void xent_sum_kernel(const float* __restrict__ part, int splits, int64_t n,
                                                        void* __restrict__ out, int dtype) {
   typedef float vec __attribute__((ext_vector_type(VE)));
-  const int64_t i = VE * (blockIdx.x * 256 + (int64_t)threadIdx.x);
-  if (i >= n) return;
-  vec s = 0.f;
-  int k = 0;
-  for (; k + 8 <= splits; k += 8) {  // 8 loads in flight
-    vec v[8];
+  for (int64_t i = VE * (blockIdx.x * 256 + (int64_t)threadIdx.x); i < n; i += VE * 256 * (int64_t)gridDim.x) {
+    vec s = 0.f;
+    int k = 0;
+    for (; k + 8 <= splits; k += 8) {  // 8 loads in flight
+      vec v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = *(const vec*)(part + (k + e) * n + i);
+      for (int e = 0; e < 8; ++e) v[e] = *(const vec*)(part + (k + e) * n + i);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += v[e];
+      for (int e = 0; e < 8; ++e) s += v[e];
+    }
+    for (; k < splits; ++k) s += *(const vec*)(part + k * n + i);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) store_as(out, i + e, s[e], dtype);
   }
-  for (; k < splits; ++k) s += *(const vec*)(part + k * n + i);
-#pragma unroll
-  for (int e = 0; e < VE; ++e) store_as(out, i + e, s[e], dtype);
 }
 
 void sum_splits(const float* part, int splits, int64_t n, void* out, int dtype, hipStream_t s) {
   if (n % 4 == 0 && n >= (1 << 19))
     xent_sum_kernel<4><<<(unsigned)cdiv(n, 1024), 256, 0, s>>>(part, splits, n, out, dtype);
   else
-    xent_sum_kernel<1><<<(unsigned)cdiv(n, 256), 256, 0, s>>>(part, splits, n, out, dtype);
+    xent_sum_kernel<1><<<(unsigned)std::min<int64_t>(cdiv(n, 256), 1 << 20), 256, 0, s>>>(part, splits, n, out, dtype);
 }
 
 // --------------------------------------------------------------------- host
@@ -830,10 +830,12 @@ struct Call {
   int d;
 };
 
-// Grids are 32-bit: tiles of 128 x 128, and 2,048 elements a workgroup of a copy.
+// A grid has less than 2^32 threads: 512 for a tile of 256 x 256, one for 8
+// elements of a copy, for 4 of the sums (or for one, in turns), 8 for a token of
+// the join.
 bool sizes_ok(int64_t R, int64_t V, int d, int dtype) {
   return R >= 0 && V > 0 && d > 0 && d <= 65536 && R <= (1ll << 31) && V <= (1ll << 31) &&
-         cdiv(R, 128) * cdiv(V, 128) < (1ll << 31) && (R + V) * up(d, 64) / 2048 < (1ll << 31) - 2 &&
+         cdiv(R, 256) * cdiv(V, 256) < (1ll << 23) && (R + V) * up(d, 64) < (1ll << 34) &&
          (dtype == MPL_F32 || dtype == MPL_F16 || dtype == MPL_BF16);
 }
 

@@ -49,6 +49,26 @@ def test_workspace_bytes():
         assert L.mpl_vocab_cross_entropy_workspace_bytes(rows, vocab, d, dtype, 0) == 0
 
 
+@pytest.mark.parametrize("rows,vocab,d,ok", [
+    (1 << 20, 1 << 18, 1024, True),  # 2^22 tiles
+    (1 << 20, 1 << 19, 1024, False),  # 2^23: 2^32 threads of the tiles' grid
+    (1 << 19, 1 << 19, 16384, False),  # 2^34 elements: 2^32 threads of the sums
+    ((1 << 19) - 1, 1 << 19, 16384, True),
+    (1 << 29, 1, 1, False)])  # 2^32 threads of the join
+def test_largest_sizes(rows, vocab, d, ok):
+    L = _lib.lib()
+    for dtype in (_lib.MPL_F32, _lib.MPL_F16, _lib.MPL_BF16):
+        for backward in (0, 1):
+            assert (L.mpl_vocab_cross_entropy_workspace_bytes(rows, vocab, d, dtype, backward) > 0) == ok
+
+
+def test_width_does_not_wrap():
+    d = (1 << 32) + 64
+    t = [torch.empty(1, d, device="meta", dtype=torch.float16) for _ in range(2)]
+    with pytest.raises(ValueError, match="at most 65536"):
+        vocab_cross_entropy(*t, torch.zeros(1, dtype=torch.int64, device="meta"))
+
+
 def test_c_entries_validate_before_launch():
     L = _lib.lib()
     one = ctypes.c_void_p(4096)  # never read: every call below is refused
