@@ -431,3 +431,131 @@ def test_second_derivative_is_refused(gpu_lib):
     assert torch.equal(g.detach(), plain)
     with pytest.raises(RuntimeError, match="differentiable once"):
         g.sum().backward()
+
+
+def _far(x, pitch):
+    """x with its rows `pitch` elements apart, in a buffer of more than 2^32 bytes."""
+    out = torch.empty(x.shape[0] * pitch, dtype=x.dtype, device="cuda").reshape(x.shape[0], pitch)[:, :x.shape[1]]
+    out.copy_(x)
+    return out
+
+
+@pytest.mark.parametrize("dtype,R,d", [(torch.float32, 5, 40), (torch.float32, 300, 40), (torch.float16, 300, 128),
+                                       (torch.bfloat16, 9, 128), (torch.bfloat16, 300, 70)])
+def test_offsets_past_32_bits(gpu_lib, dtype, R, d):
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    print(f"cross entropy, far rows R={R} d={d} {dtype}", flush=True)
+    h, e, t, gl, gs = _inputs(R, 300, d, dtype)
+    want = vocab_cross_entropy_grads(h, e, t, gl, gs)
+    pitch = 1 << 22 if dtype == torch.float32 else (1 << 23) - 8
+    far_e = _far(e, pitch)
+    assert 299 * pitch * e.element_size() > 1 << 32
+    for x, y in zip(vocab_cross_entropy_grads(h, far_e, t, gl, gs), want):
+        assert torch.equal(x, y)
+    if R == 300:
+        far_h = _far(h, pitch)
+        for x, y in zip(vocab_cross_entropy_grads(far_h, far_e, t, gl, gs), want):
+            assert torch.equal(x, y)
+
+
+def test_table_past_2_32_elements(gpu_lib):
+    """The last words of a table of more than 2^32 elements: the others are zeros, logits of 0."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    V, d, R = (1 << 24) + 300, 256, 20
+    print(f"cross entropy, V={V} d={d}", flush=True)
+    h, small, t, gl, gs = _inputs(R, 300, d, torch.bfloat16, ignored=0.0)
+    e = torch.zeros((V, d), dtype=torch.bfloat16, device="cuda")
+    e[-300:] = small
+    loss, lse, dh, de = vocab_cross_entropy_grads(h, e, t + (1 << 24), gl, gs)
+    H, E = h.double(), small.double()
+    z = H @ E.t()
+    ref = torch.logsumexp(torch.cat([z, torch.full((R, 1), math.log(V - 300), device="cuda", dtype=torch.float64)], 1), 1)
+    at = t[:, None]
+    z_tol = d * 2.0 ** -24 * (H.abs() @ E.abs().t()) + 2.0 ** -39 * (
+        E.abs().max() * H.abs().sum(1)[:, None] + H.abs().max() * E.abs().sum(1)[None])
+    lse_tol = z_tol.amax(1) + 2.0 ** -20 * (1 + ref)
+    _near("lse", lse, (ref, lse_tol))
+    _near("loss", loss, (ref - z.gather(1, at)[:, 0], 2 * lse_tol))
+    # the gradients of the last words; the zeros add nothing to dh, and get the sum of their own dz
+    g, a = gl.double(), (gl + gs).double()
+    most = max(g.abs().max().item(), a.abs().max().item())
+    p = torch.exp(z - ref[:, None]) * a[:, None]
+    dz = p.scatter_add(1, at, -g[:, None])
+    dz_tol = p.abs() * (z_tol + lse_tol[:, None] + 2.0 ** -20) + dz.abs() * 2.0 ** -11 + 2.0 ** -38 * most
+    zero = torch.exp(-ref) * a
+    zero_tol = zero.abs() * (lse_tol + 2.0 ** -20 + 2.0 ** -11) + 2.0 ** -38 * most
+
+    def product(x, x_tol, y, K):
+        out = x @ y
+        return out, ((x_tol + K * 2.0 ** -24 * x.abs()) @ y.abs() + 2.0 ** -39 * y.abs().max() * x.abs().sum(-1, keepdim=True)
+                     + 2.0 ** -8 * out.abs())
+
+    _near("dh", dh, product(dz, dz_tol, E, 300))
+    _near("de", de[-300:], product(dz.t().contiguous(), dz_tol.t().contiguous(), H, R))
+    for row in (0, 1 << 20, (1 << 24) - 1):
+        _near("de of zeros", de[row], product(zero, zero_tol, H, R))
+
+
+def test_one_tensor_as_both(gpu_lib):
+    """The table's own rows as hidden: both gradients reach the one leaf."""
+    from model_amd.cross_entropy import vocab_cross_entropy, vocab_cross_entropy_grads
+
+    _, e, _, _, _ = _inputs(1, 200, 96, torch.float32)
+    t = torch.arange(200, device="cuda")
+    gl = torch.linspace(-1, 1, 200, device="cuda")
+    leaf = e.clone().requires_grad_()
+    vocab_cross_entropy(leaf, leaf, t).backward(gl)
+    _, _, dh, de = vocab_cross_entropy_grads(e, e, t, gl)
+    assert torch.equal(leaf.grad, dh + de)
+
+
+def test_two_threads(gpu_lib):
+    """Autograd steps in two threads, each on a stream of its own."""
+    import threading
+
+    from model_amd.cross_entropy import vocab_cross_entropy, vocab_cross_entropy_grads
+
+    args = [_inputs(500, 3000, 128, torch.float16, seed=s) for s in (3, 4)]
+    want = [vocab_cross_entropy_grads(h, e, t, gl) for h, e, t, gl, _ in args]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        h, e, t, gl, _ = args[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(8):
+                a, b = h.clone().requires_grad_(), e.clone().requires_grad_()
+                loss = vocab_cross_entropy(a, b, t)
+                loss.backward(gl)
+            torch.cuda.current_stream().synchronize()
+            got[i] = (loss.detach(), a.grad, b.grad)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    for (loss, _, dh, de), g in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip((loss, dh, de), g))
+
+
+def test_memory_is_freed(gpu_lib):
+    from model_amd.cross_entropy import vocab_cross_entropy
+
+    h, e, t, gl, _ = _inputs(300, 3000, 128, torch.bfloat16)
+    h.requires_grad_(), e.requires_grad_()
+
+    def step(backward):
+        loss, lse = vocab_cross_entropy(h, e, t, return_lse=True)
+        if backward:
+            (loss + lse).sum().backward()
+            h.grad = e.grad = None
+
+    used = []
+    for i in range(6):
+        step(i % 2)
+        torch.cuda.synchronize()
+        used.append(torch.cuda.memory_allocated())
+    assert used[4] == used[2] and used[5] == used[3]

@@ -337,3 +337,95 @@ def test_changed_in_place_is_refused(gpu_lib):
         s.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 40), (torch.bfloat16, 1000), (torch.float16, 3001)])
+def test_offsets_past_32_bits(gpu_lib, dtype, d):
+    """Rows 16 MiB apart, in buffers of more than 2^32 bytes."""
+    print(f"layer norm, far rows d={d} {dtype}", flush=True)
+    R, pitch = 300, 1 << (22 if dtype == torch.float32 else 23)
+    x, w, b, r, gy, gs = _inputs(R, d, dtype, add=True)
+    want, s = _run(x, w, b, r, gy, gs)
+
+    def far(t):
+        out = torch.empty(R * pitch, dtype=dtype, device="cuda").reshape(R, pitch)[:, :d]
+        return out.copy_(t)
+
+    got, s2 = _run(far(x), w, b, far(r), far(gy), far(gs))
+    assert torch.equal(s2, s)
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+
+
+def test_more_than_2_31_elements(gpu_lib):
+    """Rows stand alone, so the last of many are those of a small call."""
+    from model_amd.layer_norm import layer_norm_backward, layer_norm_forward
+
+    R, d, n = (1 << 17) + 5, 16384, 7
+    print(f"layer norm, R={R} d={d}", flush=True)
+    x, w, b, _, gy, _ = _inputs(n, d, torch.bfloat16)
+    many = torch.zeros((R, d), dtype=torch.bfloat16, device="cuda")
+    grad = torch.zeros_like(many)
+    many[-n:], grad[-n:] = x, gy
+    y, s, mean, rstd = layer_norm_forward(many, w, b)
+    dx, ds, db = layer_norm_backward(grad, s, w, mean, rstd)
+    y1, s1, mean1, rstd1 = layer_norm_forward(x, w, b)
+    dx1, ds1, db1 = layer_norm_backward(gy, s1, w, mean1, rstd1)
+    for a, c in ((y, y1), (mean, mean1), (rstd, rstd1), (dx, dx1)):
+        assert torch.equal(a[-n:], c)
+    # the other rows pass no gradient to the parameters: sums of n terms in another order
+    hat = (x.double() - mean1.double()[:, None]) * rstd1.double()[:, None]
+    for got, ref, size in ((ds, gy.double() * hat, 1), (ds1, gy.double() * hat, 1), (db, gy.double(), 0), (db1, gy.double(), 0)):
+        assert ((got.double() - ref.sum(0)).abs() <= (n + 4) * 2.0 ** -24 * ref.abs().sum(0) + size * 2.0 ** -126).all()
+
+
+def test_one_tensor_as_rows_and_residual(gpu_lib):
+    """x as its own residual: the sum's gradient reaches it twice."""
+    from model_amd.layer_norm import layer_norm, layer_norm_backward, layer_norm_forward
+
+    x, w, b, _, gy, gs = _inputs(50, 200, torch.float32, add=True)
+    leaf = x.clone().requires_grad_()
+    y, s = layer_norm(leaf, w, b, residual=leaf)
+    torch.autograd.backward([y, s], [gy, gs])
+    _, total, mean, rstd = layer_norm_forward(x, w, b, residual=x)
+    dx, _, _ = layer_norm_backward(gy, total, w, mean, rstd, g_residual=gs)
+    assert torch.equal(leaf.grad, dx + dx)
+
+
+def test_residual_gradients_are_apart(gpu_lib):
+    """x and the residual get gradients that one may change without the other."""
+    from model_amd.layer_norm import layer_norm
+
+    for only_sum in (False, True):
+        x, w, b, r, gy, gs = _inputs(20, 64, torch.float32, add=True)
+        x.requires_grad_(), r.requires_grad_()
+        y, s = layer_norm(x, w, b, residual=r)
+        if only_sum:
+            s.backward(gs)
+        else:
+            torch.autograd.backward([y, s], [gy, gs])
+        want = r.grad.clone()
+        assert torch.equal(x.grad, want)
+        x.grad.zero_()
+        assert torch.equal(r.grad, want)
+
+
+def test_memory_is_freed(gpu_lib):
+    from model_amd.layer_norm import layer_norm
+
+    x, w, b, r, _, _ = _inputs(300, 512, torch.float32, add=True)
+    for t in (x, w, b, r):
+        t.requires_grad_()
+
+    def step(backward):
+        y, s = layer_norm(x, w, b, residual=r)
+        if backward:
+            (y + s).sum().backward()
+            x.grad = w.grad = b.grad = r.grad = None
+
+    used = []
+    for i in range(6):
+        step(i % 2)
+        torch.cuda.synchronize()
+        used.append(torch.cuda.memory_allocated())
+    assert used[4] == used[2] and used[5] == used[3]
