@@ -784,7 +784,8 @@ int mpl_layer_norm_bwd(const void* dy, int64_t dy_pitch, const void* x, int64_t 
  * g_loss 0 where ignored, held in fp16 between the products (fp32: hi + lo, 2^-23
  * of each) under a power of two that leaves 2^-38 of the largest |g_loss| or
  * |g_loss + g_lse|.  bf16 operands are read as fp16 under a power of two of each
- * array there, exact above 2^-29 of its largest.  rows > 0.  A row of an invalid
+ * array there, exact above 2^-29 of its largest.  Up to 64 rows (fewer in 16 bits)
+ * may keep dz and the operands of its products in fp32 instead.  rows > 0.  A row of an invalid
  * target makes both gradients NaN.
  *
  * The workspace (256-byte aligned) takes mpl_vocab_cross_entropy_workspace_bytes

@@ -74,7 +74,8 @@ def vocab_cross_entropy(hidden: torch.Tensor, embedding: torch.Tensor, targets: 
     where the formula has a logit of -inf.  Up to some 2^39 logits and 2^34
     elements of both arrays.
     The gradients hold dz in fp16 under a power of two (fp32: hi and lo, to
-    2^-23), down to 2^-38 of the largest gradient of a token.  For gradients
+    2^-23), down to 2^-38 of the largest gradient of a token, those of few
+    tokens (64 in fp32) in fp32.  For gradients
     inside a captured HIP graph use vocab_cross_entropy_grads."""
     _check(hidden, embedding, targets, "vocab_cross_entropy")
     autograd = torch.is_grad_enabled() and (hidden.requires_grad or embedding.requires_grad)

@@ -23,7 +23,8 @@
 // operands go through fp16 under a power of two of their own, which holds bf16
 // exactly): 8 bits of dz would put an error of bf16's own rounding into the
 // gradients before they are rounded (2-norm error 1.45 times that of fp32 sums
-// rounded once; 1.0 so).
+// rounded once; 1.0 so).  Few tokens keep dz in fp32, by the same kernel as their
+// forward, and one pass over the table makes both gradients (xent_few_kernel).
 //
 // Bound: the MFMAs.  At 16,384 x 131,072 x 1,024 bf16 the four products take 4.0,
 // 4.6, 3.6 and 3.4 ms (1,100, 955, 1,230 and 1,305 TFLOP/s; a library product
@@ -416,8 +417,9 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
 // their sums of z meet in LDS, from where each wave keeps the running maximum
 // and sum of 8 of the words.  fp32 rows go to v_mfma_f32_32x32x2_f32 as they
 // are: 4 products a vector, for which lanes of half h take dims 4h .. 4h + 3 of
-// each 8.  Bound: the table's bytes, and the fp32 products from some 100 tokens
-// on.  One token of 16,384 x 256 fp32 6.6 us with 4.4 to join (tiles, with the
+// each 8.  Two blocks of 32 tokens share the table's vectors (64 tokens of
+// 131,072 x 1,024 fp32 406 -> 260 us), and LDS with a second barrier.  Bound: the
+// table's bytes, and the fp32 products from some 100 tokens on.  One token of 16,384 x 256 fp32 6.6 us with 4.4 to join (tiles, with the
 // table's copy: 27); of 131,072 x 1,024 142 us, 3.8 TB/s of the table.
 struct RowsArgs {
   const void* E;
@@ -427,6 +429,12 @@ struct RowsArgs {
   const int64_t* target;
   float2* part;  // [workgroups][R]
   float* z_target;
+  // backward
+  const float* lse;
+  const float* g_loss;
+  const float* g_lse;
+  int64_t ignore;
+  float* dz;  // [group][32 words][TOK tokens], then as much of [group][TOK tokens][32 words]
 };
 
 template <typename T>
@@ -440,24 +448,41 @@ __device__ __forceinline__ uint4 row_vector(const T* row, int at, int d) {
   return *(const uint4*)v;
 }
 
-template <typename T>
+// BWD: z becomes dz, in both orders that the products with it read.  NT: blocks
+// of 32 tokens.
+template <typename T, int NT, bool BWD>
 __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs p) {
-  constexpr int VE = 16 / sizeof(T);
-  __shared__ float s[2][4][16][64];
+  constexpr int VE = 16 / sizeof(T), TOK = 32 * NT, kBuffers = NT == 1 ? 2 : 1;
+  constexpr int kAhead = NT == 1 ? 8 : 4;
+  __shared__ float s[kBuffers][NT][4][16][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int64_t tok = blockIdx.y * 32 + col;
-  const T* h = (const T*)p.H + min(tok, p.R - 1) * p.h_pitch;
-  const int64_t to = p.target[min(tok, p.R - 1)];
+  const T* h[NT];
+  int64_t to[NT];
+  float m[NT], l[NT], all[NT], gt[NT], lse[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int64_t tok = 32 * n + col, at = min(tok, p.R - 1);
+    h[n] = (const T*)p.H + at * p.h_pitch;
+    to[n] = p.target[at];
+    m[n] = -INFINITY, l[n] = 0.f;
+    if constexpr (BWD) {
+      gt[n] = to[n] == p.ignore || !p.g_loss ? 0.f : p.g_loss[at];
+      if (to[n] != p.ignore && (to[n] < 0 || to[n] >= p.V)) gt[n] = NAN;
+      all[n] = gt[n] + (p.g_lse ? p.g_lse[at] : 0.f);
+      lse[n] = p.lse[at] * kLog2e;
+    }
+  }
   const int chunks = (p.d + 2 * VE - 1) / (2 * VE);
   const int c0 = chunks * wave / 4, c1 = chunks * (wave + 1) / 4;
   const int64_t groups = (p.V + 31) / 32;
-  float m = -INFINITY, l = 0.f;
   int turn = 0;
-  for (int64_t g = blockIdx.x; g < groups; g += gridDim.x, turn ^= 1) {
+  for (int64_t g = blockIdx.x; g < groups; g += gridDim.x, turn = kBuffers - 1 - turn) {
     const T* e = (const T*)p.E + min(32 * g + col, p.V - 1) * p.e_pitch;
-    f32x16 acc = f32x16{};
-    auto product = [&](uint4 a, uint4 b) __attribute__((always_inline)) {
+    f32x16 acc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n] = f32x16{};
+    auto product = [&](uint4 a, uint4 b, f32x16& acc) __attribute__((always_inline)) {
       if constexpr (sizeof(T) == 4) {
         acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), acc, 0, 0, 0);
@@ -472,49 +497,80 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs p) {
       }
     };
     int c = c0;
-    for (; c + 8 <= c1 && (c + 8) * 2 * VE <= p.d; c += 8) {
-      uint4 a[8], b[8];
+    for (; c + kAhead <= c1 && (c + kAhead) * 2 * VE <= p.d; c += kAhead) {
+      uint4 a[kAhead], b[NT][kAhead];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) a[k] = row_vector(e, VE * (2 * (c + k) + half), 0x7FFFFFFF);
+      for (int k = 0; k < kAhead; ++k) a[k] = row_vector(e, VE * (2 * (c + k) + half), 0x7FFFFFFF);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) b[k] = row_vector(h, VE * (2 * (c + k) + half), 0x7FFFFFFF);
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) product(a[k], b[k]);
+        for (int k = 0; k < kAhead; ++k) b[n][k] = row_vector(h[n], VE * (2 * (c + k) + half), 0x7FFFFFFF);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) product(a[k], b[n][k], acc[n]);
     }
-    for (; c < c1; ++c) product(row_vector(e, VE * (2 * c + half), p.d), row_vector(h, VE * (2 * c + half), p.d));
+    for (; c < c1; ++c) {
+      const uint4 a = row_vector(e, VE * (2 * c + half), p.d);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[turn][wave][r][lane] = acc[r];
-    __syncthreads();  // the other half of s is written next: no second barrier
-    float z[4], n = m;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 4 * wave + i;
-      z[i] = ((s[turn][0][r][lane] + s[turn][1][r][lane]) + s[turn][2][r][lane]) + s[turn][3][r][lane];
-      const int64_t v = 32 * g + 8 * wave + 4 * half + i;
-      if (v == to && tok < p.R) p.z_target[tok] = z[i];
-      z[i] = v < p.V ? z[i] * kLog2e : -INFINITY;
-      n = fmaxf(n, z[i]);
+      for (int n = 0; n < NT; ++n) product(a, row_vector(h[n], VE * (2 * c + half), p.d), acc[n]);
     }
-    const float ref = n == -INFINITY ? 0.f : n;
-    l *= __builtin_amdgcn_exp2f(m - ref);
+    if (kBuffers == 1) __syncthreads();  // with two, the other one is written next
 #pragma unroll
-    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(z[i] - ref);
-    m = n;
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[turn][n][wave][r][lane] = acc[n][r];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int64_t tok = 32 * n + col;
+      const float (*z4)[16][64] = s[turn][n];
+      float z[4], most = m[n];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * wave + i;
+        z[i] = ((z4[0][r][lane] + z4[1][r][lane]) + z4[2][r][lane]) + z4[3][r][lane];
+        const int64_t v = 32 * g + 8 * wave + 4 * half + i;
+        if constexpr (BWD) {
+          z[i] = all[n] * __builtin_amdgcn_exp2f(fmaf(z[i], kLog2e, -lse[n])) - (v == to[n] ? gt[n] : 0.f);
+          z[i] = v < p.V && tok < p.R ? z[i] : 0.f;
+          p.dz[(g * 32 + 8 * wave + 4 * half + i) * TOK + tok] = z[i];
+        } else {
+          if (v == to[n] && tok < p.R) p.z_target[tok] = z[i];
+          z[i] = v < p.V ? z[i] * kLog2e : -INFINITY;
+          most = fmaxf(most, z[i]);
+        }
+      }
+      if constexpr (BWD) {
+        *(float4*)(p.dz + (groups * 32 + g * 32) * TOK + tok * 32 + 8 * wave + 4 * half) =
+            make_float4(z[0], z[1], z[2], z[3]);
+      } else {
+        const float ref = most == -INFINITY ? 0.f : most;
+        l[n] *= __builtin_amdgcn_exp2f(m[n] - ref);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[n] += __builtin_amdgcn_exp2f(z[i] - ref);
+        m[n] = most;
+      }
+    }
   }
-  // the token's 8 pairs: two halves of four waves
-  __shared__ float2 pair[4][64];
-  pair[wave][lane] = make_float2(m, l);
-  __syncthreads();
-  if (threadIdx.x >= 32 || tok >= p.R) return;
-  float n = -INFINITY, sum = 0.f;
+  if constexpr (!BWD) {
+    // a token's 8 pairs: two halves of four waves
+    __shared__ float2 pair[4][NT][64];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) n = fmaxf(n, fmaxf(pair[w][lane].x, pair[w][lane + 32].x));
-  const float ref = n == -INFINITY ? 0.f : n;
+    for (int n = 0; n < NT; ++n) pair[wave][n][lane] = make_float2(m[n], l[n]);
+    __syncthreads();
+    const int n = threadIdx.x >> 5, tok = threadIdx.x;
+    if (n >= NT || tok >= p.R) return;
+    float most = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w)
-    sum += pair[w][lane].y * __builtin_amdgcn_exp2f(pair[w][lane].x - ref) +
-           pair[w][lane + 32].y * __builtin_amdgcn_exp2f(pair[w][lane + 32].x - ref);
-  p.part[(int64_t)blockIdx.x * p.R + tok] = make_float2(n, sum);
+    for (int w = 0; w < 4; ++w) most = fmaxf(most, fmaxf(pair[w][n][col].x, pair[w][n][col + 32].x));
+    const float ref = most == -INFINITY ? 0.f : most;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      sum += pair[w][n][col].y * __builtin_amdgcn_exp2f(pair[w][n][col].x - ref) +
+             pair[w][n][col + 32].y * __builtin_amdgcn_exp2f(pair[w][n][col + 32].x - ref);
+    p.part[(int64_t)blockIdx.x * p.R + tok] = make_float2(most, sum);
+  }
 }
 
 // ----------------------------------------------------------------- backward
@@ -703,6 +759,167 @@ __global__ __launch_bounds__(C::kThreads) void xent_grad_kernel(GradArgs p) {
 #undef MPL_STORE
 }
 
+// Few tokens' gradients: the table is read once more, and its gradient written,
+// in one pass with v_mfma_f32_32x32x2_f32.  A wave has 128 columns, 4 next to
+// each other a lane: their hidden rows stay in registers, and so do its sums of
+// d hidden over the groups of 32 words that it walks.  Lanes of half h take words
+// (and tokens) 8 m + 4 h + t at step (m, t) of a contraction.  At the end of a
+// ragged row lanes take the last 4 columns again, and the same values.  Parts of
+// d hidden are added by the next launch, in a fixed order.
+//
+// Bound: the table read and its gradient written; 1 and 32 tokens of 131,072 x
+// 1,024 fp32 212 and 203 us (5.1 TB/s, what a large copy reaches), 64 tokens 328;
+// 16 bits 145, 215 (2.5 TB/s: the fp32 products, at one wave a SIMD).  Two columns
+// a lane and two waves a SIMD were slower (fp32, 1 and 32 tokens 265 and 298), as
+// were two waves with rows widened at each use (16 bits 303 and 368: spills).
+struct FewArgs {
+  const void* E;
+  const void* H;
+  int64_t e_pitch, h_pitch, R, V;
+  int d;
+  const float* dz;  // as RowsArgs
+  void* de;         // or null
+  float* part;      // [workgroups.x][R][d], or null
+};
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+// 4 elements of any alignment, kept as they are until a product takes them.
+template <typename T>
+struct Four {
+  typedef T vec __attribute__((ext_vector_type(4)));
+  typedef T any __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  vec v;
+  __device__ __forceinline__ void load(const T* q) { v = *(const any*)q; }
+  __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
+  __device__ static __forceinline__ void store(T* q, f4 x) { *(any*)q = __builtin_convertvector(x, vec); }
+};
+
+template <typename T, int NT>
+__global__ __launch_bounds__(64) void xent_few_kernel(FewArgs p) {
+  constexpr int TOK = 32 * NT;
+  const int lane = threadIdx.x, col = lane & 31, half = lane >> 5;
+  const int c0 = min((int)blockIdx.y * 128 + 4 * col, p.d - 4);
+  const bool owns = (int)blockIdx.y * 128 + 4 * col < p.d;
+  const int64_t groups = (p.V + 31) / 32;
+  const int64_t g0 = groups * blockIdx.x / gridDim.x, g1 = groups * (blockIdx.x + 1) / gridDim.x;
+  const float* turned = p.dz + groups * 32 * TOK;
+  Four<T> h[4 * NT][4];
+#pragma unroll
+  for (int m = 0; m < 4 * NT; ++m)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int64_t tok = 8 * m + 4 * half + t;
+      h[m][t].load((const T*)p.H + min(tok, p.R - 1) * p.h_pitch + c0);
+    }
+  f32x16 dh[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dh[n][j] = f32x16{};
+  struct Group {  // of 32 words: their rows, and their dz by tokens
+    Four<T> e[4][4];
+    f4 at[NT][4];
+  };
+  auto load = [&](int64_t g, Group& x) __attribute__((always_inline)) {
+    g = min(g, groups - 1);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) x.at[n][m] = *(const f4*)(turned + (g * TOK + 32 * n + col) * 32 + 8 * m + 4 * half);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        x.e[m][t].load((const T*)p.E + min(32 * g + 8 * m + 4 * half + t, p.V - 1) * p.e_pitch + c0);
+    }
+  };
+  // The next group is on the way during both products, or (two blocks of tokens
+  // have no registers for that) the second.
+  constexpr bool kBoth = NT == 1;
+  auto step = [&](int64_t g, Group& x, Group& next) __attribute__((always_inline)) {
+    if (kBoth) load(g + 1, next);
+    f4 a[4 * NT];
+#pragma unroll
+    for (int m = 0; m < 4 * NT; ++m) a[m] = *(const f4*)(p.dz + (g * 32 + col) * TOK + 8 * m + 4 * half);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            dh[n][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.at[n][m][t], x.e[m][t][j], dh[n][j], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!kBoth) load(g + 1, next);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!p.de) return;
+    f32x16 o[4] = {f32x16{}, f32x16{}, f32x16{}, f32x16{}};
+#pragma unroll
+    for (int m = 0; m < 4 * NT; ++m) {
+      if (8 * m >= p.R) break;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[m][t], h[m][t][j], o[j], 0, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int64_t v = 32 * g + 8 * (r >> 2) + 4 * half + (r & 3);
+      if (owns && v < p.V) Four<T>::store((T*)p.de + v * p.d + c0, (f4){o[0][r], o[1][r], o[2][r], o[3][r]});
+    }
+  };
+  Group x[kBoth ? 2 : 1];
+  load(g0, x[0]);
+  int64_t g = g0;
+  if constexpr (kBoth) {
+    for (; g + 1 < g1; g += 2) {
+      step(g, x[0], x[1]);
+      step(g + 1, x[1], x[0]);
+    }
+    if (g < g1) step(g, x[0], x[1]);
+  } else {
+    for (; g < g1; ++g) step(g, x[0], x[0]);
+  }
+  if (!p.part) return;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int64_t tok = 32 * n + 8 * (r >> 2) + 4 * half + (r & 3);
+      if (owns && tok < p.R)
+        Four<float>::store(p.part + (blockIdx.x * p.R + tok) * p.d + c0,
+                           (f4){dh[n][0][r], dh[n][1][r], dh[n][2][r], dh[n][3][r]});
+    }
+}
+
+// Adds many parts of few values: 32 values a workgroup, 32 threads a value, each
+// every 32nd part in order, then the 32 in order.
+__global__ __launch_bounds__(1024) void xent_sum_parts_kernel(const float* __restrict__ part, int parts, int64_t n,
+                                                              void* __restrict__ out, int dtype) {
+  __shared__ float s[32][33];
+  const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
+  const int64_t i = blockIdx.x * 32 + (int64_t)c;
+  float sum = 0.f;
+  if (i < n) {
+    int g = k;
+    for (; g + 7 * 32 < parts; g += 8 * 32) {  // 8 loads in flight
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = part[(int64_t)(g + 32 * e) * n + i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += v[e];
+    }
+    for (; g < parts; g += 32) sum += part[(int64_t)g * n + i];
+  }
+  s[k][c] = sum;
+  __syncthreads();
+  if (k || i >= n) return;
+  float all = 0.f;
+#pragma unroll
+  for (int g = 0; g < 32; ++g) all += s[g][c];
+  store_as(out, i, all, dtype);
+}
+
 // Adds the splits' sums in order; VE values a thread (1 where n is no multiple
 // of 4, or small).
 template <int VE>
@@ -742,7 +959,8 @@ struct Plan {
   bool split;
   bool big_z, big_h, big_e;
   uint32_t tiles_v;    // of the forward
-  uint32_t rows_grid;  // workgroups of the few-token forward, 0: tiles
+  uint32_t rows_grid;  // workgroups of the few-token forward, and of the backward's dz; 0: tiles
+  int few, parts;      // few-token backward: blocks of 32 tokens, parts of d hidden's sums
   int splits_h, splits_e;
   // offsets into the workspace
   size_t scal, amax, e, h, part, zt, coef, P, ph, pe, bytes;
@@ -757,6 +975,19 @@ constexpr int64_t kPieceBytes = 512ll << 20;
 // 131,072 x 1,024: 142 / 524, 404 / 531, 602 / 536.  bf16: 1, 32 tokens of
 // 131,072 x 1,024: 53 / 62, 79 / 64; of 50,021 x 500: 22 / 44, 28 / 45, 64: 43 / 45.
 inline int64_t few_rows(int d, int dtype) { return dtype == MPL_F32 || d % 64 ? 64 : 16; }
+
+// The same of the backward, where few tokens' products are in fp32: bf16 tiles
+// read a copy of the table as fp16, fp16 ones the table as it lies.  Forward and
+// backward, us, few tokens / tiles, fp32: 1, 32, 64 tokens of 16,384 x 256: 30 /
+// 57, 40 / 62, 61 / 69; of 131,072 x 1,024: 504 / 950, 628 / 1,012, 842 / 1,242.
+// bf16, 1, 32, 64 tokens of 131,072 x 1,024: 276 / 474, 372 / 486, 598 / 497.  fp16:
+// 274 / 279, 380 / 293, 8: 291 / 285; of 37,484 x 640 68 / 85, 87 / 88; of 16,384 x
+// 256 25 / 33, 37 / 39; of 50,021 x 500 77 / 112, 104 / 123, 64: 164 / 141.  dz has 8
+// bytes a word and token: up to the bytes of a piece.
+inline int64_t few_grad_rows(int64_t V, int d, int dtype) {
+  if (d < 4 || V * 64 * 8 > kPieceBytes) return 0;
+  return dtype == MPL_F32 ? 64 : dtype == MPL_BF16 || d % 64 || V * d < (1 << 26) ? 32 : 8;
+}
 
 inline int64_t up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
 
@@ -779,6 +1010,16 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
     p.rows_grid = (uint32_t)std::min<int64_t>(cdiv(V, 32), 2048);
     p.part = take((size_t)p.rows_grid * R * 8);
     p.zt = take((size_t)R * 4);
+    p.bytes = at;
+    return p;
+  }
+  if (backward && R <= few_grad_rows(V, d, dtype)) {
+    const int64_t groups = cdiv(V, 32), waves = std::max<int64_t>(8, 1024 / cdiv(d, 128) / 8 * 8);
+    p.few = R <= 32 ? 1 : 2;
+    p.rows_grid = (uint32_t)std::min<int64_t>(groups, 2048);
+    p.parts = (int)std::min(groups, waves);
+    p.P = take((size_t)groups * 32 * p.few * 32 * 8);
+    p.ph = take((size_t)p.parts * R * d * 4);
     p.bytes = at;
     return p;
   }
@@ -895,6 +1136,25 @@ void operands(const Call& c, const Plan& p, char* ws, const CoefArgs* q, hipStre
   H = {ws + p.h, row, c.R, row};
 }
 
+template <typename T, bool BWD>
+void rows_kernel(unsigned grid, hipStream_t s, const RowsArgs& a) {
+  if (a.R <= 32) xent_rows_kernel<T, 1, BWD><<<grid, 256, 0, s>>>(a);
+  else xent_rows_kernel<T, 2, BWD><<<grid, 256, 0, s>>>(a);
+}
+
+template <bool BWD>
+void rows_kernel(int dtype, unsigned grid, hipStream_t s, const RowsArgs& a) {
+  if (dtype == MPL_F32) rows_kernel<float, BWD>(grid, s, a);
+  else if (dtype == MPL_F16) rows_kernel<_Float16, BWD>(grid, s, a);
+  else rows_kernel<__bf16, BWD>(grid, s, a);
+}
+
+template <typename T>
+void few_kernel(int blocks, dim3 grid, hipStream_t s, const FewArgs& a) {
+  if (blocks == 1) xent_few_kernel<T, 1><<<grid, 64, 0, s>>>(a);
+  else xent_few_kernel<T, 2><<<grid, 64, 0, s>>>(a);
+}
+
 // The instantiation of one product for the operands' type and the tile.
 #define MPL_TILE(KERNEL, S, BF, AST, BST, big, grid, s, args)                                           \
   do {                                                                                                  \
@@ -939,11 +1199,9 @@ extern "C" int mpl_vocab_cross_entropy(const void* hidden, int64_t hidden_pitch,
     return check_launch(what);
   };
   if (p.rows_grid) {
-    const RowsArgs a{embedding, hidden, embedding_pitch, hidden_pitch, rows, vocab, d, target, part, z_target};
-    const dim3 grid(p.rows_grid, (unsigned)cdiv(rows, 32));
-    if (dtype == MPL_F32) xent_rows_kernel<float><<<grid, 256, 0, s>>>(a);
-    else if (dtype == MPL_F16) xent_rows_kernel<_Float16><<<grid, 256, 0, s>>>(a);
-    else xent_rows_kernel<__bf16><<<grid, 256, 0, s>>>(a);
+    RowsArgs a{embedding, hidden, embedding_pitch, hidden_pitch, rows, vocab, d, target};
+    a.part = part, a.z_target = z_target;
+    rows_kernel<false>(dtype, p.rows_grid, s, a);
     return join((int)p.rows_grid);
   }
   LogitArgs a{};
@@ -980,6 +1238,21 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
   MPL_REQUIRE(target && lse && (g_loss || g_lse) && (d_hidden || d_embedding), MPL_EINVAL, "%s: null buffer", what);
   char* ws = (char*)workspace;
   hipStream_t s = (hipStream_t)stream;
+  if (p.few) {
+    RowsArgs r{embedding, hidden, embedding_pitch, hidden_pitch, rows, vocab, d, target};
+    r.lse = lse, r.g_loss = g_loss, r.g_lse = g_lse, r.ignore = ignore_index;
+    r.dz = (float*)(ws + p.P);
+    rows_kernel<true>(dtype, p.rows_grid, s, r);
+    FewArgs f{embedding, hidden, embedding_pitch, hidden_pitch, rows, vocab, d, r.dz, d_embedding};
+    f.part = d_hidden ? (float*)(ws + p.ph) : nullptr;
+    const dim3 grid(p.parts, (unsigned)cdiv(d, 128));
+    if (dtype == MPL_F32) few_kernel<float>(p.few, grid, s, f);
+    else if (dtype == MPL_F16) few_kernel<_Float16>(p.few, grid, s, f);
+    else few_kernel<__bf16>(p.few, grid, s, f);
+    if (d_hidden)
+      xent_sum_parts_kernel<<<(unsigned)cdiv(rows * d, 32), 1024, 0, s>>>(f.part, p.parts, rows * d, d_hidden, dtype);
+    return check_launch(what);
+  }
   const int S = p.split ? 2 : 1;
   LogitArgs a{};
   float* scal = (float*)(ws + p.scal);

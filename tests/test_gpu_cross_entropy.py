@@ -559,3 +559,53 @@ def test_memory_is_freed(gpu_lib):
         torch.cuda.synchronize()
         used.append(torch.cuda.memory_allocated())
     assert used[4] == used[2] and used[5] == used[3]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,V,d", [(1, 1, 4), (1, 33, 5), (7, 31, 127), (8, 64, 128), (16, 1000, 129), (17, 300, 64),
+                                   (32, 5003, 257), (33, 70, 130), (40, 2000, 6), (64, 3001, 384), (64, 40000, 40)])
+def test_few_tokens(gpu_lib, R, V, d, dtype):
+    """Blocks of tokens, groups of words and columns that end anywhere; the
+    gradients of both outputs and of either."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    print(f"cross entropy, few tokens R={R} V={V} d={d} {dtype}", flush=True)
+    h, e, t, gl, gs = _inputs(R, V, d, dtype)
+    t[0] = V - 1
+    for a, b in ((gl, gs), (gl, None), (None, gs)):
+        want = _formula(h, e, t, a, b)
+        for name, got in zip(("loss", "lse", "dh", "de"), vocab_cross_entropy_grads(h, e, t, a, b)):
+            _near(name, got, want[name])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R", [3, 40, 100])
+def test_one_of_the_gradients(gpu_lib, R, dtype):
+    """A frozen table, or frozen rows: the other's gradient is the same, and nothing else is written."""
+    from model_amd.cross_entropy import vocab_cross_entropy, vocab_cross_entropy_grads
+
+    h, e, t, gl, _ = _inputs(R, 700, 72, dtype)
+    _, _, dh, de = vocab_cross_entropy_grads(h, e, t, gl)
+    a, b = h.clone().requires_grad_(), e.clone().requires_grad_()
+    vocab_cross_entropy(a, e, t).backward(gl)
+    vocab_cross_entropy(h, b, t).backward(gl)
+    assert torch.equal(a.grad, dh) and torch.equal(b.grad, de)
+
+
+@pytest.mark.parametrize("R", [20, 60])
+def test_few_tokens_leave_the_rest(gpu_lib, R):
+    """The C entry writes d hidden and d embedding and nothing behind them."""
+    from model_amd import _lib
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    h, e, t, gl, _ = _inputs(R, 333, 70, torch.float32)
+    _, lse, want_h, want_e = vocab_cross_entropy_grads(h, e, t, gl)
+    L = _lib.lib()
+    n = L.mpl_vocab_cross_entropy_workspace_bytes(R, 333, 70, _lib.MPL_F32, 1)
+    ws = torch.full((n + 1024,), 77, dtype=torch.uint8, device="cuda")
+    dh, de = (torch.full(((rows + 1) * 70,), 7.0, device="cuda") for rows in (R, 333))
+    _lib.check(L.mpl_vocab_cross_entropy_bwd(h.data_ptr(), 70, e.data_ptr(), 70, _lib.MPL_F32, t.data_ptr(), R, 333, 70,
+                                             IGNORE, lse.data_ptr(), gl.data_ptr(), None, ws.data_ptr(), n,
+                                             dh.data_ptr(), de.data_ptr(), _lib.stream_ptr(h.device)))
+    assert torch.equal(dh[:R * 70].view(R, 70), want_h) and torch.equal(de[:333 * 70].view(333, 70), want_e)
+    assert (dh[R * 70:] == 7).all() and (de[333 * 70:] == 7).all() and (ws[n:] == 77).all()
