@@ -609,3 +609,37 @@ def test_few_tokens_leave_the_rest(gpu_lib, R):
                                              dh.data_ptr(), de.data_ptr(), _lib.stream_ptr(h.device)))
     assert torch.equal(dh[:R * 70].view(R, 70), want_h) and torch.equal(de[:333 * 70].view(333, 70), want_e)
     assert (dh[R * 70:] == 7).all() and (de[333 * 70:] == 7).all() and (ws[n:] == 77).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R", [8, 50, 200])
+def test_two_graphs(gpu_lib, R, dtype):
+    """Two captured graphs replayed in turn and on two streams at once, between
+    eager calls, equal the eager ones."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    args = [_inputs(R, 1500, 128, dtype, seed=s) for s in (5, 6)]
+    want = [vocab_cross_entropy_grads(*x) for x in args]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x in args:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(vocab_cross_entropy_grads(*x))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(4):
+        for out in outs:
+            for x in out:
+                x.fill_(math.nan)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            if turn % 2:
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            else:
+                graph.replay()
+                vocab_cross_entropy_grads(*args[0])
+        torch.cuda.synchronize()
+        for out, ref in zip(outs, want):
+            assert all(torch.equal(x, y) for x, y in zip(out, ref))
