@@ -129,7 +129,7 @@ struct CoefArgs {
   const float* g_loss;
   const float* g_lse;
   const float* lse;
-  float* coef;  // [3][rows_p]: g + gl, g, lse log2(e)
+  float* coef;  // [3][rows_p]: g + gl, g, lse
 };
 __device__ __forceinline__ uint32_t coefficients(const CoefArgs& p, int64_t first, int64_t step) {
   uint32_t m = 0;
@@ -142,7 +142,7 @@ __device__ __forceinline__ uint32_t coefficients(const CoefArgs& p, int64_t firs
     if (i < p.R) {
       g = at == p.ignore ? 0.f : at < 0 || at >= p.V ? NAN : gk;
       all = g + sk;
-      l = lk * kLog2e;
+      l = lk;
     }
     p.coef[i] = all;
     p.coef[p.rows_p + i] = g;
@@ -285,11 +285,11 @@ struct LogitArgs {
   bool scaled;  // the operands carry powers of two
   const int64_t* target;
   // forward
-  float2* part;  // [tiles_v][R]: maximum of z log2(e), sum of 2^(z log2(e) - maximum)
+  float2* part;  // [tiles_v][R]: maximum of z, sum of exp(z - maximum)
   float* z_target;
   // backward: the piece starts at row v0 of the table
   int64_t v0, rows_p, pitch_p;  // rows_p: rows of dz that exist (zero past R); pitch in bytes
-  const float* coef;            // [3][rows_p]: g + gl, g, lse log2(e)
+  const float* coef;            // [3][rows_p]: g + gl, g, lse
   char* P;
   bool stream;  // dz is written past the caches
 };
@@ -299,6 +299,13 @@ struct LogitArgs {
 // of fp32's range.
 __device__ __forceinline__ float unscale_z(const LogitArgs& p) {
   return p.scaled ? fminf(fmaxf(p.scal[kInvE] * p.scal[kInvH], 1.17549435e-38f), 1e38f) : 1.f;
+}
+
+// exp(z - at) for z <= at: exactly 1 at z = at, whatever their size (the powers
+// are of the difference; z log2(e) - at log2(e) by a fused multiply-add leaves the
+// rounding of at log2(e), 4e-6 at 100 and infinite powers from 1e9 on).
+__device__ __forceinline__ float exp_below(float z, float at) {
+  return __builtin_amdgcn_exp2f((z - at) * kLog2e);
 }
 
 #define MPL_TILE_LDS(C)                                      \
@@ -317,13 +324,16 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
   const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
   f32x16 acc[C::TM][C::TN];
   C::run(p.E, p.H, v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
-  // z log2(e) = acc * unit: one multiply and add before each exp2
-  const float unscale = unscale_z(p), unit = unscale * kLog2e;
+  const float unscale = unscale_z(p);
   const int64_t vw = v0 + wm * C::TM * 32 + 4 * (lane >> 5);  // of acc[0][.][0]
   float2* pair = (float2*)a0;  // [WM][BN]: the stages are free
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) {
     const int64_t tok = t0 + (wn * C::TN + j) * 32 + (lane & 31);
+    if (C::S == 2) {
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) acc[i][j] *= unscale;
+    }
     const int64_t at = tok < p.R ? p.target[tok] - vw : -1;  // place of the target among the lane's, if it is there
     const int place = at >= 0 && at < C::TM * 32 && !(at & 4) ? (int)at : -1;
     if (__any(place >= 0)) {
@@ -332,7 +342,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
       for (int i = 0; i < C::TM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) z = place == 32 * i + 8 * (r >> 2) + (r & 3) ? acc[i][j][r] : z;
-      if (place >= 0) p.z_target[tok] = z * unscale;
+      if (place >= 0) p.z_target[tok] = z;
     }
     if (v0 + C::BM > p.V) {
 #pragma unroll
@@ -349,13 +359,12 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
     float x = m, y = m;
     half_swap(x, y);
     m = fmaxf(x, y);
-    m *= unit;
     const float ref = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], unit, -ref));
+      for (int r = 0; r < 16; ++r) s += exp_below(acc[i][j][r], ref);
     x = s, y = s;
     half_swap(x, y);
     if (lane < 32) pair[wm * C::BN + (wn * C::TN + j) * 32 + lane] = make_float2(m, x + y);
@@ -370,7 +379,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < C::WM; ++w)
-      s += pair[w * C::BN + t].y * __builtin_amdgcn_exp2f(pair[w * C::BN + t].x - ref);
+      s += pair[w * C::BN + t].y * exp_below(pair[w * C::BN + t].x, ref);
     p.part[(int64_t)tv * p.R + t0 + t] = make_float2(m, s);
   }
 }
@@ -389,7 +398,7 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
   float m = -INFINITY, l = 0.f;
   auto add = [&](float2 v) __attribute__((always_inline)) {
     const float n = fmaxf(m, v.x), ref = n == -INFINITY ? 0.f : n;
-    l = l * __builtin_amdgcn_exp2f(m - ref) + v.y * __builtin_amdgcn_exp2f(v.x - ref);
+    l = l * exp_below(m, ref) + v.y * exp_below(v.x, ref);
     m = n;
   };
   int i = g;
@@ -405,10 +414,12 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
   __syncthreads();
   if (g || tok >= R) return;
   for (int k = 1; k < N; ++k) add(s[k][t]);
-  const float out = (m + log2f(l)) * kLn2;
+  // l >= 1 and m >= the target's z, both exact where the target is the largest: the
+  // loss of a learned token is log(l), not a difference of two numbers of m's size
+  const float rest = log2f(l) * kLn2;
   const int64_t to = target[tok];
-  lse[tok] = out;
-  loss[tok] = to == ignore ? 0.f : (to < 0 || to >= V) ? NAN : out - z_target[tok];
+  lse[tok] = m + rest;
+  loss[tok] = to == ignore ? 0.f : (to < 0 || to >= V) ? NAN : rest + (m - z_target[tok]);
 }
 
 // Few tokens: the table is read once, straight into the operands (no copy of
@@ -470,7 +481,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs p) {
       gt[n] = to[n] == p.ignore || !p.g_loss ? 0.f : p.g_loss[at];
       if (to[n] != p.ignore && (to[n] < 0 || to[n] >= p.V)) gt[n] = NAN;
       all[n] = gt[n] + (p.g_lse ? p.g_lse[at] : 0.f);
-      lse[n] = p.lse[at] * kLog2e;
+      lse[n] = p.lse[at];
     }
   }
   const int chunks = (p.d + 2 * VE - 1) / (2 * VE);
@@ -532,12 +543,12 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs p) {
         z[i] = ((z4[0][r][lane] + z4[1][r][lane]) + z4[2][r][lane]) + z4[3][r][lane];
         const int64_t v = 32 * g + 8 * wave + 4 * half + i;
         if constexpr (BWD) {
-          z[i] = all[n] * __builtin_amdgcn_exp2f(fmaf(z[i], kLog2e, -lse[n])) - (v == to[n] ? gt[n] : 0.f);
+          z[i] = all[n] * exp_below(z[i], lse[n]) - (v == to[n] ? gt[n] : 0.f);
           z[i] = v < p.V && tok < p.R ? z[i] : 0.f;
           p.dz[(g * 32 + 8 * wave + 4 * half + i) * TOK + tok] = z[i];
         } else {
           if (v == to[n] && tok < p.R) p.z_target[tok] = z[i];
-          z[i] = v < p.V ? z[i] * kLog2e : -INFINITY;
+          z[i] = v < p.V ? z[i] : -INFINITY;
           most = fmaxf(most, z[i]);
         }
       }
@@ -546,9 +557,9 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs p) {
             make_float4(z[0], z[1], z[2], z[3]);
       } else {
         const float ref = most == -INFINITY ? 0.f : most;
-        l[n] *= __builtin_amdgcn_exp2f(m[n] - ref);
+        l[n] *= exp_below(m[n], ref);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) l[n] += __builtin_amdgcn_exp2f(z[i] - ref);
+        for (int i = 0; i < 4; ++i) l[n] += exp_below(z[i], ref);
         m[n] = most;
       }
     }
@@ -567,8 +578,8 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs p) {
     const float ref = most == -INFINITY ? 0.f : most;
 #pragma unroll
     for (int w = 0; w < 4; ++w)
-      sum += pair[w][n][col].y * __builtin_amdgcn_exp2f(pair[w][n][col].x - ref) +
-             pair[w][n][col + 32].y * __builtin_amdgcn_exp2f(pair[w][n][col + 32].x - ref);
+      sum += pair[w][n][col].y * exp_below(pair[w][n][col].x, ref) +
+             pair[w][n][col + 32].y * exp_below(pair[w][n][col + 32].x, ref);
     p.part[(int64_t)blockIdx.x * p.R + tok] = make_float2(most, sum);
   }
 }
@@ -587,7 +598,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
   const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
   f32x16 acc[C::TM][C::TN];
   C::run(p.E, p.H, p.v0 + v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
-  const float unit = unscale_z(p) * kLog2e;
+  const float unscale = unscale_z(p);
   const float up = p.scal[kScaleP];
   const int half = lane >> 5;
   const int64_t vw = v0 + wm * C::TM * 32;  // the wave's first column of the piece
@@ -615,7 +626,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
     for (int i = 0; i < C::TM; ++i) {
       float x[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = ga * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], unit, -lse));
+      for (int r = 0; r < 16; ++r) x[r] = ga * exp_below(acc[i][j][r] * unscale, lse);
       if (hit) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
