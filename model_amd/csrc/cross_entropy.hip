@@ -979,28 +979,30 @@ struct Plan {
 
 constexpr int64_t kPieceBytes = 512ll << 20;
 
-// Tokens up to which the forward reads the table into the operands: the tiles
-// read a copy of it that has to be made first (fp32, and 16-bit rows of d % 64
-// != 0), or go over it with mostly empty columns.  Measured, us, few tokens /
-// tiles, fp32: 1, 64, 96 tokens of 16,384 x 256: 9.9 / 27, 16 / 30, 20 / 30; of
-// 131,072 x 1,024: 142 / 524, 404 / 531, 602 / 536.  bf16: 1, 32 tokens of
-// 131,072 x 1,024: 53 / 62, 79 / 64; of 50,021 x 500: 22 / 44, 28 / 45, 64: 43 / 45.
-inline int64_t few_rows(int d, int dtype) { return dtype == MPL_F32 || d % 64 ? 64 : 16; }
-
-// The same of the backward, where few tokens' products are in fp32: bf16 tiles
-// read a copy of the table as fp16, fp16 ones the table as it lies.  Forward and
-// backward, us, few tokens / tiles, fp32: 1, 32, 64 tokens of 16,384 x 256: 30 /
-// 57, 40 / 62, 61 / 69; of 131,072 x 1,024: 504 / 950, 628 / 1,012, 842 / 1,242.
-// bf16, 1, 32, 64 tokens of 131,072 x 1,024: 276 / 474, 372 / 486, 598 / 497.  fp16:
-// 274 / 279, 380 / 293, 8: 291 / 285; of 37,484 x 640 68 / 85, 87 / 88; of 16,384 x
-// 256 25 / 33, 37 / 39; of 50,021 x 500 77 / 112, 104 / 123, 64: 164 / 141.  dz has 8
-// bytes a word and token: up to the bytes of a piece.
-inline int64_t few_grad_rows(int64_t V, int d, int dtype) {
-  if (d < 4 || V * 64 * 8 > kPieceBytes) return 0;
-  return dtype == MPL_F32 ? 64 : dtype == MPL_BF16 || d % 64 || V * d < (1 << 26) ? 32 : 8;
-}
-
 inline int64_t up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
+
+// Tokens up to which the table is read into the operands: the tiles read a copy
+// of it that has to be made first (fp32, bf16's gradients, and 16-bit rows of
+// d % 64 != 0), or go over it with mostly empty columns.  The backward has to
+// take the forward's way: other kernels add z's products in another order, and
+// exp(z - lse) of a learned token turns the difference, 2^-24 of z, into an error
+// of p.  The few tokens' backward holds 8 bytes of dz a word and token, at most
+// kFewBytes.
+//
+// Measured, us, few tokens / tiles.  Forward, fp32: 1, 64, 96 tokens of 16,384 x
+// 256: 9.9 / 27, 16 / 30, 20 / 30; of 131,072 x 1,024: 142 / 524, 404 / 531, 602 /
+// 536.  bf16: 1, 32 tokens of 131,072 x 1,024: 53 / 62, 79 / 64; of 50,021 x 500:
+// 22 / 44, 28 / 45, 64: 43 / 45.
+// Forward and backward, fp32: 1, 32, 64 tokens of 16,384 x 256: 30 / 57, 40 / 62,
+// 61 / 69; of 131,072 x 1,024: 504 / 950, 628 / 1,012, 842 / 1,242.  bf16, 1, 32, 64
+// tokens of 131,072 x 1,024: 276 / 474, 372 / 486, 598 / 497.  fp16: 274 / 279, 380 /
+// 293, 8: 291 / 285; of 37,484 x 640 68 / 85, 87 / 88; of 16,384 x 256 25 / 33, 37 /
+// 39; of 50,021 x 500 77 / 112, 104 / 123, 64: 164 / 141.
+constexpr int64_t kFewBytes = 4ll << 30;
+inline bool few_tokens(int64_t R, int64_t V, int d, int dtype) {
+  const int64_t most = dtype == MPL_F32 ? 64 : dtype == MPL_BF16 || d % 64 ? 32 : 16;
+  return d >= 4 && R <= most && up(V, 32) * up(R, 32) * 8 <= kFewBytes;
+}
 
 Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
   Plan p{};
@@ -1017,14 +1019,14 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
     at = (at + bytes + 1023) / 1024 * 1024;
     return o;
   };
-  if (!backward && R <= few_rows(d, dtype)) {
+  if (!backward && few_tokens(R, V, d, dtype)) {
     p.rows_grid = (uint32_t)std::min<int64_t>(cdiv(V, 32), 2048);
     p.part = take((size_t)p.rows_grid * R * 8);
     p.zt = take((size_t)R * 4);
     p.bytes = at;
     return p;
   }
-  if (backward && R <= few_grad_rows(V, d, dtype)) {
+  if (backward && few_tokens(R, V, d, dtype)) {
     const int64_t groups = cdiv(V, 32), waves = std::max<int64_t>(8, 1024 / cdiv(d, 128) / 8 * 8);
     p.few = R <= 32 ? 1 : 2;
     p.rows_grid = (uint32_t)std::min<int64_t>(groups, 2048);

@@ -1,5 +1,7 @@
 """vocab_cross_entropy where rows, words and token weights are of unlike size."""
 
+import math
+
 import pytest
 import torch
 
@@ -69,3 +71,24 @@ def test_logits_of_any_size(gpu_lib, R, size, dtype):
     near = dz.abs() * (2.0 ** -11 + u) if dtype != torch.float32 else dz.abs() * 2.0 ** -20
     assert ((dh.double() - dz).abs() <= near + 2.0 ** -37).all()
     assert torch.isfinite(de).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R", [1, 9, 16, 17, 20, 32])
+@pytest.mark.parametrize("V,d", [(300, 128), (1000, 100), (700, 320)])
+def test_few_tokens_form_z_twice_alike(gpu_lib, R, V, d, dtype):
+    """Learned tokens with logits of some 10^4, where another order of z's sum is
+    off by 2^-24 of that: p is exactly 1 where the backward's z has the forward's
+    bits, and every gradient exactly 0 (the other words are 104 and more below)."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    e = torch.randn((V, d), generator=gen, device="cuda")
+    e = (e / e.norm(dim=1, keepdim=True)).to(dtype)
+    t = torch.randint(0, V, (R,), generator=gen, device="cuda")
+    h = (3e4 * e[t].float()).to(dtype)
+    z = h.double() @ e.double().t()
+    z.scatter_(1, t[:, None], -math.inf)
+    assert (z.amax(1) < 3e4 - 200).all()
+    loss, _, dh, de = vocab_cross_entropy_grads(h, e, t, torch.ones(R, device="cuda"))
+    assert (loss == 0).all() and (dh == 0).all() and (de == 0).all()
