@@ -773,9 +773,9 @@ int mpl_layer_norm_bwd(const void* dy, int64_t dy_pitch, const void* x, int64_t 
  * embedding_pitch elements apart (>= d); 16-bit arrays of d % 64 == 0 are read
  * as they lie and must have 16-byte aligned rows less than 2^23 elements apart.
  * d <= 65,536, (rows + vocab) d below 2^34 with d rounded up to 64, and less than
- * 2^23 tiles of 256 x 256 logits.  Sums are fp32; fp32 operands are held to 2^-23
- * of each (hi + lo fp16 under a power of two), and one that is not finite may
- * give NaN where z is -inf.  target int64 [rows].  Deterministic.
+ * 2^23 tiles of 256 x 256 logits.  Sums are fp32; in z fp32 operands are held
+ * to 2^-23 of each and 2^-39 of the largest of their row (hi + lo fp16 under a power
+ * of two a row), and one that is not finite may give NaN where z is -inf.  target int64 [rows].  Deterministic.
  *
  * mpl_vocab_cross_entropy_bwd writes d_hidden [rows, d] and d_embedding [vocab,
  * d] (dense, of dtype; either may be NULL) from the forward's lse and the

@@ -70,7 +70,7 @@ def vocab_cross_entropy(hidden: torch.Tensor, embedding: torch.Tensor, targets: 
     counted tokens is loss.sum() / (targets != ignore_index).sum().
 
     Logits are sums in fp32 of the exact products (fp32 operands are held to
-    2^-23 of each).  fp32 rows or table entries that are not finite may give NaN
+    2^-23 of each and 2^-39 of the largest of their row).  fp32 rows or table entries that are not finite may give NaN
     where the formula has a logit of -inf.  Up to some 2^39 logits and 2^34
     elements of both arrays.
     The gradients hold dz in fp16 under a power of two (fp32: hi and lo, to

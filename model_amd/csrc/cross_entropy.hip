@@ -50,11 +50,18 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // operands were multiplied by, and dz's with its inverse.
 enum { kInvE = 0, kInvH, kScaleP, kInvP, kScalars = 16 };
 
-// 2^(top - exponent of the largest magnitude), given by its bits; 1 for 0.
+// The operands of z in fp32 calls are split row by row: a hidden row and a word
+// each under a power of two of its own, which z's tile undoes, so that no row's
+// size costs another's logits bits.  The operands of the gradients' products are
+// summed over words or tokens, and have one power of two an array.
+
+// The power that brings the largest magnitude, given by its bits, to [2^top,
+// 2^(top + 1)); 0 for 0.
+__device__ __forceinline__ int power_for(uint32_t bits, int top) {
+  return bits == 0 ? 0 : max(-126, min(126, top + 127 - (int)(bits >> 23)));
+}
 __device__ __forceinline__ float scale_for(uint32_t bits, int top) {
-  const int e = (int)(bits >> 23) - 127;
-  const int s = bits == 0 ? 0 : max(-126, min(126, top - e));
-  return __uint_as_float((uint32_t)(127 + s) << 23);
+  return __uint_as_float((uint32_t)(127 + power_for(bits, top)) << 23);
 }
 // Magnitude bits of x, 0 if it is not finite.
 __device__ __forceinline__ uint32_t finite_bits(float x) {
@@ -215,21 +222,38 @@ __global__ __launch_bounds__(256) void amax_kernel(PackArgs p, CoefArgs q) {
   if (threadIdx.x == 0) p.part[a * kAmaxBlocks + blockIdx.x] = m;
 }
 
+__device__ __forceinline__ void load_split(const PackOne& o, int64_t r, int64_t c, int64_t d, float (&v)[8]) {
+  Source<kSplit>::load(o, r, c, d, *(float(*)[4])v);
+  Source<kSplit>::load(o, r, c + 4, d, *(float(*)[4])(v + 4));
+}
+__device__ __forceinline__ void store_split(char* dst, int64_t r, int64_t dpad, int c, const float (&v)[8], int power) {
+  half8 hi, lo;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float y = ldexpf(v[j], power);
+    hi[j] = (_Float16)y;
+    lo[j] = (_Float16)(y - (float)hi[j]);
+  }
+  char* q = dst + (r * dpad + c / 32 * 32) * 4 + (c % 32) * 2;
+  *(half8*)q = hi;
+  *(half8*)(q + 64) = lo;
+}
+
 // Rows of an array as a tile product's operand, zero-filled to whole stages.  A
 // thread writes 8 elements.
 template <int MODE>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   const int a = blockIdx.x < p.e.blocks ? 0 : 1;
   const PackOne o = a ? p.h : p.e;
-  float scale = 1.f;
+  int power = 0;
   if constexpr (MODE != kCopy16) {
     auto most = [&](int k) __attribute__((always_inline)) {
       const uint32_t* q = p.part + k * kAmaxBlocks + threadIdx.x;
       return block_max<256>(max(q[0], q[256]));
     };
-    scale = scale_for(most(a), 14);
+    power = power_for(most(a), 14);
     if (threadIdx.x == 0 && (blockIdx.x == 0 || blockIdx.x == p.e.blocks))
-      p.scal[a == 0 ? kInvE : kInvH] = 1.f / scale;
+      p.scal[a == 0 ? kInvE : kInvH] = __uint_as_float((uint32_t)(127 - power) << 23);
     if (p.coefs && blockIdx.x == 0) {
       __syncthreads();  // block_max's words are used again
       const uint32_t m = most(2);
@@ -243,24 +267,14 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   const int c = 8 * (int)(i - r * per);
   if constexpr (MODE == kSplit) {
     float v[8];
-    Source<MODE>::load(o, r, c, p.d, *(float(*)[4])v);
-    Source<MODE>::load(o, r, c + 4, p.d, *(float(*)[4])(v + 4));
-    half8 hi, lo;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float y = v[j] * scale;
-      hi[j] = (_Float16)y;
-      lo[j] = (_Float16)(y - (float)hi[j]);
-    }
-    char* q = o.dst + (r * p.dpad + c / 32 * 32) * 4 + (c % 32) * 2;
-    *(half8*)q = hi;
-    *(half8*)(q + 64) = lo;
+    load_split(o, r, c, p.d, v);
+    store_split(o.dst, r, p.dpad, c, v, power);
   } else if constexpr (MODE == kBf16ToF16) {
     float v[8];
     Source<MODE>::load(o, r, c, p.d, v);
     half8 h;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] = (_Float16)(v[j] * scale);
+    for (int j = 0; j < 8; ++j) h[j] = (_Float16)ldexpf(v[j], power);
     *(half8*)(o.dst + (r * p.dpad + c) * 2) = h;
   } else {
     const uint16_t* x = (const uint16_t*)o.src + r * o.pitch + c;
@@ -275,14 +289,63 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   }
 }
 
+// fp32 rows of both arrays as z's operands: hi and lo under the row's own power of
+// two, whose undoing power is written beside.  A team of `width` lanes takes a row
+// and holds its first kHold vectors of 8 a lane.
+struct SplitArgs {
+  PackOne e, h;
+  int d, dpad, width;
+  int* undo_e;
+  int* undo_h;
+};
+__global__ __launch_bounds__(256) void split_rows_kernel(SplitArgs p) {
+  constexpr int kHold = 2;
+  const PackOne o = blockIdx.y ? p.h : p.e;
+  int* undo = blockIdx.y ? p.undo_h : p.undo_e;
+  const int lane = threadIdx.x & (p.width - 1), vecs = p.dpad / 8;
+  const int64_t teams = (int64_t)gridDim.x * (256 / p.width);
+  for (int64_t r = (int64_t)blockIdx.x * (256 / p.width) + threadIdx.x / p.width; r < o.rows; r += teams) {
+    float v[kHold][8];
+    uint32_t most = 0;
+    auto take = [&](const float(&u)[8]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = max(most, finite_bits(u[j]));
+    };
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) {
+      const int c = lane + k * p.width;
+      if (c >= vecs) continue;
+      load_split(o, r, 8 * c, p.d, v[k]);
+      take(v[k]);
+    }
+    for (int c = lane + kHold * p.width; c < vecs; c += p.width) {
+      float u[8];
+      load_split(o, r, 8 * c, p.d, u);
+      take(u);
+    }
+    for (int h = p.width / 2; h; h >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, h));  // a team's lanes
+    const int power = power_for(most, 14);
+    if (lane == 0) undo[r] = -power;
+#pragma unroll
+    for (int k = 0; k < kHold; ++k)
+      if (lane + k * p.width < vecs) store_split(o.dst, r, p.dpad, 8 * (lane + k * p.width), v[k], power);
+    for (int c = lane + kHold * p.width; c < vecs; c += p.width) {
+      float u[8];
+      load_split(o, r, 8 * c, p.d, u);
+      store_split(o.dst, r, p.dpad, 8 * c, u, power);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ forward
 struct LogitArgs {
   TileOperand E, H;
   int64_t R, V;
   int iters;
   uint32_t tiles_v, tiles_t;
+  const int* undo_e;  // fp32 calls: the powers that undo those of the words (to up(V, 256)) and of the rows
+  const int* undo_h;
   const float* scal;
-  bool scaled;  // the operands carry powers of two
   const int64_t* target;
   // forward
   float2* part;  // [tiles_v][R]: maximum of z, sum of exp(z - maximum)
@@ -293,13 +356,6 @@ struct LogitArgs {
   char* P;
   bool stream;  // dz is written past the caches
 };
-
-// What accumulators are multiplied by to give z: finite and not 0, so that a
-// masked -inf and an exact 0 stay what they are where both arrays lie at an end
-// of fp32's range.
-__device__ __forceinline__ float unscale_z(const LogitArgs& p) {
-  return p.scaled ? fminf(fmaxf(p.scal[kInvE] * p.scal[kInvH], 1.17549435e-38f), 1e38f) : 1.f;
-}
 
 // exp(z - at) for z <= at: exactly 1 at z = at, whatever their size (the powers
 // are of the difference; z log2(e) - at log2(e) by a fused multiply-add leaves the
@@ -314,6 +370,29 @@ __device__ __forceinline__ float exp_below(float z, float at) {
   __shared__ __attribute__((aligned(1024))) char a1[C::kStageA]; \
   __shared__ __attribute__((aligned(1024))) char b1[C::kStageB];
 
+// The powers that undo those of a tile's words, in LDS before the tile's product
+// (whose barriers show them to all waves); and a lane's accumulators of token
+// `undo_h` as z: a product of the two powers need not be a finite number, their sum
+// is one power.
+template <class C>
+__device__ __forceinline__ void hold_undo(const int* undo_e, int64_t v0, int* undo) {
+  if (C::S == 2)
+    for (int i = threadIdx.x; i < C::BM; i += C::kThreads) undo[i] = undo_e[v0 + i];
+}
+template <class C>
+__device__ __forceinline__ void undo_powers(f32x16& acc, const int* undo, int undo_h) {
+  if (C::S == 2) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int4 k = *(const int4*)(undo + 8 * q);
+      acc[4 * q] = ldexpf(acc[4 * q], undo_h + k.x);
+      acc[4 * q + 1] = ldexpf(acc[4 * q + 1], undo_h + k.y);
+      acc[4 * q + 2] = ldexpf(acc[4 * q + 2], undo_h + k.z);
+      acc[4 * q + 3] = ldexpf(acc[4 * q + 3], undo_h + k.w);
+    }
+  }
+}
+
 template <class C>
 __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
   MPL_TILE_LDS(C)
@@ -323,17 +402,17 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
   tile_of(blockIdx.x, gridDim.x, p.tiles_v, p.tiles_t, 8, tv, tt);
   const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
   f32x16 acc[C::TM][C::TN];
+  __shared__ __attribute__((aligned(16))) int undo[C::S == 2 ? C::BM : 1];
+  hold_undo<C>(p.undo_e, v0, undo);
   C::run(p.E, p.H, v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
-  const float unscale = unscale_z(p);
   const int64_t vw = v0 + wm * C::TM * 32 + 4 * (lane >> 5);  // of acc[0][.][0]
   float2* pair = (float2*)a0;  // [WM][BN]: the stages are free
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) {
     const int64_t tok = t0 + (wn * C::TN + j) * 32 + (lane & 31);
-    if (C::S == 2) {
+    const int undo_h = C::S == 2 ? p.undo_h[min(tok, p.R - 1)] : 0;
 #pragma unroll
-      for (int i = 0; i < C::TM; ++i) acc[i][j] *= unscale;
-    }
+    for (int i = 0; i < C::TM; ++i) undo_powers<C>(acc[i][j], undo + (wm * C::TM + i) * 32 + 4 * (lane >> 5), undo_h);
     const int64_t at = tok < p.R ? p.target[tok] - vw : -1;  // place of the target among the lane's, if it is there
     const int place = at >= 0 && at < C::TM * 32 && !(at & 4) ? (int)at : -1;
     if (__any(place >= 0)) {
@@ -597,8 +676,9 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
   tile_of(blockIdx.x, gridDim.x, p.tiles_v, p.tiles_t, 8, tv, tt);
   const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
   f32x16 acc[C::TM][C::TN];
+  __shared__ __attribute__((aligned(16))) int undo[C::S == 2 ? C::BM : 1];
+  hold_undo<C>(p.undo_e, p.v0 + v0, undo);
   C::run(p.E, p.H, p.v0 + v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
-  const float unscale = unscale_z(p);
   const float up = p.scal[kScaleP];
   const int half = lane >> 5;
   const int64_t vw = v0 + wm * C::TM * 32;  // the wave's first column of the piece
@@ -622,11 +702,13 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
     const int to = at >= 0 && at < C::TM * 32 ? (int)at : -1;
     const bool hit = __any(to >= 0);
     const bool edge = p.v0 + v0 + C::BM > p.V;
+    const int undo_h = C::S == 2 ? p.undo_h[min(tok, p.R - 1)] : 0;
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) {
+      undo_powers<C>(acc[i][j], undo + (wm * C::TM + i) * 32 + 4 * half, undo_h);
       float x[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = ga * exp_below(acc[i][j][r] * unscale, lse);
+      for (int r = 0; r < 16; ++r) x[r] = ga * exp_below(acc[i][j][r], lse);
       if (hit) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -966,7 +1048,8 @@ template <int S, bool BF, bool AST, bool BST> using Mid = TileMma<S, BF, AST, BS
 
 struct Plan {
   int64_t rows_p, v_piece, pieces;
-  int dpad, mode;  // mode: what the operands need, -1 nothing
+  int dpad;
+  int mode_z, mode;  // what the operands of z and of the gradients need, -1 nothing (the gradients: z's serve)
   bool split;
   bool big_z, big_h, big_e;
   uint32_t tiles_v;    // of the forward
@@ -974,7 +1057,7 @@ struct Plan {
   int few, parts;      // few-token backward: blocks of 32 tokens, parts of d hidden's sums
   int splits_h, splits_e;
   // offsets into the workspace
-  size_t scal, amax, e, h, part, zt, coef, P, ph, pe, bytes;
+  size_t scal, amax, ze, zh, undo_e, undo_h, e, h, part, zt, coef, P, ph, pe, bytes;
 };
 
 constexpr int64_t kPieceBytes = 512ll << 20;
@@ -1008,7 +1091,8 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
   Plan p{};
   p.split = dtype == MPL_F32;
   const int S = p.split ? 2 : 1;
-  p.mode = p.split ? kSplit : backward && dtype == MPL_BF16 ? kBf16ToF16 : d % 64 ? kCopy16 : -1;
+  p.mode_z = p.split ? kSplit : d % 64 ? kCopy16 : -1;
+  p.mode = p.split ? kSplit : dtype == MPL_BF16 ? kBf16ToF16 : -1;
   p.dpad = (int)up(d, 64);
   p.rows_p = up(R, 64);
   p.big_z = cdiv(R, 256) * cdiv(V, 256) >= 256;
@@ -1036,16 +1120,20 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
     p.bytes = at;
     return p;
   }
-  p.scal = take(kScalars * 4);
-  p.amax = take(3 * kAmaxBlocks * 4);
-  p.e = take(p.mode >= 0 ? (size_t)V * p.dpad * 2 * S : 0);
-  p.h = take(p.mode >= 0 ? (size_t)R * p.dpad * 2 * S : 0);
+  p.ze = take(p.mode_z >= 0 ? (size_t)V * p.dpad * 2 * S : 0);
+  p.zh = take(p.mode_z >= 0 ? (size_t)R * p.dpad * 2 * S : 0);
+  p.undo_e = take(p.split ? (size_t)up(V, 256) * 4 : 0);
+  p.undo_h = take(p.split ? (size_t)R * 4 : 0);
   if (!backward) {
     p.part = take((size_t)p.tiles_v * R * 8);
     p.zt = take((size_t)R * 4);
     p.bytes = at;
     return p;
   }
+  p.scal = take(kScalars * 4);
+  p.amax = take(3 * kAmaxBlocks * 4);
+  p.e = take(p.mode >= 0 ? (size_t)V * p.dpad * 2 * S : 0);
+  p.h = take(p.mode >= 0 ? (size_t)R * p.dpad * 2 * S : 0);
   // Pieces of the vocabulary: as few as their dz's bytes allow, and where the
   // table's gradient has 256 tiles in a piece, whole multiples of that: each
   // product of a piece then fills the 256 CUs evenly.
@@ -1111,39 +1199,61 @@ int check_call(const char* what, const Call& c, const void* ws, size_t ws_bytes,
   return MPL_OK;
 }
 
-// Brings both arrays into operand form; E and H are the rows forms.
-// In the backward `q` also gets the coefficients formed.
-void operands(const Call& c, const Plan& p, char* ws, const CoefArgs* q, hipStream_t s, TileOperand& E, TileOperand& H) {
+PackOne pack_of(const void* src, char* dst, int64_t rows, int64_t pitch, const Plan& p) {
+  const bool vec = ((uintptr_t)src & 15) == 0 && pitch % (p.split ? 4 : 8) == 0;
+  return PackOne{src, dst, rows, pitch, cdiv(rows * (p.dpad / 8), 256), vec};
+}
+
+// Both arrays as z's operands, the forward's and the backward's, in rows form.
+void z_operands(const Call& c, const Plan& p, char* ws, hipStream_t s, LogitArgs& a) {
   const int64_t row = (int64_t)p.dpad * (p.split ? 4 : 2);
-  const bool apart = q && p.mode <= kCopy16;
-  if (apart) xent_coef_kernel<<<1, 1024, 0, s>>>(*q, (float*)(ws + p.scal));
-  if (p.mode < 0) {
-    E = {(const char*)c.embedding, c.embedding_pitch * 2, c.V, row};
-    H = {(const char*)c.hidden, c.hidden_pitch * 2, c.R, row};
+  if (p.mode_z < 0) {
+    a.E = {(const char*)c.embedding, c.embedding_pitch * 2, c.V, row};
+    a.H = {(const char*)c.hidden, c.hidden_pitch * 2, c.R, row};
     return;
   }
-  auto one = [&](const void* src, char* dst, int64_t rows, int64_t pitch) {
-    const bool vec = ((uintptr_t)src & 15) == 0 && pitch % (p.split ? 4 : 8) == 0;
-    return PackOne{src, dst, rows, pitch, cdiv(rows * (p.dpad / 8), 256), vec};
-  };
+  a.E = {ws + p.ze, row, c.V, row};
+  a.H = {ws + p.zh, row, c.R, row};
+  const PackOne e = pack_of(c.embedding, ws + p.ze, c.V, c.embedding_pitch, p),
+                h = pack_of(c.hidden, ws + p.zh, c.R, c.hidden_pitch, p);
+  if (p.mode_z == kSplit) {
+    int width = 8;
+    while (width < 64 && width < p.dpad / 8) width *= 2;
+    a.undo_e = (int*)(ws + p.undo_e), a.undo_h = (int*)(ws + p.undo_h);
+    const SplitArgs q{e, h, c.d, p.dpad, width, (int*)(ws + p.undo_e), (int*)(ws + p.undo_h)};
+    const int64_t groups = cdiv(std::max(c.V, c.R), 256 / width);
+    split_rows_kernel<<<dim3((unsigned)std::min<int64_t>(groups, 1 << 20), 2), 256, 0, s>>>(q);
+  } else {
+    PackArgs q{};
+    q.e = e, q.h = h, q.d = c.d, q.dpad = p.dpad;
+    pack_kernel<kCopy16><<<(unsigned)(e.blocks + h.blocks), 256, 0, s>>>(q);
+  }
+}
+
+// Both arrays as the operands of the gradients' products, and the coefficients.
+void grad_operands(const Call& c, const Plan& p, char* ws, const CoefArgs& q, const LogitArgs& z, hipStream_t s,
+                   TileOperand& E, TileOperand& H) {
+  const int64_t row = (int64_t)p.dpad * (p.split ? 4 : 2);
+  if (p.mode < 0) {
+    xent_coef_kernel<<<1, 1024, 0, s>>>(q, (float*)(ws + p.scal));
+    E = z.E, H = z.H;
+    return;
+  }
   PackArgs a{};
-  a.e = one(c.embedding, ws + p.e, c.V, c.embedding_pitch);
-  a.h = one(c.hidden, ws + p.h, c.R, c.hidden_pitch);
+  a.e = pack_of(c.embedding, ws + p.e, c.V, c.embedding_pitch, p);
+  a.h = pack_of(c.hidden, ws + p.h, c.R, c.hidden_pitch, p);
   a.d = c.d, a.dpad = p.dpad;
   a.scal = (float*)(ws + p.scal);
   a.part = (uint32_t*)(ws + p.amax);
-  a.coefs = q && !apart;
-  const dim3 maxima(kAmaxBlocks, a.coefs ? 3 : 2);
-  const CoefArgs coef = q ? *q : CoefArgs{};
+  a.coefs = true;
+  const dim3 maxima(kAmaxBlocks, 3);
   const unsigned grid = (unsigned)(a.e.blocks + a.h.blocks);
   if (p.mode == kSplit) {
-    amax_kernel<kSplit><<<maxima, 256, 0, s>>>(a, coef);
+    amax_kernel<kSplit><<<maxima, 256, 0, s>>>(a, q);
     pack_kernel<kSplit><<<grid, 256, 0, s>>>(a);
-  } else if (p.mode == kBf16ToF16) {
-    amax_kernel<kBf16ToF16><<<maxima, 256, 0, s>>>(a, coef);
-    pack_kernel<kBf16ToF16><<<grid, 256, 0, s>>>(a);
   } else {
-    pack_kernel<kCopy16><<<grid, 256, 0, s>>>(a);
+    amax_kernel<kBf16ToF16><<<maxima, 256, 0, s>>>(a, q);
+    pack_kernel<kBf16ToF16><<<grid, 256, 0, s>>>(a);
   }
   E = {ws + p.e, row, c.V, row};
   H = {ws + p.h, row, c.R, row};
@@ -1218,13 +1328,11 @@ extern "C" int mpl_vocab_cross_entropy(const void* hidden, int64_t hidden_pitch,
     return join((int)p.rows_grid);
   }
   LogitArgs a{};
-  operands(c, p, ws, nullptr, s, a.E, a.H);
+  z_operands(c, p, ws, s, a);
   a.R = rows, a.V = vocab;
   a.iters = p.dpad * (p.split ? 2 : 1) / 64;
   a.tiles_v = p.tiles_v;
   a.tiles_t = (uint32_t)cdiv(rows, p.big_z ? 256 : 128);
-  a.scal = (const float*)(ws + p.scal);
-  a.scaled = p.split;
   a.target = target;
   a.part = part;
   a.z_target = z_target;
@@ -1271,13 +1379,14 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
   float* scal = (float*)(ws + p.scal);
   float* coef = (float*)(ws + p.coef);
   const CoefArgs q{target, rows, p.rows_p, vocab, ignore_index, g_loss, g_lse, lse, coef};
-  operands(c, p, ws, &q, s, a.E, a.H);
+  TileOperand E, H;
+  z_operands(c, p, ws, s, a);
+  grad_operands(c, p, ws, q, a, s, E, H);
   a.R = rows, a.V = vocab;
   a.iters = p.dpad * S / 64;
   const int bz = p.big_z ? 256 : 128;
   a.tiles_t = (uint32_t)cdiv(rows, bz);
   a.scal = scal;
-  a.scaled = p.mode > kCopy16;
   a.target = target;
   a.rows_p = p.rows_p;
   a.pitch_p = p.v_piece * 2 * S;
@@ -1294,18 +1403,19 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
     const int64_t nvp = up(nv, 256);
     a.tiles_v = (uint32_t)(nvp / bz);
     if (p.split) MPL_TILE(xent_dz_kernel, 2, false, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
+    else if (dtype == MPL_BF16) MPL_TILE(xent_dz_kernel, 1, true, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
     else MPL_TILE(xent_dz_kernel, 1, false, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
     if (d_hidden) {
       GradArgs g{};
       g.A = {a.P, a.pitch_p, p.rows_p, a.pitch_p};
-      g.B = {a.E.base + a.v0 * a.E.pitch, a.E.pitch, nv, a.E.width};
+      g.B = {E.base + a.v0 * E.pitch, E.pitch, nv, E.width};
       g.rows = rows, g.cols = d;
       g.iters = (int)(nvp * S / 64);
       // a short last piece has fewer stages than parts: the others' sums stand
       g.splits = std::min(p.splits_h, g.iters);
       const int b = p.big_h ? 256 : 128;
       g.tiles_m = (uint32_t)cdiv(rows, b), g.tiles_n = (uint32_t)cdiv(d, b);
-      g.u0 = scal + kInvP, g.u1 = a.scaled ? scal + kInvE : nullptr;
+      g.u0 = scal + kInvP, g.u1 = p.mode >= 0 ? scal + kInvE : nullptr;
       g.part = p.splits_h > 1 || p.pieces > 1 ? (float*)(ws + p.ph) : nullptr;
       g.add = i > 0;
       g.out = d_hidden, g.dtype = dtype;
@@ -1316,13 +1426,13 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
     if (d_embedding) {
       GradArgs g{};
       g.A = {a.P, a.pitch_p, p.rows_p, nvp * 2 * S};
-      g.B = {a.H.base, a.H.pitch, rows, a.H.width};
+      g.B = {H.base, H.pitch, rows, H.width};
       g.rows = nv, g.cols = d;
       g.iters = (int)(p.rows_p * S / 64);
       g.splits = p.splits_e;
       const int b = p.big_e ? 256 : 128;
       g.tiles_m = (uint32_t)cdiv(nv, b), g.tiles_n = (uint32_t)cdiv(d, b);
-      g.u0 = scal + kInvP, g.u1 = a.scaled ? scal + kInvH : nullptr;
+      g.u0 = scal + kInvP, g.u1 = p.mode >= 0 ? scal + kInvH : nullptr;
       g.part = p.splits_e > 1 ? (float*)(ws + p.pe) : nullptr;
       g.out = (char*)d_embedding + a.v0 * d * (dtype == MPL_F32 ? 4 : 2);
       g.dtype = dtype;

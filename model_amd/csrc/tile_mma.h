@@ -16,9 +16,9 @@
 // it), so no array is ever transposed in memory.
 //
 // fp32 operands (S = 2) are split: x = hi + lo, both fp16, after a power of
-// two that brings the largest of the array to [2^14, 2^15); 11 + 11 bits and
-// lo's sign hold x to 2^-23 of it (and to 2^-39 of the array's largest, where
-// fp16's own range ends).  A row is then 32 hi, 32 lo, 32 hi, ... and a
+// two that brings the largest of those that share it (a row, or the array) to
+// [2^14, 2^15); 11 + 11 bits and lo's sign hold x to 2^-23 of it (and to 2^-39 of
+// that largest, where fp16's own range ends).  A row is then 32 hi, 32 lo, 32 hi, ... and a
 // product is hi hi + hi lo + lo hi; lo lo is below 2^-22 of the product.
 // Three fp16 products run at 5 times the rate of one fp32 product.
 //

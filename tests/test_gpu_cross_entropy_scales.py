@@ -1,13 +1,120 @@
-"""vocab_cross_entropy where rows, words and token weights are of unlike size."""
+"""vocab_cross_entropy where rows, words and token weights are of unlike size.
+
+Tolerances as in test_gpu_cross_entropy.py, but with the ends of fp16's range
+where the operands' own powers of two put them:
+
+  z        2^-39 of a row's largest and of a word's largest (fp32 calls; 16-bit
+           calls multiply their operands as they are)
+  lse      twice sum_v p z's error (the weights shift by less than half), and
+           2^-20 (1 + |lse|)
+  dz       2^-38 of the token's own largest coefficient
+  d h      the table to 2^-39 of its largest entry (fp32 and bf16 calls)
+  d e      hidden rows times their tokens' coefficients, in dz's powers of two
+           (each within a factor of 2 of the largest coefficient, so 4 for a
+           quotient of two), to 2^-39 of the largest such product
+"""
 
 import math
 
 import pytest
 import torch
 
-from tests.test_gpu_cross_entropy import DTYPES, _inputs
+from tests.test_gpu_cross_entropy import IGNORE, DTYPES, _inputs, _near
 
 pytestmark = pytest.mark.gpu
+
+
+def _formula(h, e, t, gl):
+    dtype, (R, d), V = h.dtype, h.shape, e.shape[0]
+    u = torch.finfo(dtype).eps / 2
+    fp32 = dtype == torch.float32
+    H, E = h.double(), e.double()
+    hm, em = H.abs().amax(1), E.abs().amax(1)
+    z = H @ E.t()
+    z_tol = (d * 2.0 ** -24 + (2.0 ** -21 if fp32 else 0)) * (H.abs() @ E.abs().t())
+    if fp32:
+        z_tol = z_tol + 2.0 ** -39 * (em[None] * H.abs().sum(1)[:, None] + hm[:, None] * E.abs().sum(1)[None])
+    lse = torch.logsumexp(z, 1)
+    soft = torch.exp(z - lse[:, None])
+    lse_tol = 2 * (soft * z_tol).sum(1) + 2.0 ** -20 * (1 + lse.abs())
+    keep = t != IGNORE
+    at = torch.where(keep, t, 0)[:, None]
+    zt, zt_tol = z.gather(1, at)[:, 0], z_tol.gather(1, at)[:, 0]
+    loss = torch.where(keep, lse - zt, 0.0)
+    g = torch.where(keep, gl.double(), 0.0)
+    p = soft * g[:, None]
+    dz = p.clone().scatter_add_(1, at, -g[:, None])
+    own = g.abs()
+    dz_tol = (p.abs() * (z_tol + lse_tol[:, None] + 2.0 ** -20) + dz.abs() * 2.0 ** (-22 if fp32 else -11)
+              + (2.0 ** -38 * own + 2.0 ** -126 * own.clamp_max(1.0))[:, None])
+
+    def product(x, x_tol, y, K):
+        out = x @ y
+        acc = K * 2.0 ** -24 + (2.0 ** -21 if fp32 else 0)
+        floor = 2.0 ** -126 * (K + 1) + (2.0 ** -25 if dtype == torch.float16 else 0)
+        return out, (x_tol + acc * x.abs()) @ y.abs() + u * out.abs() + floor
+
+    dh, dh_tol = product(dz, dz_tol, E, V)
+    if dtype != torch.float16:
+        dh_tol = dh_tol + 2.0 ** -39 * em.max() * dz.abs().sum(1)[:, None]
+    Hg = torch.where(own[:, None] > 0, H, 0.0)
+    de, de_tol = product(dz.t().contiguous(), dz_tol.t().contiguous(), Hg, R)
+    share = torch.where(own[:, None] > 0, dz.abs() / own[:, None].clamp_min(1e-300), 0.0)
+    de_tol = de_tol + 4 * 2.0 ** -39 * (own * Hg.abs().amax(1)).max() * share.sum(0)[:, None]
+    return {"loss": (loss, lse_tol + zt_tol + 2.0 ** -23 * zt.abs()), "lse": (lse, lse_tol), "dh": (dh, dh_tol),
+            "de": (de, de_tol)}
+
+
+def _check(got, want, rows=slice(None)):
+    for name, x in zip(("loss", "lse", "dh", "de"), got):
+        ref, tol = want[name]
+        if name == "de":
+            _near(name, x, (ref, tol))
+        else:
+            _near(name, x[rows], (ref[rows], tol[rows]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e4, 1e8, 1e13])
+@pytest.mark.parametrize("R,V,d", [(20, 300, 64), (100, 700, 96), (300, 2000, 128)])
+def test_one_large_row(gpu_lib, R, V, d, size, dtype):
+    """A token whose hidden row is far from the others' size (a diverged one, or
+    what stands in padding) changes no other token's loss and gradient."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    if dtype == torch.float16 and size > 1e4:
+        pytest.skip("past fp16's range")
+    print(f"one large row R={R} V={V} d={d} {dtype} {size}", flush=True)
+    h, e, t, gl, _ = _inputs(R, V, d, dtype, ignored=0.1)
+    t[:3] = torch.tensor([5, 6, 7], device="cuda")
+    t[R - 2] = 8
+    plain = vocab_cross_entropy_grads(h, e, t, gl)
+    h2 = h.clone()
+    h2[R - 2] *= size
+    got = vocab_cross_entropy_grads(h2, e, t, gl)
+    others = torch.arange(R, device="cuda") != R - 2
+    for a, b in zip(plain[:3], got[:3]):
+        assert torch.equal(a[others], b[others])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e4, 1e8, 1e13])
+@pytest.mark.parametrize("R,V,d", [(20, 300, 64), (100, 700, 96), (300, 2000, 128)])
+def test_one_large_word(gpu_lib, R, V, d, size, dtype):
+    """A word that its row bans (a large negative logit of every token) leaves
+    the other words' logits as they are; one with a row of nearly 0 too."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    if dtype == torch.float16 and size > 1e4:
+        pytest.skip("past fp16's range")
+    h, e, t, gl, _ = _inputs(R, V, d, dtype)
+    h[:, 3] = h[:, 3].abs() + 1
+    t[t == 11] = 12
+    e[11] = 0
+    e[11, 3] = -size
+    e[12] = e[12] / size
+    got = vocab_cross_entropy_grads(h, e, t, gl)
+    _check(got, _formula(h, e, t, gl))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
