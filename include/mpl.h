@@ -774,19 +774,23 @@ int mpl_layer_norm_bwd(const void* dy, int64_t dy_pitch, const void* x, int64_t 
  * as they lie and must have 16-byte aligned rows less than 2^23 elements apart.
  * d <= 65,536, (rows + vocab) d below 2^34 with d rounded up to 64, and less than
  * 2^23 tiles of 256 x 256 logits.  Sums are fp32; in z fp32 operands are held
- * to 2^-23 of each and 2^-39 of the largest of their row (hi + lo fp16 under a power
- * of two a row), and one that is not finite may give NaN where z is -inf.  target int64 [rows].  Deterministic.
+ * to 2^-23 of each and 2^-39 of the largest of their row, 2^-33 of a table row's (hi
+ * + lo fp16 under a power of two a row), and one that is not finite may give NaN
+ * where z is -inf.  target int64 [rows].  Deterministic.
  *
  * mpl_vocab_cross_entropy_bwd writes d_hidden [rows, d] and d_embedding [vocab,
  * d] (dense, of dtype; either may be NULL) from the forward's lse and the
  * gradients g_loss and g_lse of loss and lse (fp32 [rows]; either may be NULL,
  * for zeros): dz = (g_loss + g_lse) exp(z - lse) - g_loss [v = target], with
- * g_loss 0 where ignored, held in fp16 between the products (fp32: hi + lo, 2^-23
- * of each) under a power of two that leaves 2^-38 of the largest |g_loss| or
- * |g_loss + g_lse|.  bf16 operands are read as fp16 under a power of two of each
- * array there, exact above 2^-29 of its largest.  Up to 64 rows (fewer in 16 bits)
- * may keep dz and the operands of its products in fp32 instead.  rows > 0.  A row of an invalid
- * target makes both gradients NaN.
+ * g_loss 0 where ignored, held in fp16 between the products (fp32: hi + lo) under a
+ * power of two a token: to 2^-12 (2^-23) of itself and 2^-38 of the token's largest
+ * |g_loss| or |g_loss + g_lse|.  d_hidden takes the table and d_embedding each hidden
+ * row times its token's coefficient to 2^-23 of each and 2^-39 of the largest of them
+ * all in fp32, bf16 exactly above 2^-29 of it; fp16 tables as they are.  The gradients
+ * of up to 64 rows (fewer in 16 bits) keep dz and the operands in fp32 instead.
+ * rows > 0.  A row whose coefficients are 0 (ignored, g_lse 0) adds nothing to
+ * d_embedding, whatever it holds.  A row of an invalid target makes its d_hidden and
+ * all of d_embedding NaN.
  *
  * The workspace (256-byte aligned) takes mpl_vocab_cross_entropy_workspace_bytes
  * (0 for sizes out of range); calls that may run at the same time need one each.

@@ -69,13 +69,17 @@ def vocab_cross_entropy(hidden: torch.Tensor, embedding: torch.Tensor, targets: 
     differentiable as well (a z-loss, or logits' norms).  A mean over the
     counted tokens is loss.sum() / (targets != ignore_index).sum().
 
-    Logits are sums in fp32 of the exact products (fp32 operands are held to
-    2^-23 of each and 2^-39 of the largest of their row).  fp32 rows or table entries that are not finite may give NaN
+    Logits are sums in fp32 of the exact products (of more than 64 rows fp32
+    operands are held to 2^-23 of each and 2^-39 of the largest of their row, 2^-33
+    of a table row's).  fp32 rows or table entries that are not finite may give NaN
     where the formula has a logit of -inf.  Up to some 2^39 logits and 2^34
     elements of both arrays.
-    The gradients hold dz in fp16 under a power of two (fp32: hi and lo, to
-    2^-23), down to 2^-38 of the largest gradient of a token, those of few
-    tokens (64 in fp32) in fp32.  For gradients
+    The gradients hold dz in fp16 under a power of two a token (fp32: hi and lo,
+    to 2^-23), down to 2^-38 of the token's own gradient; the table in d hidden and
+    the tokens' weighted rows in d embedding down to 2^-39 of their largest (bf16
+    exactly above 2^-29 of it, fp16 tables as they are); those of few tokens (64 in
+    fp32) are in fp32.  A row that passes no gradient adds nothing to the table's,
+    whatever it holds: padding may be NaN.  For gradients
     inside a captured HIP graph use vocab_cross_entropy_grads."""
     _check(hidden, embedding, targets, "vocab_cross_entropy")
     autograd = torch.is_grad_enabled() and (hidden.requires_grad or embedding.requires_grad)

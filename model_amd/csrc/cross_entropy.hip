@@ -16,14 +16,16 @@
 //
 // Backward: the vocabulary goes in pieces of up to 512 MiB of dz.  A piece's
 // tiles of z are formed again from the same products and written as dz, fp16
-// under a power of two (fp32 calls: hi and lo); two products read it from there,
-// dz . embedding with its sums kept over the pieces, dz^T . hidden piece by
+// under a power of two a token (fp32 calls: hi and lo); two products read it from
+// there, dz . embedding with its sums kept over the pieces, dz^T . hidden piece by
 // piece.  Forming z again is the fourth product of size rows x vocab x d where
-// three would do with the logits in memory.  dz is fp16 for bf16 calls too (their
-// operands go through fp16 under a power of two of their own, which holds bf16
-// exactly): 8 bits of dz would put an error of bf16's own rounding into the
-// gradients before they are rounded (2-norm error 1.45 times that of fp32 sums
-// rounded once; 1.0 so).  Few tokens keep dz in fp32, by the same kernel as their
+// three would do with the logits in memory.  dz is fp16 for bf16 calls too (the
+// other operand of its products goes through fp16 under a power of two, exact
+// above 2^-29 of the largest there): 8 bits of dz would put an error of bf16's own
+// rounding into the gradients before they are rounded (2-norm error 1.45 times that
+// of fp32 sums rounded once; 1.0 so).  In fp16 calls dz's rounding is of the
+// result's size: 2-norm error 2.8e-4 where fp32 sums rounded once have 2.1e-4
+// (1,001 x 50,021 x 500); hi and lo would double two of the four products.  Few tokens keep dz in fp32, by the same kernel as their
 // forward, and one pass over the table makes both gradients (xent_few_kernel).
 //
 // Bound: the MFMAs.  At 16,384 x 131,072 x 1,024 bf16 the four products take 4.0,
@@ -37,6 +39,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "tile_mma.h"
@@ -44,24 +47,26 @@
 namespace mpl {
 namespace {
 
+typedef float f4 __attribute__((ext_vector_type(4)));
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Device scalars of a call (floats): the inverses of the powers of two that the
-// operands were multiplied by, and dz's with its inverse.
-enum { kInvE = 0, kInvH, kScaleP, kInvP, kScalars = 16 };
-
-// The operands of z in fp32 calls are split row by row: a hidden row and a word
-// each under a power of two of its own, which z's tile undoes, so that no row's
-// size costs another's logits bits.  The operands of the gradients' products are
-// summed over words or tokens, and have one power of two an array.
+// Powers of two.  z's fp32 operands are split row by row: a hidden row and a word
+// each under a power of its own, which z's tile undoes, so that no row's size costs
+// another's logits bits.  dz has a power a token, 2^c, undone in d hidden's rows;
+// in d embedding, which sums over tokens, the hidden rows carry 2^-c (and one power
+// for all): they come weighted by their tokens' coefficients, and tokens without
+// any as zeros, whatever their rows hold.  The table of dz . embedding, summed over
+// words, has one power for the array.
+//
+// Device scalars of a call: the powers that undo those of the table and of the
+// weighted hidden rows.
+enum { kUndoE = 0, kUndoH, kScalars = 16 };
 
 // The power that brings the largest magnitude, given by its bits, to [2^top,
 // 2^(top + 1)); 0 for 0.
 __device__ __forceinline__ int power_for(uint32_t bits, int top) {
   return bits == 0 ? 0 : max(-126, min(126, top + 127 - (int)(bits >> 23)));
-}
-__device__ __forceinline__ float scale_for(uint32_t bits, int top) {
-  return __uint_as_float((uint32_t)(127 + power_for(bits, top)) << 23);
 }
 // Magnitude bits of x, 0 if it is not finite.
 __device__ __forceinline__ uint32_t finite_bits(float x) {
@@ -83,12 +88,15 @@ struct PackOne {
 };
 struct PackArgs {
   PackOne e, h;  // embedding, hidden
-  int d, dpad;
-  float* scal;
-  uint32_t* part;  // [kAmaxBlocks] maxima of each array, and of the coefficients
-  bool coefs;
+  int d, dpad, width;  // width: lanes of a team
+  int* undo_e;         // of the rows (z's fp32 operands)
+  int* undo_h;
+  int* scal;
+  uint32_t* part;    // [kParts] of the table: largest magnitudes; of the weighted rows: their exponents
+  const int* power;  // of dz's rows
 };
-constexpr int kAmaxBlocks = 512;
+constexpr int kParts = 512;
+constexpr int kNoWeight = 1 << 16;  // the power of a token without coefficients
 
 // i / n in 32 bits where i allows it (wave-uniform branch mostly): a 64-bit
 // division is some hundred instructions.
@@ -96,137 +104,46 @@ __device__ __forceinline__ int64_t divide(int64_t i, int n) {
   return (uint64_t)i >> 32 ? i / n : (int64_t)((uint32_t)i / (uint32_t)n);
 }
 
-// Source types of packed operands and what becomes of them: 16-bit rows that are
-// only filled up; bf16 rows as scaled fp16; fp32 rows as scaled hi and lo.
-enum { kCopy16 = 0, kBf16ToF16, kSplit };
+// Types of rows and what becomes of them: 16-bit rows that are only filled up;
+// 16-bit rows as fp16 under a power of two; fp32 rows as hi and lo under one.
+enum { kCopy16 = 0, kBf16ToF16, kF16, kSplit };
 
-// 8 (fp32: 4) elements from element c of row r, zero past d.
+// 8 elements from element c of row r, zero past d.
 template <int MODE>
-struct Source {
-  static constexpr int VE = MODE == kSplit ? 4 : 8;
-  __device__ static void load(const PackOne& o, int64_t r, int64_t c, int64_t d, float (&v)[VE]) {
-    if constexpr (MODE == kSplit) {
-      const float* x = (const float*)o.src + r * o.pitch + c;
-      if (o.vec && c + VE <= d) {
-        *(float4*)v = *(const float4*)x;
+__device__ __forceinline__ void load8(const PackOne& o, int64_t r, int64_t c, int64_t d, float (&v)[8]) {
+  if constexpr (MODE == kSplit) {
+    const float* x = (const float*)o.src + r * o.pitch + c;
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+      if (o.vec && c + k + 4 <= d) {
+        *(float4*)(v + k) = *(const float4*)(x + k);
       } else {
 #pragma unroll
-        for (int j = 0; j < VE; ++j) v[j] = c + j < d ? x[j] : 0.f;
+        for (int j = k; j < k + 4; ++j) v[j] = c + j < d ? x[j] : 0.f;
       }
-    } else {  // bf16
-      const uint16_t* x = (const uint16_t*)o.src + r * o.pitch + c;
-      uint16_t u[VE] __attribute__((aligned(16)));
-      if (o.vec && c + VE <= d) {
-        *(uint4*)u = *(const uint4*)x;
-      } else {
-#pragma unroll
-        for (int j = 0; j < VE; ++j) u[j] = c + j < d ? x[j] : (uint16_t)0;
-      }
-#pragma unroll
-      for (int j = 0; j < VE; ++j) v[j] = __uint_as_float((uint32_t)u[j] << 16);
     }
-  }
-};
-
-// Coefficients of the rows [first, last) of dz (threads stride through them),
-// zero for those that only fill it up; their largest finite magnitude.
-struct CoefArgs {
-  const int64_t* target;
-  int64_t R, rows_p, V, ignore;
-  const float* g_loss;
-  const float* g_lse;
-  const float* lse;
-  float* coef;  // [3][rows_p]: g + gl, g, lse
-};
-__device__ __forceinline__ uint32_t coefficients(const CoefArgs& p, int64_t first, int64_t step) {
-  uint32_t m = 0;
-#pragma unroll 4
-  for (int64_t i = first; i < p.rows_p; i += step) {
-    float all = 0.f, g = 0.f, l = 0.f;
-    const int64_t k = min(i, p.R - 1);  // loads without branches, so that they fly together
-    const int64_t at = p.target[k];
-    const float gk = p.g_loss ? p.g_loss[k] : 0.f, sk = p.g_lse ? p.g_lse[k] : 0.f, lk = p.lse[k];
-    if (i < p.R) {
-      g = at == p.ignore ? 0.f : at < 0 || at >= p.V ? NAN : gk;
-      all = g + sk;
-      l = lk;
-    }
-    p.coef[i] = all;
-    p.coef[p.rows_p + i] = g;
-    p.coef[2 * p.rows_p + i] = l;
-    m = max(m, max(finite_bits(all), finite_bits(g)));
-  }
-  return m;
-}
-
-// The largest of a workgroup's THREADS values, in its first thread.
-template <int THREADS>
-__device__ __forceinline__ uint32_t block_max(uint32_t m) {
-  __shared__ uint32_t s[THREADS / 64];
-  for (int h = 32; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < THREADS / 64; ++i) m = max(m, s[i]);
-  return m;
-}
-
-// dz's power of two: |dz| <= |g + gl| + |g|, below 2^15 after it.
-__device__ __forceinline__ void write_scale_p(float* scal, uint32_t most) {
-  const float scale = scale_for(most, 13);
-  scal[kScaleP] = scale;
-  scal[kInvP] = 1.f / scale;
-}
-
-// The coefficients where the operands are read as they lie.  One workgroup.
-__global__ __launch_bounds__(1024) void xent_coef_kernel(CoefArgs p, float* __restrict__ scal) {
-  const uint32_t m = block_max<1024>(coefficients(p, threadIdx.x, 1024));
-  if (threadIdx.x == 0) write_scale_p(scal, m);
-}
-
-// Largest finite magnitudes of both arrays, one partial maximum a workgroup; in
-// the backward a third row of workgroups forms the coefficients.
-template <int MODE>
-__global__ __launch_bounds__(256) void amax_kernel(PackArgs p, CoefArgs q) {
-  constexpr int VE = Source<MODE>::VE;
-  const int a = blockIdx.y;
-  if (a == 2) {
-    const uint32_t m = block_max<256>(coefficients(q, blockIdx.x * 256 + threadIdx.x, 256 * (int64_t)gridDim.x));
-    if (threadIdx.x == 0) p.part[2 * kAmaxBlocks + blockIdx.x] = m;
-    return;
-  }
-  const PackOne o = a ? p.h : p.e;
-  const int vecs = (p.d + VE - 1) / VE;
-  const int64_t n = o.rows * vecs, step = 256 * (int64_t)gridDim.x;
-  uint32_t m = 0;
-  auto take = [&](int64_t r, int64_t c, int64_t d) __attribute__((always_inline)) {
-    float v[VE];
-    Source<MODE>::load(o, r, c, d, v);
-#pragma unroll
-    for (int j = 0; j < VE; ++j) m = max(m, finite_bits(v[j]));
-  };
-  int64_t i = blockIdx.x * 256 + threadIdx.x;
-  if (o.vec && o.pitch == p.d && p.d % VE == 0) {  // one long row
-    for (; i + 7 * step < n; i += 8 * step) {  // 8 loads in flight
-#pragma unroll
-      for (int k = 0; k < 8; ++k) take(0, VE * (i + k * step), VE * n);
-    }
-    for (; i < n; i += step) take(0, VE * i, VE * n);
   } else {
-    for (; i < n; i += step) {
-      const int64_t r = divide(i, vecs);
-      take(r, VE * (i - r * vecs), p.d);
+    const uint16_t* x = (const uint16_t*)o.src + r * o.pitch + c;
+    uint16_t u[8] __attribute__((aligned(16)));
+    if (o.vec && c + 8 <= d) {
+      *(uint4*)u = *(const uint4*)x;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = c + j < d ? x[j] : (uint16_t)0;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = MODE == kBf16ToF16 ? __uint_as_float((uint32_t)u[j] << 16) : (float)__builtin_bit_cast(_Float16, u[j]);
   }
-  m = block_max<256>(m);
-  if (threadIdx.x == 0) p.part[a * kAmaxBlocks + blockIdx.x] = m;
 }
-
-__device__ __forceinline__ void load_split(const PackOne& o, int64_t r, int64_t c, int64_t d, float (&v)[8]) {
-  Source<kSplit>::load(o, r, c, d, *(float(*)[4])v);
-  Source<kSplit>::load(o, r, c + 4, d, *(float(*)[4])(v + 4));
+__device__ __forceinline__ uint32_t most_of(const float (&v)[8], uint32_t most) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) most = max(most, finite_bits(v[j]));
+  return most;
 }
-__device__ __forceinline__ void store_split(char* dst, int64_t r, int64_t dpad, int c, const float (&v)[8], int power) {
+// ... and what is written of them, under a power of two.
+template <int MODE>
+__device__ __forceinline__ void store8(char* dst, int64_t r, int64_t dpad, int c, const float (&v)[8], int power) {
   half8 hi, lo;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -234,48 +151,202 @@ __device__ __forceinline__ void store_split(char* dst, int64_t r, int64_t dpad, 
     hi[j] = (_Float16)y;
     lo[j] = (_Float16)(y - (float)hi[j]);
   }
-  char* q = dst + (r * dpad + c / 32 * 32) * 4 + (c % 32) * 2;
-  *(half8*)q = hi;
-  *(half8*)(q + 64) = lo;
+  if constexpr (MODE == kSplit) {
+    char* q = dst + (r * dpad + c / 32 * 32) * 4 + (c % 32) * 2;
+    *(half8*)q = hi;
+    *(half8*)(q + 64) = lo;
+  } else {
+    *(half8*)(dst + (r * dpad + c) * 2) = hi;
+  }
 }
 
-// Rows of an array as a tile product's operand, zero-filled to whole stages.  A
-// thread writes 8 elements.
+// A token's coefficients, under a power of two that leaves |dz| <= |g + gl| + |g|
+// below 2^15: zeros for rows of dz that only fill it up (i >= R).  Returns the
+// exponent of the hidden row's largest magnitude (its bits `most`) times the
+// coefficients, from 1 on, 0 for none.
+struct CoefArgs {
+  const int64_t* target;
+  int64_t R, rows_p, V, ignore;
+  const float* g_loss;
+  const float* g_lse;
+  const float* lse;
+  float* coef;  // [3][rows_p]: (g + gl) 2^c, g 2^c, lse
+  int* power;   // [rows_p]: c
+};
+constexpr int kExponents = 512;  // what makes those exponents positive
+__device__ __forceinline__ uint32_t coefficients(const CoefArgs& p, int64_t i, uint32_t most) {
+  float all = 0.f, g = 0.f, l = 0.f;
+  if (i < p.R) {
+    const int64_t at = p.target[i];
+    g = at == p.ignore || !p.g_loss ? 0.f : p.g_loss[i];
+    if (at != p.ignore && (at < 0 || at >= p.V)) g = NAN;
+    all = g + (p.g_lse ? p.g_lse[i] : 0.f);
+    l = p.lse[i];
+  }
+  const int c = power_for(max(finite_bits(all), finite_bits(g)), 13);
+  const bool weighs = all != 0.f || g != 0.f;
+  p.coef[i] = ldexpf(all, c);
+  p.coef[p.rows_p + i] = ldexpf(g, c);
+  p.coef[2 * p.rows_p + i] = l;
+  p.power[i] = weighs ? c : kNoWeight;
+  return weighs && most ? kExponents + (int)(most >> 23) - c : 0;
+}
+
+// The largest of a workgroup's values, in every thread.
+__device__ __forceinline__ uint32_t block_max(uint32_t m) {
+  __shared__ uint32_t s[4];
+  for (int h = 32; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, s[i]);
+  return m;
+}
+
+// The largest of a value that a team's lanes hold.
+__device__ __forceinline__ uint32_t team_max(uint32_t m, int width) {
+  for (int h = width / 2; h; h >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, h));
+  return m;
+}
+
+// 16-bit calls' backward: the coefficients with the exponents of the weighted
+// hidden rows (blockIdx.y = 0; a team of `width` lanes a row), and for bf16 the
+// table's largest magnitude (1).
 template <int MODE>
-__global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
-  const int a = blockIdx.x < p.e.blocks ? 0 : 1;
-  const PackOne o = a ? p.h : p.e;
-  int power = 0;
-  if constexpr (MODE != kCopy16) {
-    auto most = [&](int k) __attribute__((always_inline)) {
-      const uint32_t* q = p.part + k * kAmaxBlocks + threadIdx.x;
-      return block_max<256>(max(q[0], q[256]));
+__global__ __launch_bounds__(256) void weigh_kernel(PackArgs p, CoefArgs q) {
+  const PackOne o = blockIdx.y ? p.e : p.h;
+  const int vecs = (p.d + 7) / 8;
+  uint32_t m = 0;
+  if (blockIdx.y == 0) {
+    const int lane = threadIdx.x & (p.width - 1);
+    const int64_t teams = (int64_t)gridDim.x * (256 / p.width);
+    for (int64_t r = (int64_t)blockIdx.x * (256 / p.width) + threadIdx.x / p.width; r < q.rows_p; r += teams) {
+      uint32_t most = 0;
+      for (int c = r < o.rows ? lane : vecs; c < vecs; c += p.width) {
+        float v[8];
+        load8<MODE>(o, r, 8 * c, p.d, v);
+        most = most_of(v, most);
+      }
+      most = team_max(most, p.width);
+      if (lane == 0) m = max(m, coefficients(q, r, most));
+    }
+  } else {
+    const int64_t n = o.rows * vecs, step = 256 * (int64_t)gridDim.x;
+    auto take = [&](int64_t r, int64_t c, int64_t d) __attribute__((always_inline)) {
+      float v[8];
+      load8<MODE>(o, r, c, d, v);
+      m = most_of(v, m);
     };
-    power = power_for(most(a), 14);
-    if (threadIdx.x == 0 && (blockIdx.x == 0 || blockIdx.x == p.e.blocks))
-      p.scal[a == 0 ? kInvE : kInvH] = __uint_as_float((uint32_t)(127 - power) << 23);
-    if (p.coefs && blockIdx.x == 0) {
-      __syncthreads();  // block_max's words are used again
-      const uint32_t m = most(2);
-      if (threadIdx.x == 0) write_scale_p(p.scal, m);
+    int64_t i = blockIdx.x * 256 + threadIdx.x;
+    if (o.vec && o.pitch == p.d && p.d % 8 == 0) {  // one long row
+      for (; i + 7 * step < n; i += 8 * step) {  // 8 loads in flight
+#pragma unroll
+        for (int k = 0; k < 8; ++k) take(0, 8 * (i + k * step), 8 * n);
+      }
+      for (; i < n; i += step) take(0, 8 * i, 8 * n);
+    } else {
+      for (; i < n; i += step) {
+        const int64_t r = divide(i, vecs);
+        take(r, 8 * (i - r * vecs), p.d);
+      }
     }
   }
+  m = block_max(m);
+  if (threadIdx.x == 0) p.part[blockIdx.y * kParts + blockIdx.x] = m;
+}
+
+// fp32 rows of both arrays as z's operands: hi and lo under a power of two a row,
+// whose undoing power is written beside.  Of a group of 32 words those whose largest
+// is within 2^-kNear of the group's take the group's power (at the cost of that many
+// of 39 bits): z's tiles then undo one power a fragment.  A workgroup takes 32 rows,
+// 8 lanes each, which hold their first kHold vectors of 8.  BWD: with weigh_kernel's
+// part.
+constexpr int kNear = 6;
+template <bool BWD>
+__global__ __launch_bounds__(256) void split_rows_kernel(PackArgs p, CoefArgs q) {
+  constexpr int kHold = 4;
+  __shared__ uint32_t largest[32];
+  const bool hidden = blockIdx.y == 0;
+  const PackOne o = hidden ? p.h : p.e;
+  int* undo = hidden ? p.undo_h : p.undo_e;
+  const int lane = threadIdx.x & 7, row = threadIdx.x >> 3, vecs = p.dpad / 8;
+  const int64_t rows = BWD && hidden ? q.rows_p : o.rows;
+  uint32_t m = 0;
+  for (int64_t r0 = 32 * (int64_t)blockIdx.x; r0 < rows; r0 += 32 * (int64_t)gridDim.x) {
+    const int64_t r = r0 + row;
+    const int all = r < o.rows ? vecs : 0;
+    float v[kHold][8];
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) {
+      const int c = lane + 8 * k;
+      if (c >= all) continue;
+      load8<kSplit>(o, r, 8 * c, p.d, v[k]);
+      most = most_of(v[k], most);
+    }
+    for (int c = lane + 8 * kHold; c < all; c += 8) {
+      float u[8];
+      load8<kSplit>(o, r, 8 * c, p.d, u);
+      most = most_of(u, most);
+    }
+    most = team_max(most, 8);
+    uint32_t shared = most;
+    if (!hidden) {
+      if (lane == 0) largest[row] = most;
+      __syncthreads();
+      uint32_t group = largest[threadIdx.x & 31];
+      group = team_max(group, 32);
+      if (most == 0 || (most >> 23) + kNear >= group >> 23) shared = group;
+      __syncthreads();
+    }
+    const int power = power_for(shared, 14);
+    if (lane == 0 && all) undo[r] = -power;
+#pragma unroll
+    for (int k = 0; k < kHold; ++k)
+      if (lane + 8 * k < all) store8<kSplit>(o.dst, r, p.dpad, 8 * (lane + 8 * k), v[k], power);
+    for (int c = lane + 8 * kHold; c < all; c += 8) {
+      float u[8];
+      load8<kSplit>(o, r, 8 * c, p.d, u);
+      store8<kSplit>(o.dst, r, p.dpad, 8 * c, u, power);
+    }
+    if (BWD && !hidden) m = max(m, most);
+    if (BWD && hidden && lane == 0 && r < rows) m = max(m, coefficients(q, r, most));
+  }
+  if (!BWD) return;
+  m = block_max(m);
+  if (threadIdx.x == 0) p.part[blockIdx.y * kParts + blockIdx.x] = m;
+}
+
+// Rows of an array as a tile product's operand, zero-filled to whole stages: z's
+// (kCopy16), or the gradients' products'.  A thread writes 8 elements.
+template <int MODE>
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
+  const bool hidden = blockIdx.x >= p.e.blocks;
+  const PackOne o = hidden ? p.h : p.e;
+  int power = 0;
+  if constexpr (MODE != kCopy16) {
+    const uint32_t* q = p.part + (hidden ? 0 : kParts) + threadIdx.x;
+    const uint32_t most = block_max(max(q[0], q[256]));
+    power = !hidden ? power_for(most, 14) : most ? 14 + 127 + kExponents - (int)most : 0;
+    if (threadIdx.x == 0 && (blockIdx.x == 0 || blockIdx.x == p.e.blocks)) p.scal[hidden ? kUndoH : kUndoE] = -power;
+  }
   const int per = p.dpad / 8;
-  const int64_t i = (int64_t)(blockIdx.x - (a ? p.e.blocks : 0)) * 256 + threadIdx.x;
+  const int64_t i = (int64_t)(blockIdx.x - (hidden ? p.e.blocks : 0)) * 256 + threadIdx.x;
   if (i >= o.rows * per) return;
   const int64_t r = divide(i, per);
   const int c = 8 * (int)(i - r * per);
-  if constexpr (MODE == kSplit) {
+  if constexpr (MODE != kCopy16) {
     float v[8];
-    load_split(o, r, c, p.d, v);
-    store_split(o.dst, r, p.dpad, c, v, power);
-  } else if constexpr (MODE == kBf16ToF16) {
-    float v[8];
-    Source<MODE>::load(o, r, c, p.d, v);
-    half8 h;
+    load8<MODE>(o, r, c, p.d, v);
+    if (hidden) {
+      const int weight = p.power[r];
+      power -= weight;
+      if (weight == kNoWeight) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] = (_Float16)ldexpf(v[j], power);
-    *(half8*)(o.dst + (r * p.dpad + c) * 2) = h;
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      }
+    }
+    store8<MODE>(o.dst, r, p.dpad, c, v, power);
   } else {
     const uint16_t* x = (const uint16_t*)o.src + r * o.pitch + c;
     uint16_t v[8] __attribute__((aligned(16)));
@@ -289,70 +360,21 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   }
 }
 
-// fp32 rows of both arrays as z's operands: hi and lo under the row's own power of
-// two, whose undoing power is written beside.  A team of `width` lanes takes a row
-// and holds its first kHold vectors of 8 a lane.
-struct SplitArgs {
-  PackOne e, h;
-  int d, dpad, width;
-  int* undo_e;
-  int* undo_h;
-};
-__global__ __launch_bounds__(256) void split_rows_kernel(SplitArgs p) {
-  constexpr int kHold = 2;
-  const PackOne o = blockIdx.y ? p.h : p.e;
-  int* undo = blockIdx.y ? p.undo_h : p.undo_e;
-  const int lane = threadIdx.x & (p.width - 1), vecs = p.dpad / 8;
-  const int64_t teams = (int64_t)gridDim.x * (256 / p.width);
-  for (int64_t r = (int64_t)blockIdx.x * (256 / p.width) + threadIdx.x / p.width; r < o.rows; r += teams) {
-    float v[kHold][8];
-    uint32_t most = 0;
-    auto take = [&](const float(&u)[8]) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most = max(most, finite_bits(u[j]));
-    };
-#pragma unroll
-    for (int k = 0; k < kHold; ++k) {
-      const int c = lane + k * p.width;
-      if (c >= vecs) continue;
-      load_split(o, r, 8 * c, p.d, v[k]);
-      take(v[k]);
-    }
-    for (int c = lane + kHold * p.width; c < vecs; c += p.width) {
-      float u[8];
-      load_split(o, r, 8 * c, p.d, u);
-      take(u);
-    }
-    for (int h = p.width / 2; h; h >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, h));  // a team's lanes
-    const int power = power_for(most, 14);
-    if (lane == 0) undo[r] = -power;
-#pragma unroll
-    for (int k = 0; k < kHold; ++k)
-      if (lane + k * p.width < vecs) store_split(o.dst, r, p.dpad, 8 * (lane + k * p.width), v[k], power);
-    for (int c = lane + kHold * p.width; c < vecs; c += p.width) {
-      float u[8];
-      load_split(o, r, 8 * c, p.d, u);
-      store_split(o.dst, r, p.dpad, 8 * c, u, power);
-    }
-  }
-}
-
 // ------------------------------------------------------------------ forward
 struct LogitArgs {
   TileOperand E, H;
   int64_t R, V;
   int iters;
   uint32_t tiles_v, tiles_t;
-  const int* undo_e;  // fp32 calls: the powers that undo those of the words (to up(V, 256)) and of the rows
+  const int* undo_e;  // fp32 calls: the powers that undo those of the words and of the hidden rows
   const int* undo_h;
-  const float* scal;
   const int64_t* target;
   // forward
   float2* part;  // [tiles_v][R]: maximum of z, sum of exp(z - maximum)
   float* z_target;
   // backward: the piece starts at row v0 of the table
   int64_t v0, rows_p, pitch_p;  // rows_p: rows of dz that exist (zero past R); pitch in bytes
-  const float* coef;            // [3][rows_p]: g + gl, g, lse
+  const float* coef;            // [3][rows_p]: (g + gl) 2^c, g 2^c, lse
   char* P;
   bool stream;  // dz is written past the caches
 };
@@ -370,28 +392,55 @@ __device__ __forceinline__ float exp_below(float z, float at) {
   __shared__ __attribute__((aligned(1024))) char a1[C::kStageA]; \
   __shared__ __attribute__((aligned(1024))) char b1[C::kStageB];
 
-// The powers that undo those of a tile's words, in LDS before the tile's product
-// (whose barriers show them to all waves); and a lane's accumulators of token
-// `undo_h` as z: a product of the two powers need not be a finite number, their sum
-// is one power.
-template <class C>
-__device__ __forceinline__ void hold_undo(const int* undo_e, int64_t v0, int* undo) {
-  if (C::S == 2)
-    for (int i = threadIdx.x; i < C::BM; i += C::kThreads) undo[i] = undo_e[v0 + i];
+// What undoes the powers of a tile's words and of a lane's tokens (S = 2): z is an
+// accumulator times 2^(word's + token's), no product of two powers, which may pass
+// fp32's range on the way.  The 32 words of a fragment nearly always share one
+// (kNear), and then the factor is one for all of a lane's accumulators there and
+// costs no operation: it makes the difference in exp_below a fused multiply-add.
+// 8,192 x 16,384 x 256 fp32, z's kernels without powers a row 196 and 253 us, so 203
+// and 268 (v_ldexp by every word's own: 237 and 308).  The words' lie in LDS since
+// before the tile's product, whose barriers show them to all waves.
+__device__ __forceinline__ float power_of_2(int e) {
+  return __uint_as_float((uint32_t)(127 + max(-126, min(127, e))) << 23);
 }
 template <class C>
-__device__ __forceinline__ void undo_powers(f32x16& acc, const int* undo, int undo_h) {
-  if (C::S == 2) {
+__device__ __forceinline__ void hold_undo(const int* undo_e, int64_t v0, int64_t V, int* undo) {
+  if (C::S == 2)
+    for (int i = threadIdx.x; i < C::BM; i += C::kThreads) undo[i] = undo_e[min(v0 + i, V - 1)];
+}
+// The tokens' powers are read before the product too: behind it a tile would wait
+// for them.
+template <class C>
+struct Undo {
+  const int* words;  // of acc[0][.][0]
+  int first[C::TM], token[C::TN];
+  bool shared;  // by the words of each fragment
+  __device__ __forceinline__ Undo(const int* undo_h, int64_t tok, int64_t R) {
+    if constexpr (C::S == 2) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int4 k = *(const int4*)(undo + 8 * q);
-      acc[4 * q] = ldexpf(acc[4 * q], undo_h + k.x);
-      acc[4 * q + 1] = ldexpf(acc[4 * q + 1], undo_h + k.y);
-      acc[4 * q + 2] = ldexpf(acc[4 * q + 2], undo_h + k.z);
-      acc[4 * q + 3] = ldexpf(acc[4 * q + 3], undo_h + k.w);
+      for (int j = 0; j < C::TN; ++j) token[j] = undo_h[min(tok + 32 * j, R - 1)];
     }
   }
-}
+  __device__ __forceinline__ void behind_product(const int* undo, int lane) {
+    shared = true;
+    if constexpr (C::S == 2) {
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i) {
+        const int u = undo[32 * i + (lane & 31)];
+        first[i] = __builtin_amdgcn_readfirstlane(u);
+        shared = shared && __all(u == first[i]);
+      }
+      words = undo + 4 * (lane >> 5);
+    }
+  }
+  // of accumulator r (SHARED: of all) of fragment i, j
+  template <bool SHARED>
+  __device__ __forceinline__ float factor(int i, int j, int r) const {
+    if constexpr (C::S == 1) return 1.f;
+    else if constexpr (SHARED) return power_of_2(first[i] + token[j]);
+    else return power_of_2(words[32 * i + 8 * (r >> 2) + (r & 3)] + token[j]);
+  }
+};
 
 template <class C>
 __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
@@ -402,17 +451,16 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
   tile_of(blockIdx.x, gridDim.x, p.tiles_v, p.tiles_t, 8, tv, tt);
   const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
   f32x16 acc[C::TM][C::TN];
-  __shared__ __attribute__((aligned(16))) int undo[C::S == 2 ? C::BM : 1];
-  hold_undo<C>(p.undo_e, v0, undo);
+  __shared__ int undo[C::S == 2 ? C::BM : 1];
+  hold_undo<C>(p.undo_e, v0, p.V, undo);
+  Undo<C> z_of(p.undo_h, t0 + wn * C::TN * 32 + (lane & 31), p.R);
   C::run(p.E, p.H, v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
   const int64_t vw = v0 + wm * C::TM * 32 + 4 * (lane >> 5);  // of acc[0][.][0]
+  z_of.behind_product(undo + wm * C::TM * 32, lane);
   float2* pair = (float2*)a0;  // [WM][BN]: the stages are free
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) {
     const int64_t tok = t0 + (wn * C::TN + j) * 32 + (lane & 31);
-    const int undo_h = C::S == 2 ? p.undo_h[min(tok, p.R - 1)] : 0;
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i) undo_powers<C>(acc[i][j], undo + (wm * C::TM + i) * 32 + 4 * (lane >> 5), undo_h);
     const int64_t at = tok < p.R ? p.target[tok] - vw : -1;  // place of the target among the lane's, if it is there
     const int place = at >= 0 && at < C::TM * 32 && !(at & 4) ? (int)at : -1;
     if (__any(place >= 0)) {
@@ -421,7 +469,7 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
       for (int i = 0; i < C::TM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) z = place == 32 * i + 8 * (r >> 2) + (r & 3) ? acc[i][j][r] : z;
-      if (place >= 0) p.z_target[tok] = z;
+      if (place >= 0) p.z_target[tok] = C::S == 2 ? z * power_of_2(z_of.words[place] + z_of.token[j]) : z;
     }
     if (v0 + C::BM > p.V) {
 #pragma unroll
@@ -430,20 +478,28 @@ __global__ __launch_bounds__(C::kThreads) void xent_lse_kernel(LogitArgs p) {
         for (int r = 0; r < 16; ++r)
           if (vw + 32 * i + 8 * (r >> 2) + (r & 3) >= p.V) acc[i][j][r] = -INFINITY;
     }
-    float m = acc[0][j][0];
+    float m = -INFINITY, s = 0.f, x, y;
+    auto sums = [&](auto shared) __attribute__((always_inline)) {
+      constexpr bool SHARED = decltype(shared)::value;
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i)
+      for (int i = 0; i < C::TM; ++i) {
+        float most = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
-    float x = m, y = m;
-    half_swap(x, y);
-    m = fmaxf(x, y);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
+        for (int r = 0; r < 16; ++r)
+          most = fmaxf(most, SHARED ? acc[i][j][r] : acc[i][j][r] * z_of.template factor<false>(i, j, r));
+        m = fmaxf(m, SHARED ? most * z_of.template factor<true>(i, j, 0) : most);
+      }
+      x = m, y = m;
+      half_swap(x, y);
+      m = fmaxf(x, y);
+      const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i)
+      for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s += exp_below(acc[i][j][r], ref);
+        for (int r = 0; r < 16; ++r) s += exp_below(acc[i][j][r] * z_of.template factor<SHARED>(i, j, r), ref);
+    };
+    if (C::S == 1 || z_of.shared) sums(std::true_type{});
+    else sums(std::false_type{});
     x = s, y = s;
     half_swap(x, y);
     if (lane < 32) pair[wm * C::BN + (wn * C::TN + j) * 32 + lane] = make_float2(m, x + y);
@@ -676,10 +732,10 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
   tile_of(blockIdx.x, gridDim.x, p.tiles_v, p.tiles_t, 8, tv, tt);
   const int64_t v0 = (int64_t)tv * C::BM, t0 = (int64_t)tt * C::BN;
   f32x16 acc[C::TM][C::TN];
-  __shared__ __attribute__((aligned(16))) int undo[C::S == 2 ? C::BM : 1];
-  hold_undo<C>(p.undo_e, p.v0 + v0, undo);
+  __shared__ int undo[C::S == 2 ? C::BM : 1];
+  hold_undo<C>(p.undo_e, p.v0 + v0, p.V, undo);
+  Undo<C> z_of(p.undo_h, t0 + wn * C::TN * 32 + (lane & 31), p.R);
   C::run(p.E, p.H, p.v0 + v0, t0, 0, p.iters, a0, b0, a1, b1, acc);
-  const float up = p.scal[kScaleP];
   const int half = lane >> 5;
   const int64_t vw = v0 + wm * C::TM * 32;  // the wave's first column of the piece
   // 32 tokens' rows of the wave go through LDS (the stages are free), so that a
@@ -689,26 +745,30 @@ __global__ __launch_bounds__(C::kThreads) void xent_dz_kernel(LogitArgs p) {
   static_assert(kWaves * 32 * ROW <= C::kStageA && kWaves * 32 * ROW <= C::kStageB, "");
   const int place = wave / kWaves;
   char* rows = (place == 0 ? a0 : place == 1 ? b0 : place == 2 ? a1 : b1) + wave % kWaves * 32 * ROW;
+  z_of.behind_product(undo + wm * C::TM * 32, lane);
   auto piece = [&](int t, int c) __attribute__((always_inline)) {
     return (uint4*)(rows + t * ROW + ((c ^ (t & 15 & (kPieces - 1))) << 4));
   };
 #pragma unroll
   for (int j = 0; j < C::TN; ++j) {
     const int64_t tok = t0 + (wn * C::TN + j) * 32 + (lane & 31);
-    const bool there = tok < p.R;
     const int64_t row = min(tok, p.rows_p - 1);
-    const float ga = p.coef[row] * up, gb = p.coef[p.rows_p + row] * up, lse = p.coef[2 * p.rows_p + row];
+    const float ga = p.coef[row], gb = p.coef[p.rows_p + row], lse = p.coef[2 * p.rows_p + row];
+    const bool there = tok < p.R && (ga != 0.f || gb != 0.f);  // else dz is 0, whatever z is
     const int64_t at = (there ? p.target[tok] - p.v0 : -1) - (vw + 4 * half);
     const int to = at >= 0 && at < C::TM * 32 ? (int)at : -1;
     const bool hit = __any(to >= 0);
     const bool edge = p.v0 + v0 + C::BM > p.V;
-    const int undo_h = C::S == 2 ? p.undo_h[min(tok, p.R - 1)] : 0;
 #pragma unroll
     for (int i = 0; i < C::TM; ++i) {
-      undo_powers<C>(acc[i][j], undo + (wm * C::TM + i) * 32 + 4 * half, undo_h);
       float x[16];
+      auto soft = [&](auto shared) __attribute__((always_inline)) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = ga * exp_below(acc[i][j][r], lse);
+        for (int r = 0; r < 16; ++r)
+          x[r] = ga * exp_below(acc[i][j][r] * z_of.template factor<decltype(shared)::value>(i, j, r), lse);
+      };
+      if (C::S == 1 || z_of.shared) soft(std::true_type{});
+      else soft(std::false_type{});
       if (hit) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -773,8 +833,8 @@ struct GradArgs {
   int64_t rows;
   int cols, iters, splits;
   uint32_t tiles_m, tiles_n;
-  const float* u0;  // device scalars that undo the operands' scaling
-  const float* u1;
+  const int* undo;   // device scalar: the power that undoes the operands', or null
+  const int* power;  // those of dz's rows, where they are the output's, or null
   float* part;  // [splits][rows][cols] sums, or null: the result goes to out
   bool add;     // onto what part holds
   void* out;
@@ -790,9 +850,9 @@ __device__ __forceinline__ void store_as(void* out, int64_t i, float x, int dtyp
 // DTYPE: of what is stored, fp32 sums or the result; ADD: onto the sums there.
 template <class C, int DTYPE, bool ADD>
 __device__ __forceinline__ void grad_store(const GradArgs& p, const f32x16 (&acc)[C::TM][C::TN], int64_t m0, int n0,
-                                           int wm, int wn, int lane, void* out, bool whole) {
+                                           int wm, int wn, int lane, const int* powers, void* out, bool whole) {
   constexpr int size = DTYPE == MPL_F32 ? 4 : 2;
-  const float u0 = *p.u0, u1 = p.u1 ? *p.u1 : 1.f;
+  const int undo = p.undo ? *p.undo : 0;
   // the tile's rows from a scalar address, the lane's place in 32 bits
   char* base = (char*)out + m0 * p.cols * size;
   const int last = (int)min(p.rows - m0, (int64_t)C::BM);
@@ -804,6 +864,13 @@ __device__ __forceinline__ void grad_store(const GradArgs& p, const f32x16 (&acc
       const int row0 = (wm * C::TM + i) * 32 + 4 * (lane >> 5);
       const uint32_t at = (uint32_t)(row0 * p.cols + col) * size;
       const int rows = col < p.cols ? last - row0 : 0;  // below it there are rows
+      int power[16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int4 w = p.power ? *(const int4*)(powers + row0 + 8 * q) : int4{};
+        power[4 * q] = undo - w.x, power[4 * q + 1] = undo - w.y;
+        power[4 * q + 2] = undo - w.z, power[4 * q + 3] = undo - w.w;
+      }
       float old[16];
       if (ADD) {
 #pragma unroll
@@ -815,7 +882,7 @@ __device__ __forceinline__ void grad_store(const GradArgs& p, const f32x16 (&acc
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int step = 8 * (r >> 2) + (r & 3);
-        float x = acc[i][j][r] * u0 * u1;
+        float x = ldexpf(acc[i][j][r], power[r]);
         if (ADD) x += old[r];
         char* q = base + (int64_t)step * p.cols * size + at;
         if (whole || step < rows) store_as(q, 0, x, DTYPE);
@@ -836,13 +903,17 @@ __global__ __launch_bounds__(C::kThreads) void xent_grad_kernel(GradArgs p) {
   const int split = blockIdx.y;
   const int it0 = (int)((int64_t)p.iters * split / p.splits), it1 = (int)((int64_t)p.iters * (split + 1) / p.splits);
   f32x16 acc[C::TM][C::TN];
+  // dz's powers, shown to all waves by the product's barriers
+  __shared__ __attribute__((aligned(16))) int powers[C::BM];
+  if (p.power)
+    for (int i = tid; i < C::BM; i += C::kThreads) powers[i] = p.power[min(m0 + i, p.rows - 1)];
   C::run(p.A, p.B, m0, n0, it0, it1, a0, b0, a1, b1, acc);
   float* part = p.part + (int64_t)split * p.rows * p.cols;
   const bool whole = m0 + C::BM <= p.rows && n0 + C::BN <= p.cols;
 #define MPL_STORE(DTYPE, ADD, out)                                                      \
   do {                                                                                  \
-    if (whole) grad_store<C, DTYPE, ADD>(p, acc, m0, n0, wm, wn, lane, out, true);      \
-    else grad_store<C, DTYPE, ADD>(p, acc, m0, n0, wm, wn, lane, out, false);           \
+    if (whole) grad_store<C, DTYPE, ADD>(p, acc, m0, n0, wm, wn, lane, powers, out, true);      \
+    else grad_store<C, DTYPE, ADD>(p, acc, m0, n0, wm, wn, lane, powers, out, false);           \
   } while (0)
   if (p.part && p.add) MPL_STORE(MPL_F32, true, part);
   else if (p.part) MPL_STORE(MPL_F32, false, part);
@@ -875,7 +946,6 @@ struct FewArgs {
   float* part;      // [workgroups.x][R][d], or null
 };
 
-typedef float f4 __attribute__((ext_vector_type(4)));
 // 4 elements of any alignment, kept as they are until a product takes them.
 template <typename T>
 struct Four {
@@ -1049,7 +1119,7 @@ template <int S, bool BF, bool AST, bool BST> using Mid = TileMma<S, BF, AST, BS
 struct Plan {
   int64_t rows_p, v_piece, pieces;
   int dpad;
-  int mode_z, mode;  // what the operands of z and of the gradients need, -1 nothing (the gradients: z's serve)
+  int mode_z, mode;  // what the operands of z need (-1: nothing), and those of the gradients
   bool split;
   bool big_z, big_h, big_e;
   uint32_t tiles_v;    // of the forward
@@ -1057,7 +1127,7 @@ struct Plan {
   int few, parts;      // few-token backward: blocks of 32 tokens, parts of d hidden's sums
   int splits_h, splits_e;
   // offsets into the workspace
-  size_t scal, amax, ze, zh, undo_e, undo_h, e, h, part, zt, coef, P, ph, pe, bytes;
+  size_t scal, maxima, ze, zh, undo_e, undo_h, e, h, power, part, zt, coef, P, ph, pe, bytes;
 };
 
 constexpr int64_t kPieceBytes = 512ll << 20;
@@ -1092,7 +1162,7 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
   p.split = dtype == MPL_F32;
   const int S = p.split ? 2 : 1;
   p.mode_z = p.split ? kSplit : d % 64 ? kCopy16 : -1;
-  p.mode = p.split ? kSplit : dtype == MPL_BF16 ? kBf16ToF16 : -1;
+  p.mode = p.split ? kSplit : dtype == MPL_BF16 ? kBf16ToF16 : kF16;
   p.dpad = (int)up(d, 64);
   p.rows_p = up(R, 64);
   p.big_z = cdiv(R, 256) * cdiv(V, 256) >= 256;
@@ -1122,7 +1192,7 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
   }
   p.ze = take(p.mode_z >= 0 ? (size_t)V * p.dpad * 2 * S : 0);
   p.zh = take(p.mode_z >= 0 ? (size_t)R * p.dpad * 2 * S : 0);
-  p.undo_e = take(p.split ? (size_t)up(V, 256) * 4 : 0);
+  p.undo_e = take(p.split ? (size_t)V * 4 : 0);
   p.undo_h = take(p.split ? (size_t)R * 4 : 0);
   if (!backward) {
     p.part = take((size_t)p.tiles_v * R * 8);
@@ -1131,9 +1201,10 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
     return p;
   }
   p.scal = take(kScalars * 4);
-  p.amax = take(3 * kAmaxBlocks * 4);
-  p.e = take(p.mode >= 0 ? (size_t)V * p.dpad * 2 * S : 0);
-  p.h = take(p.mode >= 0 ? (size_t)R * p.dpad * 2 * S : 0);
+  p.maxima = take(2 * kParts * 4);
+  p.e = take(p.mode == kF16 ? 0 : (size_t)V * p.dpad * 2 * S);  // fp16: z's serves
+  p.h = take((size_t)R * p.dpad * 2 * S);
+  p.power = take((size_t)p.rows_p * 4);
   // Pieces of the vocabulary: as few as their dz's bytes allow, and where the
   // table's gradient has 256 tiles in a piece, whole multiples of that: each
   // product of a piece then fills the 256 CUs evenly.
@@ -1199,13 +1270,27 @@ int check_call(const char* what, const Call& c, const void* ws, size_t ws_bytes,
   return MPL_OK;
 }
 
-PackOne pack_of(const void* src, char* dst, int64_t rows, int64_t pitch, const Plan& p) {
-  const bool vec = ((uintptr_t)src & 15) == 0 && pitch % (p.split ? 4 : 8) == 0;
-  return PackOne{src, dst, rows, pitch, cdiv(rows * (p.dpad / 8), 256), vec};
+// Both arrays on their way to operands at e and h.
+PackArgs pack_args(const Call& c, const Plan& p, char* ws, char* e, char* h) {
+  auto one = [&](const void* src, char* dst, int64_t rows, int64_t pitch) {
+    const bool vec = ((uintptr_t)src & 15) == 0 && pitch % (p.split ? 4 : 8) == 0;
+    return PackOne{src, dst, rows, pitch, cdiv(rows * (p.dpad / 8), 256), vec};
+  };
+  PackArgs a{};
+  a.e = one(c.embedding, e, c.V, c.embedding_pitch);
+  a.h = one(c.hidden, h, c.R, c.hidden_pitch);
+  a.d = c.d, a.dpad = p.dpad;
+  for (a.width = 8; a.width < 64 && a.width < p.dpad / 8;) a.width *= 2;
+  a.undo_e = (int*)(ws + p.undo_e), a.undo_h = (int*)(ws + p.undo_h);
+  a.scal = (int*)(ws + p.scal);
+  a.part = (uint32_t*)(ws + p.maxima);
+  a.power = (const int*)(ws + p.power);
+  return a;
 }
 
-// Both arrays as z's operands, the forward's and the backward's, in rows form.
-void z_operands(const Call& c, const Plan& p, char* ws, hipStream_t s, LogitArgs& a) {
+// Both arrays as z's operands, the forward's and the backward's, in rows form.  In
+// the backward (q) fp32 calls form the coefficients in the same launch.
+void z_operands(const Call& c, const Plan& p, char* ws, const CoefArgs* q, hipStream_t s, LogitArgs& a) {
   const int64_t row = (int64_t)p.dpad * (p.split ? 4 : 2);
   if (p.mode_z < 0) {
     a.E = {(const char*)c.embedding, c.embedding_pitch * 2, c.V, row};
@@ -1214,48 +1299,36 @@ void z_operands(const Call& c, const Plan& p, char* ws, hipStream_t s, LogitArgs
   }
   a.E = {ws + p.ze, row, c.V, row};
   a.H = {ws + p.zh, row, c.R, row};
-  const PackOne e = pack_of(c.embedding, ws + p.ze, c.V, c.embedding_pitch, p),
-                h = pack_of(c.hidden, ws + p.zh, c.R, c.hidden_pitch, p);
+  PackArgs g = pack_args(c, p, ws, ws + p.ze, ws + p.zh);
   if (p.mode_z == kSplit) {
-    int width = 8;
-    while (width < 64 && width < p.dpad / 8) width *= 2;
-    a.undo_e = (int*)(ws + p.undo_e), a.undo_h = (int*)(ws + p.undo_h);
-    const SplitArgs q{e, h, c.d, p.dpad, width, (int*)(ws + p.undo_e), (int*)(ws + p.undo_h)};
-    const int64_t groups = cdiv(std::max(c.V, c.R), 256 / width);
-    split_rows_kernel<<<dim3((unsigned)std::min<int64_t>(groups, 1 << 20), 2), 256, 0, s>>>(q);
+    a.undo_e = g.undo_e, a.undo_h = g.undo_h;
+    const int64_t groups = cdiv(std::max(c.V, c.R), 32);
+    if (q) split_rows_kernel<true><<<dim3(kParts, 2), 256, 0, s>>>(g, *q);
+    else split_rows_kernel<false><<<dim3((unsigned)std::min<int64_t>(groups, 1 << 20), 2), 256, 0, s>>>(g, CoefArgs{});
   } else {
-    PackArgs q{};
-    q.e = e, q.h = h, q.d = c.d, q.dpad = p.dpad;
-    pack_kernel<kCopy16><<<(unsigned)(e.blocks + h.blocks), 256, 0, s>>>(q);
+    pack_kernel<kCopy16><<<(unsigned)(g.e.blocks + g.h.blocks), 256, 0, s>>>(g);
   }
 }
 
-// Both arrays as the operands of the gradients' products, and the coefficients.
-void grad_operands(const Call& c, const Plan& p, char* ws, const CoefArgs& q, const LogitArgs& z, hipStream_t s,
-                   TileOperand& E, TileOperand& H) {
+// The operands of the gradients' products: the table for d hidden, the weighted
+// hidden rows for d embedding, each if it is wanted; for 16-bit calls the
+// coefficients first.
+void grad_operands(const Call& c, const Plan& p, char* ws, const CoefArgs& q, const LogitArgs& z, bool want_h,
+                   bool want_e, hipStream_t s, TileOperand& E, TileOperand& H) {
   const int64_t row = (int64_t)p.dpad * (p.split ? 4 : 2);
-  if (p.mode < 0) {
-    xent_coef_kernel<<<1, 1024, 0, s>>>(q, (float*)(ws + p.scal));
-    E = z.E, H = z.H;
-    return;
+  PackArgs g = pack_args(c, p, ws, ws + p.e, ws + p.h);
+  const bool table = want_h && p.mode != kF16;
+  if (p.mode == kBf16ToF16) weigh_kernel<kBf16ToF16><<<dim3(kParts, table ? 2 : 1), 256, 0, s>>>(g, q);
+  else if (p.mode == kF16) weigh_kernel<kF16><<<dim3(kParts, 1), 256, 0, s>>>(g, q);
+  if (!table) g.e.blocks = 0;
+  if (!want_e) g.h.blocks = 0;
+  const unsigned grid = (unsigned)(g.e.blocks + g.h.blocks);
+  if (grid) {
+    if (p.mode == kSplit) pack_kernel<kSplit><<<grid, 256, 0, s>>>(g);
+    else if (p.mode == kBf16ToF16) pack_kernel<kBf16ToF16><<<grid, 256, 0, s>>>(g);
+    else pack_kernel<kF16><<<grid, 256, 0, s>>>(g);
   }
-  PackArgs a{};
-  a.e = pack_of(c.embedding, ws + p.e, c.V, c.embedding_pitch, p);
-  a.h = pack_of(c.hidden, ws + p.h, c.R, c.hidden_pitch, p);
-  a.d = c.d, a.dpad = p.dpad;
-  a.scal = (float*)(ws + p.scal);
-  a.part = (uint32_t*)(ws + p.amax);
-  a.coefs = true;
-  const dim3 maxima(kAmaxBlocks, 3);
-  const unsigned grid = (unsigned)(a.e.blocks + a.h.blocks);
-  if (p.mode == kSplit) {
-    amax_kernel<kSplit><<<maxima, 256, 0, s>>>(a, q);
-    pack_kernel<kSplit><<<grid, 256, 0, s>>>(a);
-  } else {
-    amax_kernel<kBf16ToF16><<<maxima, 256, 0, s>>>(a, q);
-    pack_kernel<kBf16ToF16><<<grid, 256, 0, s>>>(a);
-  }
-  E = {ws + p.e, row, c.V, row};
+  E = p.mode == kF16 ? z.E : TileOperand{ws + p.e, row, c.V, row};
   H = {ws + p.h, row, c.R, row};
 }
 
@@ -1328,7 +1401,7 @@ extern "C" int mpl_vocab_cross_entropy(const void* hidden, int64_t hidden_pitch,
     return join((int)p.rows_grid);
   }
   LogitArgs a{};
-  z_operands(c, p, ws, s, a);
+  z_operands(c, p, ws, nullptr, s, a);
   a.R = rows, a.V = vocab;
   a.iters = p.dpad * (p.split ? 2 : 1) / 64;
   a.tiles_v = p.tiles_v;
@@ -1376,17 +1449,17 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
   }
   const int S = p.split ? 2 : 1;
   LogitArgs a{};
-  float* scal = (float*)(ws + p.scal);
+  const int* scal = (const int*)(ws + p.scal);
   float* coef = (float*)(ws + p.coef);
-  const CoefArgs q{target, rows, p.rows_p, vocab, ignore_index, g_loss, g_lse, lse, coef};
+  int* power = (int*)(ws + p.power);
+  const CoefArgs q{target, rows, p.rows_p, vocab, ignore_index, g_loss, g_lse, lse, coef, power};
   TileOperand E, H;
-  z_operands(c, p, ws, s, a);
-  grad_operands(c, p, ws, q, a, s, E, H);
+  z_operands(c, p, ws, &q, s, a);
+  grad_operands(c, p, ws, q, a, d_hidden, d_embedding, s, E, H);
   a.R = rows, a.V = vocab;
   a.iters = p.dpad * S / 64;
   const int bz = p.big_z ? 256 : 128;
   a.tiles_t = (uint32_t)cdiv(rows, bz);
-  a.scal = scal;
   a.target = target;
   a.rows_p = p.rows_p;
   a.pitch_p = p.v_piece * 2 * S;
@@ -1415,7 +1488,7 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
       g.splits = std::min(p.splits_h, g.iters);
       const int b = p.big_h ? 256 : 128;
       g.tiles_m = (uint32_t)cdiv(rows, b), g.tiles_n = (uint32_t)cdiv(d, b);
-      g.u0 = scal + kInvP, g.u1 = p.mode >= 0 ? scal + kInvE : nullptr;
+      g.undo = p.mode == kF16 ? nullptr : scal + kUndoE, g.power = power;
       g.part = p.splits_h > 1 || p.pieces > 1 ? (float*)(ws + p.ph) : nullptr;
       g.add = i > 0;
       g.out = d_hidden, g.dtype = dtype;
@@ -1432,7 +1505,7 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
       g.splits = p.splits_e;
       const int b = p.big_e ? 256 : 128;
       g.tiles_m = (uint32_t)cdiv(nv, b), g.tiles_n = (uint32_t)cdiv(d, b);
-      g.u0 = scal + kInvP, g.u1 = p.mode >= 0 ? scal + kInvH : nullptr;
+      g.undo = scal + kUndoH;
       g.part = p.splits_e > 1 ? (float*)(ws + p.pe) : nullptr;
       g.out = (char*)d_embedding + a.v0 * d * (dtype == MPL_F32 ? 4 : 2);
       g.dtype = dtype;

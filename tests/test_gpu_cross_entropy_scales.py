@@ -3,8 +3,9 @@
 Tolerances as in test_gpu_cross_entropy.py, but with the ends of fp16's range
 where the operands' own powers of two put them:
 
-  z        2^-39 of a row's largest and of a word's largest (fp32 calls; 16-bit
-           calls multiply their operands as they are)
+  z        2^-39 of a row's largest and 2^-33 of a word's (32 words may share the
+           power of the largest where theirs are within 2^-6 of it); fp32 calls,
+           16-bit ones multiply their operands as they are
   lse      twice sum_v p z's error (the weights shift by less than half), and
            2^-20 (1 + |lse|)
   dz       2^-38 of the token's own largest coefficient
@@ -33,7 +34,8 @@ def _formula(h, e, t, gl):
     z = H @ E.t()
     z_tol = (d * 2.0 ** -24 + (2.0 ** -21 if fp32 else 0)) * (H.abs() @ E.abs().t())
     if fp32:
-        z_tol = z_tol + 2.0 ** -39 * (em[None] * H.abs().sum(1)[:, None] + hm[:, None] * E.abs().sum(1)[None])
+        z_tol = z_tol + (2.0 ** -33 * em[None] * H.abs().sum(1)[:, None]
+                         + 2.0 ** -39 * hm[:, None] * E.abs().sum(1)[None])
     lse = torch.logsumexp(z, 1)
     soft = torch.exp(z - lse[:, None])
     lse_tol = 2 * (soft * z_tol).sum(1) + 2.0 ** -20 * (1 + lse.abs())
@@ -76,18 +78,19 @@ def _check(got, want, rows=slice(None)):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size", [1e4, 1e8, 1e13])
+@pytest.mark.parametrize("ignored", [False, True])
 @pytest.mark.parametrize("R,V,d", [(20, 300, 64), (100, 700, 96), (300, 2000, 128)])
-def test_one_large_row(gpu_lib, R, V, d, size, dtype):
+def test_one_large_row(gpu_lib, R, V, d, ignored, size, dtype):
     """A token whose hidden row is far from the others' size (a diverged one, or
     what stands in padding) changes no other token's loss and gradient."""
     from model_amd.cross_entropy import vocab_cross_entropy_grads
 
     if dtype == torch.float16 and size > 1e4:
         pytest.skip("past fp16's range")
-    print(f"one large row R={R} V={V} d={d} {dtype} {size}", flush=True)
+    print(f"one large row R={R} V={V} d={d} {dtype} {size} ignored={ignored}", flush=True)
     h, e, t, gl, _ = _inputs(R, V, d, dtype, ignored=0.1)
     t[:3] = torch.tensor([5, 6, 7], device="cuda")
-    t[R - 2] = 8
+    t[R - 2] = IGNORE if ignored else 8
     plain = vocab_cross_entropy_grads(h, e, t, gl)
     h2 = h.clone()
     h2[R - 2] *= size
@@ -95,6 +98,12 @@ def test_one_large_row(gpu_lib, R, V, d, size, dtype):
     others = torch.arange(R, device="cuda") != R - 2
     for a, b in zip(plain[:3], got[:3]):
         assert torch.equal(a[others], b[others])
+    if ignored:
+        assert torch.equal(plain[3], got[3])
+        return
+    # what the large row itself adds to the words is as uncertain as its logits
+    want = _formula(h2, e, t, gl)
+    _check(got, want, others)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -115,6 +124,63 @@ def test_one_large_word(gpu_lib, R, V, d, size, dtype):
     e[12] = e[12] / size
     got = vocab_cross_entropy_grads(h, e, t, gl)
     _check(got, _formula(h, e, t, gl))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("spread", [0.5, 3.0, 9.0])
+@pytest.mark.parametrize("R,V,d", [(40, 300, 64), (100, 701, 96), (300, 2000, 128), (4100, 4300, 40)])
+def test_words_and_rows_of_every_size(gpu_lib, R, V, d, spread, dtype):
+    """Sizes of words and rows by powers of ten: some fragments of 32 words share a
+    power of two, some do not."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    h, e, t, gl, _ = _inputs(R, V, d, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    some = torch.rand((V, 1), generator=gen, device="cuda") < 0.3
+    some[V // 2:] = False
+    e = torch.where(some, e * 10 ** (spread * (torch.rand((V, 1), generator=gen, device="cuda") * 2 - 1)), e).to(dtype)
+    e[5] = 0
+    h = (h * 10 ** (spread * (torch.rand((R, 1), generator=gen, device="cuda") * 2 - 1))).to(dtype)
+    _check(vocab_cross_entropy_grads(h, e, t, gl), _formula(h, e, t, gl))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("least", [2.0 ** -12, 2.0 ** -24, 2.0 ** -60])
+@pytest.mark.parametrize("R,V,d", [(30, 300, 64), (100, 700, 96), (300, 2000, 128), (257, 40000, 320)])
+def test_weights_of_unlike_size(gpu_lib, R, V, d, least, dtype):
+    """Each token's d hidden is judged by its own size, however small its weight beside the others'."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    print(f"token weights R={R} V={V} d={d} {dtype} {least}", flush=True)
+    h, e, t, gl, _ = _inputs(R, V, d, dtype)
+    if dtype == torch.float16:  # d hidden within fp16's normal numbers
+        least, gl = max(least, 2.0 ** -20), gl * 1024
+    gl = gl * torch.logspace(math.log2(least), 0, R, base=2.0, device="cuda")[torch.randperm(R, device="cuda")]
+    _check(vocab_cross_entropy_grads(h, e, t, gl), _formula(h, e, t, gl))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,V,d", [(100, 700, 96), (300, 2000, 128)])
+@pytest.mark.parametrize("junk", [math.nan, math.inf, 3e4])
+def test_ignored_rows_hold_anything(gpu_lib, R, V, d, junk, dtype):
+    """Padding may hold NaN and infinities: the gradients are those of a call
+    with zeros there, the last row (whose memory the tiles read on) among them."""
+    from model_amd.cross_entropy import vocab_cross_entropy, vocab_cross_entropy_grads
+
+    h, e, t, gl, _ = _inputs(R, V, d, dtype, ignored=0.3)
+    t[R - 1] = IGNORE
+    pad = t == IGNORE
+    zeros, junked = h.clone(), h.clone()
+    zeros[pad] = 0
+    junked[pad] = junk
+    loss, lse, dh, de = vocab_cross_entropy_grads(zeros, e, t, gl)
+    got = vocab_cross_entropy_grads(junked, e, t, gl)
+    assert torch.equal(got[0], loss) and torch.equal(got[1][~pad], lse[~pad])
+    assert torch.equal(got[2], dh) and torch.equal(got[3], de)
+    assert (dh[pad] == 0).all()
+    a, b = junked.clone().requires_grad_(), e.clone().requires_grad_()
+    vocab_cross_entropy(a, b, t).backward(gl)
+    assert torch.equal(a.grad, dh) and torch.equal(b.grad, de)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
