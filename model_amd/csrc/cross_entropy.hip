@@ -581,6 +581,7 @@ struct RowsArgs {
   const float* g_lse;
   int64_t ignore;
   float* dz;  // [group][32 words][TOK tokens], then as much of [group][TOK tokens][32 words]
+  int* live;  // [TOK]: whether a token has coefficients
 };
 
 template <typename T>
@@ -617,6 +618,8 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs p) {
       if (to[n] != p.ignore && (to[n] < 0 || to[n] >= p.V)) gt[n] = NAN;
       all[n] = gt[n] + (p.g_lse ? p.g_lse[at] : 0.f);
       lse[n] = p.lse[at];
+      if (tok >= p.R) all[n] = gt[n] = 0.f;
+      if (blockIdx.x == 0 && wave == 0 && half == 0) p.live[tok] = all[n] != 0.f || gt[n] != 0.f;
     }
   }
   const int chunks = (p.d + 2 * VE - 1) / (2 * VE);
@@ -679,7 +682,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs p) {
         const int64_t v = 32 * g + 8 * wave + 4 * half + i;
         if constexpr (BWD) {
           z[i] = all[n] * exp_below(z[i], lse[n]) - (v == to[n] ? gt[n] : 0.f);
-          z[i] = v < p.V && tok < p.R ? z[i] : 0.f;
+          z[i] = v < p.V && (all[n] != 0.f || gt[n] != 0.f) ? z[i] : 0.f;
           p.dz[(g * 32 + 8 * wave + 4 * half + i) * TOK + tok] = z[i];
         } else {
           if (v == to[n] && tok < p.R) p.z_target[tok] = z[i];
@@ -942,6 +945,7 @@ struct FewArgs {
   int64_t e_pitch, h_pitch, R, V;
   int d;
   const float* dz;  // as RowsArgs
+  const int* live;
   void* de;         // or null
   float* part;      // [workgroups.x][R][d], or null
 };
@@ -973,6 +977,7 @@ __global__ __launch_bounds__(64) void xent_few_kernel(FewArgs p) {
     for (int t = 0; t < 4; ++t) {
       const int64_t tok = 8 * m + 4 * half + t;
       h[m][t].load((const T*)p.H + min(tok, p.R - 1) * p.h_pitch + c0);
+      if (!p.live[tok]) h[m][t].v = (T)0.f;  // its dz is 0, but the row may hold NaN
     }
   f32x16 dh[NT][4];
 #pragma unroll
@@ -1127,7 +1132,7 @@ struct Plan {
   int few, parts;      // few-token backward: blocks of 32 tokens, parts of d hidden's sums
   int splits_h, splits_e;
   // offsets into the workspace
-  size_t scal, maxima, ze, zh, undo_e, undo_h, e, h, power, part, zt, coef, P, ph, pe, bytes;
+  size_t scal, maxima, ze, zh, undo_e, undo_h, e, h, power, live, part, zt, coef, P, ph, pe, bytes;
 };
 
 constexpr int64_t kPieceBytes = 512ll << 20;
@@ -1186,6 +1191,7 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
     p.rows_grid = (uint32_t)std::min<int64_t>(groups, 2048);
     p.parts = (int)std::min(groups, waves);
     p.P = take((size_t)groups * 32 * p.few * 32 * 8);
+    p.live = take(64 * 4);
     p.ph = take((size_t)p.parts * R * d * 4);
     p.bytes = at;
     return p;
@@ -1435,9 +1441,9 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
   if (p.few) {
     RowsArgs r{embedding, hidden, embedding_pitch, hidden_pitch, rows, vocab, d, target};
     r.lse = lse, r.g_loss = g_loss, r.g_lse = g_lse, r.ignore = ignore_index;
-    r.dz = (float*)(ws + p.P);
+    r.dz = (float*)(ws + p.P), r.live = (int*)(ws + p.live);
     rows_kernel<true>(dtype, p.rows_grid, s, r);
-    FewArgs f{embedding, hidden, embedding_pitch, hidden_pitch, rows, vocab, d, r.dz, d_embedding};
+    FewArgs f{embedding, hidden, embedding_pitch, hidden_pitch, rows, vocab, d, r.dz, r.live, d_embedding};
     f.part = d_hidden ? (float*)(ws + p.ph) : nullptr;
     const dim3 grid(p.parts, (unsigned)cdiv(d, 128));
     if (dtype == MPL_F32) few_kernel<float>(p.few, grid, s, f);

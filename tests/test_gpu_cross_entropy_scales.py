@@ -160,7 +160,8 @@ def test_weights_of_unlike_size(gpu_lib, R, V, d, least, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("R,V,d", [(100, 700, 96), (300, 2000, 128)])
+@pytest.mark.parametrize("R,V,d", [(1, 40, 64), (20, 300, 64), (40, 300, 70), (64, 900, 128), (100, 700, 96),
+                                   (300, 2000, 128)])
 @pytest.mark.parametrize("junk", [math.nan, math.inf, 3e4])
 def test_ignored_rows_hold_anything(gpu_lib, R, V, d, junk, dtype):
     """Padding may hold NaN and infinities: the gradients are those of a call
