@@ -80,7 +80,8 @@ def vocab_cross_entropy(hidden: torch.Tensor, embedding: torch.Tensor, targets: 
     exactly above 2^-29 of it, fp16 tables as they are); those of few tokens (64 in
     fp32) are in fp32.  A row that passes no gradient adds nothing to the table's,
     whatever it holds: padding may be NaN.  For gradients
-    inside a captured HIP graph use vocab_cross_entropy_grads."""
+    inside a captured HIP graph use vocab_cross_entropy_grads.  Dual tensors,
+    torch.func's transforms and tracing are refused."""
     _check(hidden, embedding, targets, "vocab_cross_entropy")
     autograd = torch.is_grad_enabled() and (hidden.requires_grad or embedding.requires_grad)
     if autograd and _capturing():

@@ -8,13 +8,17 @@
 // Host code only: built by the host compiler against torch's headers and linked
 // to libmpl.so beside it.
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <initializer_list>
 #include <optional>
 #include <tuple>
 
@@ -39,6 +43,28 @@ void check(int rc, const char* what) { TORCH_CHECK(rc == MPL_OK, what, " failed 
 
 void* stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream();
+}
+
+// The calls below read memory and launch kernels that no transform sees: a trace
+// would record an empty output, and a tangent or a batch would be left out without
+// a word.  `args` may hold undefined tensors.
+void refuse_transforms(const char* what, std::initializer_list<Tensor> args) {
+  using c10::DispatchKey;
+  TORCH_CHECK(!at::tracer::impl::is_dispatch_enabled(), what, " cannot be traced (torch.jit.trace)");
+  TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(DispatchKey::FuncTorchDynamicLayerFrontMode), what,
+              " cannot be transformed by torch.func (vmap, grad, jvp, ...)");
+  for (const auto mode : {c10::impl::TorchDispatchModeKey::PROXY, c10::impl::TorchDispatchModeKey::FAKE,
+                          c10::impl::TorchDispatchModeKey::FUNCTIONAL})
+    TORCH_CHECK(!c10::impl::TorchDispatchModeTLS::get_mode(mode).has_value(), what,
+                " cannot be traced (make_fx, fake or functional tensors)");
+  constexpr c10::DispatchKeySet wrapped({DispatchKey::Python, DispatchKey::FuncTorchBatched,
+                                         DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched,
+                                         DispatchKey::Functionalize});
+  for (const Tensor& t : args) {
+    if (!t.defined()) continue;
+    TORCH_CHECK(!t.key_set().has_any(wrapped), what, " takes plain tensors, no wrappers or subclasses with their own dispatch");
+    TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivative: an argument is a dual tensor");
+  }
 }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -143,6 +169,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
     const bool nx = ctx->needs_input_grad(0), ns = ctx->needs_input_grad(1), nb = ctx->needs_input_grad(2),
                nr = added && ctx->needs_input_grad(3);
     const Tensor g_sum = added ? grads[1] : Tensor();
+    refuse_transforms("layer_norm's gradient", {grads[0], g_sum});
     variable_list out(5);
     if (!grads[0].defined()) {  // only the sum was used
       if (nx) out[0] = g_sum;
@@ -167,6 +194,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
 py::object layer_norm(const Tensor& x, const Tensor& scale, const Tensor& bias, double eps,
                       const std::optional<Tensor>& residual, bool autograd) {
   const Tensor r = or_none(residual);
+  refuse_transforms("layer_norm", {x, scale, bias, r});
   if (autograd) {
     const variable_list out = LayerNormFunction::apply(x, scale, bias, eps, residual);
     return r.defined() ? py::cast(std::make_tuple(out[0], out[1])) : py::cast(out[0]);
@@ -177,6 +205,7 @@ py::object layer_norm(const Tensor& x, const Tensor& scale, const Tensor& bias, 
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> layer_norm_forward(const Tensor& x, const Tensor& scale, const Tensor& bias,
                                                               double eps, const std::optional<Tensor>& residual) {
+  refuse_transforms("layer_norm_forward", {x, scale, bias, or_none(residual)});
   const at::AutoGradMode no_grad(false);
   auto [y, total, st] = ln_forward(x, scale, bias, eps, or_none(residual), true);
   return {y, total.defined() ? total : x, st.select(0, 0), st.select(0, 1)};
@@ -185,6 +214,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> layer_norm_forward(const Tensor& x, c
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& g_y, const Tensor& s, const Tensor& scale,
                                                        const Tensor& mean, const Tensor& rstd,
                                                        const std::optional<Tensor>& g_residual) {
+  refuse_transforms("layer_norm_backward", {g_y, s, scale, mean, rstd, or_none(g_residual)});
   const at::AutoGradMode no_grad(false);
   return ln_backward(g_y, s, scale, (const float*)mean.data_ptr(), (const float*)rstd.data_ptr(), or_none(g_residual),
                      true, true);
@@ -261,6 +291,7 @@ struct CrossEntropyFunction : torch::autograd::Function<CrossEntropyFunction> {
     TORCH_CHECK(!capturing(), "torch autograd through vocab_cross_entropy is not supported under HIP graph capture: use "
                 "vocab_cross_entropy_grads, which captures");
     variable_list out(4);
+    refuse_transforms("vocab_cross_entropy's gradient", {grads[0], grads[1]});
     if (!grads[0].defined() && !grads[1].defined()) return out;
     const variable_list s = ctx->get_saved_variables();
     {
@@ -275,6 +306,7 @@ struct CrossEntropyFunction : torch::autograd::Function<CrossEntropyFunction> {
 
 std::tuple<Tensor, Tensor> vocab_cross_entropy(const Tensor& hidden, const Tensor& embedding, const Tensor& targets,
                                                int64_t ignore_index, bool autograd) {
+  refuse_transforms("vocab_cross_entropy", {hidden, embedding, targets});
   const Tensor ids = ids_of(targets);
   if (!autograd) return ce_forward(hidden, embedding, ids, ignore_index);
   const variable_list out = CrossEntropyFunction::apply(hidden, embedding, ids, ignore_index);
@@ -286,6 +318,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> vocab_cross_entropy_grads(const Tenso
                                                                      const std::optional<Tensor>& g_loss,
                                                                      const std::optional<Tensor>& g_lse,
                                                                      int64_t ignore_index) {
+  refuse_transforms("vocab_cross_entropy_grads", {hidden, embedding, targets, or_none(g_loss), or_none(g_lse)});
   const at::AutoGradMode no_grad(false);
   const Tensor ids = ids_of(targets);
   auto [loss, lse] = ce_forward(hidden, embedding, ids, ignore_index);

@@ -63,7 +63,8 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, eps: fl
 
     Gradients come from mpl_layer_norm_bwd, those of scale and bias as fixed-order
     fp32 sums over the rows; the gradient of s joins that of x in the same pass.
-    Inside a captured HIP graph use layer_norm_forward and layer_norm_backward."""
+    Inside a captured HIP graph use layer_norm_forward and layer_norm_backward.
+    Dual tensors, torch.func's transforms and tracing are refused."""
     others = () if residual is None else (("residual", residual),)
     _check("layer_norm", x, (("scale", scale), ("bias", bias)), others)
     autograd = torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or bias.requires_grad
