@@ -14,11 +14,13 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/util/ThreadLocalDebugInfo.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <initializer_list>
+#include <memory>
 #include <optional>
 #include <tuple>
 
@@ -70,11 +72,19 @@ void refuse_transforms(const char* what, std::initializer_list<Tensor> args) {
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // A captured backward of leaves that an eager graph holds ends the process, so
-// the nodes refuse to run under capture; tests set `pretend`.
-bool pretend_capturing = false;
+// the nodes refuse to run under capture.  `Pretended` makes one thread, and the
+// backward passes that it starts (torch hands them the thread's debug information,
+// on whichever thread they run), behave as under capture: for tests.
+struct Pretended : c10::DebugInfoBase {};
+constexpr auto kPretended = c10::DebugInfoKind::TEST_INFO;
 bool capturing() {
-  return pretend_capturing ||
+  return dynamic_cast<Pretended*>(c10::ThreadLocalDebugInfo::get(kPretended)) != nullptr ||
          c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+void pretend_capturing(bool on) {
+  const bool now = dynamic_cast<Pretended*>(c10::ThreadLocalDebugInfo::get(kPretended)) != nullptr;
+  if (on && !now) c10::ThreadLocalDebugInfo::_push(kPretended, std::make_shared<Pretended>());
+  else if (!on && now) c10::ThreadLocalDebugInfo::_pop(kPretended);
 }
 
 // First derivatives only: what a node returns under create_graph raises when it
@@ -334,5 +344,5 @@ PYBIND11_MODULE(_ops, m) {
   m.def("layer_norm_backward", &layer_norm_backward);
   m.def("vocab_cross_entropy", &vocab_cross_entropy);
   m.def("vocab_cross_entropy_grads", &vocab_cross_entropy_grads);
-  m.def("pretend_capturing", [](bool on) { pretend_capturing = on; });
+  m.def("pretend_capturing", &pretend_capturing);
 }
