@@ -101,20 +101,28 @@ def _link(cmd, out: str) -> None:
     os.replace(tmp, out)
 
 
+def _link_ops(obj: str) -> None:
+    from torch.utils import cpp_extension
+
+    libs = [f"-L{p}" for p in cpp_extension.library_paths()]
+    _link([host_cxx(), "-shared", "-fPIC", obj, f"-L{HERE}", "-lmpl", *libs, "-ltorch", "-ltorch_cpu", "-ltorch_hip",
+           "-lc10", "-lc10_hip", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], OPS)
+
+
 def build(verbose: bool = False, jobs: int = 8) -> str:
+    """Builds both libraries.  libmpl.so needs hipcc and a host compiler alone: it
+    is linked first, whatever becomes of the extension module, which needs torch."""
     cc = hipcc()
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")) + glob.glob(os.path.join(CSRC, "*.cpp")))
     with cf.ThreadPoolExecutor(max_workers=max(1, min(jobs, len(srcs) + 1))) as ex:
         ops = ex.submit(_compile_ops)
         objs = list(ex.map(lambda s: _compile(s, cc), srcs))
-        ops = ops.result()
-    _link([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread", *objs], LIB)
-    from torch.utils import cpp_extension
-
-    libs = [f"-L{p}" for p in cpp_extension.library_paths()]
-    _link([host_cxx(), "-shared", "-fPIC", ops, f"-L{HERE}", "-lmpl", *libs, "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
-           "-ltorch_python", "-Wl,-rpath,$ORIGIN"], OPS)
+        _link([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-pthread", *objs], LIB)
+        try:
+            _link_ops(ops.result())
+        except Exception as e:
+            raise RuntimeError(f"{LIB} is built, {OPS} is not: {e}") from e
     if verbose:
         print(f"built {LIB} from {len(srcs)} sources, and {OPS}")
     return LIB
