@@ -99,6 +99,14 @@ variable_list once(variable_list grads, const char* what) {
   return grads;
 }
 
+// Contiguous, and what its memory says: torch marks some tensors as negated
+// (the imaginary part of a conjugate) or as zeros without memory.
+Tensor dense(const Tensor& t) {
+  if (!t.defined()) return t;
+  if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
+  return t.resolve_neg().contiguous();
+}
+
 // Rows of d elements next to each other and the elements from row to row (at
 // least d); copied only where they do not lie so.
 struct Rows {
@@ -108,6 +116,7 @@ struct Rows {
 };
 Rows rows_of(const Tensor& t, int64_t d) {
   if (!t.defined()) return {};
+  if (t.is_neg() || t._is_zerotensor()) return {dense(t), d};
   if (t.is_contiguous()) return {t, d};
   Tensor r = t.reshape({-1, d});
   if ((d > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < d)) return {r.contiguous(), d};
@@ -125,7 +134,7 @@ std::tuple<Tensor, Tensor, Tensor> ln_forward(const Tensor& x, const Tensor& sca
   if (stats) st = at::empty({2, rows}, x.options().dtype(at::kFloat));
   if (rows) {
     const Rows a = rows_of(x, d), r = rows_of(residual, d);
-    const Tensor w = scale.contiguous(), b = bias.contiguous();
+    const Tensor w = dense(scale), b = dense(bias);
     float* mean = (float*)ptr(st);
     check(mpl_layer_norm(a.data(), a.pitch, r.data(), r.pitch, dtype_code(x), w.data_ptr(), b.data_ptr(), dtype_code(w),
                          rows, (int)d, (float)eps, y.data_ptr(), ptr(total), mean, mean ? mean + rows : nullptr,
@@ -149,7 +158,7 @@ std::tuple<Tensor, Tensor, Tensor> ln_backward(const Tensor& g_y, const Tensor& 
   }
   if (rows && (want_x || want_params)) {
     const Rows a = rows_of(s, d), g = rows_of(g_y, d), r = rows_of(g_residual, d);
-    const Tensor w = scale.contiguous();
+    const Tensor w = dense(scale);
     const int code = dtype_code(s);
     const size_t n = want_params ? mpl_layer_norm_bwd_workspace_bytes(rows, (int)d, code) : 0;
     Tensor ws;
@@ -226,8 +235,9 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& g_y, const 
                                                        const std::optional<Tensor>& g_residual) {
   refuse_transforms("layer_norm_backward", {g_y, s, scale, mean, rstd, or_none(g_residual)});
   const at::AutoGradMode no_grad(false);
-  return ln_backward(g_y, s, scale, (const float*)mean.data_ptr(), (const float*)rstd.data_ptr(), or_none(g_residual),
-                     true, true);
+  const Tensor m = dense(mean), r = dense(rstd);
+  return ln_backward(g_y, s, scale, (const float*)m.data_ptr(), (const float*)r.data_ptr(), or_none(g_residual), true,
+                     true);
 }
 
 // ---------------------------------------------------------- cross entropy
@@ -275,7 +285,7 @@ std::tuple<Tensor, Tensor> ce_backward(const Tensor& hidden, const Tensor& embed
   if (want_h) dh = at::empty(hidden.sizes(), hidden.options());
   if (want_e) de = R ? at::empty({V, d}, hidden.options()) : at::zeros({V, d}, hidden.options());
   if (R && (want_h || want_e)) {
-    auto row_grad = [](const Tensor& g) { return g.defined() ? g.to(at::kFloat).contiguous() : g; };
+    auto row_grad = [](const Tensor& g) { return g.defined() ? dense(g.to(at::kFloat)) : g; };
     const Tensor gl = row_grad(g_loss), gs = row_grad(g_lse);
     const Rows h = operand_of(hidden, d), e = operand_of(embedding, d);
     const Tensor ws = workspace(R, V, d, hidden, true);
