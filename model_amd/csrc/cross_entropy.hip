@@ -1208,7 +1208,6 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
   }
   p.scal = take(kScalars * 4);
   p.maxima = take(2 * kParts * 4);
-  p.e = take(p.mode == kF16 ? 0 : (size_t)V * p.dpad * 2 * S);  // fp16: z's serves
   p.h = take((size_t)R * p.dpad * 2 * S);
   p.power = take((size_t)p.rows_p * 4);
   // Pieces of the vocabulary: as few as their dz's bytes allow, and where the
@@ -1231,6 +1230,7 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
   };
   pick(R, p.v_piece, p.big_h, p.splits_h);
   pick(p.v_piece, p.rows_p, p.big_e, p.splits_e);
+  p.e = take(p.mode == kF16 ? 0 : (size_t)std::min(V, p.v_piece) * p.dpad * 2 * S);  // fp16: z's serves
   p.coef = take((size_t)p.rows_p * 12);
   p.P = take((size_t)p.v_piece * col);
   p.ph = take(p.splits_h > 1 || p.pieces > 1 ? (size_t)p.splits_h * R * d * 4 : 0);
@@ -1316,25 +1316,29 @@ void z_operands(const Call& c, const Plan& p, char* ws, const CoefArgs* q, hipSt
   }
 }
 
-// The operands of the gradients' products: the table for d hidden, the weighted
-// hidden rows for d embedding, each if it is wanted; for 16-bit calls the
-// coefficients first.
-void grad_operands(const Call& c, const Plan& p, char* ws, const CoefArgs& q, const LogitArgs& z, bool want_h,
-                   bool want_e, hipStream_t s, TileOperand& E, TileOperand& H) {
+// The operands of the gradients' products of a piece of the table, rows v0 to v0 +
+// nv: those for d hidden, and with the first piece the weighted hidden rows for d
+// embedding, each if it is wanted; 16-bit calls form the coefficients before the
+// first.  fp16 calls' table is z's.
+void grad_operands(const Call& c, const Plan& p, char* ws, const CoefArgs& q, const LogitArgs& z, int64_t v0,
+                   int64_t nv, bool want_h, bool want_e, hipStream_t s, TileOperand& E, TileOperand& H) {
   const int64_t row = (int64_t)p.dpad * (p.split ? 4 : 2);
+  const bool table = want_h && p.mode != kF16, rows = want_e && v0 == 0;
   PackArgs g = pack_args(c, p, ws, ws + p.e, ws + p.h);
-  const bool table = want_h && p.mode != kF16;
-  if (p.mode == kBf16ToF16) weigh_kernel<kBf16ToF16><<<dim3(kParts, table ? 2 : 1), 256, 0, s>>>(g, q);
-  else if (p.mode == kF16) weigh_kernel<kF16><<<dim3(kParts, 1), 256, 0, s>>>(g, q);
-  if (!table) g.e.blocks = 0;
-  if (!want_e) g.h.blocks = 0;
+  if (v0 == 0 && p.mode == kBf16ToF16) weigh_kernel<kBf16ToF16><<<dim3(kParts, table ? 2 : 1), 256, 0, s>>>(g, q);
+  else if (v0 == 0 && p.mode == kF16) weigh_kernel<kF16><<<dim3(kParts, 1), 256, 0, s>>>(g, q);
+  g.e.src = (const char*)g.e.src + v0 * g.e.pitch * (p.split ? 4 : 2);
+  g.e.rows = nv;
+  g.e.blocks = table ? cdiv(nv * (p.dpad / 8), 256) : 0;
+  if (!rows) g.h.blocks = 0;
   const unsigned grid = (unsigned)(g.e.blocks + g.h.blocks);
   if (grid) {
     if (p.mode == kSplit) pack_kernel<kSplit><<<grid, 256, 0, s>>>(g);
     else if (p.mode == kBf16ToF16) pack_kernel<kBf16ToF16><<<grid, 256, 0, s>>>(g);
     else pack_kernel<kF16><<<grid, 256, 0, s>>>(g);
   }
-  E = p.mode == kF16 ? z.E : TileOperand{ws + p.e, row, c.V, row};
+  E = p.mode == kF16 ? TileOperand{z.E.base + v0 * z.E.pitch, z.E.pitch, nv, z.E.width}
+                     : TileOperand{ws + p.e, row, nv, row};
   H = {ws + p.h, row, c.R, row};
 }
 
@@ -1461,7 +1465,6 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
   const CoefArgs q{target, rows, p.rows_p, vocab, ignore_index, g_loss, g_lse, lse, coef, power};
   TileOperand E, H;
   z_operands(c, p, ws, &q, s, a);
-  grad_operands(c, p, ws, q, a, d_hidden, d_embedding, s, E, H);
   a.R = rows, a.V = vocab;
   a.iters = p.dpad * S / 64;
   const int bz = p.big_z ? 256 : 128;
@@ -1480,6 +1483,7 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
     a.v0 = i * p.v_piece;
     const int64_t nv = p.v_piece < vocab - a.v0 ? p.v_piece : vocab - a.v0;  // rows of the table in the piece
     const int64_t nvp = up(nv, 256);
+    grad_operands(c, p, ws, q, a, a.v0, nv, d_hidden, d_embedding, s, E, H);
     a.tiles_v = (uint32_t)(nvp / bz);
     if (p.split) MPL_TILE(xent_dz_kernel, 2, false, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
     else if (dtype == MPL_BF16) MPL_TILE(xent_dz_kernel, 1, true, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
@@ -1487,7 +1491,7 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
     if (d_hidden) {
       GradArgs g{};
       g.A = {a.P, a.pitch_p, p.rows_p, a.pitch_p};
-      g.B = {E.base + a.v0 * E.pitch, E.pitch, nv, E.width};
+      g.B = E;
       g.rows = rows, g.cols = d;
       g.iters = (int)(nvp * S / 64);
       // a short last piece has fewer stages than parts: the others' sums stand
@@ -1505,7 +1509,7 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
     if (d_embedding) {
       GradArgs g{};
       g.A = {a.P, a.pitch_p, p.rows_p, nvp * 2 * S};
-      g.B = {H.base, H.pitch, rows, H.width};
+      g.B = H;
       g.rows = nv, g.cols = d;
       g.iters = (int)(p.rows_p * S / 64);
       g.splits = p.splits_e;

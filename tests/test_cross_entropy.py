@@ -101,3 +101,18 @@ def test_c_entries_validate_before_launch():
     assert bwd(rows=0) == _lib.MPL_EINVAL
     assert bwd(gl=None) == _lib.MPL_EINVAL and bwd(lse=None) == _lib.MPL_EINVAL
     assert bwd(dh=None, de=None) == _lib.MPL_EINVAL
+
+
+@pytest.mark.parametrize("rows,vocab,d", [(16384, 131072, 1024), (8192, 1 << 18, 512)])
+def test_backward_holds_a_piece_of_the_gradients_table(rows, vocab, d):
+    """Beside z's operands (fp32: both arrays split, 4 bytes an element) the
+    backward holds operands of one piece of the vocabulary: at most 512 MiB of dz
+    (2 bytes an element; fp32 4), the piece's table, the weighted rows, and both
+    gradients' fp32 sums in at most 8 parts."""
+    L = _lib.lib()
+    for dtype, size in ((_lib.MPL_F32, 4), (_lib.MPL_F16, 2), (_lib.MPL_BF16, 2)):
+        n = L.mpl_vocab_cross_entropy_workspace_bytes(rows, vocab, d, dtype, 1)
+        z = (rows + vocab) * d * 4 if dtype == _lib.MPL_F32 else 0
+        piece = (512 << 20) // (rows * size)
+        most = z + (512 << 20) + (piece + rows) * d * size + rows * d * 4 * 8 + piece * d * 4 * 8 + (16 << 20)
+        assert n <= most, (dtype, n, most)
