@@ -1147,18 +1147,25 @@ inline int64_t up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
 // of p.  The few tokens' backward holds 8 bytes of dz a word and token, at most
 // kFewBytes.
 //
-// Measured, us, few tokens / tiles.  Forward, fp32: 1, 64, 96 tokens of 16,384 x
-// 256: 9.9 / 27, 16 / 30, 20 / 30; of 131,072 x 1,024: 142 / 524, 404 / 531, 602 /
-// 536.  bf16: 1, 32 tokens of 131,072 x 1,024: 53 / 62, 79 / 64; of 50,021 x 500:
-// 22 / 44, 28 / 45, 64: 43 / 45.
-// Forward and backward, fp32: 1, 32, 64 tokens of 16,384 x 256: 30 / 57, 40 / 62,
-// 61 / 69; of 131,072 x 1,024: 504 / 950, 628 / 1,012, 842 / 1,242.  bf16, 1, 32, 64
-// tokens of 131,072 x 1,024: 276 / 474, 372 / 486, 598 / 497.  fp16: 274 / 279, 380 /
-// 293, 8: 291 / 285; of 37,484 x 640 68 / 85, 87 / 88; of 16,384 x 256 25 / 33, 37 /
-// 39; of 50,021 x 500 77 / 112, 104 / 123, 64: 164 / 141.
+// Measured, us, few tokens / tiles, of forward and of forward with backward:
+//                                  1 token              16                   32                   64
+//   fp32 16,384 x 256        10 / 30  30 / 73    11 / 31  35 / 75    12 / 31  40 / 77    15 / 31  65 / 82
+//        131,072 x 1,024   137 / 481 508 / 1,473 172 / 481 568 / 1,479 206 / 482 630 / 1,486 257 / 484 1,077 / 1,536
+//   bf16 16,384 x 256         10 / 11  27 / 50    10 / 11  31 / 49    10 / 11  38 / 51    12 / 11  52 / 57
+//        37,484 x 640         19 / 18  69 / 118   21 / 19  79 / 121   24 / 20  93 / 124   31 / 20 143 / 130
+//        131,072 x 1,024      53 / 61 276 / 487   67 / 62 329 / 494   80 / 63 405 / 496  113 / 65 656 / 510
+//        50,021 x 500         22 / 43  79 / 193   25 / 44  91 / 195   28 / 45 106 / 198   38 / 45 167 / 202
+//   fp16 16,384 x 256         10 / 11  27 / 43    10 / 11  31 / 46    10 / 11  37 / 47    12 / 12  50 / 52
+//        37,484 x 640         19 / 18  69 / 92    21 / 19  79 / 96    24 / 20  93 / 98    31 / 20 140 / 103
+//        131,072 x 1,024      53 / 64 276 / 303   66 / 64 329 / 307   80 / 64 405 / 310  113 / 66 649 / 322
+//        50,021 x 500         22 / 44  79 / 141   25 / 44  90 / 144   28 / 45 106 / 147   38 / 45 163 / 153
+// 8 tokens of fp16 131,072 x 1,024: 59 / 62 and 293 / 304.  So fp32 and ragged 16-bit
+// rows take it as far as the kernels go, bf16 up to 32 tokens for its gradients'
+// sake (the forward alone pays up to 17 us from 16 tokens on), fp16 the same up to
+// 2^26 elements of the table and 8 tokens of larger ones.
 constexpr int64_t kFewBytes = 4ll << 30;
 inline bool few_tokens(int64_t R, int64_t V, int d, int dtype) {
-  const int64_t most = dtype == MPL_F32 ? 64 : dtype == MPL_BF16 || d % 64 ? 32 : 16;
+  const int64_t most = dtype == MPL_F32 || d % 64 ? 64 : dtype == MPL_BF16 || V * d < (1 << 26) ? 32 : 8;
   return d >= 4 && R <= most && up(V, 32) * up(R, 32) * 8 <= kFewBytes;
 }
 

@@ -248,8 +248,8 @@ def test_logits_of_any_size(gpu_lib, R, size, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("R", [1, 9, 16, 17, 20, 32])
-@pytest.mark.parametrize("V,d", [(300, 128), (1000, 100), (700, 320)])
+@pytest.mark.parametrize("R", [1, 8, 9, 16, 17, 20, 32, 33, 50, 64, 65])
+@pytest.mark.parametrize("V,d", [(300, 128), (1000, 100), (700, 320), (70000, 960)])
 def test_few_tokens_form_z_twice_alike(gpu_lib, R, V, d, dtype):
     """Learned tokens with logits of some 10^4, where another order of z's sum is
     off by 2^-24 of that: p is exactly 1 where the backward's z has the forward's
