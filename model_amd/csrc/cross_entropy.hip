@@ -581,7 +581,7 @@ struct RowsArgs {
   const float* g_lse;
   int64_t ignore;
   float* dz;  // [group][32 words][TOK tokens], then as much of [group][TOK tokens][32 words]
-  int* live;  // [TOK]: whether a token has coefficients
+  void* rows;  // [R][d]: the hidden rows, zeros for tokens without coefficients (their dz is 0, but they may hold NaN)
 };
 
 template <typename T>
@@ -619,7 +619,17 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs p) {
       all[n] = gt[n] + (p.g_lse ? p.g_lse[at] : 0.f);
       lse[n] = p.lse[at];
       if (tok >= p.R) all[n] = gt[n] = 0.f;
-      if (blockIdx.x == 0 && wave == 0 && half == 0) p.live[tok] = all[n] != 0.f || gt[n] != 0.f;
+    }
+  }
+  if constexpr (BWD) {
+    __shared__ int weighs[TOK];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      if (threadIdx.x < 32) weighs[32 * n + col] = all[n] != 0.f || gt[n] != 0.f;
+    __syncthreads();
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < (int)p.R * p.d; i += 256 * gridDim.x) {
+      const int r = i / p.d;
+      ((T*)p.rows)[i] = weighs[r] ? ((const T*)p.H)[r * p.h_pitch + (i - r * p.d)] : (T)0.f;
     }
   }
   const int chunks = (p.d + 2 * VE - 1) / (2 * VE);
@@ -941,11 +951,10 @@ __global__ __launch_bounds__(C::kThreads) void xent_grad_kernel(GradArgs p) {
 // were two waves with rows widened at each use (16 bits 303 and 368: spills).
 struct FewArgs {
   const void* E;
-  const void* H;
-  int64_t e_pitch, h_pitch, R, V;
+  const void* H;  // RowsArgs' rows
+  int64_t e_pitch, R, V;
   int d;
   const float* dz;  // as RowsArgs
-  const int* live;
   void* de;         // or null
   float* part;      // [workgroups.x][R][d], or null
 };
@@ -976,8 +985,7 @@ __global__ __launch_bounds__(64) void xent_few_kernel(FewArgs p) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int64_t tok = 8 * m + 4 * half + t;
-      h[m][t].load((const T*)p.H + min(tok, p.R - 1) * p.h_pitch + c0);
-      if (!p.live[tok]) h[m][t].v = (T)0.f;  // its dz is 0, but the row may hold NaN
+      h[m][t].load((const T*)p.H + min(tok, p.R - 1) * p.d + c0);
     }
   f32x16 dh[NT][4];
 #pragma unroll
@@ -1132,7 +1140,7 @@ struct Plan {
   int few, parts;      // few-token backward: blocks of 32 tokens, parts of d hidden's sums
   int splits_h, splits_e;
   // offsets into the workspace
-  size_t scal, maxima, ze, zh, undo_e, undo_h, e, h, power, live, part, zt, coef, P, ph, pe, bytes;
+  size_t scal, maxima, ze, zh, undo_e, undo_h, e, h, power, part, zt, coef, P, ph, pe, bytes;
 };
 
 constexpr int64_t kPieceBytes = 512ll << 20;
@@ -1149,8 +1157,8 @@ inline int64_t up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
 //
 // Measured, us, few tokens / tiles, of forward and of forward with backward:
 //                                  1 token              16                   32                   64
-//   fp32 16,384 x 256        10 / 30  30 / 73    11 / 31  35 / 75    12 / 31  40 / 77    15 / 31  65 / 82
-//        131,072 x 1,024   137 / 481 508 / 1,473 172 / 481 568 / 1,479 206 / 482 630 / 1,486 257 / 484 1,077 / 1,536
+//   fp32 16,384 x 256        10 / 30  30 / 73    11 / 31  35 / 75    12 / 31  40 / 77    15 / 31  60 / 82
+//        131,072 x 1,024   137 / 481 508 / 1,473 172 / 481 568 / 1,479 206 / 482 630 / 1,486 257 / 484 844 / 1,536
 //   bf16 16,384 x 256         10 / 11  27 / 50    10 / 11  31 / 49    10 / 11  38 / 51    12 / 11  52 / 57
 //        37,484 x 640         19 / 18  69 / 118   21 / 19  79 / 121   24 / 20  93 / 124   31 / 20 143 / 130
 //        131,072 x 1,024      53 / 61 276 / 487   67 / 62 329 / 494   80 / 63 405 / 496  113 / 65 656 / 510
@@ -1198,7 +1206,7 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
     p.rows_grid = (uint32_t)std::min<int64_t>(groups, 2048);
     p.parts = (int)std::min(groups, waves);
     p.P = take((size_t)groups * 32 * p.few * 32 * 8);
-    p.live = take(64 * 4);
+    p.h = take((size_t)R * d * (dtype == MPL_F32 ? 4 : 2));
     p.ph = take((size_t)p.parts * R * d * 4);
     p.bytes = at;
     return p;
@@ -1452,9 +1460,9 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
   if (p.few) {
     RowsArgs r{embedding, hidden, embedding_pitch, hidden_pitch, rows, vocab, d, target};
     r.lse = lse, r.g_loss = g_loss, r.g_lse = g_lse, r.ignore = ignore_index;
-    r.dz = (float*)(ws + p.P), r.live = (int*)(ws + p.live);
+    r.dz = (float*)(ws + p.P), r.rows = ws + p.h;
     rows_kernel<true>(dtype, p.rows_grid, s, r);
-    FewArgs f{embedding, hidden, embedding_pitch, hidden_pitch, rows, vocab, d, r.dz, r.live, d_embedding};
+    FewArgs f{embedding, r.rows, embedding_pitch, rows, vocab, d, r.dz, d_embedding};
     f.part = d_hidden ? (float*)(ws + p.ph) : nullptr;
     const dim3 grid(p.parts, (unsigned)cdiv(d, 128));
     if (dtype == MPL_F32) few_kernel<float>(p.few, grid, s, f);
