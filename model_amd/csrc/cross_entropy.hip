@@ -360,6 +360,29 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   }
 }
 
+// The words of a piece, which z no longer needs, as the operand of dz . embedding in
+// fp32 calls: their rows' powers become the table's, in place.  Most groups of 32
+// have it already (their largest lies in the binade of the table's) and are left.
+__global__ __launch_bounds__(256) void rescale_kernel(char* __restrict__ words, const int* __restrict__ undo, int64_t n,
+                                                      int dpad, const uint32_t* __restrict__ part,
+                                                      int* __restrict__ scal) {
+  const int power = power_for(block_max(max(part[threadIdx.x], part[256 + threadIdx.x])), 14);
+  if (blockIdx.x == 0 && threadIdx.x == 0) scal[kUndoE] = -power;
+  const int per = dpad / 8;
+  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n * per; i += 256 * (int64_t)gridDim.x) {
+    const int64_t r = divide(i, per);
+    const int by = power + undo[r];
+    if (by == 0) continue;
+    const int c = 8 * (int)(i - r * per);
+    const char* q = words + (r * dpad + c / 32 * 32) * 4 + (c % 32) * 2;
+    const half8 hi = *(const half8*)q, lo = *(const half8*)(q + 64);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)hi[j] + (float)lo[j];
+    store8<kSplit>(words, r, dpad, c, v, by);
+  }
+}
+
 // ------------------------------------------------------------------ forward
 struct LogitArgs {
   TileOperand E, H;
@@ -1245,7 +1268,7 @@ Plan make_plan(int64_t R, int64_t V, int d, int dtype, bool backward) {
   };
   pick(R, p.v_piece, p.big_h, p.splits_h);
   pick(p.v_piece, p.rows_p, p.big_e, p.splits_e);
-  p.e = take(p.mode == kF16 ? 0 : (size_t)std::min(V, p.v_piece) * p.dpad * 2 * S);  // fp16: z's serves
+  p.e = take(p.mode == kBf16ToF16 ? (size_t)std::min(V, p.v_piece) * p.dpad * 2 : 0);  // else z's serves
   p.coef = take((size_t)p.rows_p * 12);
   p.P = take((size_t)p.v_piece * col);
   p.ph = take(p.splits_h > 1 || p.pieces > 1 ? (size_t)p.splits_h * R * d * 4 : 0);
@@ -1334,15 +1357,15 @@ void z_operands(const Call& c, const Plan& p, char* ws, const CoefArgs* q, hipSt
 // The operands of the gradients' products of a piece of the table, rows v0 to v0 +
 // nv: those for d hidden, and with the first piece the weighted hidden rows for d
 // embedding, each if it is wanted; 16-bit calls form the coefficients before the
-// first.  fp16 calls' table is z's.
+// first.  fp16 calls' table is z's as it is, fp32 calls' once it is rescaled.
 void grad_operands(const Call& c, const Plan& p, char* ws, const CoefArgs& q, const LogitArgs& z, int64_t v0,
                    int64_t nv, bool want_h, bool want_e, hipStream_t s, TileOperand& E, TileOperand& H) {
   const int64_t row = (int64_t)p.dpad * (p.split ? 4 : 2);
-  const bool table = want_h && p.mode != kF16, rows = want_e && v0 == 0;
+  const bool table = want_h && p.mode == kBf16ToF16, rows = want_e && v0 == 0;
   PackArgs g = pack_args(c, p, ws, ws + p.e, ws + p.h);
   if (v0 == 0 && p.mode == kBf16ToF16) weigh_kernel<kBf16ToF16><<<dim3(kParts, table ? 2 : 1), 256, 0, s>>>(g, q);
   else if (v0 == 0 && p.mode == kF16) weigh_kernel<kF16><<<dim3(kParts, 1), 256, 0, s>>>(g, q);
-  g.e.src = (const char*)g.e.src + v0 * g.e.pitch * (p.split ? 4 : 2);
+  g.e.src = (const char*)g.e.src + v0 * g.e.pitch * 2;
   g.e.rows = nv;
   g.e.blocks = table ? cdiv(nv * (p.dpad / 8), 256) : 0;
   if (!rows) g.h.blocks = 0;
@@ -1352,8 +1375,8 @@ void grad_operands(const Call& c, const Plan& p, char* ws, const CoefArgs& q, co
     else if (p.mode == kBf16ToF16) pack_kernel<kBf16ToF16><<<grid, 256, 0, s>>>(g);
     else pack_kernel<kF16><<<grid, 256, 0, s>>>(g);
   }
-  E = p.mode == kF16 ? TileOperand{z.E.base + v0 * z.E.pitch, z.E.pitch, nv, z.E.width}
-                     : TileOperand{ws + p.e, row, nv, row};
+  E = p.mode == kBf16ToF16 ? TileOperand{ws + p.e, row, nv, row}
+                           : TileOperand{z.E.base + v0 * z.E.pitch, z.E.pitch, nv, z.E.width};
   H = {ws + p.h, row, c.R, row};
 }
 
@@ -1503,6 +1526,10 @@ extern "C" int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pi
     if (p.split) MPL_TILE(xent_dz_kernel, 2, false, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
     else if (dtype == MPL_BF16) MPL_TILE(xent_dz_kernel, 1, true, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
     else MPL_TILE(xent_dz_kernel, 1, false, false, false, p.big_z, a.tiles_v * a.tiles_t, s, a);
+    if (p.split && d_hidden)
+      rescale_kernel<<<(unsigned)std::min<int64_t>(cdiv(nv * (p.dpad / 8), 256), 8192), 256, 0, s>>>(
+          ws + p.ze + a.v0 * a.E.pitch, a.undo_e + a.v0, nv, p.dpad, (const uint32_t*)(ws + p.maxima) + kParts,
+          (int*)(ws + p.scal));
     if (d_hidden) {
       GradArgs g{};
       g.A = {a.P, a.pitch_p, p.rows_p, a.pitch_p};
