@@ -25,17 +25,19 @@
 // rounding into the gradients before they are rounded (2-norm error 1.45 times that
 // of fp32 sums rounded once; 1.0 so).  In fp16 calls dz's rounding is of the
 // result's size: 2-norm error 2.8e-4 where fp32 sums rounded once have 2.1e-4
-// (1,001 x 50,021 x 500); hi and lo would double two of the four products.  Few tokens keep dz in fp32, by the same kernel as their
-// forward, and one pass over the table makes both gradients (xent_few_kernel).
+// (1,001 x 50,021 x 500); hi and lo would double two of the four products.  Few
+// tokens keep dz in fp32, by the same kernel as their forward, and one pass over
+// the table makes both gradients (xent_few_kernel).
 //
-// Bound: the MFMAs.  At 16,384 x 131,072 x 1,024 bf16 the four products take 4.0,
-// 4.6, 3.6 and 3.4 ms (1,100, 955, 1,230 and 1,305 TFLOP/s; a library product
-// without the softmax reaches 1,210 there), 15.0 ms in all against 105 for the
-// formula in fp32 tensors.  What they lose is the epilogues at the end of each
-// tile, which no other wave of the CU covers (128 exp a lane, 3 us beside 26 us
-// of a tile at d = 1,024, and dz's bytes), and the copies of the operands
-// (0.2 ms).  fp32 calls run three fp16 products for one: 8,192 x 16,384 x 256 in
-// 0.86 ms (202, 284, 196 and 179 us the products), 2.70 in fp32 tensors.
+// Bound: the MFMAs.  At 16,384 x 131,072 x 1,024 bf16 the four products take 3.75,
+// 4.62, 3.72 and 3.41 ms (1,175, 950, 1,185 and 1,290 TFLOP/s; a library product
+// without the softmax reaches 1,210 there), the rest 0.29 (the table's largest
+// magnitude, the copies of the operands, d hidden's sums): 15.8 ms in all, 105.5 the
+// formula in fp32 tensors on the same machine.  What they lose is the epilogues at
+// the end of each tile, which no other wave of the CU covers (128 exp a lane, 3 us
+// beside 26 us of a tile at d = 1,024, and dz's bytes).  fp32 calls run three fp16
+// products for one: 8,192 x 16,384 x 256 in 0.906 ms (200, 265, 194 and 169 us the
+// products, 78 the operands, powers and sums), 2.71 in fp32 tensors.
 #include <math.h>
 
 #include <algorithm>
@@ -420,8 +422,9 @@ __device__ __forceinline__ float exp_below(float z, float at) {
 // fp32's range on the way.  The 32 words of a fragment nearly always share one
 // (kNear), and then the factor is one for all of a lane's accumulators there and
 // costs no operation: it makes the difference in exp_below a fused multiply-add.
-// 8,192 x 16,384 x 256 fp32, z's kernels without powers a row 196 and 253 us, so 203
-// and 268 (v_ldexp by every word's own: 237 and 308).  The words' lie in LDS since
+// 8,192 x 16,384 x 256 fp32, z's two kernels with one power an array 198 and 259 us,
+// so 203 and 268 (on one machine; by v_ldexp of every word's own the calls of 4,096
+// rows took 117 us for 109).  The words' lie in LDS since
 // before the tile's product, whose barriers show them to all waves.
 __device__ __forceinline__ float power_of_2(int e) {
   return __uint_as_float((uint32_t)(127 + max(-126, min(127, e))) << 23);
@@ -588,8 +591,8 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
 // are: 4 products a vector, for which lanes of half h take dims 4h .. 4h + 3 of
 // each 8.  Two blocks of 32 tokens share the table's vectors (64 tokens of
 // 131,072 x 1,024 fp32 406 -> 260 us), and LDS with a second barrier.  Bound: the
-// table's bytes, and the fp32 products from some 100 tokens on.  One token of 16,384 x 256 fp32 6.6 us with 4.4 to join (tiles, with the
-// table's copy: 27); of 131,072 x 1,024 142 us, 3.8 TB/s of the table.
+// table's bytes, and the fp32 products from some 100 tokens on.  One token of 16,384 x 256 fp32 6.5 us and 3.8 to join (tiles, with the
+// table's copy: 30 in all); of 131,072 x 1,024 143 us, 3.7 TB/s of the table.
 struct RowsArgs {
   const void* E;
   const void* H;
@@ -968,8 +971,8 @@ __global__ __launch_bounds__(C::kThreads) void xent_grad_kernel(GradArgs p) {
 // d hidden are added by the next launch, in a fixed order.
 //
 // Bound: the table read and its gradient written; 1 and 32 tokens of 131,072 x
-// 1,024 fp32 212 and 203 us (5.1 TB/s, what a large copy reaches), 64 tokens 328;
-// 16 bits 145, 215 (2.5 TB/s: the fp32 products, at one wave a SIMD).  Two columns
+// 1,024 fp32 210 and 202 us (5.1 TB/s, what a large copy reaches), 64 tokens 306;
+// 16 bits 137, 198 (2.7 TB/s: the fp32 products, at one wave a SIMD).  Two columns
 // a lane and two waves a SIMD were slower (fp32, 1 and 32 tokens 265 and 298), as
 // were two waves with rows widened at each use (16 bits 303 and 368: spills).
 struct FewArgs {
@@ -1180,8 +1183,8 @@ inline int64_t up(int64_t x, int64_t to) { return cdiv(x, to) * to; }
 //
 // Measured, us, few tokens / tiles, of forward and of forward with backward:
 //                                  1 token              16                   32                   64
-//   fp32 16,384 x 256        10 / 30  30 / 73    11 / 31  35 / 75    12 / 31  40 / 77    15 / 31  60 / 82
-//        131,072 x 1,024   137 / 481 508 / 1,473 172 / 481 568 / 1,479 206 / 482 630 / 1,486 257 / 484 844 / 1,536
+//   fp32 16,384 x 256        10 / 30  30 / 82    11 / 31  34 / 82    12 / 31  39 / 85    15 / 31  60 / 89
+//        131,072 x 1,024   137 / 483 508 / 1,338 171 / 482 568 / 1,339 205 / 482 630 / 1,356 257 / 485 844 / 1,396
 //   bf16 16,384 x 256         10 / 11  27 / 50    10 / 11  31 / 49    10 / 11  38 / 51    12 / 11  52 / 57
 //        37,484 x 640         19 / 18  69 / 118   21 / 19  79 / 121   24 / 20  93 / 124   31 / 20 143 / 130
 //        131,072 x 1,024      53 / 61 276 / 487   67 / 62 329 / 494   80 / 63 405 / 496  113 / 65 656 / 510

@@ -20,13 +20,14 @@
 // them unaligned); the last vector of a ragged row is read from its end and the
 // elements that it shares with the one before are masked out of the sums.
 //
-// Bound: memory.  16,384 x 4,096 bf16 with the residual: forward 4 arrays in 100 us
-// (5.4 TB/s; a large copy 5.1), backward 4 arrays and 512 partial rows in 117 us
-// (4.6 TB/s); 8,192 x 2,048 fp32 41 and 49 us (6.5 and 5.5 TB/s).  Small calls: 64 x
-// 256 3.3 us, 8,192 x 256 5.2 and 9.5 us.  Few wide rows leave CUs idle: 300 x
-// 16,384 10.5 and 29 us (3.7 and 2.0 TB/s).  512 workgroups of the backward are two a
-// CU; 768 or 1,024 were slower (87 and 96 us for 69 at 4,096 x 8,192 bf16): a CU's
-// share is uneven and the partial rows more.
+// Bound: memory.  16,384 x 4,096 bf16 with the residual: forward 4 arrays in 88 us
+// (6.1 TB/s; a large copy 5.1), backward 4 arrays and 512 partial rows in 120 us
+// (4.5 TB/s) and 4.7 for the second launch.  Small calls: 64 x 256 fp32 3.4 us,
+// 8,192 x 256 5.9, and 7.5 and 2.9; 4,001 x 1,283 fp16 with the residual 12.5, and
+// 18.8 and 4.9.  Few wide rows leave CUs idle: 300 x 16,384 12.6, and 22.9 and 6.1
+// (3.1 and 2.6 TB/s).  512 workgroups of the backward are two a CU; 768 or 1,024 were
+// slower (87 and 96 us for 69 at 4,096 x 8,192 bf16): a CU's share is uneven and the
+// partial rows more.
 #include <math.h>
 
 #include <algorithm>
