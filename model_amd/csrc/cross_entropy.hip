@@ -363,8 +363,8 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
 }
 
 // The words of a piece, which z no longer needs, as the operand of dz . embedding in
-// fp32 calls: their rows' powers become the table's, in place.  Most groups of 32
-// have it already (their largest lies in the binade of the table's) and are left.
+// fp32 calls: their rows' powers become the table's, in place.  Groups of 32 whose
+// largest lies in the binade of the table's have it already and are left.
 __global__ __launch_bounds__(256) void rescale_kernel(char* __restrict__ words, const int* __restrict__ undo, int64_t n,
                                                       int dpad, const uint32_t* __restrict__ part,
                                                       int* __restrict__ scal) {
