@@ -262,3 +262,14 @@ def test_few_tokens_form_z_twice_alike(gpu_lib, R, V, d, dtype):
     assert (z.amax(1) < 3e4 - 200).all()
     loss, _, dh, de = vocab_cross_entropy_grads(h, e, t, torch.ones(R, device="cuda"))
     assert (loss == 0).all() and (dh == 0).all() and (de == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,V,d", [(70, 300, 20000), (66, 40, 65536), (65, 33, 4100), (200, 90, 2), (130, 513, 264)])
+def test_widths(gpu_lib, R, V, d, dtype):
+    """Rows far wider than a team of lanes holds, and narrower than a vector."""
+    from model_amd.cross_entropy import vocab_cross_entropy_grads
+
+    print(f"width R={R} V={V} d={d} {dtype}", flush=True)
+    h, e, t, gl, _ = _inputs(R, V, d, dtype)
+    _check(vocab_cross_entropy_grads(h, e, t, gl), _formula(h, e, t, gl))
