@@ -806,6 +806,60 @@ int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pitch, const 
                                 const float* g_lse, void* workspace, size_t workspace_bytes, void* d_hidden,
                                 void* d_embedding, void* stream);
 
+/*
+ * Causal attention over packed sequences of unlike lengths, with grouped heads
+ * (model.py:88-95 for documents of a batch, prompts, and single tokens over a
+ * cache).  q [tokens, heads, head_dim], k and v [keys, groups, head_dim] of dtype
+ * MPL_F32, MPL_F16 or MPL_BF16, head_dim 32, 64 or 128 elements next to each other,
+ * tokens and heads at the given strides (in elements, >= 0, 16-byte aligned rows).
+ * Head h reads key head h / (heads / groups).
+ *
+ * starts [sequences + 1] ascends in [0, tokens]: sequence i has the queries from
+ * starts[i] to starts[i + 1] - 1, and the keys from key_starts[i] (ascending in [0,
+ * keys]) on, up to key_starts[i + 1] - 1, or the first key_lengths[i] of them where
+ * that is not NULL.  All three are device arrays of int32 (index_bytes 4) or int64
+ * (8); key_starts may be starts.  The queries are the last of their sequence: of Lq
+ * queries and Lk keys query j sees the keys s <= j + Lk - Lq.
+ *
+ *   z = scale q . k,  lse = log sum exp z,  out = sum_s exp(z - lse) v_s
+ *
+ * out [tokens, heads, head_dim] of dtype and lse fp32 [tokens, heads] (or NULL) are
+ * dense; a query that sees no key, or that lies in no sequence, has out 0 and lse
+ * -inf.  Sums are fp32.  Starts that do not ascend, or lie outside the arrays, give
+ * rows of unspecified content, never an access outside.  What is not finite may
+ * reach every row of its own sequence, and no other.
+ *
+ * mpl_packed_attention_bwd writes dq, dk and dv (dense, as q, k and v; each may be
+ * NULL) from the forward's out and lse (dense) and the gradients g_out [tokens,
+ * heads, head_dim] (strides g_token, g_head) and g_lse (dense, or NULL): with p =
+ * exp(z - lse) and delta = g_out . out - g_lse, dz = p (g_out . v - delta), dq =
+ * scale sum dz k, dk = scale sum dz q, dv = sum p g_out.  Keys that no query
+ * reads have gradients 0.
+ *
+ * Deterministic.  The workspace (256-byte aligned) takes
+ * mpl_packed_attention_workspace_bytes (0 for sizes that are refused), which reads
+ * the sizes alone; calls that may run at the same time need one each.
+ */
+typedef struct mpl_packed_attention_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  int dtype, heads, groups, head_dim;
+  int64_t tokens, keys, sequences;
+  const void* starts;
+  const void* key_starts;
+  const void* key_lengths;
+  int index_bytes;
+  float scale;
+} mpl_packed_attention_args;
+size_t mpl_packed_attention_workspace_bytes(const mpl_packed_attention_args* args, int backward);
+int mpl_packed_attention(const mpl_packed_attention_args* args, void* workspace, size_t workspace_bytes, void* out,
+                         float* lse, void* stream);
+int mpl_packed_attention_bwd(const mpl_packed_attention_args* args, const void* g_out, int64_t g_token, int64_t g_head,
+                             const void* out, const float* lse, const float* g_lse, void* workspace,
+                             size_t workspace_bytes, void* dq, void* dk, void* dv, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

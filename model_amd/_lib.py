@@ -93,6 +93,9 @@ SIGNATURES = {
     "mpl_vocab_cross_entropy": (_I, [_P, _I64, _P, _I64, _I, _P, _I64, _I64, _I, _I64, _P, _SZ, _P, _P, _P]),
     "mpl_vocab_cross_entropy_bwd": (_I, [_P, _I64, _P, _I64, _I, _P, _I64, _I64, _I, _I64, _P, _P, _P, _P, _SZ, _P,
                                          _P, _P]),
+    "mpl_packed_attention_workspace_bytes": (_SZ, [_P, _I]),
+    "mpl_packed_attention": (_I, [_P, _P, _SZ, _P, _P, _P]),
+    "mpl_packed_attention_bwd": (_I, [_P, _P, _I64, _I64, _P, _P, _P, _P, _SZ, _P, _P, _P, _P]),
     "mpl_vocab_logits": (_I, [_P, _P, _P, _F, _P, _I64, _I, _I64, _P, _P]),
     "mpl_rows_linear_pair": (_I, [_P, _P, _P, _F, _P, _P, _I, _I, _I64, _I, _I, _I, _P, _P, _P]),
     "mpl_balance_state_bytes": (_SZ, [_I64, _I]),
@@ -130,9 +133,9 @@ _ops = None
 
 
 def ops():
-    """The extension module of csrc/torch/ops.cpp: layer_norm's and
-    vocab_cross_entropy's calls and autograd nodes (raises MplError if it was
-    not built)."""
+    """The extension module of csrc/torch/ops.cpp: the calls and autograd
+    nodes of layer_norm, vocab_cross_entropy and packed_attention, and the
+    calls of clip_global_norm (raises MplError if it was not built)."""
     global _ops
     if _ops is None:
         lib()

@@ -1,0 +1,594 @@
+// Causal attention over packed sequences of unlike lengths with grouped heads
+// (the backbone's attention, model.py:88-95, for sequences of lengths of their
+// own), and its gradients:
+//
+//   z = scale q . k over the keys s <= j + Lk - Lq of query j,  lse = log sum exp z,
+//   out = sum_s exp(z - lse) v_s;
+//   delta = g_out . out - g_lse,  p = exp(z - lse),  dz = p (g_out . v - delta),
+//   dq = scale sum_s dz k_s,  dk = scale sum_rows dz q,  dv = sum_rows p g_out.
+//
+// Kernels on fp32 products (v_mfma_f32_32x32x2_f32).  A tile of scores is formed
+// transposed or not so that the lane holds one column of it and its registers are
+// directly an operand of the next product; the operands come from L2.  The four
+// waves of a workgroup take every fourth block along the contraction (keys, or
+// rows in dk and dv) and join in LDS, in a fixed order.
+#include <math.h>
+
+#include <type_traits>
+
+#include "packed_attn.h"
+
+namespace mpl {
+namespace {
+
+constexpr int kWaves = 4, kThreads = kWaves * kWave;
+
+// Register r of a 32 x 32 tile holds this row of it.
+__device__ __forceinline__ int tile_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+template <int HD, class T>
+__device__ __forceinline__ void load_operand(float4 (&x)[HD / 8], const T* row, int half) {
+#pragma unroll
+  for (int g = 0; g < HD / 8; ++g) x[g] = load4(row + 8 * g + 4 * half);
+}
+
+// c += A . B over HD, both operands one row a lane.
+template <int HD>
+__device__ __forceinline__ f32x16 products(const float4 (&x)[HD / 8], const float4 (&y)[HD / 8]) {
+  f32x16 s = f32x16{};
+#pragma unroll
+  for (int g = 0; g < HD / 8; ++g) {
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[g].x, y[g].x, s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[g].y, y[g].y, s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[g].z, y[g].z, s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[g].w, y[g].w, s, 0, 0, 0);
+  }
+  return s;
+}
+
+template <class T>
+__device__ __forceinline__ const T* row_at(const char* base, int64_t tok, int64_t head, int t, int h) {
+  return (const T*)(base + t * tok + h * head);
+}
+
+// ------------------------------------------------------------------ forward
+// A workgroup of 32 rows of one group; `splits` > 1: of one part of their keys,
+// whose sums go to `part` [split][group][T R][HD] and `stats` [..][2] (the running
+// maximum in base 2, the sum).
+template <class T, int HD>
+__global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a, int splits, T* __restrict__ out,
+                                                                  float* __restrict__ lse, float* __restrict__ part,
+                                                                  float2* __restrict__ stats) {
+  constexpr int DT = HD / 32, PO = HD + 4;
+  __shared__ float so[kWaves][32][PO];
+  __shared__ float sm[kWaves][32], sl[kWaves][32];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int group = blockIdx.x % a.G;
+  const Segment seg = segment_of<5>(a.starts, a.wide, a.n, a.T, a.R, blockIdx.x / a.G);
+  const int rows = seg.len * a.R, tiles = (rows + 31) >> 5;
+  if (seg.tile >= tiles) return;
+  const int row0 = 32 * (tiles - 1 - seg.tile);  // the rows with the most keys first
+  const Keys keys = keys_of(a, seg.seq);
+  const int ri = min(row0 + col, rows - 1), tok = div_r(a, ri);
+  const int sees = min(tok + 1 + keys.len - seg.len, keys.len);  // keys of this lane's row; <= 0 for none
+  const int most = min(div_r(a, min(row0 + 31, rows - 1)) + 1 + keys.len - seg.len, keys.len);
+  const int least = min(div_r(a, row0) + 1 + keys.len - seg.len, keys.len);
+
+  float4 q[HD / 8];
+  load_operand<HD>(q, row_at<T>(a.q, a.qt, a.qh, seg.first + tok, group * a.R + ri - tok * a.R), half);
+  float m = -INFINITY, l = 0.f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+
+  const int blocks = most > 0 ? (most + 31) >> 5 : 0, per = (blocks + splits - 1) / splits;
+  const int j1 = min(blocks, ((int)blockIdx.y + 1) * per);
+  const char* kb = a.k + group * a.kh + keys.first * a.kt;
+  const char* vb = a.v + group * a.vh + keys.first * a.vt;
+  for (int j = blockIdx.y * per + wave; j < j1; j += kWaves) {
+    const int k0 = 32 * j;
+    float4 kv[HD / 8];
+    load_operand<HD>(kv, (const T*)(kb + min(k0 + col, keys.len - 1) * a.kt), half);
+    float v[16][DT];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const T* vrow = (const T*)(vb + min(k0 + tile_row(r, half), keys.len - 1) * a.vt) + col;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) v[r][d] = (float)vrow[32 * d];
+    }
+    f32x16 s = products<HD>(kv, q);
+    if (k0 + 32 > least) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (k0 + tile_row(r, half) >= sees) s[r] = -INFINITY;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    float a0 = mx, a1 = mx;
+    half_swap(a0, a1);
+    mx = fmaxf(m, fmaxf(a0, a1) * a.c);
+    const float ref = mx == -INFINITY ? 0.f : mx;  // no key of the row yet
+    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = mx;
+    float sum = 0.f, p[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -ref));
+      sum += p[r];
+    }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[r][d], p[r], acc[d], 0, 0, 0);
+    }
+  }
+
+  float l0 = l, l1 = l;
+  half_swap(l0, l1);
+  if (half == 0) {
+    sm[wave][col] = m;
+    sl[wave][col] = l0 + l1;
+  }
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      *(float4*)&so[wave][col][32 * d + tile_row(r, half)] =
+          make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+  __syncthreads();
+  for (int i = tid; i < 32 * HD / 4; i += kThreads) {
+    const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
+    if (row0 + t >= rows) continue;
+    float mm = sm[0][t];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, sm[w][t]);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sm[w][t] - ref);  // 0 for a wave that had no block
+      const float4 x = *(const float4*)&so[w][t][d];
+      num.x += f * x.x; num.y += f * x.y; num.z += f * x.z; num.w += f * x.w;
+      den += f * sl[w][t];
+    }
+    if (splits > 1) {
+      const int64_t at = ((int64_t)blockIdx.y * a.G + group) * ((int64_t)a.T * a.R) + (int64_t)seg.first * a.R + row0 + t;
+      *(float4*)(part + at * HD + d) = num;
+      if (d == 0) stats[at] = make_float2(mm, den);
+      continue;
+    }
+    const int tk = div_r(a, row0 + t);
+    const int64_t at = (int64_t)(seg.first + tk) * a.H + group * a.R + row0 + t - tk * a.R;
+    const float inv = den == 0.f ? 0.f : 1.f / den;  // a row without keys gives 0
+    store4(out + at * HD + d, make_float4(num.x * inv, num.y * inv, num.z * inv, num.w * inv));
+    if (d == 0 && lse) lse[at] = (mm + __builtin_amdgcn_logf(den)) * kLn2;
+  }
+}
+
+// Joins the parts of the keys: HD / 4 lanes a row.
+template <class T, int HD>
+__global__ __launch_bounds__(256) void packed_join_kernel(const Packed a, int splits, const float* __restrict__ part,
+                                                          const float2* __restrict__ stats, T* __restrict__ out,
+                                                          float* __restrict__ lse) {
+  const uint32_t rows = (uint32_t)a.T * a.R;
+  const int64_t all = (int64_t)rows * a.G;
+  const uint32_t at = (blockIdx.x * 256u + threadIdx.x) / (HD / 4);  // below 2^29 for all rows
+  const int d = 4 * (threadIdx.x % (HD / 4));
+  if (at >= all) return;
+  float mm = -INFINITY;
+  for (int s = 0; s < splits; ++s) mm = fmaxf(mm, stats[s * all + at].x);
+  const float ref = mm == -INFINITY ? 0.f : mm;
+  float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+  float den = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const float2 st = stats[s * all + at];
+    const float f = __builtin_amdgcn_exp2f(st.x - ref);
+    const float4 x = *(const float4*)(part + (s * all + at) * HD + d);
+    num.x += f * x.x; num.y += f * x.y; num.z += f * x.z; num.w += f * x.w;
+    den += f * st.y;
+  }
+  const int group = at / rows, row = at % rows, tk = div_r(a, row);
+  const int64_t to = (int64_t)tk * a.H + group * a.R + row - tk * a.R;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  store4(out + to * HD + d, make_float4(num.x * inv, num.y * inv, num.z * inv, num.w * inv));
+  if (d == 0 && lse) lse[to] = (mm + __builtin_amdgcn_logf(den)) * kLn2;
+}
+
+// ----------------------------------------------------------------- backward
+struct Grads {
+  const char* g_out;
+  int64_t gt, gh;  // bytes
+  const float *lse2, *delta;  // [group][T R]: base 2, +inf for a row without keys
+  float scale;
+};
+
+// lse2 and delta of every row, HD / 4 lanes a row.
+template <class T, int HD>
+__global__ __launch_bounds__(256) void packed_delta_kernel(const Packed a, const char* __restrict__ g_out, int64_t gt,
+                                                           int64_t gh, const T* __restrict__ out,
+                                                           const float* __restrict__ lse,
+                                                           const float* __restrict__ g_lse, float* __restrict__ lse2,
+                                                           float* __restrict__ delta) {
+  constexpr int L = HD / 4;
+  const uint32_t at = (blockIdx.x * 256u + threadIdx.x) / L;  // below 2^29 for all rows
+  const int d = 4 * (threadIdx.x % L);
+  const bool in = at < (uint32_t)a.T * a.H;
+  const uint32_t row = in ? at : 0;
+  const int t = row / (uint32_t)a.H, h = row % (uint32_t)a.H;
+  const float4 x = load4(row_at<T>(g_out, gt, gh, t, h) + d), y = load4(out + (int64_t)row * HD + d);
+  float s = x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+#pragma unroll
+  for (int o = L / 2; o; o >>= 1) s += __shfl_xor(s, o);
+  if (!in || d) return;
+  const int g = div_r(a, h);
+  const int64_t to = (int64_t)g * a.T * a.R + (int64_t)t * a.R + h - g * a.R;
+  const float z = lse[row];
+  lse2[to] = z == -INFINITY ? INFINITY : z * kLog2e;
+  delta[to] = g_lse ? s - g_lse[row] : s;
+}
+
+// dq: 32 rows a workgroup, tiles of scores transposed (the lane's column a row).
+template <class T, int HD>
+__global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, const Grads g, T* __restrict__ dq) {
+  constexpr int DT = HD / 32, PO = HD + 4;
+  __shared__ float so[kWaves][32][PO];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int group = blockIdx.x % a.G;
+  const Segment seg = segment_of<5>(a.starts, a.wide, a.n, a.T, a.R, blockIdx.x / a.G);
+  const int rows = seg.len * a.R, tiles = (rows + 31) >> 5;
+  if (seg.tile >= tiles) return;
+  const int row0 = 32 * (tiles - 1 - seg.tile);
+  const Keys keys = keys_of(a, seg.seq);
+  const int ri = min(row0 + col, rows - 1), tok = div_r(a, ri);
+  const int sees = min(tok + 1 + keys.len - seg.len, keys.len);
+  const int most = min(div_r(a, min(row0 + 31, rows - 1)) + 1 + keys.len - seg.len, keys.len);
+  const int least = min(div_r(a, row0) + 1 + keys.len - seg.len, keys.len);
+  const int head = group * a.R + ri - tok * a.R;
+
+  float4 q[HD / 8], go[HD / 8];
+  load_operand<HD>(q, row_at<T>(a.q, a.qt, a.qh, seg.first + tok, head), half);
+  load_operand<HD>(go, row_at<T>(g.g_out, g.gt, g.gh, seg.first + tok, head), half);
+  const int64_t st = (int64_t)group * a.T * a.R + (int64_t)seg.first * a.R + ri;
+  const float lse2 = g.lse2[st], delta = g.delta[st];
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  const int blocks = most > 0 ? (most + 31) >> 5 : 0;
+  const char* kb = a.k + group * a.kh + keys.first * a.kt;
+  const char* vb = a.v + group * a.vh + keys.first * a.vt;
+  for (int j = wave; j < blocks; j += kWaves) {
+    const int k0 = 32 * j, key = min(k0 + col, keys.len - 1);
+    float4 x[HD / 8];
+    load_operand<HD>(x, (const T*)(kb + key * a.kt), half);
+    const f32x16 s = products<HD>(x, q);
+    load_operand<HD>(x, (const T*)(vb + key * a.vt), half);
+    f32x16 ds = products<HD>(x, go);
+    const bool masked = k0 + 32 > least;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2)) * (ds[r] - delta);
+      if (masked && k0 + tile_row(r, half) >= sees) ds[r] = 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float kx = (float)((const T*)(kb + min(k0 + tile_row(r, half), keys.len - 1) * a.kt))[32 * d + col];
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx, ds[r], acc[d], 0, 0, 0);
+      }
+  }
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      *(float4*)&so[wave][col][32 * d + tile_row(r, half)] =
+          make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+  __syncthreads();
+  for (int i = tid; i < 32 * HD / 4; i += kThreads) {
+    const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
+    if (row0 + t >= rows) continue;
+    float4 x = *(const float4*)&so[0][t][d];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+      const float4 y = *(const float4*)&so[w][t][d];
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    const int tk = div_r(a, row0 + t);
+    const int64_t at = (int64_t)(seg.first + tk) * a.H + group * a.R + row0 + t - tk * a.R;
+    store4(dq + at * HD + d, make_float4(x.x * g.scale, x.y * g.scale, x.z * g.scale, x.w * g.scale));
+  }
+}
+
+// dk and dv: 32 keys a workgroup, the lane's column a key, rows in the registers.
+template <class T, int HD>
+__global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, const Grads g, T* __restrict__ dk,
+                                                              T* __restrict__ dv) {
+  constexpr int DT = HD / 32, PO = HD + 4;
+  __shared__ float so[kWaves][32][PO];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int group = blockIdx.x % a.G;
+  const Segment seg = segment_of<5>(a.key_starts, a.wide, a.n, a.S, 1, blockIdx.x / a.G);
+  if (32 * seg.tile >= seg.len) return;
+  const int k0 = 32 * seg.tile;
+  const bool real = seg.seq >= 0 && seg.seq < a.n;
+  const int len = real ? keys_of(a, seg.seq).len : 0;  // of the segment's keys those in use
+  int first = 0, rows = 0, behind = 0;
+  if (real) {
+    first = __builtin_amdgcn_readfirstlane(segment_start(a.starts, a.wide, a.n, a.T, seg.seq + 1));
+    const int end = __builtin_amdgcn_readfirstlane(segment_start(a.starts, a.wide, a.n, a.T, seg.seq + 2));
+    const int tokens = max(end - first, 0);
+    rows = tokens * a.R;
+    behind = len - tokens;  // token j sees the keys below j + 1 + behind
+  }
+  f32x16 ak[DT], av[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) ak[d] = av[d] = f32x16{};
+  if (k0 < len) {
+    const int key = min(k0 + col, len - 1);
+    const T* krow = row_at<T>(a.k, a.kt, a.kh, seg.first + key, group);
+    const T* vrow = row_at<T>(a.v, a.vt, a.vh, seg.first + key, group);
+    float4 k[HD / 8], v[HD / 8];
+    if (HD <= 64) {
+      load_operand<HD>(k, krow, half);
+      load_operand<HD>(v, vrow, half);
+    }
+    const int64_t st = (int64_t)group * a.T * a.R + (int64_t)first * a.R;
+    const int row_from = max(k0 - behind, 0) * a.R, blocks = (rows + 31) >> 5;
+    for (int j = (row_from >> 5) + wave; j < blocks; j += kWaves) {
+      const int r0 = 32 * j;
+      float4 x[HD / 8];
+      const int ri = min(r0 + col, rows - 1), tk = div_r(a, ri), h = group * a.R + ri - tk * a.R;
+      if (HD > 64) load_operand<HD>(k, krow, half);
+      load_operand<HD>(x, row_at<T>(a.q, a.qt, a.qh, first + tk, h), half);
+      f32x16 s = products<HD>(x, k);
+      if (HD > 64) load_operand<HD>(v, vrow, half);
+      load_operand<HD>(x, row_at<T>(g.g_out, g.gt, g.gh, first + tk, h), half);
+      f32x16 ds = products<HD>(x, v);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = r0 + tile_row(r, half), at = min(row, rows - 1);
+        const bool off = row >= rows || k0 + col > div_r(a, at) + behind || k0 + col >= len;
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -g.lse2[st + at]));
+        s[r] = off ? 0.f : p;
+        ds[r] = off ? 0.f : p * (ds[r] - g.delta[st + at]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int at = min(r0 + tile_row(r, half), rows - 1), t = div_r(a, at), hh = group * a.R + at - t * a.R;
+        const T* qrow = row_at<T>(a.q, a.qt, a.qh, first + t, hh) + col;
+        const T* grow = row_at<T>(g.g_out, g.gt, g.gh, first + t, hh) + col;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          ak[d] = __builtin_amdgcn_mfma_f32_32x32x2f32((float)qrow[32 * d], ds[r], ak[d], 0, 0, 0);
+          av[d] = __builtin_amdgcn_mfma_f32_32x32x2f32((float)grow[32 * d], s[r], av[d], 0, 0, 0);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    T* to = which ? dv : dk;
+    if (!to) continue;
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const f32x16& c = which ? av[d] : ak[d];
+        *(float4*)&so[wave][col][32 * d + tile_row(r, half)] = make_float4(c[r], c[r + 1], c[r + 2], c[r + 3]);
+      }
+    __syncthreads();
+    const float f = which ? 1.f : g.scale;
+    for (int i = tid; i < 32 * HD / 4; i += kThreads) {
+      const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
+      if (k0 + t >= seg.len) continue;
+      float4 x = *(const float4*)&so[0][t][d];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) {
+        const float4 y = *(const float4*)&so[w][t][d];
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+      store4(to + ((int64_t)(seg.first + k0 + t) * a.G + group) * HD + d,
+             make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+    }
+  }
+}
+
+// --------------------------------------------------------------------- host
+typedef mpl_packed_attention_args Args;
+
+int element_size(int dtype) { return dtype == MPL_F32 ? 4 : 2; }
+
+// What does not depend on the buffers.
+int check_sizes(const Args* p, const char* what) {
+  MPL_REQUIRE(p, MPL_EINVAL, "%s: null arguments", what);
+  MPL_REQUIRE(p->dtype == MPL_F32 || p->dtype == MPL_F16 || p->dtype == MPL_BF16, MPL_EINVAL, "%s: dtype %d", what, p->dtype);
+  MPL_REQUIRE(p->heads > 0 && p->groups > 0 && p->heads % p->groups == 0, MPL_EINVAL,
+              "%s: %d heads for %d key heads", what, p->heads, p->groups);
+  MPL_REQUIRE(p->head_dim == 32 || p->head_dim == 64 || p->head_dim == 128, MPL_EUNSUPPORTED,
+              "%s: head_dim %d (32, 64 or 128)", what, p->head_dim);
+  MPL_REQUIRE(p->tokens >= 0 && p->keys >= 0 && p->sequences >= 0, MPL_EINVAL,
+              "%s: bad sizes tokens=%lld keys=%lld sequences=%lld", what, (long long)p->tokens, (long long)p->keys,
+              (long long)p->sequences);
+  MPL_REQUIRE(p->index_bytes == 4 || p->index_bytes == 8, MPL_EINVAL, "%s: index_bytes %d (4 or 8)", what, p->index_bytes);
+  // rows are counted in 32 bits, and a grid's threads too
+  constexpr int64_t kMost = (int64_t)1 << 30;
+  MPL_REQUIRE(p->heads <= 65536 && p->tokens <= kMost && p->keys <= kMost && p->sequences <= kMost &&
+                  p->tokens * (p->heads / p->groups) <= kMost &&
+                  (p->tokens * (p->heads / p->groups) / 32 + p->sequences + 2) * p->groups < ((int64_t)1 << 24) &&
+                  (p->keys / 32 + p->sequences + 2) * p->groups < ((int64_t)1 << 24) &&
+                  p->tokens * p->heads * (p->head_dim / 4) < ((int64_t)1 << 32),
+              MPL_EUNSUPPORTED, "%s: %lld tokens and %lld keys in %lld sequences of %d and %d heads are too many", what,
+              (long long)p->tokens, (long long)p->keys, (long long)p->sequences, p->heads, p->groups);
+  return MPL_OK;
+}
+
+int check_rows(const Args* p, const void* x, int64_t tok, int64_t head, const char* name, const char* what) {
+  const int64_t unit = 16 / element_size(p->dtype);
+  MPL_REQUIRE(x, MPL_EINVAL, "%s: null %s", what, name);
+  MPL_REQUIRE(((uintptr_t)x & 15) == 0 && tok >= 0 && head >= 0 && tok % unit == 0 && head % unit == 0, MPL_EINVAL,
+              "%s: the rows of %s must be 16-byte aligned (token %lld, head %lld)", what, name, (long long)tok,
+              (long long)head);
+  return MPL_OK;
+}
+
+int check_inputs(const Args* p, const char* what) {
+  if (int rc = check_sizes(p, what)) return rc;
+  MPL_REQUIRE(p->scale > 0.f && p->scale < INFINITY, MPL_EINVAL, "%s: scale must be positive and finite", what);
+  MPL_REQUIRE(p->starts && p->key_starts, MPL_EINVAL, "%s: null starts", what);
+  MPL_REQUIRE((((uintptr_t)p->starts | (uintptr_t)p->key_starts | (uintptr_t)p->key_lengths) & (p->index_bytes - 1)) == 0,
+              MPL_EINVAL, "%s: starts must be aligned", what);
+  if (p->tokens)
+    if (int rc = check_rows(p, p->q, p->q_token, p->q_head, "q", what)) return rc;
+  if (p->keys) {
+    if (int rc = check_rows(p, p->k, p->k_token, p->k_head, "k", what)) return rc;
+    if (int rc = check_rows(p, p->v, p->v_token, p->v_head, "v", what)) return rc;
+  }
+  return MPL_OK;
+}
+
+Packed device_args(const Args* p) {
+  Packed a;
+  const int64_t e = element_size(p->dtype);
+  a.q = (const char*)p->q; a.k = (const char*)p->k; a.v = (const char*)p->v;
+  a.qt = p->q_token * e; a.qh = p->q_head * e;
+  a.kt = p->k_token * e; a.kh = p->k_head * e;
+  a.vt = p->v_token * e; a.vh = p->v_head * e;
+  a.starts = p->starts; a.key_starts = p->key_starts; a.key_lengths = p->key_lengths;
+  a.n = (int)p->sequences;
+  a.wide = p->index_bytes == 8;
+  a.T = (int)p->tokens; a.S = (int)p->keys;
+  a.H = p->heads; a.G = p->groups; a.R = p->heads / p->groups;
+  a.shift = 0;
+  while (((int64_t)1 << a.shift) < a.R) ++a.shift;
+  a.magic = (uint32_t)((((uint64_t)1 << (31 + a.shift)) + a.R - 1) / a.R);
+  a.c = p->scale * kLog2e;
+  return a;
+}
+
+// Parts of the keys: where the tiles of rows do not fill the chip and the keys of
+// a sequence are many.  Only sums over the sequences are known here.
+int splits_of(const Args* p) {
+  const int64_t r = p->heads / p->groups, n = p->sequences ? p->sequences : 1;
+  const int64_t tiles = (p->tokens * r / 32 + (p->tokens < n ? p->tokens : n)) * p->groups;
+  const int64_t per = p->keys / n;  // keys of a sequence
+  if (tiles <= 0 || tiles >= 1024 || per < 512) return 1;
+  const int64_t want = 1024 / tiles, most = per / 256;
+  const int64_t s = want < most ? want : most;
+  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+
+size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+size_t workspace_bytes(const Args* p, bool backward) {
+  const size_t rows = (size_t)p->tokens * p->heads;
+  if (backward) return 2 * round256(rows * 4);
+  const int s = splits_of(p);
+  return s > 1 ? round256(s * rows * p->head_dim * 4) + round256(s * rows * 8) : 0;
+}
+
+template <class T, int HD>
+void forward(const Args* p, void* out, float* lse, void* ws, hipStream_t s) {
+  const Packed a = device_args(p);
+  const int splits = splits_of(p);
+  const size_t rows = (size_t)p->tokens * p->heads;
+  float* part = (float*)ws;
+  float2* stats = (float2*)((char*)ws + round256(splits * rows * HD * 4));
+  const int64_t tiles = ((int64_t)a.T * a.R / 32 + a.n + 2) * a.G;
+  packed_forward_kernel<T, HD><<<dim3((unsigned)tiles, splits), kThreads, 0, s>>>(a, splits, (T*)out, lse, part, stats);
+  if (splits > 1)
+    packed_join_kernel<T, HD><<<(unsigned)cdiv(rows * (HD / 4), 256), 256, 0, s>>>(a, splits, part, stats, (T*)out, lse);
+}
+
+template <class T, int HD>
+void backward(const Args* p, const void* g_out, int64_t gt, int64_t gh, const void* out, const float* lse,
+              const float* g_lse, void* ws, void* dq, void* dk, void* dv, hipStream_t s) {
+  const Packed a = device_args(p);
+  const size_t rows = (size_t)p->tokens * p->heads;
+  float* lse2 = (float*)ws;
+  float* delta = (float*)((char*)ws + round256(rows * 4));
+  Grads g{(const char*)g_out, gt * (int64_t)sizeof(T), gh * (int64_t)sizeof(T), lse2, delta, p->scale};
+  if (rows)
+    packed_delta_kernel<T, HD><<<(unsigned)cdiv(rows * (HD / 4), 256), 256, 0, s>>>(a, g.g_out, g.gt, g.gh, (const T*)out,
+                                                                                   lse, g_lse, lse2, delta);
+  if (rows && dq)
+    packed_dq_kernel<T, HD><<<(unsigned)(((int64_t)a.T * a.R / 32 + a.n + 2) * a.G), kThreads, 0, s>>>(a, g, (T*)dq);
+  if (a.S && (dk || dv))
+    packed_dkv_kernel<T, HD><<<(unsigned)(((int64_t)a.S / 32 + a.n + 2) * a.G), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
+}
+
+template <class F>
+void with_types(const Args* p, F&& f) {
+  auto width = [&](auto t) {
+    if (p->head_dim == 32) f(t, std::integral_constant<int, 32>{});
+    else if (p->head_dim == 64) f(t, std::integral_constant<int, 64>{});
+    else f(t, std::integral_constant<int, 128>{});
+  };
+  if (p->dtype == MPL_F32) width(float{});
+  else if (p->dtype == MPL_F16) width(_Float16{});
+  else width(__bf16{});
+}
+
+}  // namespace
+}  // namespace mpl
+
+using namespace mpl;
+
+extern "C" size_t mpl_packed_attention_workspace_bytes(const mpl_packed_attention_args* args, int backward) {
+  clear_error();
+  if (check_sizes(args, "mpl_packed_attention_workspace_bytes")) return 0;
+  const size_t n = workspace_bytes(args, backward != 0);
+  return n ? n : 256;
+}
+
+extern "C" int mpl_packed_attention(const mpl_packed_attention_args* args, void* workspace, size_t workspace_bytes_,
+                                    void* out, float* lse, void* stream) {
+  clear_error();
+  if (int rc = check_inputs(args, "mpl_packed_attention")) return rc;
+  if (!args->tokens) return MPL_OK;
+  MPL_REQUIRE(out && ((uintptr_t)out & 15) == 0, MPL_EINVAL, "mpl_packed_attention: out must be 16-byte aligned");
+  const size_t need = workspace_bytes(args, false);
+  MPL_REQUIRE(!need || (workspace && ((uintptr_t)workspace & 255) == 0), MPL_EINVAL,
+              "mpl_packed_attention: a 256-byte aligned workspace is needed");
+  MPL_REQUIRE(workspace_bytes_ >= need, MPL_EWORKSPACE, "mpl_packed_attention: workspace of %zu bytes needed", need);
+  with_types(args, [&](auto t, auto hd) {
+    forward<decltype(t), decltype(hd)::value>(args, out, lse, workspace, (hipStream_t)stream);
+  });
+  return check_launch("mpl_packed_attention");
+}
+
+extern "C" int mpl_packed_attention_bwd(const mpl_packed_attention_args* args, const void* g_out, int64_t g_token,
+                                        int64_t g_head, const void* out, const float* lse, const float* g_lse,
+                                        void* workspace, size_t workspace_bytes_, void* dq, void* dk, void* dv,
+                                        void* stream) {
+  clear_error();
+  if (int rc = check_inputs(args, "mpl_packed_attention_bwd")) return rc;
+  MPL_REQUIRE(dq || dk || dv, MPL_EINVAL, "mpl_packed_attention_bwd: no gradient is asked for");
+  MPL_REQUIRE((((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, MPL_EINVAL,
+              "mpl_packed_attention_bwd: gradients must be 16-byte aligned");
+  if (args->tokens) {
+    if (int rc = check_rows(args, g_out, g_token, g_head, "g_out", "mpl_packed_attention_bwd")) return rc;
+    MPL_REQUIRE(out && ((uintptr_t)out & 15) == 0 && lse, MPL_EINVAL,
+                "mpl_packed_attention_bwd: out (16-byte aligned) and lse are needed");
+    const size_t need = workspace_bytes(args, true);
+    MPL_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0, MPL_EINVAL,
+                "mpl_packed_attention_bwd: a 256-byte aligned workspace is needed");
+    MPL_REQUIRE(workspace_bytes_ >= need, MPL_EWORKSPACE, "mpl_packed_attention_bwd: workspace of %zu bytes needed", need);
+  }
+  with_types(args, [&](auto t, auto hd) {
+    backward<decltype(t), decltype(hd)::value>(args, g_out, g_token, g_head, out, lse, g_lse, workspace, dq, dk, dv,
+                                               (hipStream_t)stream);
+  });
+  return check_launch("mpl_packed_attention_bwd");
+}

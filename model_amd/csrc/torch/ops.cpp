@@ -1,9 +1,10 @@
-// The host path of layer_norm and vocab_cross_entropy (model_amd/layer_norm.py,
-// model_amd/cross_entropy.py check the arguments and document them): output and
-// workspace tensors, the calls into libmpl.so (include/mpl.h), and the autograd
-// nodes.  In C++ because a training step's small calls are bound by host time:
-// torch runs backward nodes on a thread of its own, where a Python node of these
-// two operators took 40 to 80 us a call, several times its kernels.
+// The host path of layer_norm, vocab_cross_entropy and packed_attention
+// (model_amd/layer_norm.py, cross_entropy.py and attention.py check the arguments
+// and document them): output and workspace tensors, the calls into libmpl.so
+// (include/mpl.h), and the autograd nodes; and of clip_global_norm
+// (model_amd/grad_clip.py).  In C++ because a training step's small calls are bound
+// by host time: torch runs backward nodes on a thread of its own, where a Python
+// node of the first two took 40 to 80 us a call, several times its kernels.
 //
 // Host code only: built by the host compiler against torch's headers and linked
 // to libmpl.so beside it.
@@ -346,6 +347,147 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> vocab_cross_entropy_grads(const Tenso
   return {loss, lse, dh, de};
 }
 
+// ------------------------------------------------------- packed attention
+// [tokens, heads, hd] with hd elements next to each other and rows at 16 bytes;
+// copied only where they do not lie so.
+struct Heads {
+  Tensor t;
+  int64_t token = 0, head = 0;
+};
+Heads heads_of(const Tensor& x) {
+  Tensor t = x._is_zerotensor() ? dense(x) : x.resolve_neg();
+  const int64_t unit = 16 / t.element_size();
+  auto lies = [&](const Tensor& y) {
+    return y.numel() == 0 ||
+           (y.stride(2) == 1 && (uintptr_t)y.data_ptr() % 16 == 0 && (y.size(0) == 1 || y.stride(0) % unit == 0) &&
+            (y.size(1) == 1 || y.stride(1) % unit == 0));
+  };
+  if (!lies(t)) t = t.clone(at::MemoryFormat::Contiguous);
+  if (t.numel() == 0) return {t, 0, 0};
+  return {t, t.size(0) == 1 ? 0 : t.stride(0), t.size(1) == 1 ? 0 : t.stride(1)};
+}
+
+// The arguments of a call, and the tensors that they point into.
+struct PackedCall {
+  mpl_packed_attention_args a;
+  Heads q, k, v;
+  Tensor starts, key_starts, key_lengths;
+  PackedCall(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& starts_, const Tensor& key_starts_,
+             const Tensor& key_lengths_, double scale)
+      : q(heads_of(q_)), k(heads_of(k_)), v(heads_of(v_)), starts(dense(starts_)), key_starts(dense(key_starts_)),
+        key_lengths(dense(key_lengths_)) {
+    a.q = ptr(q.t); a.k = ptr(k.t); a.v = ptr(v.t);
+    a.q_token = q.token; a.q_head = q.head;
+    a.k_token = k.token; a.k_head = k.head;
+    a.v_token = v.token; a.v_head = v.head;
+    a.dtype = dtype_code(q_);
+    a.heads = (int)q_.size(1); a.groups = (int)k_.size(1); a.head_dim = (int)q_.size(2);
+    a.tokens = q_.size(0); a.keys = k_.size(0); a.sequences = starts.numel() - 1;
+    a.starts = ptr(starts);
+    a.key_starts = key_starts.defined() ? ptr(key_starts) : ptr(starts);
+    a.key_lengths = ptr(key_lengths);
+    a.index_bytes = (int)starts.element_size();
+    a.scale = (float)scale;
+  }
+  Tensor workspace(bool backward) const {
+    const size_t n = mpl_packed_attention_workspace_bytes(&a, backward);
+    TORCH_CHECK_VALUE(n, "packed_attention: ", mpl_last_error());
+    return at::empty({(int64_t)n}, q.t.options().dtype(at::kByte));
+  }
+};
+
+std::tuple<Tensor, Tensor> pa_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& starts,
+                                      const Tensor& key_starts, const Tensor& key_lengths, double scale, bool want_lse) {
+  const c10::DeviceGuard guard(q.device());
+  const PackedCall c(q, k, v, starts, key_starts, key_lengths, scale);
+  Tensor out = at::empty(q.sizes(), q.options()), lse;
+  if (want_lse) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  if (q.size(0)) {
+    const Tensor ws = c.workspace(false);
+    check(mpl_packed_attention(&c.a, ws.data_ptr(), ws.numel(), out.data_ptr(), (float*)ptr(lse), stream_of(q)),
+          "mpl_packed_attention");
+  }
+  return {out, lse};
+}
+
+// (dq, dk, dv), undefined where not wanted
+std::tuple<Tensor, Tensor, Tensor> pa_backward(const Tensor& g_out, const Tensor& g_lse, const Tensor& q, const Tensor& k,
+                                               const Tensor& v, const Tensor& out, const Tensor& lse, const Tensor& starts,
+                                               const Tensor& key_starts, const Tensor& key_lengths, double scale,
+                                               bool want_q, bool want_k, bool want_v) {
+  const c10::DeviceGuard guard(q.device());
+  Tensor dq, dk, dv;
+  if (want_q) dq = at::empty(q.sizes(), q.options());
+  if (want_k) dk = at::empty(k.sizes(), k.options());
+  if (want_v) dv = at::empty(v.sizes(), v.options());
+  if ((q.size(0) || k.size(0)) && (want_q || want_k || want_v)) {
+    const PackedCall c(q, k, v, starts, key_starts, key_lengths, scale);
+    const Heads g = heads_of(g_out.defined() ? g_out : at::zeros(q.sizes(), q.options()));
+    const Tensor o = heads_of(out.contiguous()).t, l = dense(lse);
+    const Tensor gl = g_lse.defined() ? dense(g_lse.to(at::kFloat)) : g_lse;
+    const Tensor ws = c.workspace(true);
+    check(mpl_packed_attention_bwd(&c.a, ptr(g.t), g.token, g.head, ptr(o), (const float*)ptr(l), (const float*)ptr(gl),
+                                   ws.data_ptr(), ws.numel(), ptr(dq), ptr(dk), ptr(dv), stream_of(q)),
+          "mpl_packed_attention_bwd");
+  }
+  return {dq, dk, dv};
+}
+
+struct PackedAttentionFunction : torch::autograd::Function<PackedAttentionFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                               const Tensor& starts, const std::optional<Tensor>& key_starts,
+                               const std::optional<Tensor>& key_lengths, double scale) {
+    auto [out, lse] = pa_forward(q, k, v, starts, or_none(key_starts), or_none(key_lengths), scale, true);
+    ctx->save_for_backward({q, k, v, out, lse, starts, or_none(key_starts), or_none(key_lengths)});
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    return {out, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!capturing(), "torch autograd through packed_attention is not supported under HIP graph capture: use "
+                "packed_attention_forward and packed_attention_backward, which capture");
+    variable_list out(7);
+    refuse_transforms("packed_attention's gradient", {grads[0], grads[1]});
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    {
+      const at::AutoGradMode no_grad(false);
+      std::tie(out[0], out[1], out[2]) =
+          pa_backward(grads[0], grads[1], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7],
+                      ctx->saved_data["scale"].toDouble(), ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                      ctx->needs_input_grad(2));
+    }
+    return once(std::move(out), "packed_attention");
+  }
+};
+
+// (out, lse or none)
+std::tuple<Tensor, std::optional<Tensor>> packed_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                           const Tensor& starts, const std::optional<Tensor>& key_starts,
+                                                           const std::optional<Tensor>& key_lengths, double scale,
+                                                           bool want_lse, bool autograd) {
+  refuse_transforms("packed_attention", {q, k, v, starts, or_none(key_starts), or_none(key_lengths)});
+  if (autograd) {
+    const variable_list out = PackedAttentionFunction::apply(q, k, v, starts, key_starts, key_lengths, scale);
+    return {out[0], want_lse ? std::optional<Tensor>(out[1]) : std::nullopt};
+  }
+  const at::AutoGradMode no_grad(false);
+  auto [out, lse] = pa_forward(q, k, v, starts, or_none(key_starts), or_none(key_lengths), scale, want_lse);
+  return {out, want_lse ? std::optional<Tensor>(lse) : std::nullopt};
+}
+
+std::tuple<Tensor, Tensor, Tensor> packed_attention_backward(const Tensor& g_out, const Tensor& q, const Tensor& k,
+                                                             const Tensor& v, const Tensor& out, const Tensor& lse,
+                                                             const Tensor& starts, const std::optional<Tensor>& key_starts,
+                                                             const std::optional<Tensor>& key_lengths, double scale,
+                                                             const std::optional<Tensor>& g_lse) {
+  refuse_transforms("packed_attention_backward",
+                    {g_out, q, k, v, out, lse, starts, or_none(key_starts), or_none(key_lengths), or_none(g_lse)});
+  const at::AutoGradMode no_grad(false);
+  return pa_backward(g_out, or_none(g_lse), q, k, v, out, lse, starts, or_none(key_starts), or_none(key_lengths), scale,
+                     true, true, true);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ops, m) {
@@ -354,5 +496,7 @@ PYBIND11_MODULE(_ops, m) {
   m.def("layer_norm_backward", &layer_norm_backward);
   m.def("vocab_cross_entropy", &vocab_cross_entropy);
   m.def("vocab_cross_entropy_grads", &vocab_cross_entropy_grads);
+  m.def("packed_attention", &packed_attention);
+  m.def("packed_attention_backward", &packed_attention_backward);
   m.def("pretend_capturing", &pretend_capturing);
 }
