@@ -860,6 +860,25 @@ int mpl_packed_attention_bwd(const mpl_packed_attention_args* args, const void* 
                              const void* out, const float* lse, const float* g_lse, void* workspace,
                              size_t workspace_bytes, void* dq, void* dk, void* dv, void* stream);
 
+/*
+ * The global norm of many gradients and the clip by it (train.py:395-399, over
+ * every dense gradient of a model beside the sparse rows):
+ *   gnorm = sqrt(sum of the squares of all count tensors + sum of row_sq [rows]),
+ *   scale = min(1, grad_clip / (gnorm + 1e-6)) (NaN where gnorm is),
+ * scale_gnorm[0] = scale, scale_gnorm[1] = gnorm (device), and with apply != 0
+ * every tensor is multiplied by scale in place (in fp32, rounded once to its type;
+ * left alone where scale is 1).  x, n and dtype are host arrays of device pointers
+ * (aligned to their elements), sizes in elements and types (MPL_F32, MPL_F16,
+ * MPL_BF16), read by the call; the tensors must not overlap where apply is set.
+ * row_sq is fp32 and may be NULL with rows = 0.  Sums are fp64 in a fixed order;
+ * no atomics, no memset.  Workspace (8-byte aligned):
+ * mpl_clip_grads_workspace_bytes(count) (0 for a count out of range).
+ */
+size_t mpl_clip_grads_workspace_bytes(int64_t count);
+int mpl_clip_grads(void* const* x, const int64_t* n, const int* dtype, int64_t count, const float* row_sq,
+                   int64_t rows, float grad_clip, int apply, float* scale_gnorm, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -96,6 +96,8 @@ SIGNATURES = {
     "mpl_packed_attention_workspace_bytes": (_SZ, [_P, _I]),
     "mpl_packed_attention": (_I, [_P, _P, _SZ, _P, _P, _P]),
     "mpl_packed_attention_bwd": (_I, [_P, _P, _I64, _I64, _P, _P, _P, _P, _SZ, _P, _P, _P, _P]),
+    "mpl_clip_grads_workspace_bytes": (_SZ, [_I64]),
+    "mpl_clip_grads": (_I, [_P, _P, _P, _I64, _P, _I64, _F, _I, _P, _P, _SZ, _P]),
     "mpl_vocab_logits": (_I, [_P, _P, _P, _F, _P, _I64, _I, _I64, _P, _P]),
     "mpl_rows_linear_pair": (_I, [_P, _P, _P, _F, _P, _P, _I, _I, _I64, _I, _I, _I, _P, _P, _P]),
     "mpl_balance_state_bytes": (_SZ, [_I64, _I]),

@@ -9,6 +9,7 @@
 // Host code only: built by the host compiler against torch's headers and linked
 // to libmpl.so beside it.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/TracerMode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
@@ -20,10 +21,13 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <memory>
 #include <optional>
 #include <tuple>
+#include <utility>
+#include <vector>
 
 #include "../../../include/mpl.h"
 
@@ -488,6 +492,83 @@ std::tuple<Tensor, Tensor, Tensor> packed_attention_backward(const Tensor& g_out
                      true, true, true);
 }
 
+// --------------------------------------------------------------- gradient clip
+Tensor clip_grads(const std::vector<Tensor>& grads, double grad_clip, const std::optional<Tensor>& row_sq, bool apply,
+                  const char* what) {
+  const Tensor rows = or_none(row_sq);
+  TORCH_CHECK_VALUE(!grads.empty() || rows.defined(), what, ": no gradients");
+  TORCH_CHECK_VALUE(grad_clip >= 0, what, ": grad_clip ", grad_clip, " must not be negative");
+  const auto device = (grads.empty() ? rows : grads[0]).device();
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& t = grads[i];
+    refuse_transforms(what, {t});
+    TORCH_CHECK_VALUE(t.layout() == at::kStrided && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf ||
+                                                     t.scalar_type() == at::kBFloat16),
+                      what, ": gradient ", i, " must be a dense float32, float16 or bfloat16 tensor, got ", t.scalar_type(),
+                      " ", t.layout());
+    TORCH_CHECK_VALUE(t.device() == device, what, ": gradient ", i, " on ", t.device(), ", others on ", device);
+    if (apply) {
+      TORCH_CHECK_VALUE(!(t.requires_grad() && at::GradMode::is_enabled()), what, ": gradient ", i,
+                        " requires grad itself: it cannot be scaled in place outside torch.no_grad()");
+      TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, what, ": gradient ", i,
+                        " is expanded: its elements share memory");
+    }
+  }
+  if (rows.defined()) {
+    refuse_transforms(what, {rows});
+    TORCH_CHECK_VALUE(rows.scalar_type() == at::kFloat && rows.layout() == at::kStrided && rows.device() == device, what,
+                      ": row_sq must be a dense float32 tensor on ", device);
+  }
+  TORCH_CHECK_VALUE(device.is_cuda(), what, " runs on the GPU only (libmpl.so), gradients are on ", device);
+  const at::AutoGradMode no_grad(false);
+  const c10::DeviceGuard guard(device);
+  std::vector<Tensor> held;                        // copies of what does not lie in one piece
+  std::vector<std::pair<Tensor, Tensor>> back;     // and where they go
+  std::vector<void*> x;
+  std::vector<int64_t> n;
+  std::vector<int> types;
+  std::vector<std::pair<char*, char*>> spans;
+  for (const Tensor& t : grads) {
+    if (t.numel() == 0 || t._is_zerotensor()) continue;  // add nothing, and are scaled by being what they are
+    Tensor y = t;
+    if (t.is_neg() || !t.is_non_overlapping_and_dense()) {
+      y = dense(t);
+      held.push_back(y);
+      if (apply) back.emplace_back(t, y);
+    } else if (apply) {
+      char* at = (char*)t.data_ptr();
+      spans.emplace_back(at, at + t.numel() * t.element_size());
+    }
+    x.push_back(y.data_ptr());
+    n.push_back(y.numel());
+    types.push_back(dtype_code(y));
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, what, ": two of the gradients share memory");
+  const auto opt = at::TensorOptions().device(device);
+  Tensor out = at::empty({2}, opt.dtype(at::kFloat));
+  const Tensor r = dense(rows);
+  const size_t bytes = mpl_clip_grads_workspace_bytes((int64_t)x.size());
+  TORCH_CHECK_VALUE(bytes, what, ": too many gradients");
+  const Tensor ws = at::empty({(int64_t)bytes}, opt.dtype(at::kByte));
+  check(mpl_clip_grads(x.data(), n.data(), types.data(), (int64_t)x.size(), (const float*)ptr(r), r.defined() ? r.numel() : 0,
+                       (float)grad_clip, apply, (float*)out.data_ptr(), ws.data_ptr(), bytes, stream_of(out)),
+        "mpl_clip_grads");
+  for (auto& [to, from] : back) to.copy_(from);
+  if (apply)
+    for (const Tensor& t : grads)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+
+Tensor clip_global_norm(const std::vector<Tensor>& grads, double grad_clip, const std::optional<Tensor>& row_sq) {
+  return clip_grads(grads, grad_clip, row_sq, true, "clip_global_norm");
+}
+Tensor global_norm_scale(const std::vector<Tensor>& grads, double grad_clip, const std::optional<Tensor>& row_sq) {
+  return clip_grads(grads, grad_clip, row_sq, false, "global_norm_scale");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ops, m) {
@@ -498,5 +579,7 @@ PYBIND11_MODULE(_ops, m) {
   m.def("vocab_cross_entropy_grads", &vocab_cross_entropy_grads);
   m.def("packed_attention", &packed_attention);
   m.def("packed_attention_backward", &packed_attention_backward);
+  m.def("clip_global_norm", &clip_global_norm);
+  m.def("global_norm_scale", &global_norm_scale);
   m.def("pretend_capturing", &pretend_capturing);
 }

@@ -7,6 +7,7 @@ Host mirror of the sparse half of the reference training step
   * ``merge_rows(slots, contribs, pool_size)``                 train.py:166-172
   * ``clip_scale(row_sq, rest_sq, grad_clip)``                 train.py:395-399
   * ``sum_squares(tensors, add)`` (the dense gradients' norm)   train.py:395-397
+    (of many gradients, and their clip in place: model_amd/grad_clip.py)
   * ``rowwise_adagrad(...)``                                   train.py:412-416
   * ``lazy_adam(...)``                                         train.py:417-426
   * ``warmup_cosine(step, lr, warmup_steps, steps)``           train.py:100-103
@@ -27,6 +28,7 @@ import torch
 
 from . import _lib
 from ._lib import check, ptr
+from .grad_clip import clip_global_norm, global_norm_scale
 
 MPL_F16, MPL_F32 = _lib.MPL_F16, _lib.MPL_F32
 
@@ -356,18 +358,26 @@ class SparseRowUpdate:
         return {"merged": merged, "slot_counts": counts}
 
     def apply(self, handle: Dict, rest_sq: Optional[torch.Tensor] = None,
-              dense_grads: Optional[Sequence[torch.Tensor]] = None) -> Dict[str, torch.Tensor]:
+              dense_grads: Optional[Sequence[torch.Tensor]] = None, clip_dense: bool = False) -> Dict[str, torch.Tensor]:
         """The second half (train.py:395-429): the global-norm clip over the
         merged rows and the dense gradients (rest_sq, their squared norm as
-        a device scalar, or dense_grads, the tensors, summed in the clip's
-        own pass), then the row optimizer step.  Call it on a stream that
-        has waited for the merge's."""
+        a device scalar, or dense_grads, the tensors, any number of them,
+        summed in the clip's own pass), then the row optimizer step.  With
+        ``clip_dense`` the dense gradients are clipped as well, in place, by
+        the same scale (grad_clip.clip_global_norm).  Call it on a stream
+        that has waited for the merge's."""
         merged, counts = handle["merged"], handle["slot_counts"]
         stream = torch.cuda.current_stream(merged.rows.device)
         for t in (merged.uniq, merged.rows, merged.row_sq, merged.num_unique, counts):
             if t is not None:
                 t.record_stream(stream)
-        sg = clip_scale(merged.row_sq, rest_sq, self.grad_clip, dense_grads)
+        if clip_dense or (dense_grads is not None and len(dense_grads) > 7):
+            if rest_sq is not None or dense_grads is None:
+                raise ValueError("clip_dense goes with dense_grads, and those without rest_sq")
+            norm = clip_global_norm if clip_dense else global_norm_scale
+            sg = norm(dense_grads, self.grad_clip, row_sq=merged.row_sq)
+        else:
+            sg = clip_scale(merged.row_sq, rest_sq, self.grad_clip, dense_grads)
         lr = warmup_cosine(self.step, self.lr, self.warmup_steps, self.steps) * self.pool_lr_mult
         scale = sg[0:1]
         if self.host is not None:
@@ -385,7 +395,7 @@ class SparseRowUpdate:
 
     def __call__(self, aux: Dict, probe_grads, layers: Sequence[int],
                  rest_sq: Optional[torch.Tensor] = None, count_slots: bool = False,
-                 dense_grads: Optional[Sequence[torch.Tensor]] = None) -> Dict[str, torch.Tensor]:
+                 dense_grads: Optional[Sequence[torch.Tensor]] = None, clip_dense: bool = False) -> Dict[str, torch.Tensor]:
         """One update from the fetches of ``layers`` (aux["slots"][i],
         aux["weights"][i], probe_grads[layer]): merge() then apply().  With
         count_slots the result also holds "slot_counts" [N] fp32, the fetches
@@ -394,5 +404,5 @@ class SparseRowUpdate:
         average), from the merge's own sort instead of a separate histogram.
         The global norm takes the dense gradients as rest_sq (their squared
         norm, a device scalar) or as dense_grads (the tensors, summed in the
-        clip's own pass)."""
-        return self.apply(self.merge(aux, probe_grads, layers, count_slots), rest_sq, dense_grads)
+        clip's own pass, and with clip_dense clipped in place)."""
+        return self.apply(self.merge(aux, probe_grads, layers, count_slots), rest_sq, dense_grads, clip_dense)
