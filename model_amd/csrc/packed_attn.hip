@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "packed_attn.h"
+#include "packed_attn16.h"
 
 namespace mpl {
 namespace {
@@ -51,17 +52,74 @@ __device__ __forceinline__ const T* row_at(const char* base, int64_t tok, int64_
   return (const T*)(base + t * tok + h * head);
 }
 
+// The waves' results of 32 rows in LDS: sums of weighted values, the maximum (base 2)
+// that was taken off and the sum of the weights.
+template <int HD>
+struct Join {
+  float so[kWaves][32][HD + 4];
+  float sm[kWaves][32], sl[kWaves][32];
+
+  __device__ __forceinline__ void put(int wave, int col, int half, float m, float l, const f32x16 (&acc)[HD / 32]) {
+    float l0 = l, l1 = l;
+    half_swap(l0, l1);
+    if (half == 0) {
+      sm[wave][col] = m;
+      sl[wave][col] = l0 + l1;
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *(float4*)&so[wave][col][32 * d + tile_row(r, half)] =
+            make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+  }
+
+  template <class T>
+  __device__ __forceinline__ void write(const Packed& a, int splits, const Segment& seg, int group, int row0, int rows,
+                                        T* out, float* lse, float* part, float2* stats) const {
+    for (int i = threadIdx.x; i < 32 * HD / 4; i += kThreads) {
+      const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
+      if (row0 + t >= rows) continue;
+      float mm = sm[0][t];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, sm[w][t]);
+      const float ref = mm == -INFINITY ? 0.f : mm;
+      float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+      float den = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(sm[w][t] - ref);  // 0 for a wave that had no block
+        const float4 x = *(const float4*)&so[w][t][d];
+        num.x += f * x.x; num.y += f * x.y; num.z += f * x.z; num.w += f * x.w;
+        den += f * sl[w][t];
+      }
+      if (splits > 1) {
+        const int64_t at =
+            ((int64_t)blockIdx.y * a.G + group) * ((int64_t)a.T * a.R) + (int64_t)seg.first * a.R + row0 + t;
+        *(float4*)(part + at * HD + d) = num;
+        if (d == 0) stats[at] = make_float2(mm, den);
+        continue;
+      }
+      const int tk = div_r(a, row0 + t);
+      const int64_t at = (int64_t)(seg.first + tk) * a.H + group * a.R + row0 + t - tk * a.R;
+      const float inv = den == 0.f ? 0.f : 1.f / den;  // a row without keys gives 0
+      store4(out + at * HD + d, make_float4(num.x * inv, num.y * inv, num.z * inv, num.w * inv));
+      if (d == 0 && lse) lse[at] = (mm + __builtin_amdgcn_logf(den)) * kLn2;
+    }
+  }
+};
+
 // ------------------------------------------------------------------ forward
 // A workgroup of 32 rows of one group; `splits` > 1: of one part of their keys,
 // whose sums go to `part` [split][group][T R][HD] and `stats` [..][2] (the running
 // maximum in base 2, the sum).
-template <class T, int HD>
-__global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a, int splits, T* __restrict__ out,
+template <int HD>
+__global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a, int splits, float* __restrict__ out,
                                                                   float* __restrict__ lse, float* __restrict__ part,
                                                                   float2* __restrict__ stats) {
-  constexpr int DT = HD / 32, PO = HD + 4;
-  __shared__ float so[kWaves][32][PO];
-  __shared__ float sm[kWaves][32], sl[kWaves][32];
+  typedef float T;
+  constexpr int DT = HD / 32;
+  __shared__ Join<HD> join;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -129,47 +187,212 @@ __global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a
     }
   }
 
-  float l0 = l, l1 = l;
-  half_swap(l0, l1);
-  if (half == 0) {
-    sm[wave][col] = m;
-    sl[wave][col] = l0 + l1;
-  }
+  join.put(wave, col, half, m, l, acc);
+  __syncthreads();
+  join.write(a, splits, seg, group, row0, rows, out, lse, part, stats);
+}
+
+// ------------------------------------------------- forward, fp16 and bf16
+// The running softmax of a wave's 32 rows, one a lane (both halves of the wave hold
+// the same rows and different keys).  The maximum that is taken off, m, moves only
+// when a row's scores pass it by 2^8 or more: until then the weights stay below
+// 2^8, exact in fp32 and of the same relative error in 16 bits, and the
+// accumulators need no scaling.
+template <class T, int HD>
+struct Softmax {
+  static constexpr int DT = HD / 32;
+  float m = -INFINITY, l = 0.f;
+  f32x16 acc[DT];
+  __device__ __forceinline__ Softmax() {
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  }
+  // One stage of 32 B keys, of which the row sees those below `sees` (counted from
+  // the stage's first); `masked`: some row of the wave does not see them all.
+  template <int B>
+  __device__ __forceinline__ void step(const Stage<HD>& st, const char* k, const char* v, const short8v (&q)[HD / 16],
+                                       float c, int sees, bool masked) {
+    const int half = (threadIdx.x >> 5) & 1;
+    f32x16 s[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      s[b] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) s[b] = mma16<T>(st.rows(k, b, i), q[i], s[b]);
+    }
+    if (masked) {
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * b + tile_row(r, half) >= sees) s[b][r] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+    float a0 = mx, a1 = mx;
+    half_swap(a0, a1);
+    mx = fmaxf(a0, a1) * c;
+    if (__any(mx > m + 8.f)) {
+      mx = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.f : mx));
+      m = mx;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;  // no key of the row yet
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(fmaf(s[b][8 * i + e], c, -ref));
+          sum += p[e];
+        }
+        const short8v w = round8<T>(p);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] = mma16<T>(st.cols(v, 2 * b + i, d), w, acc[d]);
+      }
+    l += sum;
+  }
+};
+
+// Many rows: 128 a workgroup, 32 a wave, 64 keys a stage that all four waves read.
+constexpr int kWideRows = 128, kWideKeys = 64;
+template <class T, int HD>
+__global__ __launch_bounds__(kThreads, 2) void packed_forward16_kernel(const Packed a, T* __restrict__ out,
+                                                                       float* __restrict__ lse) {
+  typedef Stage<HD> St;
+  constexpr int kBytes = kWideKeys * St::kRow, kLoads = kBytes / 1024 / kWaves;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int group = blockIdx.x % a.G;
+  const Segment seg = segment_of<7>(a.starts, a.wide, a.n, a.T, a.R, blockIdx.x / a.G);
+  const int rows = seg.len * a.R, tiles = (rows + kWideRows - 1) / kWideRows;
+  if (seg.tile >= tiles) return;
+  const int row0 = kWideRows * (tiles - 1 - seg.tile);  // the rows with the most keys first
+  const Keys keys = keys_of(a, seg.seq);
+  const int behind = keys.len - seg.len;
+  const int w0 = row0 + 32 * wave, ri = min(w0 + col, rows - 1), tok = div_r(a, ri);
+  const int sees = min(tok + 1 + behind, keys.len);
+  const int most = min(div_r(a, min(row0 + kWideRows, rows) - 1) + 1 + behind, keys.len);
+  const int wave_most = w0 < rows ? min(div_r(a, min(w0 + 32, rows) - 1) + 1 + behind, keys.len) : 0;
+  const int least = min(div_r(a, min(w0, rows - 1)) + 1 + behind, keys.len);
+  const char* kb = a.k + group * a.kh + keys.first * a.kt;
+  const char* vb = a.v + group * a.vh + keys.first * a.vt;
+  const char* qrow = a.q + (seg.first + tok) * a.qt + (group * a.R + ri - tok * a.R) * a.qh;
+  auto send = [&](int it, char* to) __attribute__((always_inline)) {
+    const int k0 = it * kWideKeys;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      St::load(to, wave * kLoads + i, [&](int r) { return kb + min(k0 + r, keys.len - 1) * a.kt; });
+      St::load(to + kBytes, wave * kLoads + i, [&](int r) { return vb + min(k0 + r, keys.len - 1) * a.vt; });
+    }
+  };
+  const St st;
+  const int stages = most > 0 ? (most + kWideKeys - 1) / kWideKeys : 0;
+  if (stages) send(0, lds);
+  short8v q[HD / 16];
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i) q[i] = *(const short8v*)(qrow + 32 * i + 16 * half);
+  Softmax<T, HD> sm;
+  for (int it = 0; it < stages; ++it) {
+    // behind the barrier this stage has arrived, and every wave has read the one
+    // before it, over which the next is sent
+    wait_vmcnt_le<0>();
+    reads_done();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (it + 1 < stages) send(it + 1, lds + 2 * kBytes * ((it + 1) & 1));
+    const int k0 = it * kWideKeys;
+    if (k0 < wave_most) {
+      const char* at = lds + 2 * kBytes * (it & 1);
+      sm.template step<2>(st, at, at + kBytes, q, a.c, sees - k0, k0 + kWideKeys > least);
+    }
+  }
+  float l0 = sm.l, l1 = sm.l;
+  half_swap(l0, l1);
+  const float l = l0 + l1, inv = l == 0.f ? 0.f : 1.f / l;  // a row without keys gives 0
+  if (w0 + col >= rows) return;
+  const int64_t at = (int64_t)(seg.first + tok) * a.H + group * a.R + ri - tok * a.R;
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4)
-      *(float4*)&so[wave][col][32 * d + tile_row(r, half)] =
-          make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
-  __syncthreads();
-  for (int i = tid; i < 32 * HD / 4; i += kThreads) {
-    const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
-    if (row0 + t >= rows) continue;
-    float mm = sm[0][t];
+      store4(out + at * HD + 32 * d + tile_row(r, half), make_float4(sm.acc[d][r] * inv, sm.acc[d][r + 1] * inv,
+                                                                    sm.acc[d][r + 2] * inv, sm.acc[d][r + 3] * inv));
+  if (lse && half == 0) lse[at] = (sm.m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Few rows: 32 a workgroup; every wave has keys, and stages of 32 of them, of its own.
+template <class T, int HD>
+__global__ __launch_bounds__(kThreads) void packed_forward16_few_kernel(const Packed a, int splits, T* __restrict__ out,
+                                                                        float* __restrict__ lse, float* __restrict__ part,
+                                                                        float2* __restrict__ stats) {
+  typedef Stage<HD> St;
+  constexpr int kBytes = 32 * St::kRow, kLoads = kBytes / 1024;
+  constexpr int kStages = 4 * kBytes * kWaves, kJoin = sizeof(Join<HD>);
+  __shared__ __attribute__((aligned(1024))) char lds[kStages > kJoin ? kStages : kJoin];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int group = blockIdx.x % a.G;
+  const Segment seg = segment_of<5>(a.starts, a.wide, a.n, a.T, a.R, blockIdx.x / a.G);
+  const int rows = seg.len * a.R, tiles = (rows + 31) >> 5;
+  if (seg.tile >= tiles) return;
+  const int row0 = 32 * (tiles - 1 - seg.tile);
+  const Keys keys = keys_of(a, seg.seq);
+  const int behind = keys.len - seg.len;
+  const int ri = min(row0 + col, rows - 1), tok = div_r(a, ri);
+  const int sees = min(tok + 1 + behind, keys.len);
+  const int most = min(div_r(a, min(row0 + 32, rows) - 1) + 1 + behind, keys.len);
+  const int least = min(div_r(a, row0) + 1 + behind, keys.len);
+  const char* kb = a.k + group * a.kh + keys.first * a.kt;
+  const char* vb = a.v + group * a.vh + keys.first * a.vt;
+  const char* qrow = a.q + (seg.first + tok) * a.qt + (group * a.R + ri - tok * a.R) * a.qh;
+  const int blocks = most > 0 ? (most + 31) >> 5 : 0, per = (blocks + splits - 1) / splits;
+  const int j0 = blockIdx.y * per + wave, j1 = min(blocks, ((int)blockIdx.y + 1) * per);
+  char* mine = lds + 4 * kBytes * wave;
+  auto send = [&](int j, char* to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, sm[w][t]);
-    const float ref = mm == -INFINITY ? 0.f : mm;
-    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.f;
+    for (int i = 0; i < kLoads; ++i) {
+      St::load(to, i, [&](int r) { return kb + min(32 * j + r, keys.len - 1) * a.kt; });
+      St::load(to + kBytes, i, [&](int r) { return vb + min(32 * j + r, keys.len - 1) * a.vt; });
+    }
+  };
+  const St st;
+  short8v q[HD / 16];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sm[w][t] - ref);  // 0 for a wave that had no block
-      const float4 x = *(const float4*)&so[w][t][d];
-      num.x += f * x.x; num.y += f * x.y; num.z += f * x.z; num.w += f * x.w;
-      den += f * sl[w][t];
+  for (int i = 0; i < HD / 16; ++i) q[i] = *(const short8v*)(qrow + 32 * i + 16 * half);
+  Softmax<T, HD> sm;
+  if (j0 < j1) send(j0, mine);
+  int turn = 0;
+  for (int j = j0; j < j1; j += kWaves, turn ^= 1) {
+    reads_done();  // of the stage before, over which the next is sent
+    if (j + kWaves < j1) {
+      send(j + kWaves, mine + 2 * kBytes * (turn ^ 1));
+      wait_vmcnt_le<2 * kLoads>();
+    } else {
+      wait_vmcnt_le<0>();
     }
-    if (splits > 1) {
-      const int64_t at = ((int64_t)blockIdx.y * a.G + group) * ((int64_t)a.T * a.R) + (int64_t)seg.first * a.R + row0 + t;
-      *(float4*)(part + at * HD + d) = num;
-      if (d == 0) stats[at] = make_float2(mm, den);
-      continue;
-    }
-    const int tk = div_r(a, row0 + t);
-    const int64_t at = (int64_t)(seg.first + tk) * a.H + group * a.R + row0 + t - tk * a.R;
-    const float inv = den == 0.f ? 0.f : 1.f / den;  // a row without keys gives 0
-    store4(out + at * HD + d, make_float4(num.x * inv, num.y * inv, num.z * inv, num.w * inv));
-    if (d == 0 && lse) lse[at] = (mm + __builtin_amdgcn_logf(den)) * kLn2;
+    asm volatile("" ::: "memory");
+    const char* at = mine + 2 * kBytes * turn;
+    sm.template step<1>(st, at, at + kBytes, q, a.c, sees - 32 * j, 32 * j + 32 > least);
   }
+  reads_done();
+  __syncthreads();  // the stages become the waves' results
+  Join<HD>& join = *(Join<HD>*)lds;
+  join.put(wave, col, half, sm.m, sm.l, sm.acc);
+  __syncthreads();
+  join.write(a, splits, seg, group, row0, rows, out, lse, part, stats);
 }
 
 // Joins the parts of the keys: HD / 4 lanes a row.
@@ -477,6 +700,12 @@ Packed device_args(const Args* p) {
   return a;
 }
 
+// Whether the 16-bit forward takes tiles of 128 rows: where they fill the chip.
+bool wide_of(const Args* p) {
+  const int64_t r = p->heads / p->groups;
+  return p->dtype != MPL_F32 && p->tokens * r / kWideRows * p->groups >= 256;
+}
+
 // Parts of the keys: where the tiles of rows do not fill the chip and the keys of
 // a sequence are many.  Only sums over the sequences are known here.
 int splits_of(const Args* p) {
@@ -494,7 +723,7 @@ size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 size_t workspace_bytes(const Args* p, bool backward) {
   const size_t rows = (size_t)p->tokens * p->heads;
   if (backward) return 2 * round256(rows * 4);
-  const int s = splits_of(p);
+  const int s = wide_of(p) ? 1 : splits_of(p);
   return s > 1 ? round256(s * rows * p->head_dim * 4) + round256(s * rows * 8) : 0;
 }
 
@@ -506,7 +735,17 @@ void forward(const Args* p, void* out, float* lse, void* ws, hipStream_t s) {
   float* part = (float*)ws;
   float2* stats = (float2*)((char*)ws + round256(splits * rows * HD * 4));
   const int64_t tiles = ((int64_t)a.T * a.R / 32 + a.n + 2) * a.G;
-  packed_forward_kernel<T, HD><<<dim3((unsigned)tiles, splits), kThreads, 0, s>>>(a, splits, (T*)out, lse, part, stats);
+  if constexpr (sizeof(T) == 2) {
+    if (wide_of(p)) {
+      const int64_t wide = ((int64_t)a.T * a.R / kWideRows + a.n + 2) * a.G;
+      packed_forward16_kernel<T, HD><<<(unsigned)wide, kThreads, 0, s>>>(a, (T*)out, lse);
+      return;
+    }
+    packed_forward16_few_kernel<T, HD><<<dim3((unsigned)tiles, splits), kThreads, 0, s>>>(a, splits, (T*)out, lse, part,
+                                                                                        stats);
+  } else {
+    packed_forward_kernel<HD><<<dim3((unsigned)tiles, splits), kThreads, 0, s>>>(a, splits, (T*)out, lse, part, stats);
+  }
   if (splits > 1)
     packed_join_kernel<T, HD><<<(unsigned)cdiv(rows * (HD / 4), 256), 256, 0, s>>>(a, splits, part, stats, (T*)out, lse);
 }
