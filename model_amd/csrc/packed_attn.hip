@@ -198,6 +198,11 @@ __global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a
 // when a row's scores pass it by 2^8 or more: until then the weights stay below
 // 2^8, exact in fp32 and of the same relative error in 16 bits, and the
 // accumulators need no scaling.
+// fp16's weights are 2^6 times as large, which the division takes out again: with
+// 2^8 that is 2^14, and those below 2^-20 of the largest keep all their bits.
+template <class T>
+constexpr float kLift = __is_same(T, _Float16) ? 6.f : 0.f;
+
 template <class T, int HD>
 struct Softmax {
   static constexpr int DT = HD / 32;
@@ -245,7 +250,7 @@ struct Softmax {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
     }
-    const float ref = m == -INFINITY ? 0.f : m;  // no key of the row yet
+    const float ref = (m == -INFINITY ? 0.f : m) - kLift<T>;  // no key of the row yet: weights 0
     float sum = 0.f;
 #pragma unroll
     for (int b = 0; b < B; ++b)
@@ -330,7 +335,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_forward16_kernel(const Pac
     for (int r = 0; r < 16; r += 4)
       store4(out + at * HD + 32 * d + tile_row(r, half), make_float4(sm.acc[d][r] * inv, sm.acc[d][r + 1] * inv,
                                                                     sm.acc[d][r + 2] * inv, sm.acc[d][r + 3] * inv));
-  if (lse && half == 0) lse[at] = (sm.m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (lse && half == 0) lse[at] = (sm.m - kLift<T> + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // Few rows: 32 a workgroup; every wave has keys, and stages of 32 of them, of its own.
@@ -390,7 +395,7 @@ __global__ __launch_bounds__(kThreads) void packed_forward16_few_kernel(const Pa
   reads_done();
   __syncthreads();  // the stages become the waves' results
   Join<HD>& join = *(Join<HD>*)lds;
-  join.put(wave, col, half, sm.m, sm.l, sm.acc);
+  join.put(wave, col, half, sm.m - kLift<T>, sm.l, sm.acc);
   __syncthreads();
   join.write(a, splits, seg, group, row0, rows, out, lse, part, stats);
 }
@@ -429,37 +434,74 @@ struct Grads {
   const char* g_out;
   int64_t gt, gh;  // bytes
   const float *lse2, *delta;  // [group][T R]: base 2, +inf for a row without keys
+  const float* largest;       // [3][blocks]
+  int blocks;
   float scale;
 };
 
-// lse2 and delta of every row, HD / 4 lanes a row.
+// lse2 and delta of every row, HD / 4 lanes a row.  For fp16 also each workgroup's
+// largest |g_out|^2 and |v|^2 of a row and largest |g_lse| (see unit_of); rows that
+// are not finite do not count.
+constexpr int kDeltaBlocks = 1024;
+template <int L>
+__device__ __forceinline__ float sum_lanes(float x) {
+#pragma unroll
+  for (int o = L / 2; o; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ __forceinline__ float finite_max(float top, float x) { return x < INFINITY ? fmaxf(top, x) : top; }
+
 template <class T, int HD>
 __global__ __launch_bounds__(256) void packed_delta_kernel(const Packed a, const char* __restrict__ g_out, int64_t gt,
                                                            int64_t gh, const T* __restrict__ out,
                                                            const float* __restrict__ lse,
                                                            const float* __restrict__ g_lse, float* __restrict__ lse2,
-                                                           float* __restrict__ delta) {
+                                                           float* __restrict__ delta, float* __restrict__ largest) {
   constexpr int L = HD / 4;
-  const uint32_t at = (blockIdx.x * 256u + threadIdx.x) / L;  // below 2^29 for all rows
+  constexpr bool kUnit = __is_same(T, _Float16);
   const int d = 4 * (threadIdx.x % L);
-  const bool in = at < (uint32_t)a.T * a.H;
-  const uint32_t row = in ? at : 0;
-  const int t = row / (uint32_t)a.H, h = row % (uint32_t)a.H;
-  const float4 x = load4(row_at<T>(g_out, gt, gh, t, h) + d), y = load4(out + (int64_t)row * HD + d);
-  float s = x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+  const uint32_t rows = (uint32_t)a.T * a.H, values = (uint32_t)a.S * a.G;  // below 2^29
+  float top[3] = {0.f, 0.f, 0.f};
+  for (uint32_t first = blockIdx.x * (256 / L); first < rows; first += gridDim.x * (256 / L)) {
+    const uint32_t at = first + threadIdx.x / L, row = min(at, rows - 1);
+    const int t = row / (uint32_t)a.H, h = row % (uint32_t)a.H;
+    const float4 x = load4(row_at<T>(g_out, gt, gh, t, h) + d), y = load4(out + (int64_t)row * HD + d);
+    const float s = sum_lanes<L>(x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w);
+    if (kUnit) top[0] = finite_max(top[0], sum_lanes<L>(x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w));
+    if (at < rows && d == 0) {
+      const int g = div_r(a, h);
+      const int64_t to = (int64_t)g * a.T * a.R + (int64_t)t * a.R + h - g * a.R;
+      const float z = lse[row], gl = g_lse ? g_lse[row] : 0.f;
+      lse2[to] = z == -INFINITY ? INFINITY : z * kLog2e;
+      delta[to] = s - gl;
+      if (kUnit) top[2] = finite_max(top[2], fabsf(gl));
+    }
+  }
+  if constexpr (kUnit) {
+    for (uint32_t first = blockIdx.x * (256 / L); first < values; first += gridDim.x * (256 / L)) {
+      const uint32_t row = min(first + threadIdx.x / L, values - 1);
+      const float4 x = load4(row_at<T>(a.v, a.vt, a.vh, row / (uint32_t)a.G, row % (uint32_t)a.G) + d);
+      top[1] = finite_max(top[1], sum_lanes<L>(x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w));
+    }
+    __shared__ float tops[4][3];
 #pragma unroll
-  for (int o = L / 2; o; o >>= 1) s += __shfl_xor(s, o);
-  if (!in || d) return;
-  const int g = div_r(a, h);
-  const int64_t to = (int64_t)g * a.T * a.R + (int64_t)t * a.R + h - g * a.R;
-  const float z = lse[row];
-  lse2[to] = z == -INFINITY ? INFINITY : z * kLog2e;
-  delta[to] = g_lse ? s - g_lse[row] : s;
+    for (int i = 0; i < 3; ++i) {
+#pragma unroll
+      for (int o = 32; o; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], o));
+      if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6][i] = top[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < 3) {
+      const int i = threadIdx.x;
+      largest[i * gridDim.x + blockIdx.x] = fmaxf(fmaxf(tops[0][i], tops[1][i]), fmaxf(tops[2][i], tops[3][i]));
+    }
+  }
 }
 
 // dq: 32 rows a workgroup, tiles of scores transposed (the lane's column a row).
-template <class T, int HD>
-__global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, const Grads g, T* __restrict__ dq) {
+template <int HD>
+__global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, const Grads g, float* __restrict__ dq) {
+  typedef float T;
   constexpr int DT = HD / 32, PO = HD + 4;
   __shared__ float so[kWaves][32][PO];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -532,9 +574,10 @@ __global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, con
 }
 
 // dk and dv: 32 keys a workgroup, the lane's column a key, rows in the registers.
-template <class T, int HD>
-__global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, const Grads g, T* __restrict__ dk,
-                                                              T* __restrict__ dv) {
+template <int HD>
+__global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, const Grads g, float* __restrict__ dk,
+                                                              float* __restrict__ dv) {
+  typedef float T;
   constexpr int DT = HD / 32, PO = HD + 4;
   __shared__ float so[kWaves][32][PO];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -628,6 +671,356 @@ __global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, co
   }
 }
 
+// ------------------------------------------------ backward, fp16 and bf16
+// The power of two that dz is multiplied by before it is rounded to fp16.  |dz| is at
+// most |dp| + |delta| <= B = 2 max|g_out| max|v| + max|g_lse|, and B goes to [2^13,
+// 2^14): nothing overflows, and gradients of any size keep their bits down to 2^-38
+// of B.  bf16 has fp32's range and takes 1.  Every thread of the workgroup calls it.
+template <class T>
+__device__ __forceinline__ float unit_of(const Grads& g, float* lds) {
+  if constexpr (__is_same(T, _Float16)) {
+    float top[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      top[i] = 0.f;
+      for (int b = threadIdx.x; b < g.blocks; b += kThreads) top[i] = fmaxf(top[i], g.largest[i * g.blocks + b]);
+#pragma unroll
+      for (int o = 32; o; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], o));
+      if ((threadIdx.x & 63) == 0) lds[3 * (threadIdx.x >> 6) + i] = top[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) top[i] = fmaxf(fmaxf(lds[i], lds[3 + i]), fmaxf(lds[6 + i], lds[9 + i]));
+    __syncthreads();
+    const float most = 2.f * __builtin_sqrtf(top[0]) * __builtin_sqrtf(top[1]) + top[2];
+    const int e = (int)(__float_as_uint(most) >> 23);  // biased
+    // within fp32's range with its inverse; the largest power that leaves B so
+    return e == 0 || e == 255 ? 1.f : __uint_as_float((uint32_t)min(max(127 + 13 + 127 - e, 27), 227) << 23);
+  } else {
+    return 1.f;
+  }
+}
+
+// fp16's weights in dv, at most 1, are 2^14 times as large.
+template <class T>
+constexpr float kLiftP = __is_same(T, _Float16) ? 16384.f : 1.f;
+
+// The waves' sums of 32 rows, joined in LDS and written, times f.
+template <int HD>
+struct Sums {
+  float so[kWaves][32][HD + 4];
+  __device__ __forceinline__ void put(int wave, int col, int half, const f32x16 (&acc)[HD / 32]) {
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *(float4*)&so[wave][col][32 * d + tile_row(r, half)] =
+            make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+  }
+  // `place(t)`: where row t goes, null for nowhere.
+  template <class F>
+  __device__ __forceinline__ void write(float f, F&& place) const {
+    for (int i = threadIdx.x; i < 32 * HD / 4; i += kThreads) {
+      const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
+      auto* to = place(t);
+      if (!to) continue;
+      float4 x = *(const float4*)&so[0][t][d];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) {
+        const float4 y = *(const float4*)&so[w][t][d];
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+      store4(to + d, make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+    }
+  }
+};
+
+// dq.  WIDE: 128 rows a workgroup, 32 a wave, 64 keys a stage that all waves read;
+// else 32 rows, and every wave has keys and stages of its own.
+template <class T, int HD, bool WIDE>
+__global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(const Packed a, const Grads g,
+                                                                            T* __restrict__ dq) {
+  typedef Stage<HD> St;
+  constexpr int B = WIDE ? 2 : 1, kKeys = 32 * B, kRows = WIDE ? 128 : 32;
+  constexpr int kBytes = kKeys * St::kRow, kLoads = kBytes / 1024 / (WIDE ? kWaves : 1);
+  constexpr int kStages = 4 * kBytes * (WIDE ? 1 : kWaves), kJoin = WIDE ? 0 : sizeof(Sums<HD>);
+  __shared__ __attribute__((aligned(1024))) char lds[kStages > kJoin ? kStages : kJoin];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int group = blockIdx.x % a.G;
+  const Segment seg = segment_of<WIDE ? 7 : 5>(a.starts, a.wide, a.n, a.T, a.R, blockIdx.x / a.G);
+  const int rows = seg.len * a.R, tiles = (rows + kRows - 1) / kRows;
+  if (seg.tile >= tiles) return;
+  const float unit = unit_of<T>(g, (float*)lds);
+  const int row0 = kRows * (tiles - 1 - seg.tile);
+  const Keys keys = keys_of(a, seg.seq);
+  const int behind = keys.len - seg.len;
+  const int w0 = row0 + (WIDE ? 32 * wave : 0), ri = min(w0 + col, rows - 1), tok = div_r(a, ri);
+  const int sees = min(tok + 1 + behind, keys.len);
+  const int most = min(div_r(a, min(row0 + kRows, rows) - 1) + 1 + behind, keys.len);
+  const int wave_most = w0 < rows ? min(div_r(a, min(w0 + 32, rows) - 1) + 1 + behind, keys.len) : 0;
+  const int least = min(div_r(a, min(w0, rows - 1)) + 1 + behind, keys.len);
+  const char* kb = a.k + group * a.kh + keys.first * a.kt;
+  const char* vb = a.v + group * a.vh + keys.first * a.vt;
+  const int head = group * a.R + ri - tok * a.R;
+  const char* qrow = a.q + (seg.first + tok) * a.qt + head * a.qh;
+  const char* grow = g.g_out + (seg.first + tok) * g.gt + head * g.gh;
+  char* mine = lds + (WIDE ? 0 : 4 * kBytes * wave);
+  auto send = [&](int it, char* to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int n = (WIDE ? wave * kLoads : 0) + i;
+      St::load(to, n, [&](int r) { return kb + min(it * kKeys + r, keys.len - 1) * a.kt; });
+      St::load(to + kBytes, n, [&](int r) { return vb + min(it * kKeys + r, keys.len - 1) * a.vt; });
+    }
+  };
+  const St st;
+  const int stages = most > 0 ? (most + kKeys - 1) / kKeys : 0;
+  const int from = WIDE ? 0 : wave, by = WIDE ? 1 : kWaves;
+  if (from < stages) send(from, mine);
+  short8v q[HD / 16], go[HD / 16];
+#pragma unroll
+  for (int i = 0; i < HD / 16; ++i) {
+    q[i] = *(const short8v*)(qrow + 32 * i + 16 * half);
+    go[i] = *(const short8v*)(grow + 32 * i + 16 * half);
+  }
+  const int64_t at = (int64_t)group * a.T * a.R + (int64_t)seg.first * a.R + ri;
+  const float lse2 = g.lse2[at], delta = g.delta[at];
+  f32x16 acc[HD / 32];
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d) acc[d] = f32x16{};
+  int turn = 0;
+  for (int it = from; it < stages; it += by, turn ^= 1) {
+    if (WIDE) wait_vmcnt_le<0>();
+    reads_done();
+    if (WIDE) __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (it + by < stages) {
+      send(it + by, mine + 2 * kBytes * (turn ^ 1));
+      if (!WIDE) wait_vmcnt_le<2 * kLoads>();
+    } else if (!WIDE) {
+      wait_vmcnt_le<0>();
+    }
+    asm volatile("" ::: "memory");
+    const int k0 = it * kKeys;
+    if (k0 >= wave_most) continue;
+    const char* k = mine + 2 * kBytes * turn;
+    const char* v = k + kBytes;
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      f32x16 s = f32x16{}, ds = f32x16{};
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) s = mma16<T>(st.rows(k, b, i), q[i], s);
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) ds = mma16<T>(st.rows(v, b, i), go[i], ds);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2)) * ((ds[r] - delta) * unit);
+      if (k0 + kKeys > least) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (k0 + 32 * b + tile_row(r, half) >= sees) ds[r] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = ds[8 * i + e];
+        const short8v w = round8<T>(x);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) acc[d] = mma16<T>(st.cols(k, 2 * b + i, d), w, acc[d]);
+      }
+    }
+  }
+  const float f = g.scale / unit;
+  if constexpr (WIDE) {
+    if (w0 + col >= rows) return;
+    T* to = dq + ((int64_t)(seg.first + tok) * a.H + head) * HD;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        store4(to + 32 * d + tile_row(r, half),
+               make_float4(acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f));
+  } else {
+    reads_done();
+    __syncthreads();  // the stages become the waves' sums
+    Sums<HD>& sums = *(Sums<HD>*)lds;
+    sums.put(wave, col, half, acc);
+    __syncthreads();
+    sums.write(f, [&](int t) -> T* {
+      if (row0 + t >= rows) return nullptr;
+      const int tk = div_r(a, row0 + t);
+      return dq + ((int64_t)(seg.first + tk) * a.H + group * a.R + row0 + t - tk * a.R) * HD;
+    });
+  }
+}
+
+// dk and dv.  WIDE: 128 keys a workgroup, 32 a wave, 32 rows a stage that all waves
+// read; else 32 keys, and every wave has rows and stages of its own.
+template <class T, int HD, bool WIDE>
+__global__ __launch_bounds__(kThreads, 1) void packed_dkv16_kernel(const Packed a, const Grads g, T* __restrict__ dk,
+                                                                   T* __restrict__ dv) {
+  typedef Stage<HD> St;
+  constexpr int kKeys = WIDE ? 128 : 32;
+  constexpr int kBytes = 32 * St::kRow, kLoads = kBytes / 1024;
+  constexpr int kStages = 4 * kBytes * (WIDE ? 1 : kWaves), kJoin = WIDE ? 0 : sizeof(Sums<HD>);
+  // a stage: 32 rows of q, then of g_out; each wave's own copy of the rows' lse2 and delta
+  __shared__ __attribute__((aligned(1024))) char lds[kStages > kJoin ? kStages : kJoin];
+  __shared__ __attribute__((aligned(16))) float row_stats[kWaves][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int group = blockIdx.x % a.G;
+  const Segment seg = segment_of<WIDE ? 7 : 5>(a.key_starts, a.wide, a.n, a.S, 1, blockIdx.x / a.G);
+  const int k0 = kKeys * seg.tile;
+  if (k0 >= seg.len) return;
+  const float unit = unit_of<T>(g, (float*)lds);
+  const bool real = seg.seq >= 0 && seg.seq < a.n;
+  const int len = real ? keys_of(a, seg.seq).len : 0;  // of the segment's keys those in use
+  int first = 0, tokens = 0;
+  if (real) {
+    first = __builtin_amdgcn_readfirstlane(segment_start(a.starts, a.wide, a.n, a.T, seg.seq + 1));
+    const int end = __builtin_amdgcn_readfirstlane(segment_start(a.starts, a.wide, a.n, a.T, seg.seq + 2));
+    tokens = max(end - first, 0);
+  }
+  const int rows = tokens * a.R, behind = len - tokens;  // token j sees the keys below j + 1 + behind
+  const int w0 = k0 + (WIDE ? 32 * wave : 0), key = w0 + col;
+  f32x16 ak[HD / 32], av[HD / 32];
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d) ak[d] = av[d] = f32x16{};
+  char* mine = lds + (WIDE ? 0 : 4 * kBytes * wave);
+  if (k0 < len && rows > 0) {
+    const int held = min(key, len - 1);
+    const char* krow = a.k + (seg.first + held) * a.kt + group * a.kh;
+    const char* vrow = a.v + (seg.first + held) * a.vt + group * a.vh;
+    const int64_t st0 = (int64_t)group * a.T * a.R + (int64_t)first * a.R;
+    // the first row that sees the lane's key, the wave's first key and the workgroup's
+    const int row_min = max(key - behind, 0) * a.R, wave_min = max(w0 - behind, 0) * a.R;
+    const int all_see = max(min(w0 + 31, len - 1) - behind, 0) * a.R;  // from here on a row sees all keys of the wave
+    const int base = max(k0 - behind, 0) * a.R;
+    const int stages = (rows + 31) >> 5, from = (base >> 5) + (WIDE ? 0 : wave), by = WIDE ? 1 : kWaves;
+    auto send = [&](int it, char* to) __attribute__((always_inline)) {
+      constexpr int N = WIDE ? (kLoads + kWaves - 1) / kWaves : kLoads;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int n = WIDE ? wave + i * kWaves : i;
+        if (WIDE && kLoads % kWaves && n >= kLoads) continue;
+        const int row = min(32 * it + n * St::kPer + lane / St::kPieces, rows - 1), tk = div_r(a, row);
+        const int h = group * a.R + row - tk * a.R;
+        St::load(to, n, [&](int) { return a.q + (first + tk) * a.qt + h * a.qh; });
+        St::load(to + kBytes, n, [&](int) { return g.g_out + (first + tk) * g.gt + h * g.gh; });
+      }
+    };
+    // lane l holds lse2 of row l of a stage, or delta of row l - 32; rows behind the last weigh nothing
+    auto stat = [&](int it) __attribute__((always_inline)) {
+      const int row = 32 * it + col;
+      const float x = (half ? g.delta : g.lse2)[st0 + min(row, rows - 1)];
+      return row < rows ? x : half ? 0.f : INFINITY;
+    };
+    const St st;
+    float next = 0.f;
+    if (from < stages) {
+      send(from, mine);
+      next = stat(from);
+    }
+    short8v k[HD / 16], v[HD / 16];
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) {
+      k[i] = *(const short8v*)(krow + 32 * i + 16 * half);
+      v[i] = *(const short8v*)(vrow + 32 * i + 16 * half);
+    }
+    int turn = 0;
+    for (int it = from; it < stages; it += by, turn ^= 1) {
+      wait_vmcnt_le<0>();
+      reads_done();
+      row_stats[wave][lane] = next;
+      if (WIDE) __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (it + by < stages) {
+        send(it + by, mine + 2 * kBytes * (turn ^ 1));
+        next = stat(it + by);
+      }
+      const int r0 = 32 * it;
+      if (r0 + 32 <= wave_min) continue;
+      const char* q = mine + 2 * kBytes * turn;
+      const char* go = q + kBytes;
+      f32x16 s = f32x16{}, ds = f32x16{};
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) s = mma16<T>(st.rows(q, 0, i), k[i], s);
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) ds = mma16<T>(st.rows(go, 0, i), v[i], ds);
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const float4 z = *(const float4*)&row_stats[wave][tile_row(r, half)];
+        const float4 e = *(const float4*)&row_stats[wave][32 + tile_row(r, half)];
+        const float zs[4] = {z.x, z.y, z.z, z.w}, es[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[r + i] = __builtin_amdgcn_exp2f(fmaf(s[r + i], a.c, -zs[i]));
+          ds[r + i] = s[r + i] * ((ds[r + i] - es[i]) * unit);
+        }
+      }
+      if (r0 < all_see) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (r0 + tile_row(r, half) < row_min) s[r] = ds[r] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x[8], y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = s[8 * i + e] * kLiftP<T>;
+          y[e] = ds[8 * i + e];
+        }
+        const short8v p = round8<T>(x), w = round8<T>(y);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) {
+          av[d] = mma16<T>(st.cols(go, i, d), p, av[d]);
+          ak[d] = mma16<T>(st.cols(q, i, d), w, ak[d]);
+        }
+      }
+    }
+  }
+  const float fk = g.scale / unit, fv = 1.f / kLiftP<T>;
+  if constexpr (WIDE) {
+    if (key >= seg.len) return;
+    const bool in = key < len;  // places not in use have gradients 0
+    const int64_t at = ((int64_t)(seg.first + key) * a.G + group) * HD;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int to = 32 * d + tile_row(r, half);
+        const float4 x = make_float4(ak[d][r] * fk, ak[d][r + 1] * fk, ak[d][r + 2] * fk, ak[d][r + 3] * fk);
+        const float4 y = make_float4(av[d][r] * fv, av[d][r + 1] * fv, av[d][r + 2] * fv, av[d][r + 3] * fv);
+        const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (dk) store4(dk + at + to, in ? x : none);
+        if (dv) store4(dv + at + to, in ? y : none);
+      }
+  } else {
+    Sums<HD>& sums = *(Sums<HD>*)lds;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      T* to = which ? dv : dk;
+      if (!to) continue;
+      reads_done();
+      __syncthreads();
+      const bool in = key < len;
+      f32x16 x[HD / 32];
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[d][r] = in ? (which ? av[d][r] : ak[d][r]) : 0.f;
+      sums.put(wave, col, half, x);
+      __syncthreads();
+      sums.write(which ? fv : fk, [&](int t) -> T* {
+        return k0 + t < seg.len ? to + ((int64_t)(seg.first + k0 + t) * a.G + group) * HD : nullptr;
+      });
+    }
+  }
+}
+
 // --------------------------------------------------------------------- host
 typedef mpl_packed_attention_args Args;
 
@@ -706,6 +1099,9 @@ bool wide_of(const Args* p) {
   return p->dtype != MPL_F32 && p->tokens * r / kWideRows * p->groups >= 256;
 }
 
+// Whether dk and dv in 16 bits take tiles of 128 keys.
+bool wide_keys_of(const Args* p) { return p->keys / 128 * p->groups >= 256; }
+
 // Parts of the keys: where the tiles of rows do not fill the chip and the keys of
 // a sequence are many.  Only sums over the sequences are known here.
 int splits_of(const Args* p) {
@@ -722,7 +1118,7 @@ size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 size_t workspace_bytes(const Args* p, bool backward) {
   const size_t rows = (size_t)p->tokens * p->heads;
-  if (backward) return 2 * round256(rows * 4);
+  if (backward) return 2 * round256(rows * 4) + 3 * kDeltaBlocks * 4;
   const int s = wide_of(p) ? 1 : splits_of(p);
   return s > 1 ? round256(s * rows * p->head_dim * 4) + round256(s * rows * 8) : 0;
 }
@@ -757,14 +1153,26 @@ void backward(const Args* p, const void* g_out, int64_t gt, int64_t gh, const vo
   const size_t rows = (size_t)p->tokens * p->heads;
   float* lse2 = (float*)ws;
   float* delta = (float*)((char*)ws + round256(rows * 4));
-  Grads g{(const char*)g_out, gt * (int64_t)sizeof(T), gh * (int64_t)sizeof(T), lse2, delta, p->scale};
+  float* largest = (float*)((char*)ws + 2 * round256(rows * 4));
+  const int64_t blocks = cdiv(rows * (HD / 4), 256);
+  const int used = (int)(blocks < kDeltaBlocks ? blocks : kDeltaBlocks);
+  const Grads g{(const char*)g_out, gt * (int64_t)sizeof(T), gh * (int64_t)sizeof(T), lse2, delta, largest, used, p->scale};
   if (rows)
-    packed_delta_kernel<T, HD><<<(unsigned)cdiv(rows * (HD / 4), 256), 256, 0, s>>>(a, g.g_out, g.gt, g.gh, (const T*)out,
-                                                                                   lse, g_lse, lse2, delta);
-  if (rows && dq)
-    packed_dq_kernel<T, HD><<<(unsigned)(((int64_t)a.T * a.R / 32 + a.n + 2) * a.G), kThreads, 0, s>>>(a, g, (T*)dq);
-  if (a.S && (dk || dv))
-    packed_dkv_kernel<T, HD><<<(unsigned)(((int64_t)a.S / 32 + a.n + 2) * a.G), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
+    packed_delta_kernel<T, HD><<<used, 256, 0, s>>>(a, g.g_out, g.gt, g.gh, (const T*)out, lse, g_lse, lse2, delta, largest);
+  auto tiles = [&](int64_t x, int unit) { return (unsigned)((x / unit + a.n + 2) * a.G); };
+  if constexpr (sizeof(T) == 2) {
+    if (rows && dq) {
+      if (wide_of(p)) packed_dq16_kernel<T, HD, true><<<tiles((int64_t)a.T * a.R, 128), kThreads, 0, s>>>(a, g, (T*)dq);
+      else packed_dq16_kernel<T, HD, false><<<tiles((int64_t)a.T * a.R, 32), kThreads, 0, s>>>(a, g, (T*)dq);
+    }
+    if (a.S && (dk || dv)) {
+      if (wide_keys_of(p)) packed_dkv16_kernel<T, HD, true><<<tiles(a.S, 128), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
+      else packed_dkv16_kernel<T, HD, false><<<tiles(a.S, 32), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
+    }
+  } else {
+    if (rows && dq) packed_dq_kernel<HD><<<tiles((int64_t)a.T * a.R, 32), kThreads, 0, s>>>(a, g, (T*)dq);
+    if (a.S && (dk || dv)) packed_dkv_kernel<HD><<<tiles(a.S, 32), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
+  }
 }
 
 template <class F>

@@ -397,3 +397,12 @@ def test_offsets_past_32_bits(dtype):
     small = torch.cat([kv[:50], kv[cap - 50:]])
     want = packed_attention(q, small, small, starts, key_starts=torch.tensor([0, 50, 100], device=DEV))
     assert torch.allclose(out.float(), want.float(), rtol=2 * torch.finfo(dtype).eps, atol=2 * torch.finfo(dtype).eps)
+
+
+@pytest.mark.parametrize("g_size,v_size", [(2.0 ** -14, 1.0), (1.0, 500.0), (2.0 ** 9, 100.0), (0.0, 1.0)])
+def test_fp16_gradients_of_any_size(g_size, v_size):
+    """dz is held under a power of two of the call's own: small gradients keep their bits, large ones do not overflow."""
+    lq = [300, 41]
+    q, k, v, g, _ = make(lq, lq, 4, 2, 64, torch.float16, seed=14)
+    q, k = q * 0.2, k * 0.2  # many alike weights, of 1 / 300 each
+    run_all(q, k, (v.float() * v_size).half(), lq, lq, (g.float() * g_size).half(), scale=0.01)
