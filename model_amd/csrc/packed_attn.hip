@@ -296,12 +296,9 @@ __global__ __launch_bounds__(kThreads, 2) void packed_forward16_kernel(const Pac
   const char* vb = a.v + group * a.vh + keys.first * a.vt;
   const char* qrow = a.q + (seg.first + tok) * a.qt + (group * a.R + ri - tok * a.R) * a.qh;
   auto send = [&](int it, char* to) __attribute__((always_inline)) {
-    const int k0 = it * kWideKeys;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      St::load(to, wave * kLoads + i, [&](int r) { return kb + min(k0 + r, keys.len - 1) * a.kt; });
-      St::load(to + kBytes, wave * kLoads + i, [&](int r) { return vb + min(k0 + r, keys.len - 1) * a.vt; });
-    }
+    const int k0 = it * kWideKeys, last = keys.len - 1 - k0;
+    St::template load_rows<kLoads, kWaves>(to, wave, kb + k0 * a.kt, (uint32_t)a.kt, last);
+    St::template load_rows<kLoads, kWaves>(to + kBytes, wave, vb + k0 * a.vt, (uint32_t)a.vt, last);
   };
   const St st;
   const int stages = most > 0 ? (most + kWideKeys - 1) / kWideKeys : 0;
@@ -367,11 +364,9 @@ __global__ __launch_bounds__(kThreads) void packed_forward16_few_kernel(const Pa
   const int j0 = blockIdx.y * per + wave, j1 = min(blocks, ((int)blockIdx.y + 1) * per);
   char* mine = lds + 4 * kBytes * wave;
   auto send = [&](int j, char* to) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      St::load(to, i, [&](int r) { return kb + min(32 * j + r, keys.len - 1) * a.kt; });
-      St::load(to + kBytes, i, [&](int r) { return vb + min(32 * j + r, keys.len - 1) * a.vt; });
-    }
+    const int last = keys.len - 1 - 32 * j;
+    St::template load_rows<kLoads, 1>(to, 0, kb + 32 * j * a.kt, (uint32_t)a.kt, last);
+    St::template load_rows<kLoads, 1>(to + kBytes, 0, vb + 32 * j * a.vt, (uint32_t)a.vt, last);
   };
   const St st;
   short8v q[HD / 16];
@@ -676,21 +671,23 @@ __global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, co
 // most |dp| + |delta| <= B = 2 max|g_out| max|v| + max|g_lse|, and B goes to [2^13,
 // 2^14): nothing overflows, and gradients of any size keep their bits down to 2^-38
 // of B.  bf16 has fp32's range and takes 1.  Every thread of the workgroup calls it.
-template <class T>
+template <class T, int W>
 __device__ __forceinline__ float unit_of(const Grads& g, float* lds) {
   if constexpr (__is_same(T, _Float16)) {
     float top[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
       top[i] = 0.f;
-      for (int b = threadIdx.x; b < g.blocks; b += kThreads) top[i] = fmaxf(top[i], g.largest[i * g.blocks + b]);
+      for (int b = threadIdx.x; b < g.blocks; b += 64 * W) top[i] = fmaxf(top[i], g.largest[i * g.blocks + b]);
 #pragma unroll
       for (int o = 32; o; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], o));
       if ((threadIdx.x & 63) == 0) lds[3 * (threadIdx.x >> 6) + i] = top[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 3; ++i) top[i] = fmaxf(fmaxf(lds[i], lds[3 + i]), fmaxf(lds[6 + i], lds[9 + i]));
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int w = 0; w < W; ++w) top[i] = fmaxf(top[i], lds[3 * w + i]);
     __syncthreads();
     const float most = 2.f * __builtin_sqrtf(top[0]) * __builtin_sqrtf(top[1]) + top[2];
     const int e = (int)(__float_as_uint(most) >> 23);  // biased
@@ -705,32 +702,32 @@ __device__ __forceinline__ float unit_of(const Grads& g, float* lds) {
 template <class T>
 constexpr float kLiftP = __is_same(T, _Float16) ? 16384.f : 1.f;
 
-// The waves' sums of 32 rows, joined in LDS and written, times f.
-template <int HD>
+// The sums of N sets of RW waves, 32 rows each, joined in LDS and written.
+template <int HD, int N, int RW>
 struct Sums {
-  float so[kWaves][32][HD + 4];
-  __device__ __forceinline__ void put(int wave, int col, int half, const f32x16 (&acc)[HD / 32]) {
+  float so[N][RW][32][HD + 4];
+  __device__ __forceinline__ void put(int n, int rw, int col, int half, const f32x16 (&acc)[HD / 32], float f) {
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
-        *(float4*)&so[wave][col][32 * d + tile_row(r, half)] =
-            make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+        *(float4*)&so[n][rw][col][32 * d + tile_row(r, half)] =
+            make_float4(acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f);
   }
   // `place(t)`: where row t goes, null for nowhere.
   template <class F>
-  __device__ __forceinline__ void write(float f, F&& place) const {
-    for (int i = threadIdx.x; i < 32 * HD / 4; i += kThreads) {
+  __device__ __forceinline__ void write(F&& place) const {
+    for (int i = threadIdx.x; i < N * 32 * HD / 4; i += 64 * N * RW) {
       const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
       auto* to = place(t);
       if (!to) continue;
-      float4 x = *(const float4*)&so[0][t][d];
+      float4 x = *(const float4*)&so[t >> 5][0][t & 31][d];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) {
-        const float4 y = *(const float4*)&so[w][t][d];
+      for (int w = 1; w < RW; ++w) {
+        const float4 y = *(const float4*)&so[t >> 5][w][t & 31][d];
         x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
       }
-      store4(to + d, make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+      store4(to + d, x);
     }
   }
 };
@@ -743,7 +740,7 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
   typedef Stage<HD> St;
   constexpr int B = WIDE ? 2 : 1, kKeys = 32 * B, kRows = WIDE ? 128 : 32;
   constexpr int kBytes = kKeys * St::kRow, kLoads = kBytes / 1024 / (WIDE ? kWaves : 1);
-  constexpr int kStages = 4 * kBytes * (WIDE ? 1 : kWaves), kJoin = WIDE ? 0 : sizeof(Sums<HD>);
+  constexpr int kStages = 4 * kBytes * (WIDE ? 1 : kWaves), kJoin = WIDE ? 0 : sizeof(Sums<HD, 1, kWaves>);
   __shared__ __attribute__((aligned(1024))) char lds[kStages > kJoin ? kStages : kJoin];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -751,7 +748,7 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
   const Segment seg = segment_of<WIDE ? 7 : 5>(a.starts, a.wide, a.n, a.T, a.R, blockIdx.x / a.G);
   const int rows = seg.len * a.R, tiles = (rows + kRows - 1) / kRows;
   if (seg.tile >= tiles) return;
-  const float unit = unit_of<T>(g, (float*)lds);
+  const float unit = unit_of<T, kWaves>(g, (float*)lds);
   const int row0 = kRows * (tiles - 1 - seg.tile);
   const Keys keys = keys_of(a, seg.seq);
   const int behind = keys.len - seg.len;
@@ -767,12 +764,10 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
   const char* grow = g.g_out + (seg.first + tok) * g.gt + head * g.gh;
   char* mine = lds + (WIDE ? 0 : 4 * kBytes * wave);
   auto send = [&](int it, char* to) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int n = (WIDE ? wave * kLoads : 0) + i;
-      St::load(to, n, [&](int r) { return kb + min(it * kKeys + r, keys.len - 1) * a.kt; });
-      St::load(to + kBytes, n, [&](int r) { return vb + min(it * kKeys + r, keys.len - 1) * a.vt; });
-    }
+    constexpr int BY = WIDE ? kWaves : 1;
+    const int from = it * kKeys, last = keys.len - 1 - from, n0 = WIDE ? wave : 0;
+    St::template load_rows<kLoads, BY>(to, n0, kb + from * a.kt, (uint32_t)a.kt, last);
+    St::template load_rows<kLoads, BY>(to + kBytes, n0, vb + from * a.vt, (uint32_t)a.vt, last);
   };
   const St st;
   const int stages = most > 0 ? (most + kKeys - 1) / kKeys : 0;
@@ -810,9 +805,10 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
     for (int b = 0; b < B; ++b) {
       f32x16 s = f32x16{}, ds = f32x16{};
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i) s = mma16<T>(st.rows(k, b, i), q[i], s);
-#pragma unroll
-      for (int i = 0; i < HD / 16; ++i) ds = mma16<T>(st.rows(v, b, i), go[i], ds);
+      for (int i = 0; i < HD / 16; ++i) {
+        s = mma16<T>(st.rows(k, b, i), q[i], s);
+        ds = mma16<T>(st.rows(v, b, i), go[i], ds);
+      }
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2)) * ((ds[r] - delta) * unit);
@@ -845,10 +841,10 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
   } else {
     reads_done();
     __syncthreads();  // the stages become the waves' sums
-    Sums<HD>& sums = *(Sums<HD>*)lds;
-    sums.put(wave, col, half, acc);
+    Sums<HD, 1, kWaves>& sums = *(Sums<HD, 1, kWaves>*)lds;
+    sums.put(0, wave, col, half, acc, f);
     __syncthreads();
-    sums.write(f, [&](int t) -> T* {
+    sums.write([&](int t) -> T* {
       if (row0 + t >= rows) return nullptr;
       const int tk = div_r(a, row0 + t);
       return dq + ((int64_t)(seg.first + tk) * a.H + group * a.R + row0 + t - tk * a.R) * HD;
@@ -856,25 +852,31 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
   }
 }
 
-// dk and dv.  WIDE: 128 keys a workgroup, 32 a wave, 32 rows a stage that all waves
-// read; else 32 keys, and every wave has rows and stages of its own.
-template <class T, int HD, bool WIDE>
-__global__ __launch_bounds__(kThreads, 1) void packed_dkv16_kernel(const Packed a, const Grads g, T* __restrict__ dk,
+// dk and dv.  A workgroup of KW x RW waves has 32 KW keys, 32 a wave, and its rows in
+// stages (8 KB of q and of g_out, or 32 rows) that RW sets of KW waves take in turn, each set
+// with stages of its own, and join at the end.
+template <class T, int HD, int KW, int RW>
+__global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed a, const Grads g, T* __restrict__ dk,
                                                                    T* __restrict__ dv) {
   typedef Stage<HD> St;
-  constexpr int kKeys = WIDE ? 128 : 32;
-  constexpr int kBytes = 32 * St::kRow, kLoads = kBytes / 1024;
-  constexpr int kStages = 4 * kBytes * (WIDE ? 1 : kWaves), kJoin = WIDE ? 0 : sizeof(Sums<HD>);
-  // a stage: 32 rows of q, then of g_out; each wave's own copy of the rows' lse2 and delta
+  constexpr int kKeys = 32 * KW, W = KW * RW;
+  constexpr int kBytes = KW == 1 ? 32 * St::kRow : 8192, kLoads = kBytes / 1024, kRows = kBytes / St::kRow, NB = kRows / 32;
+  // heads of 128 leave no registers for the wave's keys and values as operands: they
+  // lie in LDS, behind the stages
+  constexpr bool kHeld = HD < 128 || KW == 1;
+  constexpr int kKV = kHeld ? 0 : kKeys * St::kRow;
+  constexpr int kStages = 4 * kBytes * RW + 2 * kKV, kJoin = sizeof(Sums<HD, KW, RW>);
+  // a stage: rows of q, then of g_out; each wave's own copy of the rows' lse2 and delta
   __shared__ __attribute__((aligned(1024))) char lds[kStages > kJoin ? kStages : kJoin];
-  __shared__ __attribute__((aligned(16))) float row_stats[kWaves][64];
+  __shared__ __attribute__((aligned(16))) float row_stats[W][2 * kRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kw = wave % KW, rw = wave / KW;
   const int col = lane & 31, half = lane >> 5;
   const int group = blockIdx.x % a.G;
-  const Segment seg = segment_of<WIDE ? 7 : 5>(a.key_starts, a.wide, a.n, a.S, 1, blockIdx.x / a.G);
+  const Segment seg = segment_of<KW == 1 ? 5 : KW == 2 ? 6 : 7>(a.key_starts, a.wide, a.n, a.S, 1, blockIdx.x / a.G);
   const int k0 = kKeys * seg.tile;
   if (k0 >= seg.len) return;
-  const float unit = unit_of<T>(g, (float*)lds);
+  const float unit = unit_of<T, W>(g, (float*)lds);
   const bool real = seg.seq >= 0 && seg.seq < a.n;
   const int len = real ? keys_of(a, seg.seq).len : 0;  // of the segment's keys those in use
   int first = 0, tokens = 0;
@@ -884,11 +886,11 @@ __global__ __launch_bounds__(kThreads, 1) void packed_dkv16_kernel(const Packed 
     tokens = max(end - first, 0);
   }
   const int rows = tokens * a.R, behind = len - tokens;  // token j sees the keys below j + 1 + behind
-  const int w0 = k0 + (WIDE ? 32 * wave : 0), key = w0 + col;
+  const int w0 = k0 + 32 * kw, key = w0 + col;
   f32x16 ak[HD / 32], av[HD / 32];
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d) ak[d] = av[d] = f32x16{};
-  char* mine = lds + (WIDE ? 0 : 4 * kBytes * wave);
+  char* mine = lds + 4 * kBytes * rw;
   if (k0 < len && rows > 0) {
     const int held = min(key, len - 1);
     const char* krow = a.k + (seg.first + held) * a.kt + group * a.kh;
@@ -897,127 +899,144 @@ __global__ __launch_bounds__(kThreads, 1) void packed_dkv16_kernel(const Packed 
     // the first row that sees the lane's key, the wave's first key and the workgroup's
     const int row_min = max(key - behind, 0) * a.R, wave_min = max(w0 - behind, 0) * a.R;
     const int all_see = max(min(w0 + 31, len - 1) - behind, 0) * a.R;  // from here on a row sees all keys of the wave
-    const int base = max(k0 - behind, 0) * a.R;
-    const int stages = (rows + 31) >> 5, from = (base >> 5) + (WIDE ? 0 : wave), by = WIDE ? 1 : kWaves;
+    const int stages = (rows + kRows - 1) / kRows, from = max(k0 - behind, 0) * a.R / kRows;
+    uint32_t q_at[kLoads / KW], g_at[kLoads / KW];
+#pragma unroll
+    for (int i = 0; i < kLoads / KW; ++i) {
+      const int row = St::load_row(kw + i * KW), tk = div_r(a, row), h = row - tk * a.R;
+      q_at[i] = tk * (uint32_t)a.qt + h * (uint32_t)a.qh;
+      g_at[i] = tk * (uint32_t)g.gt + h * (uint32_t)g.gh;
+    }
     auto send = [&](int it, char* to) __attribute__((always_inline)) {
-      constexpr int N = WIDE ? (kLoads + kWaves - 1) / kWaves : kLoads;
+      // a stage is whole tokens where R divides 32: a lane's rows lie alike in every one.  Else, and in the last stage, each row's token is looked for.
+      constexpr int N = kLoads / KW;
+      const bool alike = (a.R & (a.R - 1)) == 0 && a.R <= 32 && kRows * (it + 1) <= rows;
+      const int t0 = div_r(a, kRows * it);
+      const char* qb = a.q + (int64_t)(first + t0) * a.qt + group * a.R * a.qh;
+      const char* gb = g.g_out + (int64_t)(first + t0) * g.gt + group * a.R * g.gh;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int n = WIDE ? wave + i * kWaves : i;
-        if (WIDE && kLoads % kWaves && n >= kLoads) continue;
-        const int row = min(32 * it + n * St::kPer + lane / St::kPieces, rows - 1), tk = div_r(a, row);
-        const int h = group * a.R + row - tk * a.R;
-        St::load(to, n, [&](int) { return a.q + (first + tk) * a.qt + h * a.qh; });
-        St::load(to + kBytes, n, [&](int) { return g.g_out + (first + tk) * g.gt + h * g.gh; });
+        const int n = kw + i * KW;
+        uint32_t qat = q_at[i], gat = g_at[i];
+        if (!alike) {
+          const int row = min(kRows * it + St::load_row(n), rows - 1), tk = div_r(a, row), h = row - tk * a.R;
+          qat = (uint32_t)(tk - t0) * (uint32_t)a.qt + h * (uint32_t)a.qh;
+          gat = (uint32_t)(tk - t0) * (uint32_t)g.gt + h * (uint32_t)g.gh;
+        }
+        St::load(to, n, qb, qat);
+        St::load(to + kBytes, n, gb, gat);
       }
     };
-    // lane l holds lse2 of row l of a stage, or delta of row l - 32; rows behind the last weigh nothing
+    // a stage's lse2, then its deltas, NB a lane; rows behind the last weigh nothing
+    float next[NB];
     auto stat = [&](int it) __attribute__((always_inline)) {
-      const int row = 32 * it + col;
-      const float x = (half ? g.delta : g.lse2)[st0 + min(row, rows - 1)];
-      return row < rows ? x : half ? 0.f : INFINITY;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int e = lane + 64 * i, row = kRows * it + (e & (kRows - 1));
+        const float x = (e >= kRows ? g.delta : g.lse2)[st0 + min(row, rows - 1)];
+        next[i] = row < rows ? x : e >= kRows ? 0.f : INFINITY;
+      }
     };
     const St st;
-    float next = 0.f;
-    if (from < stages) {
-      send(from, mine);
-      next = stat(from);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) next[i] = 0.f;
+    if (from + rw < stages) {
+      send(from + rw, mine);
+      stat(from + rw);
     }
     short8v k[HD / 16], v[HD / 16];
+    char* kv = lds + 4 * kBytes * RW;
+    if constexpr (kHeld) {
 #pragma unroll
-    for (int i = 0; i < HD / 16; ++i) {
-      k[i] = *(const short8v*)(krow + 32 * i + 16 * half);
-      v[i] = *(const short8v*)(vrow + 32 * i + 16 * half);
+      for (int i = 0; i < HD / 16; ++i) {
+        k[i] = *(const short8v*)(krow + 32 * i + 16 * half);
+        v[i] = *(const short8v*)(vrow + 32 * i + 16 * half);
+      }
+    } else {
+      St::template load_rows<kKV / 1024 / W, W>(kv, wave, a.k + (int64_t)(seg.first + k0) * a.kt + group * a.kh,
+                                                (uint32_t)a.kt, len - 1 - k0);
+      St::template load_rows<kKV / 1024 / W, W>(kv + kKV, wave, a.v + (int64_t)(seg.first + k0) * a.vt + group * a.vh,
+                                                (uint32_t)a.vt, len - 1 - k0);
     }
     int turn = 0;
-    for (int it = from; it < stages; it += by, turn ^= 1) {
+    for (int base = from; base < stages; base += RW, turn ^= 1) {
+      const int it = base + rw;
       wait_vmcnt_le<0>();
       reads_done();
-      row_stats[wave][lane] = next;
-      if (WIDE) __builtin_amdgcn_s_barrier();
+#pragma unroll
+      for (int i = 0; i < NB; ++i) row_stats[wave][lane + 64 * i] = next[i];
+      if (KW > 1) __builtin_amdgcn_s_barrier();  // every wave comes by here as often
       asm volatile("" ::: "memory");
-      if (it + by < stages) {
-        send(it + by, mine + 2 * kBytes * (turn ^ 1));
-        next = stat(it + by);
+      if (it + RW < stages) {
+        send(it + RW, mine + 2 * kBytes * (turn ^ 1));
+        stat(it + RW);
       }
-      const int r0 = 32 * it;
-      if (r0 + 32 <= wave_min) continue;
+      if (it >= stages) continue;
       const char* q = mine + 2 * kBytes * turn;
       const char* go = q + kBytes;
-      f32x16 s = f32x16{}, ds = f32x16{};
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i) s = mma16<T>(st.rows(q, 0, i), k[i], s);
+      for (int b = 0; b < NB; ++b) {
+        const int r0 = kRows * it + 32 * b;
+        if (r0 + 32 <= wave_min || r0 >= rows) continue;
+        f32x16 s = f32x16{}, ds = f32x16{};
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i) ds = mma16<T>(st.rows(go, 0, i), v[i], ds);
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const float4 z = *(const float4*)&row_stats[wave][tile_row(r, half)];
-        const float4 e = *(const float4*)&row_stats[wave][32 + tile_row(r, half)];
-        const float zs[4] = {z.x, z.y, z.z, z.w}, es[4] = {e.x, e.y, e.z, e.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[r + i] = __builtin_amdgcn_exp2f(fmaf(s[r + i], a.c, -zs[i]));
-          ds[r + i] = s[r + i] * ((ds[r + i] - es[i]) * unit);
+        for (int i = 0; i < HD / 16; ++i) {
+          s = mma16<T>(st.rows(q, b, i), kHeld ? k[i] : st.rows(kv, kw, i), s);
+          ds = mma16<T>(st.rows(go, b, i), kHeld ? v[i] : st.rows(kv + kKV, kw, i), ds);
         }
-      }
-      if (r0 < all_see) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (r0 + tile_row(r, half) < row_min) s[r] = ds[r] = 0.f;
-      }
+        for (int r = 0; r < 16; r += 4) {
+          const float4 z = *(const float4*)&row_stats[wave][32 * b + tile_row(r, half)];
+          const float4 e = *(const float4*)&row_stats[wave][kRows + 32 * b + tile_row(r, half)];
+          const float zs[4] = {z.x, z.y, z.z, z.w}, es[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float x[8], y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = s[8 * i + e] * kLiftP<T>;
-          y[e] = ds[8 * i + e];
+          for (int i = 0; i < 4; ++i) {
+            s[r + i] = __builtin_amdgcn_exp2f(fmaf(s[r + i], a.c, -zs[i]));
+            ds[r + i] = s[r + i] * ((ds[r + i] - es[i]) * unit);
+          }
         }
-        const short8v p = round8<T>(x), w = round8<T>(y);
+        if (r0 < all_see) {
 #pragma unroll
-        for (int d = 0; d < HD / 32; ++d) {
-          av[d] = mma16<T>(st.cols(go, i, d), p, av[d]);
-          ak[d] = mma16<T>(st.cols(q, i, d), w, ak[d]);
+          for (int r = 0; r < 16; ++r)
+            if (r0 + tile_row(r, half) < row_min) s[r] = ds[r] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x[8], y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = s[8 * i + e] * kLiftP<T>;
+            y[e] = ds[8 * i + e];
+          }
+          const short8v p = round8<T>(x), w = round8<T>(y);
+#pragma unroll
+          for (int d = 0; d < HD / 32; ++d) {
+            av[d] = mma16<T>(st.cols(go, 2 * b + i, d), p, av[d]);
+            ak[d] = mma16<T>(st.cols(q, 2 * b + i, d), w, ak[d]);
+          }
         }
       }
     }
   }
   const float fk = g.scale / unit, fv = 1.f / kLiftP<T>;
-  if constexpr (WIDE) {
-    if (key >= seg.len) return;
-    const bool in = key < len;  // places not in use have gradients 0
-    const int64_t at = ((int64_t)(seg.first + key) * a.G + group) * HD;
+  const bool in = key < len;  // places not in use have gradients 0
+  Sums<HD, KW, RW>& sums = *(Sums<HD, KW, RW>*)lds;
 #pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
+  for (int which = 0; which < 2; ++which) {
+    T* to = which ? dv : dk;
+    if (!to) continue;
+    f32x16 (&x)[HD / 32] = which ? av : ak;
+    if (!in) {
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int to = 32 * d + tile_row(r, half);
-        const float4 x = make_float4(ak[d][r] * fk, ak[d][r + 1] * fk, ak[d][r + 2] * fk, ak[d][r + 3] * fk);
-        const float4 y = make_float4(av[d][r] * fv, av[d][r + 1] * fv, av[d][r + 2] * fv, av[d][r + 3] * fv);
-        const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (dk) store4(dk + at + to, in ? x : none);
-        if (dv) store4(dv + at + to, in ? y : none);
-      }
-  } else {
-    Sums<HD>& sums = *(Sums<HD>*)lds;
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      T* to = which ? dv : dk;
-      if (!to) continue;
-      reads_done();
-      __syncthreads();
-      const bool in = key < len;
-      f32x16 x[HD / 32];
-#pragma unroll
-      for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[d][r] = in ? (which ? av[d][r] : ak[d][r]) : 0.f;
-      sums.put(wave, col, half, x);
-      __syncthreads();
-      sums.write(which ? fv : fk, [&](int t) -> T* {
-        return k0 + t < seg.len ? to + ((int64_t)(seg.first + k0 + t) * a.G + group) * HD : nullptr;
-      });
+      for (int d = 0; d < HD / 32; ++d) x[d] = f32x16{};
     }
+    reads_done();
+    __syncthreads();  // the stages become the waves' sums
+    sums.put(kw, rw, col, half, x, which ? fv : fk);
+    __syncthreads();
+    sums.write([&](int t) -> T* {
+      return k0 + t < seg.len ? to + ((int64_t)(seg.first + k0 + t) * a.G + group) * HD : nullptr;
+    });
   }
 }
 
@@ -1050,12 +1069,17 @@ int check_sizes(const Args* p, const char* what) {
   return MPL_OK;
 }
 
+constexpr int64_t kMostStride = 1 << 23;  // elements
 int check_rows(const Args* p, const void* x, int64_t tok, int64_t head, const char* name, const char* what) {
   const int64_t unit = 16 / element_size(p->dtype);
   MPL_REQUIRE(x, MPL_EINVAL, "%s: null %s", what, name);
   MPL_REQUIRE(((uintptr_t)x & 15) == 0 && tok >= 0 && head >= 0 && tok % unit == 0 && head % unit == 0, MPL_EINVAL,
               "%s: the rows of %s must be 16-byte aligned (token %lld, head %lld)", what, name, (long long)tok,
               (long long)head);
+  // places within a stage of rows are 32-bit: up to 63 tokens and a token's heads
+  const int64_t r = p->heads / p->groups;
+  MPL_REQUIRE(tok <= kMostStride && head <= kMostStride && head * (r < 32 ? 32 : r) <= 32 * kMostStride, MPL_EUNSUPPORTED,
+              "%s: the rows of %s lie too far apart (token %lld, head %lld)", what, name, (long long)tok, (long long)head);
   return MPL_OK;
 }
 
@@ -1166,8 +1190,9 @@ void backward(const Args* p, const void* g_out, int64_t gt, int64_t gh, const vo
       else packed_dq16_kernel<T, HD, false><<<tiles((int64_t)a.T * a.R, 32), kThreads, 0, s>>>(a, g, (T*)dq);
     }
     if (a.S && (dk || dv)) {
-      if (wide_keys_of(p)) packed_dkv16_kernel<T, HD, true><<<tiles(a.S, 128), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
-      else packed_dkv16_kernel<T, HD, false><<<tiles(a.S, 32), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
+      constexpr int KW = 4, RW = HD == 128 ? 2 : 1;
+      if (wide_keys_of(p)) packed_dkv16_kernel<T, HD, KW, RW><<<tiles(a.S, 32 * KW), 64 * KW * RW, 0, s>>>(a, g, (T*)dk, (T*)dv);
+      else packed_dkv16_kernel<T, HD, 1, 4><<<tiles(a.S, 32), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
     }
   } else {
     if (rows && dq) packed_dq_kernel<HD><<<tiles((int64_t)a.T * a.R, 32), kThreads, 0, s>>>(a, g, (T*)dq);

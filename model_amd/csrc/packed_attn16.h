@@ -12,10 +12,11 @@
 // to 8 c + 7 are its operand as they are, when the other operand's elements are read
 // in the same order: rows 16 c + 4 h + [0, 4) and 16 c + 8 + 4 h + [0, 4).
 //
-// Banks: DMA writes lane after lane, so places are permuted at the source.  The
-// 16-byte piece p of row r lies at p ^ f(r), f a permutation of r's low bits by
-// which 8 neighbouring rows' pieces fall on all banks, and so do the 32-byte
-// granules of 4 rows that 16 lanes read transposed.
+// Banks: DMA writes lane after lane, so places are permuted at the source: the
+// 16-byte piece p of row r lies at p ^ f(r).  f spreads the pieces that 16 lanes read
+// of 16 neighbouring rows over all 64 banks, and the 64 bytes each that 32 lanes read
+// transposed of 4 rows as well.  (With 8 and 16 lanes and half the banks, as 128 bytes
+// a cycle would have it, every read took twice its cycles.)
 #pragma once
 
 #include "mfma.h"
@@ -52,37 +53,45 @@ struct Stage {
   static constexpr int kSteps = HD / 16, kTiles = HD / 32;
 
   __device__ static __forceinline__ int f(int r) {
-    return HD >= 64 ? (r & 3) << 1 | (r >> 2 & 1) : (r & 2) | (r >> 2 & 1);
+    return HD == 128 ? (r & 3) << 2 | (r >> 2 & 3) : HD == 64 ? (r & 2) << 1 | (r >> 2 & 3) : r >> 2 & 3;
   }
 
-  uint32_t row[4], col[2];
+  uint32_t row, col0, col1;
   __device__ __forceinline__ Stage() {
     const int lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) row[c] = r * kRow + (((2 * c + h) ^ f(r)) & (kPieces - 1)) * 16;
-    const int kr = (lane & 15) >> 2, q = lane >> 4 & 1, cr = 4 * h + kr;
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
-      col[d] = cr * kRow + (((4 * d + 2 * q + ((lane & 3) >> 1)) ^ f(cr)) & (kPieces - 1)) * 16 + (lane & 1) * 8;
+    row = r * kRow + ((h ^ f(r)) << 4);
+    const int cr = 4 * h + ((lane & 15) >> 2), piece = (lane >> 3 & 2) | (lane >> 1 & 1), e = (lane & 1) * 8;
+    col0 = cr * kRow + ((piece ^ f(cr)) << 4) + e;
+    col1 = (cr + 8) * kRow + ((piece ^ f(cr + 8)) << 4) + e;
   }
   // Row 32 b + lane % 32, elements 16 c + 8 (lane / 32) + [0, 8).
   __device__ __forceinline__ short8v rows(const char* lds, int b, int c) const {
-    return *(const short8v*)(lds + row[c & 3] + (c >> 2) * 128 + b * 32 * kRow);
+    return *(const short8v*)(lds + (row ^ (c << 5)) + b * 32 * kRow);
   }
   // Column 32 d + lane % 32 of rows 16 c + 4 (lane / 32) + [0, 4) and 8 further.
   __device__ __forceinline__ short8v cols(const char* lds, int c, int d) const {
-    const char* at = lds + col[d & 1] + (d >> 1) * 128 + 16 * c * kRow;
-    const short4v u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)at);
-    const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(at + 8 * kRow));
+    const short4v u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds + (col0 ^ (d << 6)) + 16 * c * kRow));
+    const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds + (col1 ^ (d << 6)) + 16 * c * kRow));
     return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
   }
-  // Sends load i of a stage: rows i kPer to (i + 1) kPer - 1 of it; `at(row)` gives a
-  // row's address.
-  template <class F>
-  __device__ static __forceinline__ void load(char* lds, int i, F&& at) {
-    const int lane = threadIdx.x & 63, r = i * kPer + lane / kPieces;
-    const char* p = at(r) + (((lane % kPieces) ^ f(r)) << 4);
-    __builtin_amdgcn_global_load_lds((const void*)p, (lds_void*)(lds + i * 1024), 16, 0, 0);
+  // Sends load n of a stage: its rows n kPer to (n + 1) kPer - 1, of which the lane
+  // brings 16 bytes of load_row(n), at `base` (the same for the wave) + `row_at`.
+  __device__ static __forceinline__ int load_row(int n) { return n * kPer + (threadIdx.x & 63) / kPieces; }
+  __device__ static __forceinline__ void load(char* lds, int n, const char* base, uint32_t row_at) {
+    const uint32_t piece = (threadIdx.x & 63) % kPieces ^ f(load_row(n));
+    __builtin_amdgcn_global_load_lds((const void*)(base + (row_at + (piece << 4))), (lds_void*)(lds + n * 1024), 16, 0, 0);
+  }
+  // N loads, every BY-th from n0 on, of rows `pitch` bytes apart from `base` on, the
+  // stage's first; rows behind `last` are read as the last.
+  template <int N, int BY>
+  __device__ static __forceinline__ void load_rows(char* lds, int n0, const char* base, uint32_t pitch, int last) {
+    if (last >= N * BY * kPer - 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) load(lds, n0 + i * BY, base + i * BY * kPer * pitch, load_row(n0) * pitch);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) load(lds, n0 + i * BY, base, min(load_row(n0 + i * BY), last) * pitch);
+    }
   }
 };
 

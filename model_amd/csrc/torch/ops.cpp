@@ -352,8 +352,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> vocab_cross_entropy_grads(const Tenso
 }
 
 // ------------------------------------------------------- packed attention
-// [tokens, heads, hd] with hd elements next to each other and rows at 16 bytes;
-// copied only where they do not lie so.
+// [tokens, heads, hd] with hd elements next to each other, rows at 16 bytes and not
+// too far apart (mpl.h); copied only where they do not lie so.
 struct Heads {
   Tensor t;
   int64_t token = 0, head = 0;
@@ -361,10 +361,12 @@ struct Heads {
 Heads heads_of(const Tensor& x) {
   Tensor t = x._is_zerotensor() ? dense(x) : x.resolve_neg();
   const int64_t unit = 16 / t.element_size();
+  constexpr int64_t kFar = 1 << 23;
   auto lies = [&](const Tensor& y) {
     return y.numel() == 0 ||
-           (y.stride(2) == 1 && (uintptr_t)y.data_ptr() % 16 == 0 && (y.size(0) == 1 || y.stride(0) % unit == 0) &&
-            (y.size(1) == 1 || y.stride(1) % unit == 0));
+           (y.stride(2) == 1 && (uintptr_t)y.data_ptr() % 16 == 0 &&
+            (y.size(0) == 1 || (y.stride(0) % unit == 0 && y.stride(0) <= kFar)) &&
+            (y.size(1) == 1 || (y.stride(1) % unit == 0 && y.stride(1) * std::max<int64_t>(32, y.size(1)) <= 32 * kFar)));
   };
   if (!lies(t)) t = t.clone(at::MemoryFormat::Contiguous);
   if (t.numel() == 0) return {t, 0, 0};

@@ -406,3 +406,48 @@ def test_fp16_gradients_of_any_size(g_size, v_size):
     q, k, v, g, _ = make(lq, lq, 4, 2, 64, torch.float16, seed=14)
     q, k = q * 0.2, k * 0.2  # many alike weights, of 1 / 300 each
     run_all(q, k, (v.float() * v_size).half(), lq, lq, (g.float() * g_size).half(), scale=0.01)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("H,G", [(16, 16), (6, 2), (8, 2), (33, 1)])
+def test_many_rows(dtype, hd, H, G):
+    """Enough rows and keys for the tiles of large calls: 128 rows, 128 keys."""
+    rng = random.Random(H + hd)
+    total = 33_000 // G + 300
+    lq = [0, 1, 127, 128, 129, 257]
+    while sum(lq) < total:
+        lq.append(rng.choice([1, 2, 63, 65, 200, 300, 511, 640]))
+    q, k, v, g, gl = make(lq, lq, H, G, hd, dtype, seed=15, fused=H == G)
+    run_all(q, k, v, lq, lq, g, gl, wide=H == 6)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_rows_that_continue_a_cache(dtype, hd):
+    rng = random.Random(hd)
+    lq = [rng.choice([1, 40, 130, 260]) for _ in range(60)] + [0, 50]
+    cap = 700
+    used = [max(0, min(cap, x + rng.choice([0, 1, 100, 333, -20]))) for x in lq]
+    q, k, v, g, gl = make(lq, [cap] * len(lq), 8, 4, hd, dtype, seed=16)
+    begin = [cap * i for i in range(len(lq) + 1)]
+    for i, x in enumerate(used):  # places not in use hold anything
+        k[begin[i] + x:begin[i + 1]] = math.nan
+        v[begin[i] + x:begin[i + 1]] = math.inf
+    run_all(q, k, v, lq, used, g, gl, own_keys=True, key_lengths=used, begin=begin)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_many_rows_not_finite_stays_in_its_sequence(dtype):
+    lq = [1500, 700, 2000]
+    q, k, v, g, _ = make(lq, lq, 16, 16, 64, dtype, seed=17)
+    starts = torch.tensor(sums(lq), dtype=torch.int32, device=DEV)
+
+    def all_of():
+        out, lse = packed_attention_forward(q, k, v, starts)
+        return [out, lse, *packed_attention_backward(g, q, k, v, out, lse, starts)]
+
+    want = all_of()
+    q[1505], k[1700], v[2100], g[2199] = math.nan, math.inf, math.nan, -math.inf
+    for a, b in zip(want, all_of()):
+        assert torch.equal(a[:1500], b[:1500]) and torch.equal(a[2200:], b[2200:])
