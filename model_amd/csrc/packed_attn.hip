@@ -212,31 +212,18 @@ struct Softmax {
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
   }
-  // One stage of 32 B keys, of which the row sees those below `sees` (counted from
-  // the stage's first); `masked`: some row of the wave does not see them all.
-  template <int B>
-  __device__ __forceinline__ void step(const Stage<HD>& st, const char* k, const char* v, const short8v (&q)[HD / 16],
-                                       float c, int sees, bool masked) {
+  // Takes in the scores of 32 keys, of which the row sees those below `sees` (counted
+  // from the first; `masked`: some row of the wave does not see them all): the maximum.
+  __device__ __forceinline__ void top(f32x16& s, float c, int sees, bool masked) {
     const int half = (threadIdx.x >> 5) & 1;
-    f32x16 s[B];
-#pragma unroll
-    for (int b = 0; b < B; ++b) {
-      s[b] = f32x16{};
-#pragma unroll
-      for (int i = 0; i < HD / 16; ++i) s[b] = mma16<T>(st.rows(k, b, i), q[i], s[b]);
-    }
     if (masked) {
 #pragma unroll
-      for (int b = 0; b < B; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * b + tile_row(r, half) >= sees) s[b][r] = -INFINITY;
+      for (int r = 0; r < 16; ++r)
+        if (tile_row(r, half) >= sees) s[r] = -INFINITY;
     }
-    float mx = s[0][0];
+    float mx = s[0];
 #pragma unroll
-    for (int b = 0; b < B; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
     float a0 = mx, a1 = mx;
     half_swap(a0, a1);
     mx = fmaxf(a0, a1) * c;
@@ -250,34 +237,44 @@ struct Softmax {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
     }
+  }
+  // Their weights, as operands of the product with the values.
+  __device__ __forceinline__ void weights(const f32x16& s, float c, short8v (&w)[2]) {
     const float ref = (m == -INFINITY ? 0.f : m) - kLift<T>;  // no key of the row yet: weights 0
     float sum = 0.f;
 #pragma unroll
-    for (int b = 0; b < B; ++b)
+    for (int i = 0; i < 2; ++i) {
+      float p[8];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(fmaf(s[b][8 * i + e], c, -ref));
-          sum += p[e];
-        }
-        const short8v w = round8<T>(p);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] = mma16<T>(st.cols(v, 2 * b + i, d), w, acc[d]);
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * i + e], c, -ref));
+        sum += p[e];
       }
+      w[i] = round8<T>(p);
+    }
     l += sum;
+  }
+  __device__ __forceinline__ void values(const Stage<HD>& st, const char* v, int b, const short8v (&w)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[d] = mma16<T>(st.cols(v, 2 * b + i, d), w[i], acc[d]);
   }
 };
 
 // Many rows: 128 a workgroup, 32 a wave, 64 keys a stage that all four waves read.
+//
+// The scores of the next 32 keys are formed while the softmax of these 32 runs: the
+// products need the matrix unit and the softmax the vector unit, and a wave that
+// alternated them would leave one or the other idle.  So keys run half a stage ahead
+// of values, and values have one stage more.
 constexpr int kWideRows = 128, kWideKeys = 64;
 template <class T, int HD>
 __global__ __launch_bounds__(kThreads, 2) void packed_forward16_kernel(const Packed a, T* __restrict__ out,
                                                                        float* __restrict__ lse) {
   typedef Stage<HD> St;
   constexpr int kBytes = kWideKeys * St::kRow, kLoads = kBytes / 1024 / kWaves;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * kBytes];
+  __shared__ __attribute__((aligned(1024))) char lds[5 * kBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int group = blockIdx.x % a.G;
@@ -295,31 +292,69 @@ __global__ __launch_bounds__(kThreads, 2) void packed_forward16_kernel(const Pac
   const char* kb = a.k + group * a.kh + keys.first * a.kt;
   const char* vb = a.v + group * a.vh + keys.first * a.vt;
   const char* qrow = a.q + (seg.first + tok) * a.qt + (group * a.R + ri - tok * a.R) * a.qh;
-  auto send = [&](int it, char* to) __attribute__((always_inline)) {
+  auto send = [&](int it, int slot) __attribute__((always_inline)) {
     const int k0 = it * kWideKeys, last = keys.len - 1 - k0;
-    St::template load_rows<kLoads, kWaves>(to, wave, kb + k0 * a.kt, (uint32_t)a.kt, last);
-    St::template load_rows<kLoads, kWaves>(to + kBytes, wave, vb + k0 * a.vt, (uint32_t)a.vt, last);
+    St::template load_rows<kLoads, kWaves>(lds + (it & 1) * kBytes, wave, kb + k0 * a.kt, (uint32_t)a.kt, last);
+    St::template load_rows<kLoads, kWaves>(lds + (2 + slot) * kBytes, wave, vb + k0 * a.vt, (uint32_t)a.vt, last);
   };
   const St st;
   const int stages = most > 0 ? (most + kWideKeys - 1) / kWideKeys : 0;
-  if (stages) send(0, lds);
-  short8v q[HD / 16];
+  if (stages) send(0, 0);
+  short8v q[HD / 16], kf[HD / 16];
 #pragma unroll
   for (int i = 0; i < HD / 16; ++i) q[i] = *(const short8v*)(qrow + 32 * i + 16 * half);
   Softmax<T, HD> sm;
-  for (int it = 0; it < stages; ++it) {
-    // behind the barrier this stage has arrived, and every wave has read the one
-    // before it, over which the next is sent
-    wait_vmcnt_le<0>();
+  f32x16 s[2] = {f32x16{}, f32x16{}};
+  auto turn = [&]() __attribute__((always_inline)) {
     reads_done();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (it + 1 < stages) send(it + 1, lds + 2 * kBytes * ((it + 1) & 1));
-    const int k0 = it * kWideKeys;
-    if (k0 < wave_most) {
-      const char* at = lds + 2 * kBytes * (it & 1);
-      sm.template step<2>(st, at, at + kBytes, q, a.c, sees - k0, k0 + kWideKeys > least);
+  };
+  auto fetch = [&](const char* k, int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) kf[i] = st.rows(k, b, i);
+  };
+  auto scores = [&](f32x16& to) __attribute__((always_inline)) {
+    to = f32x16{};
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) to = mma16<T>(kf[i], q[i], to);
+  };
+  wait_vmcnt_le<0>();  // q too: the compiler does not count the stages' loads, and would wait for all of them
+  if (stages) {
+    turn();
+    if (stages > 1) send(1, 1);
+    fetch(lds, 0);
+    scores(s[0]);
+  }
+  // block j of the wave: its scores are there, the next one's are formed
+  auto block = [&](f32x16& now, f32x16& next, const char* v, int b, int j) __attribute__((always_inline)) {
+    sm.top(now, a.c, sees - 32 * j, 32 * j + 32 > least);
+    short8v w[2];
+    scores(next);
+    sm.weights(now, a.c, w);
+    sm.values(st, v, b, w);
+  };
+  int slot = 0;  // it % 3
+  for (int it = 0; it < stages; ++it) {
+    const char* k = lds + (it & 1) * kBytes;
+    const char* v = lds + (2 + slot) * kBytes;
+    const bool first = it * kWideKeys < wave_most, second = it * kWideKeys + 32 < wave_most;
+    if (first) {
+      fetch(k, 1);
+      block(s[0], s[1], v, 0, 2 * it);
     }
+    if (it + 1 < stages) {
+      // behind the barrier the next stage has arrived; every wave is done with this
+      // one's keys and with the values before, over which the stage after next goes
+      wait_vmcnt_le<0>();
+      turn();
+      if (it + 2 < stages) send(it + 2, slot == 0 ? 2 : slot - 1);
+    }
+    if (second) {
+      fetch(lds + ((it + 1) & 1) * kBytes, 0);  // past the last stage: not used
+      block(s[1], s[0], v, 1, 2 * it + 1);
+    }
+    slot = slot == 2 ? 0 : slot + 1;
   }
   float l0 = sm.l, l1 = sm.l;
   half_swap(l0, l1);
@@ -374,6 +409,7 @@ __global__ __launch_bounds__(kThreads) void packed_forward16_few_kernel(const Pa
   for (int i = 0; i < HD / 16; ++i) q[i] = *(const short8v*)(qrow + 32 * i + 16 * half);
   Softmax<T, HD> sm;
   if (j0 < j1) send(j0, mine);
+  wait_vmcnt_le<0>();  // q too: the compiler does not count the stages' loads, and would wait for all of them
   int turn = 0;
   for (int j = j0; j < j1; j += kWaves, turn ^= 1) {
     reads_done();  // of the stage before, over which the next is sent
@@ -385,7 +421,13 @@ __global__ __launch_bounds__(kThreads) void packed_forward16_few_kernel(const Pa
     }
     asm volatile("" ::: "memory");
     const char* at = mine + 2 * kBytes * turn;
-    sm.template step<1>(st, at, at + kBytes, q, a.c, sees - 32 * j, 32 * j + 32 > least);
+    f32x16 s = f32x16{};
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) s = mma16<T>(st.rows(at, 0, i), q[i], s);
+    short8v w[2];
+    sm.top(s, a.c, sees - 32 * j, 32 * j + 32 > least);
+    sm.weights(s, a.c, w);
+    sm.values(st, at + kBytes, 0, w);
   }
   reads_done();
   __syncthreads();  // the stages become the waves' results
@@ -784,6 +826,7 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
   f32x16 acc[HD / 32];
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d) acc[d] = f32x16{};
+  wait_vmcnt_le<0>();  // q and the rest too: the compiler does not count the stages' loads
   int turn = 0;
   for (int it = from; it < stages; it += by, turn ^= 1) {
     if (WIDE) wait_vmcnt_le<0>();

@@ -77,9 +77,21 @@ struct Stage {
   // Sends load n of a stage: its rows n kPer to (n + 1) kPer - 1, of which the lane
   // brings 16 bytes of load_row(n), at `base` (the same for the wave) + `row_at`.
   __device__ static __forceinline__ int load_row(int n) { return n * kPer + (threadIdx.x & 63) / kPieces; }
+  //
+  // In assembly, because the compiler makes every transposing read wait for all loads
+  // under way, those of the next stage among them (it does not know what either
+  // touches).  The instruction has no register for a result; whoever reads the stage
+  // waits for it with wait_vmcnt_le and a barrier.
   __device__ static __forceinline__ void load(char* lds, int n, const char* base, uint32_t row_at) {
     const uint32_t piece = (threadIdx.x & 63) % kPieces ^ f(load_row(n));
-    __builtin_amdgcn_global_load_lds((const void*)(base + (row_at + (piece << 4))), (lds_void*)(lds + n * 1024), 16, 0, 0);
+    const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)(lds + n * 1024));
+    const uint64_t from = (uint64_t)base;
+    const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(from >> 32)) << 32 |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)from);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(to), "v"(row_at + (piece << 4)), "s"(at)
+                 : "memory", "m0");
   }
   // N loads, every BY-th from n0 on, of rows `pitch` bytes apart from `base` on, the
   // stage's first; rows behind `last` are read as the last.
