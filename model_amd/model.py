@@ -9,8 +9,12 @@ MemoryPool (libmpl.so).  MemoryPoolLM.token_loss gives each token's cross
 entropy without the logits in memory, for training and evaluation on the GPU:
 its layer norms (with the residual add before each) and its output layer with
 the loss are libmpl.so launches with their own backward passes
-(model_amd/layer_norm.py, model_amd/cross_entropy.py).  Parameter names and shapes follow the Flax modules, so a checkpoint of the reference
-(model_amd/checkpoint.py) loads into it:
+(model_amd/layer_norm.py, model_amd/cross_entropy.py).  With ``starts`` the
+tokens of apply and token_loss are sequences of unlike lengths packed one behind
+the other: positions begin anew with each, and the attention
+(model_amd/attention.py) is one libmpl.so launch a layer, with its own backward
+pass, in training too.  Parameter names and shapes follow the Flax modules, so a
+checkpoint of the reference (model_amd/checkpoint.py) loads into it:
 
   embed/embedding [vocab, d]            nn.Embed (logits use embed.attend)
   pos_embed [max_len, d]
@@ -42,6 +46,7 @@ from typing import Any, Dict, List, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from .attention import packed_attention
 from .cross_entropy import vocab_cross_entropy
 from .layer_norm import LN_EPS, layer_norm
 from .memory import MemoryPool
@@ -335,6 +340,33 @@ def _add_layer_norm(x, y, p):
     if y is None:
         return layer_norm(x, p["scale"], p["bias"], LN_EPS), x
     return layer_norm(x, p["scale"], p["bias"], LN_EPS, residual=y)
+
+
+def _packed_embed(emb: torch.Tensor, pos_emb: torch.Tensor, tokens: torch.Tensor, starts: torch.Tensor) -> torch.Tensor:
+    """emb[tokens] + pos_emb[position in the token's own sequence], for tokens
+    [B, T] that hold the sequences of ``starts`` one behind the other.  A token of
+    no sequence has position 0; one at a position past the table a NaN row."""
+    at = torch.arange(tokens.numel(), device=tokens.device, dtype=starts.dtype)
+    n = starts.numel() - 1
+    seq = torch.searchsorted(starts.contiguous(), at, right=True) - 1
+    in_one = (seq >= 0) & (seq < n)
+    pos = torch.where(in_one, at - starts[seq.clamp(min=0, max=n)], 0)
+    last = pos_emb.shape[0] - 1
+    x = emb[tokens] + pos_emb[pos.clamp(min=0, max=last)].reshape(*tokens.shape, -1)
+    return x.masked_fill((pos > last).reshape(*tokens.shape, 1), math.nan)
+
+
+def _check_starts(what: str, starts, tokens, heads: int, d: int, dropout: bool) -> None:
+    if (not isinstance(starts, torch.Tensor) or starts.dim() != 1 or starts.numel() == 0
+            or starts.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"{what}: starts must be a tensor [sequences + 1] of int32 or int64")
+    if not tokens.is_cuda or starts.device != tokens.device:
+        raise ValueError(f"{what}: packed sequences run on the GPU only (libmpl.so), tokens are on {tokens.device}, starts on "
+                         f"{starts.device}")
+    if d % heads or d // heads not in (32, 64, 128):
+        raise ValueError(f"{what}: packed sequences take heads of 32, 64 or 128, not of {d} / {heads}")
+    if dropout:
+        raise ValueError(f"{what}: packed sequences have no dropout on the attention's weights")
 
 
 def merge_layer_aux(layer_aux: List[Dict[str, Any]]) -> Dict[str, Any]:
@@ -632,30 +664,37 @@ class MemoryPoolLM:
         return (plain(emb, 4) and emb.dim() == 2 and emb.shape[1] == d
                 and plain(pe, 4) and pe.dim() == 2 and pe.shape[1] == d and ln(p["ln_final"]))
 
-    def _forward_gpu(self, p, tokens, pool_off, noise_scale, shuffle_pool, rngs):
+    def _forward_gpu(self, p, tokens, pool_off, noise_scale, shuffle_pool, rngs, starts=None):
         """The general path of apply() for plain inference over whole
         sequences, as library launches: the layer norms, biases, activations
         and residual adds inside the dense layers (mpl_dense_layers), and the
         attention one launch without score matrix, mask or transposed copies
         (mpl_causal_attention)."""
         B, T = tokens.shape
-        x, layer_aux = self._trunk_gpu(p, tokens, pool_off, noise_scale, shuffle_pool, rngs)
+        x, layer_aux = self._trunk_gpu(p, tokens, pool_off, noise_scale, shuffle_pool, rngs, starts)
         logits = F.linear(_ln(x, p["ln_final"]), p["embed"]["embedding"])
         return logits.reshape(B, T, -1), _LazyMerged(layer_aux)
 
-    def _trunk_gpu(self, p, tokens, pool_off, noise_scale, shuffle_pool, rngs):
+    def _trunk_gpu(self, p, tokens, pool_off, noise_scale, shuffle_pool, rngs, starts=None):
         """_forward_gpu up to ln_final's input: ([B * T, d], the layers' aux)."""
         cfg = self.cfg
         B, T = tokens.shape
         d, H = cfg.d_model, cfg.n_heads
         emb = p["embed"]["embedding"]
-        x = (emb[tokens] + p["pos_embed"][None, :T]).reshape(B * T, d)
+        if starts is None:
+            x = emb[tokens] + p["pos_embed"][None, :T]
+        else:
+            x = _packed_embed(emb, p["pos_embed"], tokens, starts)
+        x = x.reshape(B * T, d)
         layer_aux = []
         for i in range(cfg.n_layers):
             pa = p[f"attn_{i}"]
             qkv, = dense_layers(x, [(pa[nm]["kernel"], pa[nm]["bias"], None) for nm in ("query", "key", "value")],
                                 ln=p[f"ln_attn_{i}"], joined=True)
-            a = causal_attention(qkv.reshape(B, T, 3 * d), H, (d // H) ** -0.5)
+            if starts is None:
+                a = causal_attention(qkv.reshape(B, T, 3 * d), H, (d // H) ** -0.5)
+            else:
+                a = packed_attention(*qkv.reshape(B * T, 3, H, d // H).unbind(1), starts)
             x, = dense_layers(a.reshape(B * T, d), [(pa["out"]["kernel"], pa["out"]["bias"], None)], residual=x)
             ln = p[f"ln_ffn_{i}"]
             mem_layer = self.pool is not None and i in cfg.memory_layers
@@ -674,7 +713,7 @@ class MemoryPoolLM:
                 layer_aux.append(aux)
         return x, layer_aux
 
-    def _attention(self, p, h, layer_cache, positions, drop=None):
+    def _attention(self, p, h, layer_cache, positions, drop=None, starts=None):
         cfg = self.cfg
         B, T, d = h.shape
         hd = d // cfg.n_heads
@@ -684,6 +723,9 @@ class MemoryPoolLM:
         w = torch.cat([p[nm]["kernel"].reshape(d, cfg.n_heads * hd) for nm in names], 1)
         b = torch.cat([p[nm]["bias"].reshape(cfg.n_heads * hd) for nm in names])
         qkv = (torch.matmul(h, w) + b).reshape(B, T, 3, cfg.n_heads, hd)
+        if starts is not None:
+            a = packed_attention(*qkv.reshape(B * T, 3, cfg.n_heads, hd).unbind(1), starts).reshape(B, T, d)
+            return torch.matmul(a, p["out"]["kernel"].reshape(d, d)) + p["out"]["bias"]
         q, k, v = (qkv[:, :, i].permute(0, 2, 1, 3) for i in range(3))  # [B, heads, T, hd]
         q = q * (hd ** -0.5)
         if layer_cache is not None:  # decode: write position `positions`, attend to <= it
@@ -707,9 +749,14 @@ class MemoryPoolLM:
               route_through_pool: bool = False, sparse_grad: bool = False,
               probes: Optional[Dict[int, torch.Tensor]] = None, positions: Optional[torch.Tensor] = None,
               noise_scale: float = 1.0, shuffle_pool: bool = False, cache=None, rngs=None,
-              input_rows: Optional[torch.Tensor] = None):
+              input_rows: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None):
         """model.py:27-127: (logits [B, T, vocab], aux).  In decode mode pass
         ``cache`` (init_cache) and ``positions`` (int64 device tensor [1]).
+        ``starts`` (int32 or int64 [n + 1], on the GPU) packs n sequences of unlike
+        lengths, each of at most max_len, into the B T tokens: sequence i is
+        tokens.flatten()[starts[i]:starts[i + 1]], its positions begin at 0, and its
+        tokens attend to it alone (packed_attention; T may pass max_len).  No decode
+        mode, and no dropout in training.
         ``input_rows`` (GPU decode step only): the step's input rows
         emb[tokens] + pos_embed[positions], [B, d_model] fp32, already formed
         (the greedy token step writes them, mpl_decode_next_token_embed); the
@@ -717,16 +764,20 @@ class MemoryPoolLM:
         cfg = self.cfg
         p = variables["params"] if "params" in variables else variables
         B, T = tokens.shape
+        if starts is not None:
+            if self.decode or positions is not None or cache is not None:
+                raise ValueError("packed sequences take whole sequences: no decode mode, positions or cache")
+            _check_starts("apply", starts, tokens, cfg.n_heads, cfg.d_model, train and cfg.dropout > 0)
         if (self.decode and tokens.is_cuda and cache is not None and positions is not None and T == 1 and not train
                 and not pool_off and not route_through_pool and probes is None and not shuffle_pool):
             return self._decode_step_gpu(p, tokens, positions, cache, noise_scale, rngs, input_rows)
         if (not self.decode and positions is None and not train and not route_through_pool and probes is None
                 and not sparse_grad and self._fused_forward_ok(p, tokens, pool_off)):
-            return self._forward_gpu(p, tokens, pool_off, noise_scale, shuffle_pool, rngs)
+            return self._forward_gpu(p, tokens, pool_off, noise_scale, shuffle_pool, rngs, starts)
         x, layer_aux = self._trunk(p, tokens, _add_ln, train=train, pool_off=pool_off,
                                    route_through_pool=route_through_pool, sparse_grad=sparse_grad, probes=probes,
                                    positions=positions, noise_scale=noise_scale, shuffle_pool=shuffle_pool,
-                                   cache=cache, rngs=rngs)
+                                   cache=cache, rngs=rngs, starts=starts)
         logits = F.linear(x, p["embed"]["embedding"])  # x . emb^T as one product, no transposed copy of the table
         return logits, _LazyMerged(layer_aux)
 
@@ -736,7 +787,7 @@ class MemoryPoolLM:
                    ignore_index: int = -100, return_lse: bool = False, train: bool = False, pool_off: bool = False,
                    route_through_pool: bool = False, sparse_grad: bool = False,
                    probes: Optional[Dict[int, torch.Tensor]] = None, noise_scale: float = 1.0,
-                   shuffle_pool: bool = False, rngs=None):
+                   shuffle_pool: bool = False, rngs=None, starts: Optional[torch.Tensor] = None):
         """The cross entropy of each token's target under apply()'s logits,
         without the logits in memory: (loss [B, T] fp32, aux), or (loss, lse,
         aux) with ``return_lse``; on the GPU.  targets [B, T] int64 or int32,
@@ -745,29 +796,35 @@ class MemoryPoolLM:
         apply() is (the table's gradient through the output layer and through
         the input rows); the layer norms run with the residual adds before
         them (layer_norm).  Under torch.no_grad the blocks take the fused
-        launches that apply() takes there."""
+        launches that apply() takes there.  With ``starts`` (apply) the tokens
+        are packed sequences, and the attention's backward pass is
+        packed_attention's; a sequence's last token has no next one, nor has a
+        token of no sequence: their targets are ignore_index."""
         if self.decode:
             raise ValueError("token_loss takes whole sequences: build the model without decode=True")
         if not tokens.is_cuda:
             raise ValueError(f"token_loss runs on the GPU only (libmpl.so), tokens are on {tokens.device}")
         if targets.shape != tokens.shape:
             raise ValueError(f"token_loss: targets {tuple(targets.shape)} for tokens {tuple(tokens.shape)}")
+        if starts is not None:
+            _check_starts("token_loss", starts, tokens, self.cfg.n_heads, self.cfg.d_model,
+                          train and self.cfg.dropout > 0)
         p = variables["params"] if "params" in variables else variables
         if (not train and not route_through_pool and probes is None and not sparse_grad
                 and self._fused_forward_ok(p, tokens, pool_off)):
-            x, layer_aux = self._trunk_gpu(p, tokens, pool_off, noise_scale, shuffle_pool, rngs)
+            x, layer_aux = self._trunk_gpu(p, tokens, pool_off, noise_scale, shuffle_pool, rngs, starts)
             lf = p["ln_final"]
             x = layer_norm(x, lf["scale"], lf["bias"], LN_EPS).reshape(*tokens.shape, -1)
         else:
             x, layer_aux = self._trunk(p, tokens, _add_layer_norm, train=train, pool_off=pool_off,
                                        route_through_pool=route_through_pool, sparse_grad=sparse_grad, probes=probes,
                                        positions=None, noise_scale=noise_scale, shuffle_pool=shuffle_pool, cache=None,
-                                       rngs=rngs)
+                                       rngs=rngs, starts=starts)
         loss, lse = vocab_cross_entropy(x, p["embed"]["embedding"], targets, ignore_index=ignore_index, return_lse=True)
         return (loss, lse, _LazyMerged(layer_aux)) if return_lse else (loss, _LazyMerged(layer_aux))
 
     def _trunk(self, p, tokens, add_ln, *, train, pool_off, route_through_pool, sparse_grad, probes, positions,
-               noise_scale, shuffle_pool, cache, rngs):
+               noise_scale, shuffle_pool, cache, rngs, starts=None):
         """The backbone up to the output layer: (LayerNorm of the last layer's
         output [B, T, d], the layers' aux).  ``add_ln`` adds a block's output to
         the residual stream and normalises it for the next (_add_ln,
@@ -775,7 +832,9 @@ class MemoryPoolLM:
         cfg = self.cfg
         B, T = tokens.shape
         emb = p["embed"]["embedding"]
-        if positions is None:
+        if starts is not None:
+            x = _packed_embed(emb, p["pos_embed"], tokens, starts)
+        elif positions is None:
             x = emb[tokens] + p["pos_embed"][None, :T]
         else:
             x = emb[tokens] + p["pos_embed"][positions][None]
@@ -786,7 +845,7 @@ class MemoryPoolLM:
         y = None
         for i in range(cfg.n_layers):
             h, x = add_ln(x, y, p[f"ln_attn_{i}"])
-            y = self._attention(p[f"attn_{i}"], h, cache[i] if self.decode else None, positions, drop)
+            y = self._attention(p[f"attn_{i}"], h, cache[i] if self.decode else None, positions, drop, starts)
             h, x = add_ln(x, y, p[f"ln_ffn_{i}"])
             mem_layer = self.pool is not None and i in cfg.memory_layers
             y = torch.zeros_like(x)

@@ -67,3 +67,31 @@ def test_dropout_mask_statistics():
 
     with pytest.raises(ValueError):
         _make_dropout(1.0, None, torch.device("cpu"))
+
+
+def test_packed_sequences_are_refused_where_they_cannot_run():
+    import pytest
+
+    cfg = _cfg(d_model=64)
+    model = MemoryPoolLM(cfg)
+    params = model.init(1, device="cpu")
+    toks = torch.zeros((1, 12), dtype=torch.int64)
+    for starts, match in ((torch.tensor([0.0, 12.0]), "starts must be"), ([0, 12], "starts must be"),
+                          (torch.zeros(0, dtype=torch.int32), "starts must be"),
+                          (torch.tensor([[0, 12]]), "starts must be"), (torch.tensor([0, 12]), "on the GPU only")):
+        with pytest.raises(ValueError, match=match):
+            model.apply(params, toks, starts=starts)
+    dec = MemoryPoolLM(cfg, decode=True)
+    with pytest.raises(ValueError, match="no decode mode"):
+        dec.apply(params, toks[:, :1], positions=torch.tensor([0]), cache=dec.init_cache(1, device="cpu"),
+                  starts=torch.tensor([0, 1]))
+
+
+def test_packed_embedding_rows():
+    from model_amd.model import _packed_embed
+
+    emb, pe = torch.arange(20.0)[:, None] * 100, torch.arange(4.0)[:, None]
+    tokens = torch.arange(12).reshape(2, 6) % 20
+    x = _packed_embed(emb, pe, tokens, torch.tensor([1, 3, 3, 8, 9], dtype=torch.int32)).reshape(-1)
+    want = tokens.reshape(-1) * 100.0 + torch.tensor([0, 0, 1, 0, 1, 2, 3, float("nan"), 0, 0, 0, 0])
+    torch.testing.assert_close(x, want, equal_nan=True)
