@@ -470,7 +470,9 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const Packed a, int sp
 struct Grads {
   const char* g_out;
   int64_t gt, gh;  // bytes
-  const float *lse2, *delta;  // [group][T R]: base 2, +inf for a row without keys
+  const float* lse2;  // [group][T R]: base 2, +inf for a row without keys
+  float* delta;       // [group][T R]
+  const float* g_lse;
   const float* largest;       // [3][blocks]
   int blocks;
   float scale;
@@ -776,6 +778,14 @@ struct Sums {
 
 // dq.  WIDE: 128 rows a workgroup, 32 a wave, 64 keys a stage that all waves read;
 // else 32 rows, and every wave has keys and stages of its own.
+//
+// delta = g_out . out is as good as out, which was rounded to 16 bits; where a row sees
+// few keys, out is as large as v, and that error was most of dq's and dk's (3.8e-3 of
+// their norm against 2.4e-3, bf16, 10 sequences of 56 tokens together).  So tiles of up
+// to kExactKeys keys take delta = sum p dp - g_lse in a sweep of their own, which also
+// goes to memory for dk; with more keys out is an average and that error small,
+// and the sweep would cost two thirds of dq again.
+constexpr int kExactKeys = 512;
 template <class T, int HD, bool WIDE>
 __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(const Packed a, const Grads g,
                                                                             T* __restrict__ dq) {
@@ -784,6 +794,7 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
   constexpr int kBytes = kKeys * St::kRow, kLoads = kBytes / 1024 / (WIDE ? kWaves : 1);
   constexpr int kStages = 4 * kBytes * (WIDE ? 1 : kWaves), kJoin = WIDE ? 0 : sizeof(Sums<HD, 1, kWaves>);
   __shared__ __attribute__((aligned(1024))) char lds[kStages > kJoin ? kStages : kJoin];
+  __shared__ float sigma[kWaves][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int group = blockIdx.x % a.G;
@@ -814,7 +825,6 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
   const St st;
   const int stages = most > 0 ? (most + kKeys - 1) / kKeys : 0;
   const int from = WIDE ? 0 : wave, by = WIDE ? 1 : kWaves;
-  if (from < stages) send(from, mine);
   short8v q[HD / 16], go[HD / 16];
 #pragma unroll
   for (int i = 0; i < HD / 16; ++i) {
@@ -822,55 +832,84 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
     go[i] = *(const short8v*)(grow + 32 * i + 16 * half);
   }
   const int64_t at = (int64_t)group * a.T * a.R + (int64_t)seg.first * a.R + ri;
-  const float lse2 = g.lse2[at], delta = g.delta[at];
+  const float lse2 = g.lse2[at];
+  float delta = g.delta[at];
+  // use(p, dp, k, b): the weights of 32 keys (0 where not seen) and g_out . v, transposed,
+  // and where block b of keys lies
+  auto sweep = [&](auto&& use) __attribute__((always_inline)) {
+    reads_done();
+    if (WIDE) __builtin_amdgcn_s_barrier();  // of a sweep before
+    asm volatile("" ::: "memory");
+    if (from < stages) send(from, mine);
+    wait_vmcnt_le<0>();  // q and the rest too: the compiler does not count the stages' loads
+    int turn = 0;
+    for (int it = from; it < stages; it += by, turn ^= 1) {
+      if (WIDE) wait_vmcnt_le<0>();
+      reads_done();
+      if (WIDE) __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (it + by < stages) {
+        send(it + by, mine + 2 * kBytes * (turn ^ 1));
+        if (!WIDE) wait_vmcnt_le<2 * kLoads>();
+      } else if (!WIDE) {
+        wait_vmcnt_le<0>();
+      }
+      asm volatile("" ::: "memory");
+      const int k0 = it * kKeys;
+      if (k0 >= wave_most) continue;
+      const char* k = mine + 2 * kBytes * turn;
+      const char* v = k + kBytes;
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          s = mma16<T>(st.rows(k, b, i), q[i], s);
+          dp = mma16<T>(st.rows(v, b, i), go[i], dp);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2));
+        if (k0 + kKeys > least) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (k0 + 32 * b + tile_row(r, half) >= sees) s[r] = dp[r] = 0.f;
+        }
+        use(s, dp, k, b);
+      }
+    }
+  };
+  if (most <= kExactKeys) {
+    float sum = 0.f;
+    sweep([&](const f32x16& p, const f32x16& dp, const char*, int) __attribute__((always_inline)) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum = fmaf(p[r], dp[r], sum);
+    });
+    float other = sum;
+    half_swap(sum, other);
+    sum += other;
+    if constexpr (!WIDE) {
+      if (half == 0) sigma[wave][col] = sum;
+      __syncthreads();
+      sum = (sigma[0][col] + sigma[1][col]) + (sigma[2][col] + sigma[3][col]);
+    }
+    delta = sum - (g.g_lse ? g.g_lse[(int64_t)(seg.first + tok) * a.H + head] : 0.f);
+    if (half == 0 && w0 + col < rows && (WIDE || wave == 0)) g.delta[at] = delta;
+  }
+  if (!dq) return;
   f32x16 acc[HD / 32];
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d) acc[d] = f32x16{};
-  wait_vmcnt_le<0>();  // q and the rest too: the compiler does not count the stages' loads
-  int turn = 0;
-  for (int it = from; it < stages; it += by, turn ^= 1) {
-    if (WIDE) wait_vmcnt_le<0>();
-    reads_done();
-    if (WIDE) __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (it + by < stages) {
-      send(it + by, mine + 2 * kBytes * (turn ^ 1));
-      if (!WIDE) wait_vmcnt_le<2 * kLoads>();
-    } else if (!WIDE) {
-      wait_vmcnt_le<0>();
+  sweep([&](const f32x16& p, const f32x16& dp, const char* k, int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = p[8 * i + e] * ((dp[8 * i + e] - delta) * unit);
+      const short8v w = round8<T>(x);
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d) acc[d] = mma16<T>(st.cols(k, 2 * b + i, d), w, acc[d]);
     }
-    asm volatile("" ::: "memory");
-    const int k0 = it * kKeys;
-    if (k0 >= wave_most) continue;
-    const char* k = mine + 2 * kBytes * turn;
-    const char* v = k + kBytes;
-#pragma unroll
-    for (int b = 0; b < B; ++b) {
-      f32x16 s = f32x16{}, ds = f32x16{};
-#pragma unroll
-      for (int i = 0; i < HD / 16; ++i) {
-        s = mma16<T>(st.rows(k, b, i), q[i], s);
-        ds = mma16<T>(st.rows(v, b, i), go[i], ds);
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse2)) * ((ds[r] - delta) * unit);
-      if (k0 + kKeys > least) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (k0 + 32 * b + tile_row(r, half) >= sees) ds[r] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = ds[8 * i + e];
-        const short8v w = round8<T>(x);
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d) acc[d] = mma16<T>(st.cols(k, 2 * b + i, d), w, acc[d]);
-      }
-    }
-  }
+  });
   const float f = g.scale / unit;
   if constexpr (WIDE) {
     if (w0 + col >= rows) return;
@@ -1223,12 +1262,12 @@ void backward(const Args* p, const void* g_out, int64_t gt, int64_t gh, const vo
   float* largest = (float*)((char*)ws + 2 * round256(rows * 4));
   const int64_t blocks = cdiv(rows * (HD / 4), 256);
   const int used = (int)(blocks < kDeltaBlocks ? blocks : kDeltaBlocks);
-  const Grads g{(const char*)g_out, gt * (int64_t)sizeof(T), gh * (int64_t)sizeof(T), lse2, delta, largest, used, p->scale};
+  const Grads g{(const char*)g_out, gt * (int64_t)sizeof(T), gh * (int64_t)sizeof(T), lse2, delta, g_lse, largest, used, p->scale};
   if (rows)
     packed_delta_kernel<T, HD><<<used, 256, 0, s>>>(a, g.g_out, g.gt, g.gh, (const T*)out, lse, g_lse, lse2, delta, largest);
   auto tiles = [&](int64_t x, int unit) { return (unsigned)((x / unit + a.n + 2) * a.G); };
   if constexpr (sizeof(T) == 2) {
-    if (rows && dq) {
+    if (rows) {  // for delta, too
       if (wide_of(p)) packed_dq16_kernel<T, HD, true><<<tiles((int64_t)a.T * a.R, 128), kThreads, 0, s>>>(a, g, (T*)dq);
       else packed_dq16_kernel<T, HD, false><<<tiles((int64_t)a.T * a.R, 32), kThreads, 0, s>>>(a, g, (T*)dq);
     }

@@ -91,7 +91,7 @@ struct Stage {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
                  : "s"(to), "v"(row_at + (piece << 4)), "s"(at)
-                 : "memory", "m0");
+                 : "memory");  // m0 is the compiler's for its own LDS loads alone, which set it themselves
   }
   // N loads, every BY-th from n0 on, of rows `pitch` bytes apart from `base` on, the
   // stage's first; rows behind `last` are read as the last.

@@ -19,9 +19,11 @@
 #include <c10/util/ThreadLocalDebugInfo.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <functional>
 #include <initializer_list>
 #include <memory>
 #include <optional>
@@ -55,7 +57,7 @@ void* stream_of(const Tensor& t) {
 // The calls below read memory and launch kernels that no transform sees: a trace
 // would record an empty output, and a tangent or a batch would be left out without
 // a word.  `args` may hold undefined tensors.
-void refuse_transforms(const char* what, std::initializer_list<Tensor> args) {
+void refuse_modes(const char* what) {
   using c10::DispatchKey;
   TORCH_CHECK(!at::tracer::impl::is_dispatch_enabled(), what, " cannot be traced (torch.jit.trace)");
   TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(DispatchKey::FuncTorchDynamicLayerFrontMode), what,
@@ -64,14 +66,19 @@ void refuse_transforms(const char* what, std::initializer_list<Tensor> args) {
                           c10::impl::TorchDispatchModeKey::FUNCTIONAL})
     TORCH_CHECK(!c10::impl::TorchDispatchModeTLS::get_mode(mode).has_value(), what,
                 " cannot be traced (make_fx, fake or functional tensors)");
+}
+void refuse_wrapped(const char* what, const Tensor& t) {
+  using c10::DispatchKey;
   constexpr c10::DispatchKeySet wrapped({DispatchKey::Python, DispatchKey::FuncTorchBatched,
                                          DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched,
                                          DispatchKey::Functionalize});
-  for (const Tensor& t : args) {
-    if (!t.defined()) continue;
-    TORCH_CHECK(!t.key_set().has_any(wrapped), what, " takes plain tensors, no wrappers or subclasses with their own dispatch");
-    TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivative: an argument is a dual tensor");
-  }
+  TORCH_CHECK(!t.key_set().has_any(wrapped), what, " takes plain tensors, no wrappers or subclasses with their own dispatch");
+  TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivative: an argument is a dual tensor");
+}
+void refuse_transforms(const char* what, std::initializer_list<Tensor> args) {
+  refuse_modes(what);
+  for (const Tensor& t : args)
+    if (t.defined()) refuse_wrapped(what, t);
 }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -495,15 +502,23 @@ std::tuple<Tensor, Tensor, Tensor> packed_attention_backward(const Tensor& g_out
 }
 
 // --------------------------------------------------------------- gradient clip
-Tensor clip_grads(const std::vector<Tensor>& grads, double grad_clip, const std::optional<Tensor>& row_sq, bool apply,
+// `list` holds its tensors while the call runs: references, no copies of a thousand handles.
+Tensor clip_grads(const py::list& list, double grad_clip, const std::optional<Tensor>& row_sq, bool apply,
                   const char* what) {
+  std::vector<std::reference_wrapper<const Tensor>> grads;
+  grads.reserve(list.size());
+  for (const py::handle o : list) {
+    TORCH_CHECK_TYPE(THPVariable_Check(o.ptr()), what, ": gradient ", grads.size(), " is no tensor");
+    grads.emplace_back(THPVariable_Unpack(o.ptr()));
+  }
   const Tensor rows = or_none(row_sq);
   TORCH_CHECK_VALUE(!grads.empty() || rows.defined(), what, ": no gradients");
   TORCH_CHECK_VALUE(grad_clip >= 0, what, ": grad_clip ", grad_clip, " must not be negative");
-  const auto device = (grads.empty() ? rows : grads[0]).device();
+  refuse_modes(what);
+  const auto device = (grads.empty() ? rows : grads[0].get()).device();
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& t = grads[i];
-    refuse_transforms(what, {t});
+    refuse_wrapped(what, t);
     TORCH_CHECK_VALUE(t.layout() == at::kStrided && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf ||
                                                      t.scalar_type() == at::kBFloat16),
                       what, ": gradient ", i, " must be a dense float32, float16 or bfloat16 tensor, got ", t.scalar_type(),
@@ -517,7 +532,7 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double grad_clip, const std:
     }
   }
   if (rows.defined()) {
-    refuse_transforms(what, {rows});
+    refuse_wrapped(what, rows);
     TORCH_CHECK_VALUE(rows.scalar_type() == at::kFloat && rows.layout() == at::kStrided && rows.device() == device, what,
                       ": row_sq must be a dense float32 tensor on ", device);
   }
@@ -530,20 +545,25 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double grad_clip, const std:
   std::vector<int64_t> n;
   std::vector<int> types;
   std::vector<std::pair<char*, char*>> spans;
+  n.reserve(grads.size());
+  x.reserve(grads.size());
+  types.reserve(grads.size());
+  spans.reserve(grads.size());
   for (const Tensor& t : grads) {
-    if (t.numel() == 0 || t._is_zerotensor()) continue;  // add nothing, and are scaled by being what they are
-    Tensor y = t;
+    const int64_t m = t.numel();
+    if (m == 0 || t._is_zerotensor()) continue;  // add nothing, and are scaled by being what they are
+    char* at;
     if (t.is_neg() || !t.is_non_overlapping_and_dense()) {
-      y = dense(t);
-      held.push_back(y);
-      if (apply) back.emplace_back(t, y);
-    } else if (apply) {
-      char* at = (char*)t.data_ptr();
-      spans.emplace_back(at, at + t.numel() * t.element_size());
+      held.push_back(dense(t));
+      at = (char*)held.back().data_ptr();
+      if (apply) back.emplace_back(t, held.back());
+    } else {
+      at = (char*)t.data_ptr();
+      if (apply) spans.emplace_back(at, at + m * t.element_size());
     }
-    x.push_back(y.data_ptr());
-    n.push_back(y.numel());
-    types.push_back(dtype_code(y));
+    x.push_back(at);
+    n.push_back(m);
+    types.push_back(dtype_code(t));
   }
   std::sort(spans.begin(), spans.end());
   for (size_t i = 1; i < spans.size(); ++i)
@@ -564,10 +584,10 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double grad_clip, const std:
   return out;
 }
 
-Tensor clip_global_norm(const std::vector<Tensor>& grads, double grad_clip, const std::optional<Tensor>& row_sq) {
+Tensor clip_global_norm(const py::list& grads, double grad_clip, const std::optional<Tensor>& row_sq) {
   return clip_grads(grads, grad_clip, row_sq, true, "clip_global_norm");
 }
-Tensor global_norm_scale(const std::vector<Tensor>& grads, double grad_clip, const std::optional<Tensor>& row_sq) {
+Tensor global_norm_scale(const py::list& grads, double grad_clip, const std::optional<Tensor>& row_sq) {
   return clip_grads(grads, grad_clip, row_sq, false, "global_norm_scale");
 }
 
