@@ -145,10 +145,24 @@ __global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a
   const int j1 = min(blocks, ((int)blockIdx.y + 1) * per);
   const char* kb = a.k + group * a.kh + keys.first * a.kt;
   const char* vb = a.v + group * a.vh + keys.first * a.vt;
-  for (int j = blockIdx.y * per + wave; j < j1; j += kWaves) {
+  // the next block's keys and this one's values are under way while the products run
+  // (heads of 128 have registers for the values alone)
+  constexpr bool kAhead = HD <= 64;
+  auto fetch = [&](float4 (&x)[HD / 8], int j) __attribute__((always_inline)) {
+    load_operand<HD>(x, (const T*)(kb + min(32 * j + col, keys.len - 1) * a.kt), half);
+  };
+  float4 kv[HD / 8], ahead[HD / 8];
+  const int j0 = blockIdx.y * per + wave;
+  if (kAhead && j0 < j1) fetch(ahead, j0);
+  for (int j = j0; j < j1; j += kWaves) {
     const int k0 = 32 * j;
-    float4 kv[HD / 8];
-    load_operand<HD>(kv, (const T*)(kb + min(k0 + col, keys.len - 1) * a.kt), half);
+    if (kAhead) {
+#pragma unroll
+      for (int g = 0; g < HD / 8; ++g) kv[g] = ahead[g];
+      fetch(ahead, min(j + kWaves, j1 - 1));
+    } else {
+      fetch(kv, j);
+    }
     float v[16][DT];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -156,6 +170,7 @@ __global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a
 #pragma unroll
       for (int d = 0; d < DT; ++d) v[r][d] = (float)vrow[32 * d];
     }
+    __builtin_amdgcn_sched_barrier(0);
     f32x16 s = products<HD>(kv, q);
     if (k0 + 32 > least) {
 #pragma unroll
@@ -571,11 +586,24 @@ __global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, con
   const char* vb = a.v + group * a.vh + keys.first * a.vt;
   for (int j = wave; j < blocks; j += kWaves) {
     const int k0 = 32 * j, key = min(k0 + col, keys.len - 1);
-    float4 x[HD / 8];
+    // all of the block's loads are under way before its products (of heads of 128 the
+    // rows' alone: registers)
+    constexpr bool kAhead = HD <= 64;
+    float4 x[HD / 8], y[HD / 8];
+    float kc[kAhead ? 16 : 1][DT];
     load_operand<HD>(x, (const T*)(kb + key * a.kt), half);
+    if (kAhead) {
+      load_operand<HD>(y, (const T*)(vb + key * a.vt), half);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          kc[kAhead ? r : 0][d] = ((const T*)(kb + min(k0 + tile_row(r, half), keys.len - 1) * a.kt))[32 * d + col];
+      __builtin_amdgcn_sched_barrier(0);
+    }
     const f32x16 s = products<HD>(x, q);
-    load_operand<HD>(x, (const T*)(vb + key * a.vt), half);
-    f32x16 ds = products<HD>(x, go);
+    if (!kAhead) load_operand<HD>(y, (const T*)(vb + key * a.vt), half);
+    f32x16 ds = products<HD>(y, go);
     const bool masked = k0 + 32 > least;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -586,7 +614,8 @@ __global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, con
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float kx = (float)((const T*)(kb + min(k0 + tile_row(r, half), keys.len - 1) * a.kt))[32 * d + col];
+        const float kx = kAhead ? kc[kAhead ? r : 0][d]
+                                : ((const T*)(kb + min(k0 + tile_row(r, half), keys.len - 1) * a.kt))[32 * d + col];
         acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx, ds[r], acc[d], 0, 0, 0);
       }
   }
@@ -650,23 +679,48 @@ __global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, co
     }
     const int64_t st = (int64_t)group * a.T * a.R + (int64_t)first * a.R;
     const int row_from = max(k0 - behind, 0) * a.R, blocks = (rows + 31) >> 5;
+    const int row_min = max(k0 + col - behind, 0) * a.R;  // the first row that sees the lane's key
     for (int j = (row_from >> 5) + wave; j < blocks; j += kWaves) {
       const int r0 = 32 * j;
       float4 x[HD / 8];
       const int ri = min(r0 + col, rows - 1), tk = div_r(a, ri), h = group * a.R + ri - tk * a.R;
-      if (HD > 64) load_operand<HD>(k, krow, half);
+      // as in dq; the rows' lse2 and delta by two lanes a row, and from them by shuffles
+      constexpr bool kAhead = HD <= 64;
+      float4 y[HD / 8];
+      float qc[kAhead ? 16 : 1][DT], gc[kAhead ? 16 : 1][DT];
+      const float mine = (half ? g.delta : g.lse2)[st + ri];
       load_operand<HD>(x, row_at<T>(a.q, a.qt, a.qh, first + tk, h), half);
+      if (kAhead) {
+        load_operand<HD>(y, row_at<T>(g.g_out, g.gt, g.gh, first + tk, h), half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int at = min(r0 + tile_row(r, half), rows - 1), t = div_r(a, at), hh = group * a.R + at - t * a.R;
+          const T* qrow = row_at<T>(a.q, a.qt, a.qh, first + t, hh) + col;
+          const T* grow = row_at<T>(g.g_out, g.gt, g.gh, first + t, hh) + col;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            qc[kAhead ? r : 0][d] = qrow[32 * d];
+            gc[kAhead ? r : 0][d] = grow[32 * d];
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      } else {
+        load_operand<HD>(k, krow, half);
+      }
       f32x16 s = products<HD>(x, k);
-      if (HD > 64) load_operand<HD>(v, vrow, half);
-      load_operand<HD>(x, row_at<T>(g.g_out, g.gt, g.gh, first + tk, h), half);
-      f32x16 ds = products<HD>(x, v);
+      if (!kAhead) {
+        load_operand<HD>(v, vrow, half);
+        load_operand<HD>(y, row_at<T>(g.g_out, g.gt, g.gh, first + tk, h), half);
+      }
+      f32x16 ds = products<HD>(y, v);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int row = r0 + tile_row(r, half), at = min(row, rows - 1);
-        const bool off = row >= rows || k0 + col > div_r(a, at) + behind || k0 + col >= len;
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -g.lse2[st + at]));
+        const bool off = row >= rows || at < row_min || k0 + col >= len;
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -__shfl(mine, tile_row(r, half))));
+        const float e = __shfl(mine, 32 + tile_row(r, half));
         s[r] = off ? 0.f : p;
-        ds[r] = off ? 0.f : p * (ds[r] - g.delta[st + at]);
+        ds[r] = off ? 0.f : p * (ds[r] - e);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -675,8 +729,8 @@ __global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, co
         const T* grow = row_at<T>(g.g_out, g.gt, g.gh, first + t, hh) + col;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          ak[d] = __builtin_amdgcn_mfma_f32_32x32x2f32((float)qrow[32 * d], ds[r], ak[d], 0, 0, 0);
-          av[d] = __builtin_amdgcn_mfma_f32_32x32x2f32((float)grow[32 * d], s[r], av[d], 0, 0, 0);
+          ak[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(kAhead ? qc[kAhead ? r : 0][d] : qrow[32 * d], ds[r], ak[d], 0, 0, 0);
+          av[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(kAhead ? gc[kAhead ? r : 0][d] : grow[32 * d], s[r], av[d], 0, 0, 0);
         }
       }
     }
@@ -785,7 +839,7 @@ struct Sums {
 // to kExactKeys keys take delta = sum p dp - g_lse in a sweep of their own, which also
 // goes to memory for dk; with more keys out is an average and that error small,
 // and the sweep would cost two thirds of dq again.
-constexpr int kExactKeys = 512;
+constexpr int kExactKeys = 384;
 template <class T, int HD, bool WIDE>
 __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(const Packed a, const Grads g,
                                                                             T* __restrict__ dq) {
@@ -1035,10 +1089,12 @@ __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed
         v[i] = *(const short8v*)(vrow + 32 * i + 16 * half);
       }
     } else {
-      St::template load_rows<kKV / 1024 / W, W>(kv, wave, a.k + (int64_t)(seg.first + k0) * a.kt + group * a.kh,
-                                                (uint32_t)a.kt, len - 1 - k0);
-      St::template load_rows<kKV / 1024 / W, W>(kv + kKV, wave, a.v + (int64_t)(seg.first + k0) * a.vt + group * a.vh,
-                                                (uint32_t)a.vt, len - 1 - k0);
+      if (rw < 2) {  // two sets of waves bring them
+        St::template load_rows<kKV / 2048 / KW, 2 * KW>(kv, wave, a.k + (int64_t)(seg.first + k0) * a.kt + group * a.kh,
+                                                        (uint32_t)a.kt, len - 1 - k0);
+        St::template load_rows<kKV / 2048 / KW, 2 * KW>(
+            kv + kKV, wave, a.v + (int64_t)(seg.first + k0) * a.vt + group * a.vh, (uint32_t)a.vt, len - 1 - k0);
+      }
     }
     int turn = 0;
     for (int base = from; base < stages; base += RW, turn ^= 1) {
@@ -1272,7 +1328,7 @@ void backward(const Args* p, const void* g_out, int64_t gt, int64_t gh, const vo
       else packed_dq16_kernel<T, HD, false><<<tiles((int64_t)a.T * a.R, 32), kThreads, 0, s>>>(a, g, (T*)dq);
     }
     if (a.S && (dk || dv)) {
-      constexpr int KW = 4, RW = HD == 128 ? 2 : 1;
+      constexpr int KW = HD == 128 ? 2 : 4, RW = HD == 128 ? 3 : 1;
       if (wide_keys_of(p)) packed_dkv16_kernel<T, HD, KW, RW><<<tiles(a.S, 32 * KW), 64 * KW * RW, 0, s>>>(a, g, (T*)dk, (T*)dv);
       else packed_dkv16_kernel<T, HD, 1, 4><<<tiles(a.S, 32), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
     }
