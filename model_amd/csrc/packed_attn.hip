@@ -1255,25 +1255,49 @@ Packed device_args(const Args* p) {
   return a;
 }
 
-// Whether the 16-bit forward takes tiles of 128 rows: where they fill the chip.
+// Whether the 16-bit forward and dq take tiles of 128 rows: where there are enough of
+// them, more of narrower heads, whose tiles are less work.  us, tiles of 32 / of 128 rows
+// (bf16, forward; T tokens in n sequences, H heads over G):
+//   heads of 128:  T 2,048 n 4 H 8 G 8 (128 tiles): 17.2 / 16.8;  4,096, 8 (256): 29.5 / 19.4;
+//                  2,048, 1, 16 over 4 (256): 48.3 / 49.3;  16,384, 16, 16 over 4 (2,048): 267 / 109
+//   of 64:         4,096, 8, 8, 8 (256): 15.2 / 14.2;  2,048, 1, 16 over 4 (256): 23.1 / 35.7;
+//                  8,192, 8, 8, 8 (512): 31.9 / 29.0;  4,096, 16, 16 over 4 (512): 22.3 / 13.3
+//   of 32:         8,192, 8, 8, 8 (512): 19.3 / 24.5;  8,192, 16, 16 over 4 (1,024): 22.9 / 17.3
 bool wide_of(const Args* p) {
   const int64_t r = p->heads / p->groups;
-  return p->dtype != MPL_F32 && p->tokens * r / kWideRows * p->groups >= 256;
+  return p->dtype != MPL_F32 && p->tokens * r / kWideRows * p->groups >= 256 * (128 / p->head_dim);
 }
 
-// Whether dk and dv in 16 bits take tiles of 128 keys.
-bool wide_keys_of(const Args* p) { return p->keys / 128 * p->groups >= 256; }
+// Whether dk and dv in 16 bits take tiles of more keys, which read the rows less often.
+// us of the backward pass, tiles of 32 keys / of 64 (heads of 128) or 128:
+//   heads of 128:  2,048, 4, 8, 8 (128 tiles of 128): 53.8 / 44.7;  4,096, 16, 16 over 4 (128): 124 / 112;
+//                  2,048, 1, 16 over 4 (64): 189 / 206
+//   of 64:         4,096, 8, 8, 8 (256): 44.2 / 44.6;  8,192, 8, 8, 8 (512): 89.0 / 80.1;
+//                  8,192, 64, 32 over 8 (512): 96.8 / 106;  dk and dv of 16,384, 1, 16, 16 (2,048): 1,353 / 1,129
+//   of 32:         8,192, 8, 8, 8 (512): 51.3 / 54.4;  16,384, 16, 16 over 4 (512): 140 / 165
+bool wide_keys_of(const Args* p) {
+  const int64_t tiles = p->keys / 128 * p->groups;
+  return tiles >= (p->head_dim == 128 ? 128 : 1024);
+}
 
 // Parts of the keys: where the tiles of rows do not fill the chip and the keys of
-// a sequence are many.  Only sums over the sequences are known here.
+// a sequence are many.  Only sums over the sequences are known here.  A part is worth
+// its share of the join's launch and memory from some keys on; fp32's products take
+// longer, and want more workgroups.  us by number of parts, single tokens of B streams
+// over `cap` keys each:
+//   fp32, B 1, cap 2,048, 4 heads of 64:      1: 43.4   4: 18.5   8: 14.6   16: 14.6   32: 19.4
+//   fp32, 16, 4,096, 32 over 8 of 128:        1: 221    2: 128    4: 132    8: 140     16: 160
+//   bf16, 1, 512, 4 of 64:                    1: 8.2    2: 11.1   4: 10.6
+//   bf16, 1, 8,192, 4 of 64:                  1: 42.0   4: 16.4   8: 13.3   16: 13.8   32: 18.1
+//   bf16, 1, 32,768, 32 over 8 of 128:        1: 215    8: 38.1   16: 33.9  32: 47.6   64: 64.8
+//   bf16, 16, 4,096, 32 over 8 of 128:        1: 43.7   2: 46.1   4: 48.0   8: 53.0
 int splits_of(const Args* p) {
+  const bool f32 = p->dtype == MPL_F32;
   const int64_t r = p->heads / p->groups, n = p->sequences ? p->sequences : 1;
   const int64_t tiles = (p->tokens * r / 32 + (p->tokens < n ? p->tokens : n)) * p->groups;
-  const int64_t per = p->keys / n;  // keys of a sequence
-  if (tiles <= 0 || tiles >= 1024 || per < 512) return 1;
-  const int64_t want = 1024 / tiles, most = per / 256;
+  const int64_t want = tiles ? (f32 ? 512 : 128) / tiles : 1, most = p->keys / n / (f32 ? 256 : 512);
   const int64_t s = want < most ? want : most;
-  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+  return s < 1 ? 1 : s > 16 ? 16 : (int)s;
 }
 
 size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
