@@ -57,16 +57,18 @@ struct Segment {
 template <int LOG>
 __device__ __forceinline__ Segment segment_of(const void* starts, int wide, int n, int total, int per, int b) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, len = n + 2;
-  while (len > 1) {
+  int lo = 0, len = n + 2, first, end;
+  do {
     const int step = (len + 63) >> 6, i = lo + lane * step;
-    const bool in = lane * step < len;
-    const int64_t at = ((int64_t)segment_start(starts, wide, n, total, in ? i : lo) * per >> LOG) + i;
-    const int before = 63 - __clzll((long long)(__ballot(in && at <= b) | 1));
+    const int begins = segment_start(starts, wide, n, total, i);
+    const int64_t at = ((int64_t)begins * per >> LOG) + i;
+    const int before = 63 - __clzll((long long)(__ballot(lane * step < len && at <= b) | 1));
     lo += before * step;
     len = min(step, len - before * step);
-  }
-  const int first = segment_start(starts, wide, n, total, lo), end = segment_start(starts, wide, n, total, lo + 1);
+    // a step of neighbouring segments: the lanes hold where they begin
+    first = __shfl(begins, before);
+    end = step == 1 && before < 63 ? __shfl(begins, before + 1) : segment_start(starts, wide, n, total, lo + 1);
+  } while (len > 1);
   Segment s;
   s.seq = __builtin_amdgcn_readfirstlane(lo - 1);
   s.first = __builtin_amdgcn_readfirstlane(first);
