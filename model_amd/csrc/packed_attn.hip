@@ -7,11 +7,25 @@
 //   delta = g_out . out - g_lse,  p = exp(z - lse),  dz = p (g_out . v - delta),
 //   dq = scale sum_s dz k_s,  dk = scale sum_rows dz q,  dv = sum_rows p g_out.
 //
-// Kernels on fp32 products (v_mfma_f32_32x32x2_f32).  A tile of scores is formed
-// transposed or not so that the lane holds one column of it and its registers are
-// directly an operand of the next product; the operands come from L2.  The four
-// waves of a workgroup take every fourth block along the contraction (keys, or
-// rows in dk and dv) and join in LDS, in a fixed order.
+// A tile of scores is formed transposed or not so that a lane holds one column of it
+// and its registers are directly an operand of the next product: no score goes through
+// LDS or memory.  fp32 runs on v_mfma_f32_32x32x2_f32 with operands from the caches,
+// 16 bits on the 32x32x16 products with operands staged in LDS (packed_attn16.h).  The
+// backward pass forms the scores twice, for dq by rows and for dk and dv by keys: seven
+// products instead of five, and no atomics.
+//
+// Measured (MI355X; a large bf16 product makes 1,247 TFLOP/s, an fp32 one 154), us:
+//   forward, one prompt of 16,384, 16 heads over 4 of 128, bf16      1,128   975 TFLOP/s
+//     the same of 16 heads of 64                                       670   820
+//   backward of the latter: delta 19, dq 803 (1,027), dk and dv 1,102 (998 of its four products)
+//   24 documents, 16,384 tokens, 16 heads over 4 of 128, bf16: forward 150, delta 36, dq 191,
+//     dk and dv 334: the longest document's first tiles are most of the time
+//   40 documents, 8,192 tokens, 4 heads of 64, fp32: forward 59, delta 5, dq 85, dk and dv 128
+//   64 single tokens over caches of up to 8,192, 32 heads over 8 of 128, bf16: 266, 5.2 TB/s
+// Bound: the matrix units of large 16-bit calls (half of their cycles; the vector units
+// 60 to 85 % of theirs: exponentials and conversions), memory for single tokens, for
+// short sequences the chain of loads that each workgroup begins with.  fp32's short
+// sequences spend most of their time between a block's loads and its products.
 #include <math.h>
 
 #include <type_traits>
@@ -277,12 +291,14 @@ struct Softmax {
   }
 };
 
-// Many rows: 128 a workgroup, 32 a wave, 64 keys a stage that all four waves read.
+// Many rows: 128 a workgroup, 32 a wave, 64 keys a stage that all four waves read.  Two
+// waves a SIMD of heads of 128 (225 registers, 80 KB of LDS a workgroup).
 //
 // The scores of the next 32 keys are formed while the softmax of these 32 runs: the
 // products need the matrix unit and the softmax the vector unit, and a wave that
-// alternated them would leave one or the other idle.  So keys run half a stage ahead
-// of values, and values have one stage more.
+// alternated them would leave one or the other idle (one prompt of 16,384: 1,164 us
+// without this, 1,110 with).  So keys run half a stage ahead of values, and values have
+// one stage more.
 constexpr int kWideRows = 128, kWideKeys = 64;
 template <class T, int HD>
 __global__ __launch_bounds__(kThreads, 2) void packed_forward16_kernel(const Packed a, T* __restrict__ out,
@@ -385,7 +401,8 @@ __global__ __launch_bounds__(kThreads, 2) void packed_forward16_kernel(const Pac
   if (lse && half == 0) lse[at] = (sm.m - kLift<T> + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Few rows: 32 a workgroup; every wave has keys, and stages of 32 of them, of its own.
+// Few rows: 32 a workgroup; every wave has keys, and stages of 32 of them, of its own,
+// two under way: with single tokens over a cache 64 KB a CU (heads of 128).
 template <class T, int HD>
 __global__ __launch_bounds__(kThreads) void packed_forward16_few_kernel(const Packed a, int splits, T* __restrict__ out,
                                                                         float* __restrict__ lse, float* __restrict__ part,
@@ -729,8 +746,9 @@ __global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, co
         const T* grow = row_at<T>(g.g_out, g.gt, g.gh, first + t, hh) + col;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          ak[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(kAhead ? qc[kAhead ? r : 0][d] : qrow[32 * d], ds[r], ak[d], 0, 0, 0);
-          av[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(kAhead ? gc[kAhead ? r : 0][d] : grow[32 * d], s[r], av[d], 0, 0, 0);
+          const float qx = kAhead ? qc[kAhead ? r : 0][d] : qrow[32 * d], gx = kAhead ? gc[kAhead ? r : 0][d] : grow[32 * d];
+          ak[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(qx, ds[r], ak[d], 0, 0, 0);
+          av[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(gx, s[r], av[d], 0, 0, 0);
         }
       }
     }
@@ -990,13 +1008,17 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
 
 // dk and dv.  A workgroup of KW x RW waves has 32 KW keys, 32 a wave, and its rows in
 // stages (8 KB of q and of g_out, or 32 rows) that RW sets of KW waves take in turn, each set
-// with stages of its own, and join at the end.
+// with stages of its own, and join at the end.  For heads of 128 KW 2 and RW 3: KW 4 and
+// RW 2 halve the reads of rows and take 356 us where this takes 323 (24 documents), for
+// the first keys of a long document with the heads that share them are the longest way
+// through.  Of narrower heads KW 4 and RW 1 (1,129 us; KW 4, RW 2 1,414; KW 2, RW 4 1,525).
 template <class T, int HD, int KW, int RW>
 __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed a, const Grads g, T* __restrict__ dk,
                                                                    T* __restrict__ dv) {
   typedef Stage<HD> St;
   constexpr int kKeys = 32 * KW, W = KW * RW;
-  constexpr int kBytes = KW == 1 ? 32 * St::kRow : 8192, kLoads = kBytes / 1024, kRows = kBytes / St::kRow, NB = kRows / 32;
+  constexpr int kBytes = KW == 1 ? 32 * St::kRow : 8192, kLoads = kBytes / 1024;
+  constexpr int kRows = kBytes / St::kRow, NB = kRows / 32;
   // heads of 128 leave no registers for the wave's keys and values as operands: they
   // lie in LDS, behind the stages
   constexpr bool kHeld = HD < 128 || KW == 1;
@@ -1044,7 +1066,8 @@ __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed
       g_at[i] = tk * (uint32_t)g.gt + h * (uint32_t)g.gh;
     }
     auto send = [&](int it, char* to) __attribute__((always_inline)) {
-      // a stage is whole tokens where R divides 32: a lane's rows lie alike in every one.  Else, and in the last stage, each row's token is looked for.
+      // a stage is whole tokens where R divides 32: a lane's rows lie alike in every
+      // one.  Else, and in the last stage, each row's token is looked for.
       constexpr int N = kLoads / KW;
       const bool alike = (a.R & (a.R - 1)) == 0 && a.R <= 32 && kRows * (it + 1) <= rows;
       const int t0 = div_r(a, kRows * it);

@@ -16,7 +16,8 @@
 // 16-byte piece p of row r lies at p ^ f(r).  f spreads the pieces that 16 lanes read
 // of 16 neighbouring rows over all 64 banks, and the 64 bytes each that 32 lanes read
 // transposed of 4 rows as well.  (With 8 and 16 lanes and half the banks, as 128 bytes
-// a cycle would have it, every read took twice its cycles.)
+// a cycle would have it, every read took twice its cycles: SQ_LDS_BANK_CONFLICT half of
+// SQ_LDS_IDX_ACTIVE, now 0.)
 #pragma once
 
 #include "mfma.h"
