@@ -811,8 +811,9 @@ int mpl_vocab_cross_entropy_bwd(const void* hidden, int64_t hidden_pitch, const 
  * (model.py:88-95 for documents of a batch, prompts, and single tokens over a
  * cache).  q [tokens, heads, head_dim], k and v [keys, groups, head_dim] of dtype
  * MPL_F32, MPL_F16 or MPL_BF16, head_dim 32, 64 or 128 elements next to each other,
- * tokens and heads at the given strides in elements (0 to 2^23, 16-byte aligned
- * rows, and heads / groups heads within 2^28; else MPL_EUNSUPPORTED).
+ * tokens and heads at the given strides in elements (>= 0, 16-byte aligned rows;
+ * tokens at most 2^23 apart, q's heads too, and heads / groups of them within 2^28:
+ * else MPL_EUNSUPPORTED).
  * Head h reads key head h / (heads / groups).
  *
  * starts [sequences + 1] ascends in [0, tokens]: sequence i has the queries from

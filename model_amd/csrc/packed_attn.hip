@@ -1231,7 +1231,8 @@ int check_sizes(const Args* p, const char* what) {
 }
 
 constexpr int64_t kMostStride = 1 << 23;  // elements
-int check_rows(const Args* p, const void* x, int64_t tok, int64_t head, const char* name, const char* what) {
+// `shared`: of k and v, whose heads lie where they like.
+int check_rows(const Args* p, const void* x, int64_t tok, int64_t head, bool shared, const char* name, const char* what) {
   const int64_t unit = 16 / element_size(p->dtype);
   MPL_REQUIRE(x, MPL_EINVAL, "%s: null %s", what, name);
   MPL_REQUIRE(((uintptr_t)x & 15) == 0 && tok >= 0 && head >= 0 && tok % unit == 0 && head % unit == 0, MPL_EINVAL,
@@ -1239,8 +1240,9 @@ int check_rows(const Args* p, const void* x, int64_t tok, int64_t head, const ch
               (long long)head);
   // places within a stage of rows are 32-bit: up to 63 tokens and a token's heads
   const int64_t r = p->heads / p->groups;
-  MPL_REQUIRE(tok <= kMostStride && head <= kMostStride && head * (r < 32 ? 32 : r) <= 32 * kMostStride, MPL_EUNSUPPORTED,
-              "%s: the rows of %s lie too far apart (token %lld, head %lld)", what, name, (long long)tok, (long long)head);
+  MPL_REQUIRE(tok <= kMostStride && (shared || (head <= kMostStride && head * (r < 32 ? 32 : r) <= 32 * kMostStride)),
+              MPL_EUNSUPPORTED, "%s: the rows of %s lie too far apart (token %lld, head %lld)", what, name,
+              (long long)tok, (long long)head);
   return MPL_OK;
 }
 
@@ -1251,10 +1253,10 @@ int check_inputs(const Args* p, const char* what) {
   MPL_REQUIRE((((uintptr_t)p->starts | (uintptr_t)p->key_starts | (uintptr_t)p->key_lengths) & (p->index_bytes - 1)) == 0,
               MPL_EINVAL, "%s: starts must be aligned", what);
   if (p->tokens)
-    if (int rc = check_rows(p, p->q, p->q_token, p->q_head, "q", what)) return rc;
+    if (int rc = check_rows(p, p->q, p->q_token, p->q_head, false, "q", what)) return rc;
   if (p->keys) {
-    if (int rc = check_rows(p, p->k, p->k_token, p->k_head, "k", what)) return rc;
-    if (int rc = check_rows(p, p->v, p->v_token, p->v_head, "v", what)) return rc;
+    if (int rc = check_rows(p, p->k, p->k_token, p->k_head, true, "k", what)) return rc;
+    if (int rc = check_rows(p, p->v, p->v_token, p->v_head, true, "v", what)) return rc;
   }
   return MPL_OK;
 }
@@ -1435,7 +1437,7 @@ extern "C" int mpl_packed_attention_bwd(const mpl_packed_attention_args* args, c
   MPL_REQUIRE((((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0, MPL_EINVAL,
               "mpl_packed_attention_bwd: gradients must be 16-byte aligned");
   if (args->tokens) {
-    if (int rc = check_rows(args, g_out, g_token, g_head, "g_out", "mpl_packed_attention_bwd")) return rc;
+    if (int rc = check_rows(args, g_out, g_token, g_head, false, "g_out", "mpl_packed_attention_bwd")) return rc;
     MPL_REQUIRE(out && ((uintptr_t)out & 15) == 0 && lse, MPL_EINVAL,
                 "mpl_packed_attention_bwd: out (16-byte aligned) and lse are needed");
     const size_t need = workspace_bytes(args, true);

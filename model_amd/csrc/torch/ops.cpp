@@ -365,7 +365,7 @@ struct Heads {
   Tensor t;
   int64_t token = 0, head = 0;
 };
-Heads heads_of(const Tensor& x) {
+Heads heads_of(const Tensor& x, bool shared = false) {  // shared: k and v
   Tensor t = x._is_zerotensor() ? dense(x) : x.resolve_neg();
   const int64_t unit = 16 / t.element_size();
   constexpr int64_t kFar = 1 << 23;
@@ -373,7 +373,8 @@ Heads heads_of(const Tensor& x) {
     return y.numel() == 0 ||
            (y.stride(2) == 1 && (uintptr_t)y.data_ptr() % 16 == 0 &&
             (y.size(0) == 1 || (y.stride(0) % unit == 0 && y.stride(0) <= kFar)) &&
-            (y.size(1) == 1 || (y.stride(1) % unit == 0 && y.stride(1) * std::max<int64_t>(32, y.size(1)) <= 32 * kFar)));
+            (y.size(1) == 1 || (y.stride(1) % unit == 0 &&
+                                (shared || y.stride(1) * std::max<int64_t>(32, y.size(1)) <= 32 * kFar))));
   };
   if (!lies(t)) t = t.clone(at::MemoryFormat::Contiguous);
   if (t.numel() == 0) return {t, 0, 0};
@@ -387,7 +388,7 @@ struct PackedCall {
   Tensor starts, key_starts, key_lengths;
   PackedCall(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& starts_, const Tensor& key_starts_,
              const Tensor& key_lengths_, double scale)
-      : q(heads_of(q_)), k(heads_of(k_)), v(heads_of(v_)), starts(dense(starts_)), key_starts(dense(key_starts_)),
+      : q(heads_of(q_)), k(heads_of(k_, true)), v(heads_of(v_, true)), starts(dense(starts_)), key_starts(dense(key_starts_)),
         key_lengths(dense(key_lengths_)) {
     a.q = ptr(q.t); a.k = ptr(k.t); a.v = ptr(v.t);
     a.q_token = q.token; a.q_head = q.head;

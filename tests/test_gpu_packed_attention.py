@@ -451,3 +451,61 @@ def test_many_rows_not_finite_stays_in_its_sequence(dtype):
     q[1505], k[1700], v[2100], g[2199] = math.nan, math.inf, math.nan, -math.inf
     for a, b in zip(want, all_of()):
         assert torch.equal(a[:1500], b[:1500]) and torch.equal(a[2200:], b[2200:])
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_many_rows_with_starts_that_make_no_sense(dtype):
+    """As test_starts_that_make_no_sense, at sizes that take the large calls' tiles."""
+    T = 9000
+    q, k, v, g, _ = make([T], [T], 16, 16, 64, dtype, seed=18)
+    rng = random.Random(5)
+    for n in (3, 100):
+        starts = torch.tensor([rng.randint(-T, 2 * T) for _ in range(n)], dtype=torch.int64, device=DEV)
+        for kw in ({}, {"key_starts": starts.flip(0), "key_lengths": starts[1:] * 3}):
+            out, lse = packed_attention_forward(q, k, v, starts, **kw)
+            packed_attention_backward(g, q, k, v, out, lse, starts, **kw)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_heads_that_lie_far_apart(dtype):
+    """A cache with its heads outermost is read where it lies; q's heads as far apart are copied."""
+    used, cap, G, hd = [70, 3], 1 << 18, 3, 64
+    cache = torch.zeros((2, G, cap, hd), dtype=dtype, device=DEV)  # heads 2^24 elements apart
+    g = torch.Generator(device=DEV).manual_seed(19)
+    cache[:, :, :200] = torch.randn((2, G, 200, hd), generator=g, device=DEV).to(dtype)
+    k, v = (c.permute(1, 0, 2)[:200] for c in cache)
+    q = torch.zeros((6, 1 << 19, hd), dtype=dtype, device=DEV)[:, :2].permute(1, 0, 2)
+    q.copy_(torch.randn((2, 6, hd), generator=g, device=DEV))
+    begin = [0, 100, 200]
+    run_all(q, k, v, [1, 1], used, torch.ones_like(q), own_keys=True, key_lengths=used, begin=begin)
+
+
+def test_two_graphs_at_once():
+    sets, graphs = [], []
+    for i in range(2):
+        lq = [40 + i, 1, 300]
+        q, k, v, g, gl = make(lq, lq, 4, 2, 64, torch.float16, seed=20 + i)
+        starts = torch.tensor(sums(lq), dtype=torch.int32, device=DEV)
+
+        def call(q=q, k=k, v=v, g=g, gl=gl, starts=starts):
+            out, lse = packed_attention_forward(q, k, v, starts)
+            return (out, lse, *packed_attention_backward(g, q, k, v, out, lse, starts, g_lse=gl))
+
+        want = call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = call()
+        sets.append((want, got))
+        graphs.append((graph, call))  # the graph reads the inputs where they were: the call keeps them
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for (graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for want, got in sets:
+            for a, b in zip(want, got):
+                assert torch.equal(a, b)
+                b.zero_()
