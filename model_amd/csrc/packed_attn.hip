@@ -857,7 +857,7 @@ struct Sums {
 // to kExactKeys keys take delta = sum p dp - g_lse in a sweep of their own, which also
 // goes to memory for dk; with more keys out is an average and that error small,
 // and the sweep would cost two thirds of dq again.
-constexpr int kExactKeys = 384;
+constexpr int kExactKeys = 512;
 template <class T, int HD, bool WIDE>
 __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(const Packed a, const Grads g,
                                                                             T* __restrict__ dq) {
