@@ -9,8 +9,8 @@
 //
 // A tile of scores is formed transposed or not so that a lane holds one column of it
 // and its registers are directly an operand of the next product: no score goes through
-// LDS or memory.  fp32 runs on v_mfma_f32_32x32x2_f32 with operands from the caches,
-// 16 bits on the 32x32x16 products with operands staged in LDS (packed_attn16.h).  The
+// LDS or memory.  fp32 runs on v_mfma_f32_32x32x2_f32, 16 bits on the 32x32x16
+// products, both with operands staged in LDS (packed_attn16.h).  The
 // backward pass forms the scores twice, for dq by rows and for dk and dv by keys: seven
 // products instead of five, and no atomics.
 //
@@ -47,23 +47,43 @@ __device__ __forceinline__ void load_operand(float4 (&x)[HD / 8], const T* row, 
   for (int g = 0; g < HD / 8; ++g) x[g] = load4(row + 8 * g + 4 * half);
 }
 
-// c += A . B over HD, both operands one row a lane.
-template <int HD>
-__device__ __forceinline__ f32x16 products(const float4 (&x)[HD / 8], const float4 (&y)[HD / 8]) {
-  f32x16 s = f32x16{};
-#pragma unroll
-  for (int g = 0; g < HD / 8; ++g) {
-    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[g].x, y[g].x, s, 0, 0, 0);
-    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[g].y, y[g].y, s, 0, 0, 0);
-    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[g].z, y[g].z, s, 0, 0, 0);
-    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[g].w, y[g].w, s, 0, 0, 0);
-  }
-  return s;
-}
-
 template <class T>
 __device__ __forceinline__ const T* row_at(const char* base, int64_t tok, int64_t head, int t, int h) {
   return (const T*)(base + t * tok + h * head);
+}
+
+// A wave's stage of 32 fp32 rows in LDS, by DMA: from the caches straight, a lane's own
+// row costs a line a lane and a scalar load an element of a column (40 documents of
+// 8,192 tokens, 4 heads of 64, with gradients: 264 us so, 191 with the stages).
+template <int HD>
+struct Stage32 : Stage<2 * HD> {
+  typedef Stage<2 * HD> Base;
+  static constexpr int kBytes = 128 * HD, kLoads = kBytes / 1024;
+  // The operand of the lane's row: elements 8 g + 4 (lane / 32) + [0, 4).
+  __device__ __forceinline__ float4 operand(const char* lds, int g) const {
+    return __builtin_bit_cast(float4, this->rows(lds, 0, g));
+  }
+  // Element 32 d + lane % 32 of row tile_row(r, lane / 32).
+  __device__ __forceinline__ float column(const char* lds, int r, int d) const {
+    const int lane = threadIdx.x & 63, half = lane >> 5, row = tile_row(r, half);
+    const int piece = (8 * d + (lane >> 2 & 7)) ^ Base::f(row);
+    return *(const float*)(lds + row * Base::kRow + piece * 16 + (lane & 3) * 4);
+  }
+};
+
+// One operand of a product in registers, the other a stage.
+template <int HD>
+__device__ __forceinline__ f32x16 staged_products(const Stage32<HD>& st, const char* lds, const float4 (&y)[HD / 8]) {
+  f32x16 s = f32x16{};
+#pragma unroll
+  for (int g = 0; g < HD / 8; ++g) {
+    const float4 x = st.operand(lds, g);
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y[g].x, s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y[g].y, s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y[g].z, s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y[g].w, s, 0, 0, 0);
+  }
+  return s;
 }
 
 // The waves' results of 32 rows in LDS: sums of weighted values, the maximum (base 2)
@@ -133,7 +153,8 @@ __global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a
                                                                   float2* __restrict__ stats) {
   typedef float T;
   constexpr int DT = HD / 32;
-  __shared__ Join<HD> join;
+  constexpr int kStages = 2 * Stage32<HD>::kBytes * kWaves, kJoin = sizeof(Join<HD>);
+  __shared__ __attribute__((aligned(1024))) char lds[kStages > kJoin ? kStages : kJoin];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -159,33 +180,29 @@ __global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a
   const int j1 = min(blocks, ((int)blockIdx.y + 1) * per);
   const char* kb = a.k + group * a.kh + keys.first * a.kt;
   const char* vb = a.v + group * a.vh + keys.first * a.vt;
-  // the next block's keys and this one's values are under way while the products run
-  // (heads of 128 have registers for the values alone)
-  constexpr bool kAhead = HD <= 64;
-  auto fetch = [&](float4 (&x)[HD / 8], int j) __attribute__((always_inline)) {
-    load_operand<HD>(x, (const T*)(kb + min(32 * j + col, keys.len - 1) * a.kt), half);
+  // keys and values of a block arrive in the wave's own stages, the next block's keys
+  // once this one's scores are formed, its values behind its last product
+  typedef Stage32<HD> St;
+  const St st;
+  char* ks = lds + 2 * St::kBytes * wave;
+  char* vs = ks + St::kBytes;
+  auto send = [&](const char* base, int64_t pitch, int j, char* to) __attribute__((always_inline)) {
+    St::template load_rows<St::kLoads, 1>(to, 0, base + 32 * j * pitch, (uint32_t)pitch, keys.len - 1 - 32 * j);
   };
-  float4 kv[HD / 8], ahead[HD / 8];
   const int j0 = blockIdx.y * per + wave;
-  if (kAhead && j0 < j1) fetch(ahead, j0);
+  wait_vmcnt_le<0>();  // q: the compiler does not count the stages' loads
+  if (j0 < j1) {
+    send(kb, a.kt, j0, ks);
+    send(vb, a.vt, j0, vs);
+  }
   for (int j = j0; j < j1; j += kWaves) {
     const int k0 = 32 * j;
-    if (kAhead) {
-#pragma unroll
-      for (int g = 0; g < HD / 8; ++g) kv[g] = ahead[g];
-      fetch(ahead, min(j + kWaves, j1 - 1));
-    } else {
-      fetch(kv, j);
-    }
-    float v[16][DT];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const T* vrow = (const T*)(vb + min(k0 + tile_row(r, half), keys.len - 1) * a.vt) + col;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) v[r][d] = (float)vrow[32 * d];
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    f32x16 s = products<HD>(kv, q);
+    const bool more = j + kWaves < j1;
+    wait_vmcnt_le<St::kLoads>();
+    asm volatile("" ::: "memory");
+    f32x16 s = staged_products<HD>(st, ks, q);
+    reads_done();
+    if (more) send(kb, a.kt, j + kWaves, ks);
     if (k0 + 32 > least) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -207,14 +224,22 @@ __global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a
       sum += p[r];
     }
     l = l * alpha + sum;
+    if (more) wait_vmcnt_le<St::kLoads>();
+    else wait_vmcnt_le<0>();
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[r][d], p[r], acc[d], 0, 0, 0);
+      for (int r = 0; r < 16; ++r) acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(st.column(vs, r, d), p[r], acc[d], 0, 0, 0);
     }
+    reads_done();
+    if (more) send(vb, a.vt, j + kWaves, vs);
   }
+  reads_done();
+  __syncthreads();  // the stages become the waves' results
+  Join<HD>& join = *(Join<HD>*)lds;
 
   join.put(wave, col, half, m, l, acc);
   __syncthreads();
@@ -569,12 +594,43 @@ __global__ __launch_bounds__(256) void packed_delta_kernel(const Packed a, const
   }
 }
 
+// The sums of N sets of RW waves, 32 rows each, joined in LDS and written.
+template <int HD, int N, int RW>
+struct Sums {
+  float so[N][RW][32][HD + 4];
+  __device__ __forceinline__ void put(int n, int rw, int col, int half, const f32x16 (&acc)[HD / 32], float f) {
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *(float4*)&so[n][rw][col][32 * d + tile_row(r, half)] =
+            make_float4(acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f);
+  }
+  // `place(t)`: where row t goes, null for nowhere.
+  template <class F>
+  __device__ __forceinline__ void write(F&& place) const {
+    for (int i = threadIdx.x; i < N * 32 * HD / 4; i += 64 * N * RW) {
+      const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
+      auto* to = place(t);
+      if (!to) continue;
+      float4 x = *(const float4*)&so[t >> 5][0][t & 31][d];
+#pragma unroll
+      for (int w = 1; w < RW; ++w) {
+        const float4 y = *(const float4*)&so[t >> 5][w][t & 31][d];
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+      store4(to + d, x);
+    }
+  }
+};
+
 // dq: 32 rows a workgroup, tiles of scores transposed (the lane's column a row).
 template <int HD>
 __global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, const Grads g, float* __restrict__ dq) {
   typedef float T;
-  constexpr int DT = HD / 32, PO = HD + 4;
-  __shared__ float so[kWaves][32][PO];
+  constexpr int DT = HD / 32;
+  constexpr int kStages = 2 * Stage32<HD>::kBytes * kWaves, kJoin = sizeof(Sums<HD, 1, kWaves>);
+  __shared__ __attribute__((aligned(1024))) char lds[kStages > kJoin ? kStages : kJoin];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -601,26 +657,34 @@ __global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, con
   const int blocks = most > 0 ? (most + 31) >> 5 : 0;
   const char* kb = a.k + group * a.kh + keys.first * a.kt;
   const char* vb = a.v + group * a.vh + keys.first * a.vt;
+  // as in the forward pass: values first, whose stage is free again after one product
+  typedef Stage32<HD> St;
+  const St stage;
+  char* ks = lds + 2 * St::kBytes * wave;
+  char* vs = ks + St::kBytes;
+  auto send = [&](const char* base, int64_t pitch, int j, char* to) __attribute__((always_inline)) {
+    St::template load_rows<St::kLoads, 1>(to, 0, base + 32 * j * pitch, (uint32_t)pitch, keys.len - 1 - 32 * j);
+  };
+  wait_vmcnt_le<0>();  // the rows: the compiler does not count the stages' loads
+  if (wave < blocks) {
+    send(vb, a.vt, wave, vs);
+    send(kb, a.kt, wave, ks);
+  }
   for (int j = wave; j < blocks; j += kWaves) {
-    const int k0 = 32 * j, key = min(k0 + col, keys.len - 1);
-    // all of the block's loads are under way before its products (of heads of 128 the
-    // rows' alone: registers)
-    constexpr bool kAhead = HD <= 64;
-    float4 x[HD / 8], y[HD / 8];
-    float kc[kAhead ? 16 : 1][DT];
-    load_operand<HD>(x, (const T*)(kb + key * a.kt), half);
-    if (kAhead) {
-      load_operand<HD>(y, (const T*)(vb + key * a.vt), half);
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          kc[kAhead ? r : 0][d] = ((const T*)(kb + min(k0 + tile_row(r, half), keys.len - 1) * a.kt))[32 * d + col];
-      __builtin_amdgcn_sched_barrier(0);
+    const int k0 = 32 * j;
+    const bool more = j + kWaves < blocks;
+    wait_vmcnt_le<St::kLoads>();
+    asm volatile("" ::: "memory");
+    f32x16 ds = staged_products<HD>(stage, vs, go);
+    reads_done();
+    if (more) {
+      send(vb, a.vt, j + kWaves, vs);
+      wait_vmcnt_le<St::kLoads>();
+    } else {
+      wait_vmcnt_le<0>();
     }
-    const f32x16 s = products<HD>(x, q);
-    if (!kAhead) load_operand<HD>(y, (const T*)(vb + key * a.vt), half);
-    f32x16 ds = products<HD>(y, go);
+    asm volatile("" ::: "memory");
+    const f32x16 s = staged_products<HD>(stage, ks, q);
     const bool masked = k0 + 32 > least;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -631,40 +695,31 @@ __global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, con
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float kx = kAhead ? kc[kAhead ? r : 0][d]
-                                : ((const T*)(kb + min(k0 + tile_row(r, half), keys.len - 1) * a.kt))[32 * d + col];
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx, ds[r], acc[d], 0, 0, 0);
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(stage.column(ks, r, d), ds[r], acc[d], 0, 0, 0);
       }
+    reads_done();
+    if (more) send(kb, a.kt, j + kWaves, ks);
   }
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      *(float4*)&so[wave][col][32 * d + tile_row(r, half)] =
-          make_float4(acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]);
+  reads_done();
+  __syncthreads();  // the stages become the waves' sums
+  Sums<HD, 1, kWaves>& sums = *(Sums<HD, 1, kWaves>*)lds;
+  sums.put(0, wave, col, half, acc, g.scale);
   __syncthreads();
-  for (int i = tid; i < 32 * HD / 4; i += kThreads) {
-    const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
-    if (row0 + t >= rows) continue;
-    float4 x = *(const float4*)&so[0][t][d];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-      const float4 y = *(const float4*)&so[w][t][d];
-      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-    }
+  sums.write([&](int t) -> T* {
+    if (row0 + t >= rows) return nullptr;
     const int tk = div_r(a, row0 + t);
-    const int64_t at = (int64_t)(seg.first + tk) * a.H + group * a.R + row0 + t - tk * a.R;
-    store4(dq + at * HD + d, make_float4(x.x * g.scale, x.y * g.scale, x.z * g.scale, x.w * g.scale));
-  }
+    return dq + ((int64_t)(seg.first + tk) * a.H + group * a.R + row0 + t - tk * a.R) * HD;
+  });
 }
 
 // dk and dv: 32 keys a workgroup, the lane's column a key, rows in the registers.
 template <int HD>
-__global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, const Grads g, float* __restrict__ dk,
+__global__ __launch_bounds__(kThreads, HD <= 64 ? 2 : 1) void packed_dkv_kernel(const Packed a, const Grads g, float* __restrict__ dk,
                                                               float* __restrict__ dv) {
   typedef float T;
-  constexpr int DT = HD / 32, PO = HD + 4;
-  __shared__ float so[kWaves][32][PO];
+  constexpr int DT = HD / 32;
+  constexpr int kStages = 2 * Stage32<HD>::kBytes * kWaves, kJoin = sizeof(Sums<HD, 1, kWaves>);
+  __shared__ __attribute__((aligned(1024))) char lds[kStages > kJoin ? kStages : kJoin];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -690,46 +745,48 @@ __global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, co
     const T* krow = row_at<T>(a.k, a.kt, a.kh, seg.first + key, group);
     const T* vrow = row_at<T>(a.v, a.vt, a.vh, seg.first + key, group);
     float4 k[HD / 8], v[HD / 8];
-    if (HD <= 64) {
-      load_operand<HD>(k, krow, half);
-      load_operand<HD>(v, vrow, half);
-    }
+    load_operand<HD>(k, krow, half);
+    load_operand<HD>(v, vrow, half);
     const int64_t st = (int64_t)group * a.T * a.R + (int64_t)first * a.R;
     const int row_from = max(k0 - behind, 0) * a.R, blocks = (rows + 31) >> 5;
     const int row_min = max(k0 + col - behind, 0) * a.R;  // the first row that sees the lane's key
-    for (int j = (row_from >> 5) + wave; j < blocks; j += kWaves) {
+    // rows of g_out and q in the wave's own stages, each sent again behind its last product
+    typedef Stage32<HD> St;
+    const St stage;
+    char* gs = lds + 2 * St::kBytes * wave;
+    char* qs = gs + St::kBytes;
+    auto send = [&](const char* base, int64_t tok, int64_t head, int j, char* to) __attribute__((always_inline)) {
+      const int t0 = div_r(a, 32 * j);
+      const char* at = base + (int64_t)(first + t0) * tok + group * a.R * head;
+#pragma unroll
+      for (int i = 0; i < St::kLoads; ++i) {
+        const int row = min(32 * j + St::load_row(i), rows - 1), tk = div_r(a, row);
+        St::load(to, i, at, (uint32_t)(tk - t0) * (uint32_t)tok + (row - tk * a.R) * (uint32_t)head);
+      }
+    };
+    const int from = (row_from >> 5) + wave;
+    float next = 0.f;
+    // the rows' lse2 and delta by two lanes a row, and from them by shuffles
+    auto stat = [&](int j) __attribute__((always_inline)) {
+      next = (half ? g.delta : g.lse2)[st + min(32 * j + col, rows - 1)];
+    };
+    if (from < blocks) stat(from);
+    wait_vmcnt_le<0>();  // the keys too: the compiler does not count the stages' loads
+    if (from < blocks) {
+      send(g.g_out, g.gt, g.gh, from, gs);
+      send(a.q, a.qt, a.qh, from, qs);
+    }
+    for (int j = from; j < blocks; j += kWaves) {
       const int r0 = 32 * j;
-      float4 x[HD / 8];
-      const int ri = min(r0 + col, rows - 1), tk = div_r(a, ri), h = group * a.R + ri - tk * a.R;
-      // as in dq; the rows' lse2 and delta by two lanes a row, and from them by shuffles
-      constexpr bool kAhead = HD <= 64;
-      float4 y[HD / 8];
-      float qc[kAhead ? 16 : 1][DT], gc[kAhead ? 16 : 1][DT];
-      const float mine = (half ? g.delta : g.lse2)[st + ri];
-      load_operand<HD>(x, row_at<T>(a.q, a.qt, a.qh, first + tk, h), half);
-      if (kAhead) {
-        load_operand<HD>(y, row_at<T>(g.g_out, g.gt, g.gh, first + tk, h), half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int at = min(r0 + tile_row(r, half), rows - 1), t = div_r(a, at), hh = group * a.R + at - t * a.R;
-          const T* qrow = row_at<T>(a.q, a.qt, a.qh, first + t, hh) + col;
-          const T* grow = row_at<T>(g.g_out, g.gt, g.gh, first + t, hh) + col;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            qc[kAhead ? r : 0][d] = qrow[32 * d];
-            gc[kAhead ? r : 0][d] = grow[32 * d];
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      } else {
-        load_operand<HD>(k, krow, half);
-      }
-      f32x16 s = products<HD>(x, k);
-      if (!kAhead) {
-        load_operand<HD>(v, vrow, half);
-        load_operand<HD>(y, row_at<T>(g.g_out, g.gt, g.gh, first + tk, h), half);
-      }
-      f32x16 ds = products<HD>(y, v);
+      const bool more = j + kWaves < blocks;
+      const float mine = next;
+      wait_vmcnt_le<St::kLoads>();
+      asm volatile("" ::: "memory");
+      f32x16 ds = staged_products<HD>(stage, gs, v);
+      wait_vmcnt_le<0>();
+      asm volatile("" ::: "memory");
+      f32x16 s = staged_products<HD>(stage, qs, k);
+      if (more) stat(j + kWaves);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int row = r0 + tile_row(r, half), at = min(row, rows - 1);
@@ -740,45 +797,36 @@ __global__ __launch_bounds__(kThreads) void packed_dkv_kernel(const Packed a, co
         ds[r] = off ? 0.f : p * (ds[r] - e);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int at = min(r0 + tile_row(r, half), rows - 1), t = div_r(a, at), hh = group * a.R + at - t * a.R;
-        const T* qrow = row_at<T>(a.q, a.qt, a.qh, first + t, hh) + col;
-        const T* grow = row_at<T>(g.g_out, g.gt, g.gh, first + t, hh) + col;
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const float qx = kAhead ? qc[kAhead ? r : 0][d] : qrow[32 * d], gx = kAhead ? gc[kAhead ? r : 0][d] : grow[32 * d];
-          ak[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(qx, ds[r], ak[d], 0, 0, 0);
-          av[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(gx, s[r], av[d], 0, 0, 0);
-        }
+        for (int r = 0; r < 16; ++r)
+          av[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(stage.column(gs, r, d), s[r], av[d], 0, 0, 0);
+      reads_done();
+      if (more) {
+        wait_vmcnt_le<0>();  // the next rows' lse2, before loads that the compiler does not count
+        send(g.g_out, g.gt, g.gh, j + kWaves, gs);
       }
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          ak[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(stage.column(qs, r, d), ds[r], ak[d], 0, 0, 0);
+      reads_done();
+      if (more) send(a.q, a.qt, a.qh, j + kWaves, qs);
     }
   }
+  Sums<HD, 1, kWaves>& sums = *(Sums<HD, 1, kWaves>*)lds;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     T* to = which ? dv : dk;
     if (!to) continue;
+    reads_done();
+    __syncthreads();  // the stages become the waves' sums
+    sums.put(0, wave, col, half, which ? av : ak, which ? 1.f : g.scale);
     __syncthreads();
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const f32x16& c = which ? av[d] : ak[d];
-        *(float4*)&so[wave][col][32 * d + tile_row(r, half)] = make_float4(c[r], c[r + 1], c[r + 2], c[r + 3]);
-      }
-    __syncthreads();
-    const float f = which ? 1.f : g.scale;
-    for (int i = tid; i < 32 * HD / 4; i += kThreads) {
-      const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
-      if (k0 + t >= seg.len) continue;
-      float4 x = *(const float4*)&so[0][t][d];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) {
-        const float4 y = *(const float4*)&so[w][t][d];
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-      }
-      store4(to + ((int64_t)(seg.first + k0 + t) * a.G + group) * HD + d,
-             make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
-    }
+    sums.write([&](int t) -> T* {
+      return k0 + t < seg.len ? to + ((int64_t)(seg.first + k0 + t) * a.G + group) * HD : nullptr;
+    });
   }
 }
 
@@ -817,36 +865,6 @@ __device__ __forceinline__ float unit_of(const Grads& g, float* lds) {
 // fp16's weights in dv, at most 1, are 2^14 times as large.
 template <class T>
 constexpr float kLiftP = __is_same(T, _Float16) ? 16384.f : 1.f;
-
-// The sums of N sets of RW waves, 32 rows each, joined in LDS and written.
-template <int HD, int N, int RW>
-struct Sums {
-  float so[N][RW][32][HD + 4];
-  __device__ __forceinline__ void put(int n, int rw, int col, int half, const f32x16 (&acc)[HD / 32], float f) {
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4)
-        *(float4*)&so[n][rw][col][32 * d + tile_row(r, half)] =
-            make_float4(acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f);
-  }
-  // `place(t)`: where row t goes, null for nowhere.
-  template <class F>
-  __device__ __forceinline__ void write(F&& place) const {
-    for (int i = threadIdx.x; i < N * 32 * HD / 4; i += 64 * N * RW) {
-      const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
-      auto* to = place(t);
-      if (!to) continue;
-      float4 x = *(const float4*)&so[t >> 5][0][t & 31][d];
-#pragma unroll
-      for (int w = 1; w < RW; ++w) {
-        const float4 y = *(const float4*)&so[t >> 5][w][t & 31][d];
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-      }
-      store4(to + d, x);
-    }
-  }
-};
 
 // dq.  WIDE: 128 rows a workgroup, 32 a wave, 64 keys a stage that all waves read;
 // else 32 rows, and every wave has keys and stages of its own.

@@ -54,7 +54,7 @@ struct Stage {
   static constexpr int kSteps = HD / 16, kTiles = HD / 32;
 
   __device__ static __forceinline__ int f(int r) {
-    return HD == 128 ? (r & 3) << 2 | (r >> 2 & 3) : HD == 64 ? (r & 2) << 1 | (r >> 2 & 3) : r >> 2 & 3;
+    return HD >= 128 ? (r & 3) << 2 | (r >> 2 & 3) : HD == 64 ? (r & 2) << 1 | (r >> 2 & 3) : r >> 2 & 3;
   }
 
   uint32_t row, col0, col1;
