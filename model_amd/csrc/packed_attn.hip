@@ -20,12 +20,12 @@
 //   backward of the latter: delta 19, dq 803 (1,027), dk and dv 1,102 (998 of its four products)
 //   24 documents, 16,384 tokens, 16 heads over 4 of 128, bf16: forward 150, delta 36, dq 191,
 //     dk and dv 334: the longest document's first tiles are most of the time
-//   40 documents, 8,192 tokens, 4 heads of 64, fp32: forward 59, delta 5, dq 85, dk and dv 128
+//   40 documents, 8,192 tokens, 4 heads of 64, fp32: forward 47, delta 5, dq 62, dk and dv 87
+//   4,096 tokens, 8 heads of 64, fp32: forward 169 (101 TFLOP/s), backward 557 (108 of its seven products)
 //   64 single tokens over caches of up to 8,192, 32 heads over 8 of 128, bf16: 266, 5.2 TB/s
 // Bound: the matrix units of large 16-bit calls (half of their cycles; the vector units
 // 60 to 85 % of theirs: exponentials and conversions), memory for single tokens, for
-// short sequences the chain of loads that each workgroup begins with.  fp32's short
-// sequences spend most of their time between a block's loads and its products.
+// short sequences the chain of loads that each workgroup begins with.
 #include <math.h>
 
 #include <type_traits>
@@ -1328,8 +1328,8 @@ bool wide_keys_of(const Args* p) {
 // its share of the join's launch and memory from some keys on; fp32's products take
 // longer, and want more workgroups.  us by number of parts, single tokens of B streams
 // over `cap` keys each:
-//   fp32, B 1, cap 2,048, 4 heads of 64:      1: 43.4   4: 18.5   8: 14.6   16: 14.6   32: 19.4
-//   fp32, 16, 4,096, 32 over 8 of 128:        1: 221    2: 128    4: 132    8: 140     16: 160
+//   fp32, B 1, cap 2,048, 4 heads of 64:      1: 41.9   4: 16.7   8: 14.1   16: 14.1   32: 19.3
+//   fp32, 16, 4,096, 32 over 8 of 128:        1: 170    2: 107    4: 120    8: 125     16: 150
 //   bf16, 1, 512, 4 of 64:                    1: 8.2    2: 11.1   4: 10.6
 //   bf16, 1, 8,192, 4 of 64:                  1: 42.0   4: 16.4   8: 13.3   16: 13.8   32: 18.1
 //   bf16, 1, 32,768, 32 over 8 of 128:        1: 215    8: 38.1   16: 33.9  32: 47.6   64: 64.8
