@@ -232,7 +232,8 @@ __global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(st.column(vs, r, d), p[r], acc[d], 0, 0, 0);
+      for (int r = 0; r < 16; ++r)
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(st.column(vs, r, d), p[r], acc[d], 0, 0, 0);
     }
     reads_done();
     if (more) send(vb, a.vt, j + kWaves, vs);
@@ -714,8 +715,9 @@ __global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, con
 
 // dk and dv: 32 keys a workgroup, the lane's column a key, rows in the registers.
 template <int HD>
-__global__ __launch_bounds__(kThreads, HD <= 64 ? 2 : 1) void packed_dkv_kernel(const Packed a, const Grads g, float* __restrict__ dk,
-                                                              float* __restrict__ dv) {
+__global__ __launch_bounds__(kThreads, HD <= 64 ? 2 : 1) void packed_dkv_kernel(const Packed a, const Grads g,
+                                                                               float* __restrict__ dk,
+                                                                               float* __restrict__ dv) {
   typedef float T;
   constexpr int DT = HD / 32;
   constexpr int kStages = 2 * Stage32<HD>::kBytes * kWaves, kJoin = sizeof(Sums<HD, 1, kWaves>);
@@ -1227,7 +1229,8 @@ int element_size(int dtype) { return dtype == MPL_F32 ? 4 : 2; }
 // What does not depend on the buffers.
 int check_sizes(const Args* p, const char* what) {
   MPL_REQUIRE(p, MPL_EINVAL, "%s: null arguments", what);
-  MPL_REQUIRE(p->dtype == MPL_F32 || p->dtype == MPL_F16 || p->dtype == MPL_BF16, MPL_EINVAL, "%s: dtype %d", what, p->dtype);
+  MPL_REQUIRE(p->dtype == MPL_F32 || p->dtype == MPL_F16 || p->dtype == MPL_BF16, MPL_EINVAL, "%s: dtype %d", what,
+              p->dtype);
   MPL_REQUIRE(p->heads > 0 && p->groups > 0 && p->heads % p->groups == 0, MPL_EINVAL,
               "%s: %d heads for %d key heads", what, p->heads, p->groups);
   MPL_REQUIRE(p->head_dim == 32 || p->head_dim == 64 || p->head_dim == 128, MPL_EUNSUPPORTED,
@@ -1235,7 +1238,8 @@ int check_sizes(const Args* p, const char* what) {
   MPL_REQUIRE(p->tokens >= 0 && p->keys >= 0 && p->sequences >= 0, MPL_EINVAL,
               "%s: bad sizes tokens=%lld keys=%lld sequences=%lld", what, (long long)p->tokens, (long long)p->keys,
               (long long)p->sequences);
-  MPL_REQUIRE(p->index_bytes == 4 || p->index_bytes == 8, MPL_EINVAL, "%s: index_bytes %d (4 or 8)", what, p->index_bytes);
+  MPL_REQUIRE(p->index_bytes == 4 || p->index_bytes == 8, MPL_EINVAL, "%s: index_bytes %d (4 or 8)", what,
+              p->index_bytes);
   // rows are counted in 32 bits, and a grid's threads too
   constexpr int64_t kMost = (int64_t)1 << 30;
   MPL_REQUIRE(p->heads <= 65536 && p->tokens <= kMost && p->keys <= kMost && p->sequences <= kMost &&
@@ -1250,7 +1254,8 @@ int check_sizes(const Args* p, const char* what) {
 
 constexpr int64_t kMostStride = 1 << 23;  // elements
 // `shared`: of k and v, whose heads lie where they like.
-int check_rows(const Args* p, const void* x, int64_t tok, int64_t head, bool shared, const char* name, const char* what) {
+int check_rows(const Args* p, const void* x, int64_t tok, int64_t head, bool shared, const char* name,
+               const char* what) {
   const int64_t unit = 16 / element_size(p->dtype);
   MPL_REQUIRE(x, MPL_EINVAL, "%s: null %s", what, name);
   MPL_REQUIRE(((uintptr_t)x & 15) == 0 && tok >= 0 && head >= 0 && tok % unit == 0 && head % unit == 0, MPL_EINVAL,
@@ -1385,9 +1390,11 @@ void backward(const Args* p, const void* g_out, int64_t gt, int64_t gh, const vo
   float* largest = (float*)((char*)ws + 2 * round256(rows * 4));
   const int64_t blocks = cdiv(rows * (HD / 4), 256);
   const int used = (int)(blocks < kDeltaBlocks ? blocks : kDeltaBlocks);
-  const Grads g{(const char*)g_out, gt * (int64_t)sizeof(T), gh * (int64_t)sizeof(T), lse2, delta, g_lse, largest, used, p->scale};
+  const Grads g{(const char*)g_out, gt * (int64_t)sizeof(T), gh * (int64_t)sizeof(T), lse2, delta, g_lse, largest, used,
+                p->scale};
   if (rows)
-    packed_delta_kernel<T, HD><<<used, 256, 0, s>>>(a, g.g_out, g.gt, g.gh, (const T*)out, lse, g_lse, lse2, delta, largest);
+    packed_delta_kernel<T, HD><<<used, 256, 0, s>>>(a, g.g_out, g.gt, g.gh, (const T*)out, lse, g_lse, lse2, delta,
+                                                    largest);
   auto tiles = [&](int64_t x, int unit) { return (unsigned)((x / unit + a.n + 2) * a.G); };
   if constexpr (sizeof(T) == 2) {
     if (rows) {  // for delta, too
@@ -1396,8 +1403,10 @@ void backward(const Args* p, const void* g_out, int64_t gt, int64_t gh, const vo
     }
     if (a.S && (dk || dv)) {
       constexpr int KW = HD == 128 ? 2 : 4, RW = HD == 128 ? 3 : 1;
-      if (wide_keys_of(p)) packed_dkv16_kernel<T, HD, KW, RW><<<tiles(a.S, 32 * KW), 64 * KW * RW, 0, s>>>(a, g, (T*)dk, (T*)dv);
-      else packed_dkv16_kernel<T, HD, 1, 4><<<tiles(a.S, 32), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
+      if (wide_keys_of(p))
+        packed_dkv16_kernel<T, HD, KW, RW><<<tiles(a.S, 32 * KW), 64 * KW * RW, 0, s>>>(a, g, (T*)dk, (T*)dv);
+      else
+        packed_dkv16_kernel<T, HD, 1, 4><<<tiles(a.S, 32), kThreads, 0, s>>>(a, g, (T*)dk, (T*)dv);
     }
   } else {
     if (rows && dq) packed_dq_kernel<HD><<<tiles((int64_t)a.T * a.R, 32), kThreads, 0, s>>>(a, g, (T*)dq);
