@@ -83,16 +83,27 @@ struct Stage {
   // under way, those of the next stage among them (it does not know what either
   // touches).  The instruction has no register for a result; whoever reads the stage
   // waits for it with wait_vmcnt_le and a barrier.
+  //
+  // The compiler does not look for hazards inside the statement either.  An address in
+  // scalar registers that a vector instruction wrote (v_readfirstlane, here or wherever
+  // the base comes from) may be read by a vector-memory instruction five wait states
+  // later at the earliest, so the statement copies it: a scalar read waits for the
+  // vector write, and what a scalar instruction wrote may be read at once.  The copy is
+  // the wait state, too, that m0 needs.
   __device__ static __forceinline__ void load(char* lds, int n, const char* base, uint32_t row_at) {
     const uint32_t piece = (threadIdx.x & 63) % kPieces ^ f(load_row(n));
     const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)(lds + n * 1024));
     const uint64_t from = (uint64_t)base;
     const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(from >> 32)) << 32 |
                         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)from);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
+    uint64_t copy;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: declared all the same, so that no value of it is kept across
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+                 : "=&s"(copy)
                  : "s"(to), "v"(row_at + (piece << 4)), "s"(at)
-                 : "memory");  // m0 is the compiler's for its own LDS loads alone, which set it themselves
+                 : "memory", "m0");
+#pragma clang diagnostic pop
   }
   // N loads, every BY-th from n0 on, of rows `pitch` bytes apart from `base` on, the
   // stage's first; rows behind `last` are read as the last.
