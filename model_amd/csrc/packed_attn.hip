@@ -531,14 +531,10 @@ struct Grads {
   const float* lse2;  // [group][T R]: base 2, +inf for a row without keys
   float* delta;       // [group][T R]
   const float* g_lse;
-  const float* largest;       // [3][blocks]
-  int blocks;
   float scale;
 };
 
-// lse2 and delta of every row, HD / 4 lanes a row.  For fp16 also each workgroup's
-// largest |g_out|^2 and |v|^2 of a row and largest |g_lse| (see unit_of); rows that
-// are not finite do not count.
+// lse2 and delta of every row, HD / 4 lanes a row.
 constexpr int kDeltaBlocks = 1024;
 template <int L>
 __device__ __forceinline__ float sum_lanes(float x) {
@@ -546,51 +542,27 @@ __device__ __forceinline__ float sum_lanes(float x) {
   for (int o = L / 2; o; o >>= 1) x += __shfl_xor(x, o);
   return x;
 }
-__device__ __forceinline__ float finite_max(float top, float x) { return x < INFINITY ? fmaxf(top, x) : top; }
 
 template <class T, int HD>
 __global__ __launch_bounds__(256) void packed_delta_kernel(const Packed a, const char* __restrict__ g_out, int64_t gt,
                                                            int64_t gh, const T* __restrict__ out,
                                                            const float* __restrict__ lse,
                                                            const float* __restrict__ g_lse, float* __restrict__ lse2,
-                                                           float* __restrict__ delta, float* __restrict__ largest) {
+                                                           float* __restrict__ delta) {
   constexpr int L = HD / 4;
-  constexpr bool kUnit = __is_same(T, _Float16);
   const int d = 4 * (threadIdx.x % L);
-  const uint32_t rows = (uint32_t)a.T * a.H, values = (uint32_t)a.S * a.G;  // below 2^29
-  float top[3] = {0.f, 0.f, 0.f};
+  const uint32_t rows = (uint32_t)a.T * a.H;  // below 2^29
   for (uint32_t first = blockIdx.x * (256 / L); first < rows; first += gridDim.x * (256 / L)) {
     const uint32_t at = first + threadIdx.x / L, row = min(at, rows - 1);
     const int t = row / (uint32_t)a.H, h = row % (uint32_t)a.H;
     const float4 x = load4(row_at<T>(g_out, gt, gh, t, h) + d), y = load4(out + (int64_t)row * HD + d);
     const float s = sum_lanes<L>(x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w);
-    if (kUnit) top[0] = finite_max(top[0], sum_lanes<L>(x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w));
     if (at < rows && d == 0) {
       const int g = div_r(a, h);
       const int64_t to = (int64_t)g * a.T * a.R + (int64_t)t * a.R + h - g * a.R;
-      const float z = lse[row], gl = g_lse ? g_lse[row] : 0.f;
+      const float z = lse[row];
       lse2[to] = z == -INFINITY ? INFINITY : z * kLog2e;
-      delta[to] = s - gl;
-      if (kUnit) top[2] = finite_max(top[2], fabsf(gl));
-    }
-  }
-  if constexpr (kUnit) {
-    for (uint32_t first = blockIdx.x * (256 / L); first < values; first += gridDim.x * (256 / L)) {
-      const uint32_t row = min(first + threadIdx.x / L, values - 1);
-      const float4 x = load4(row_at<T>(a.v, a.vt, a.vh, row / (uint32_t)a.G, row % (uint32_t)a.G) + d);
-      top[1] = finite_max(top[1], sum_lanes<L>(x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w));
-    }
-    __shared__ float tops[4][3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-#pragma unroll
-      for (int o = 32; o; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], o));
-      if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6][i] = top[i];
-    }
-    __syncthreads();
-    if (threadIdx.x < 3) {
-      const int i = threadIdx.x;
-      largest[i * gridDim.x + blockIdx.x] = fmaxf(fmaxf(tops[0][i], tops[1][i]), fmaxf(tops[2][i], tops[3][i]));
+      delta[to] = s - (g_lse ? g_lse[row] : 0.f);
     }
   }
 }
@@ -833,36 +805,42 @@ __global__ __launch_bounds__(kThreads, HD <= 64 ? 2 : 1) void packed_dkv_kernel(
 }
 
 // ------------------------------------------------ backward, fp16 and bf16
-// The power of two that dz is multiplied by before it is rounded to fp16.  |dz| is at
-// most |dp| + |delta| <= B = 2 max|g_out| max|v| + max|g_lse|, and B goes to [2^13,
-// 2^14): nothing overflows, and gradients of any size keep their bits down to 2^-38
-// of B.  bf16 has fp32's range and takes 1.  Every thread of the workgroup calls it.
-template <class T, int W>
-__device__ __forceinline__ float unit_of(const Grads& g, float* lds) {
-  if constexpr (__is_same(T, _Float16)) {
-    float top[3];
+// dz is rounded to fp16 under a power of two of the lane's column (a row in dq, a key
+// in dk and dv; both halves of the wave hold the same ones): the largest |dz| so far goes
+// to [2^13, 2^14) when it is found and stays below 2^15, else the power falls, and the
+// accumulators with it.  So nothing overflows, and dz keeps all its bits down to 2^-27 of
+// the column's largest, whatever the other rows and keys, sequences or places not in use
+// hold.  (One power for the whole call, of its largest |g_out| and |v|, cost a sequence
+// its bits for another's size, and a pass over all of v.)  What is not finite takes its
+// own column along.  bf16 has fp32's range and takes none.
+template <class T, int HD>
+struct Unit {
+  static constexpr bool kNone = !__is_same(T, _Float16);
+  uint32_t e = 227;  // of the power, biased by 127: at most 2^100, so that the inverse is finite
+  // x, the column's next 16 dz, times the power; acc is in the power's measure
+  __device__ __forceinline__ void scale(f32x16& x, f32x16 (&acc)[HD / 32]) {
+    if constexpr (kNone) return;
+    float top = fabsf(x[0]);
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      top[i] = 0.f;
-      for (int b = threadIdx.x; b < g.blocks; b += 64 * W) top[i] = fmaxf(top[i], g.largest[i * g.blocks + b]);
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
+    float t0 = top, t1 = top;
+    half_swap(t0, t1);
+    top = fmaxf(t0, t1);
+    if (__any(top * power() >= 32768.f)) {
+      const uint32_t now = top * power() >= 32768.f ? 127 + 13 + 127 - (__float_as_uint(top) >> 23) : e;
+      const float f = __uint_as_float((uint32_t)max(127 + (int)now - (int)e, 0) << 23);  // 0 below 2^-126
+      e = now;
 #pragma unroll
-      for (int o = 32; o; o >>= 1) top[i] = fmaxf(top[i], __shfl_xor(top[i], o));
-      if ((threadIdx.x & 63) == 0) lds[3 * (threadIdx.x >> 6) + i] = top[i];
+      for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= f;
     }
-    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
-#pragma unroll
-      for (int w = 0; w < W; ++w) top[i] = fmaxf(top[i], lds[3 * w + i]);
-    __syncthreads();
-    const float most = 2.f * __builtin_sqrtf(top[0]) * __builtin_sqrtf(top[1]) + top[2];
-    const int e = (int)(__float_as_uint(most) >> 23);  // biased
-    // within fp32's range with its inverse; the largest power that leaves B so
-    return e == 0 || e == 255 ? 1.f : __uint_as_float((uint32_t)min(max(127 + 13 + 127 - e, 27), 227) << 23);
-  } else {
-    return 1.f;
+    for (int r = 0; r < 16; ++r) x[r] *= power();
   }
-}
+  __device__ __forceinline__ float power() const { return __uint_as_float(e << 23); }
+  __device__ __forceinline__ float inverse() const { return kNone ? 1.f : __uint_as_float((254 - e) << 23); }
+};
 
 // fp16's weights in dv, at most 1, are 2^14 times as large.
 template <class T>
@@ -893,7 +871,6 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
   const Segment seg = segment_of<WIDE ? 7 : 5>(a.starts, a.wide, a.n, a.T, a.R, blockIdx.x / a.G);
   const int rows = seg.len * a.R, tiles = (rows + kRows - 1) / kRows;
   if (seg.tile >= tiles) return;
-  const float unit = unit_of<T, kWaves>(g, (float*)lds);
   const int row0 = kRows * (tiles - 1 - seg.tile);
   const Keys keys = keys_of(a, seg.seq);
   const int behind = keys.len - seg.len;
@@ -991,18 +968,23 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
   f32x16 acc[HD / 32];
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d) acc[d] = f32x16{};
+  Unit<T, HD> unit;
   sweep([&](const f32x16& p, const f32x16& dp, const char* k, int b) __attribute__((always_inline)) {
+    f32x16 dz;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dz[r] = p[r] * (dp[r] - delta);
+    unit.scale(dz, acc);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = p[8 * i + e] * ((dp[8 * i + e] - delta) * unit);
+      for (int e = 0; e < 8; ++e) x[e] = dz[8 * i + e];
       const short8v w = round8<T>(x);
 #pragma unroll
       for (int d = 0; d < HD / 32; ++d) acc[d] = mma16<T>(st.cols(k, 2 * b + i, d), w, acc[d]);
     }
   });
-  const float f = g.scale / unit;
+  const float f = g.scale * unit.inverse();
   if constexpr (WIDE) {
     if (w0 + col >= rows) return;
     T* to = dq + ((int64_t)(seg.first + tok) * a.H + head) * HD;
@@ -1054,7 +1036,6 @@ __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed
   const Segment seg = segment_of<KW == 1 ? 5 : KW == 2 ? 6 : 7>(a.key_starts, a.wide, a.n, a.S, 1, blockIdx.x / a.G);
   const int k0 = kKeys * seg.tile;
   if (k0 >= seg.len) return;
-  const float unit = unit_of<T, W>(g, (float*)lds);
   const bool real = seg.seq >= 0 && seg.seq < a.n;
   const int len = real ? keys_of(a, seg.seq).len : 0;  // of the segment's keys those in use
   int first = 0, tokens = 0;
@@ -1068,6 +1049,7 @@ __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed
   f32x16 ak[HD / 32], av[HD / 32];
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d) ak[d] = av[d] = f32x16{};
+  Unit<T, HD> unit;
   char* mine = lds + 4 * kBytes * rw;
   if (k0 < len && rows > 0) {
     const int held = min(key, len - 1);
@@ -1173,7 +1155,7 @@ __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             s[r + i] = __builtin_amdgcn_exp2f(fmaf(s[r + i], a.c, -zs[i]));
-            ds[r + i] = s[r + i] * ((ds[r + i] - es[i]) * unit);
+            ds[r + i] = s[r + i] * (ds[r + i] - es[i]);
           }
         }
         if (r0 < all_see) {
@@ -1181,6 +1163,7 @@ __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed
           for (int r = 0; r < 16; ++r)
             if (r0 + tile_row(r, half) < row_min) s[r] = ds[r] = 0.f;
         }
+        unit.scale(ds, ak);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float x[8], y[8];
@@ -1199,7 +1182,7 @@ __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed
       }
     }
   }
-  const float fk = g.scale / unit, fv = 1.f / kLiftP<T>;
+  const float fk = g.scale * unit.inverse(), fv = 1.f / kLiftP<T>;
   const bool in = key < len;  // places not in use have gradients 0
   Sums<HD, KW, RW>& sums = *(Sums<HD, KW, RW>*)lds;
 #pragma unroll
@@ -1352,7 +1335,7 @@ size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 size_t workspace_bytes(const Args* p, bool backward) {
   const size_t rows = (size_t)p->tokens * p->heads;
-  if (backward) return 2 * round256(rows * 4) + 3 * kDeltaBlocks * 4;
+  if (backward) return 2 * round256(rows * 4);
   const int s = wide_of(p) ? 1 : splits_of(p);
   return s > 1 ? round256(s * rows * p->head_dim * 4) + round256(s * rows * 8) : 0;
 }
@@ -1387,14 +1370,11 @@ void backward(const Args* p, const void* g_out, int64_t gt, int64_t gh, const vo
   const size_t rows = (size_t)p->tokens * p->heads;
   float* lse2 = (float*)ws;
   float* delta = (float*)((char*)ws + round256(rows * 4));
-  float* largest = (float*)((char*)ws + 2 * round256(rows * 4));
   const int64_t blocks = cdiv(rows * (HD / 4), 256);
   const int used = (int)(blocks < kDeltaBlocks ? blocks : kDeltaBlocks);
-  const Grads g{(const char*)g_out, gt * (int64_t)sizeof(T), gh * (int64_t)sizeof(T), lse2, delta, g_lse, largest, used,
-                p->scale};
+  const Grads g{(const char*)g_out, gt * (int64_t)sizeof(T), gh * (int64_t)sizeof(T), lse2, delta, g_lse, p->scale};
   if (rows)
-    packed_delta_kernel<T, HD><<<used, 256, 0, s>>>(a, g.g_out, g.gt, g.gh, (const T*)out, lse, g_lse, lse2, delta,
-                                                    largest);
+    packed_delta_kernel<T, HD><<<used, 256, 0, s>>>(a, g.g_out, g.gt, g.gh, (const T*)out, lse, g_lse, lse2, delta);
   auto tiles = [&](int64_t x, int unit) { return (unsigned)((x / unit + a.n + 2) * a.G); };
   if constexpr (sizeof(T) == 2) {
     if (rows) {  // for delta, too

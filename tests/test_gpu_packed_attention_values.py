@@ -1,0 +1,82 @@
+"""packed_attention: what values elsewhere do to a sequence's results.  Nothing, in whatever size they come: the same
+sequences of one call are compared bit by bit, and values of unlike sizes with the definition in 64 bits."""
+
+import pytest
+import torch
+
+from model_amd.attention import packed_attention_backward, packed_attention_forward
+from tests.test_gpu_packed_attention import DEV, DT, make, run_all, sums
+
+pytestmark = pytest.mark.gpu
+
+
+def all_of(q, k, v, g, gl, starts, **kw):
+    out, lse = packed_attention_forward(q, k, v, starts, **kw)
+    return out, lse, *packed_attention_backward(g, q, k, v, out, lse, starts, g_lse=gl, **kw)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("what", ["v", "g_out", "g_lse", "all"])
+@pytest.mark.parametrize("lq,H,G,hd", [([40, 300, 33, 70], 4, 2, 64), ([40, 300, 33, 70], 5, 1, 128),
+                                       ([1500, 700, 2000], 16, 16, 64), ([900, 5, 1700], 32, 16, 128),
+                                       ([2500, 6000, 500], 16, 16, 32)])
+def test_another_sequence_of_large_values(dtype, what, lq, H, G, hd):
+    """Sequence 1's values times 2^12 (finite in every type): the others' bits stay."""
+    q, k, v, g, gl = make(lq, lq, H, G, hd, dtype, seed=31, std=0.5)
+    starts = torch.tensor(sums(lq), dtype=torch.int32, device=DEV)
+    want = all_of(q, k, v, g, gl, starts)
+    one = slice(lq[0], lq[0] + lq[1])
+    for nm, x in (("v", v), ("g_out", g), ("g_lse", gl)):
+        if what in (nm, "all"):
+            x[one] *= 4096
+    got = all_of(q, k, v, g, gl, starts)
+    for nm, a, b in zip(("out", "lse", "dq", "dk", "dv"), want, got):
+        assert torch.equal(a[:one.start], b[:one.start]) and torch.equal(a[one.stop:], b[one.stop:]), nm
+        assert torch.isfinite(b[one].float()).all() or dtype == torch.float16, nm
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("H,G,hd,n", [(4, 2, 64, 1), (8, 1, 128, 3), (6, 3, 32, 40)])
+def test_places_not_in_use_of_large_values(dtype, H, G, hd, n):
+    """A cache's free places hold finite values of 60,000: every bit as if they held 0."""
+    cap, used = 700, [1, 700, 0, 333, 64]
+    q, k, v, g, gl = make([n] * 5, [cap] * 5, H, G, hd, dtype, seed=32)
+    starts = torch.arange(0, 5 * n + 1, n, dtype=torch.int32, device=DEV)
+    kw = {"key_starts": torch.arange(0, 5 * cap + 1, cap, dtype=torch.int32, device=DEV),
+          "key_lengths": torch.tensor(used, dtype=torch.int32, device=DEV)}
+    runs = []
+    for fill in (0.0, 60_000.0):
+        for i, x in enumerate(used):
+            k[cap * i + x:cap * (i + 1)] = fill
+            v[cap * i + x:cap * (i + 1)] = fill
+        runs.append(all_of(q, k, v, g, gl, starts, **kw))
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("H,hd", [(4, 64), (6, 128), (8, 32)])
+def test_sequences_of_unlike_sizes(dtype, H, hd):
+    """Each sequence's gradients and values have a size of their own, as small and as large as fp16 takes."""
+    lq = [60, 300, 33, 129]
+    q, k, v, g, gl = make(lq, lq, H, H // 2, hd, dtype, seed=33)
+    q, k = q * 0.2, k * 0.2
+    a = 0
+    for n, sv, sg in zip(lq, (500.0, 1.0, 2.0 ** -9, 30.0), (2.0 ** -14, 2.0 ** 9, 1.0, 2.0 ** -6)):
+        v[a:a + n] *= sv
+        g[a:a + n] *= sg
+        gl[a:a + n] *= sv * sg
+        a += n
+    run_all(q, k, v, lq, lq, g, gl, scale=0.05)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n", [90, 1300])
+def test_rows_and_keys_of_unlike_sizes(dtype, n):
+    """Within one sequence sizes grow and fall by 2^20 from row to row, so that the largest is met late, early and again."""
+    q, k, v, g, gl = make([n], [n], 4, 2, 64, dtype, seed=34)
+    gen = torch.Generator(device=DEV).manual_seed(35)
+    size = torch.exp2(torch.randint(-14, 6, (n, 1, 1), generator=gen, device=DEV).float())
+    g = (g.float() * size).to(dtype)
+    v = (v.float() * torch.exp2(torch.randint(-6, 6, (n, 1, 1), generator=gen, device=DEV).float())).to(dtype)
+    run_all(q * 0.3, k * 0.3, v, [n], [n], g, gl * size[:, :, 0])
