@@ -964,6 +964,7 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
     delta = sum - (g.g_lse ? g.g_lse[(int64_t)(seg.first + tok) * a.H + head] : 0.f);
     if (half == 0 && w0 + col < rows && (WIDE || wave == 0)) g.delta[at] = delta;
   }
+  if (sees <= 0) delta = 0.f;  // a row without keys, whose weights are 0: g_lse may be anything
   if (!dq) return;
   f32x16 acc[HD / 32];
 #pragma unroll

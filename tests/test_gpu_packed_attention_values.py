@@ -80,3 +80,21 @@ def test_rows_and_keys_of_unlike_sizes(dtype, n):
     g = (g.float() * size).to(dtype)
     v = (v.float() * torch.exp2(torch.randint(-6, 6, (n, 1, 1), generator=gen, device=DEV).float())).to(dtype)
     run_all(q * 0.3, k * 0.3, v, [n], [n], g, gl * size[:, :, 0])
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("lq,lk,H,G,hd", [([40, 100, 33], [10, 37, 32], 4, 2, 64), ([40, 100, 33], [10, 37, 32], 8, 1, 128),
+                                          ([900, 1500, 40], [700, 1400, 0], 16, 16, 64),
+                                          ([4500, 1500], [4400, 1], 16, 16, 32)])
+def test_queries_without_keys_and_a_senseless_gradient_of_lse(dtype, lq, lk, H, G, hd):
+    """The lse of such a query is -inf, and what comes back for it NaN or inf as often as not: it passes no gradient."""
+    q, k, v, g, gl = make(lq, lk, H, G, hd, dtype, seed=36)
+    starts, begin = (torch.tensor(sums(x), dtype=torch.int32, device=DEV) for x in (lq, lk))
+    lost = torch.cat([torch.arange(n, device=DEV) < n - m for n, m in zip(lq, lk)])
+    gl[lost] = 0
+    want = all_of(q, k, v, g, gl, starts, key_starts=begin)
+    assert (want[2][lost] == 0).all() and torch.isinf(want[1][lost]).all()
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        gl[lost] = bad
+        for nm, a, b in zip(("out", "lse", "dq", "dk", "dv"), want, all_of(q, k, v, g, gl, starts, key_starts=begin)):
+            assert torch.equal(a, b), (bad, nm)
