@@ -790,13 +790,19 @@ __global__ __launch_bounds__(kThreads, HD <= 64 ? 2 : 1) void packed_dkv_kernel(
     }
   }
   Sums<HD, 1, kWaves>& sums = *(Sums<HD, 1, kWaves>*)lds;
+  const bool in = k0 + col < len;  // places not in use have gradients 0
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     T* to = which ? dv : dk;
     if (!to) continue;
+    f32x16 (&x)[DT] = which ? av : ak;
+    if (!in) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) x[d] = f32x16{};
+    }
     reads_done();
     __syncthreads();  // the stages become the waves' sums
-    sums.put(0, wave, col, half, which ? av : ak, which ? 1.f : g.scale);
+    sums.put(0, wave, col, half, x, which ? 1.f : g.scale);
     __syncthreads();
     sums.write([&](int t) -> T* {
       return k0 + t < seg.len ? to + ((int64_t)(seg.first + k0 + t) * a.G + group) * HD : nullptr;

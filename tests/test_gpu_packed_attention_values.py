@@ -98,3 +98,18 @@ def test_queries_without_keys_and_a_senseless_gradient_of_lse(dtype, lq, lk, H, 
         gl[lost] = bad
         for nm, a, b in zip(("out", "lse", "dq", "dk", "dv"), want, all_of(q, k, v, g, gl, starts, key_starts=begin)):
             assert torch.equal(a, b), (bad, nm)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("H,G,hd,n", [(4, 2, 64, 3), (8, 1, 128, 1), (16, 16, 32, 2100)])
+def test_places_not_in_use_have_gradients_0(dtype, H, G, hd, n):
+    """Even beside rows whose gradient is not finite."""
+    cap, used = 2200, [3, 70, 2101]
+    q, k, v, g, gl = make([n] * 3, [cap] * 3, H, G, hd, dtype, seed=37)
+    g[0], g[2 * n - 1], gl[-1] = float("nan"), float("inf"), float("nan")
+    starts = torch.arange(0, 3 * n + 1, n, dtype=torch.int32, device=DEV)
+    got = all_of(q, k, v, g, gl, starts, key_starts=torch.arange(0, 3 * cap + 1, cap, dtype=torch.int32, device=DEV),
+                 key_lengths=torch.tensor(used, dtype=torch.int32, device=DEV))
+    for x in got[3:]:
+        for i, m in enumerate(used):
+            assert (x[cap * i + m:cap * (i + 1)] == 0).all()
