@@ -1313,8 +1313,12 @@ bool wide_of(const Args* p) {
 //   of 64:         4,096, 8, 8, 8 (256): 44.2 / 44.6;  8,192, 8, 8, 8 (512): 89.0 / 80.1;
 //                  8,192, 64, 32 over 8 (512): 96.8 / 106;  dk and dv of 16,384, 1, 16, 16 (2,048): 1,353 / 1,129
 //   of 32:         8,192, 8, 8, 8 (512): 51.3 / 54.4;  16,384, 16, 16 over 4 (512): 140 / 165
+//
+// Heads of 128 have 384 threads a workgroup then: with more than some 11 million tiles
+// (sequences times key heads) the grid's threads would pass 32 bits, where 256 do not.
 bool wide_keys_of(const Args* p) {
   const int64_t tiles = p->keys / 128 * p->groups;
+  if (p->head_dim == 128 && (p->keys / 64 + p->sequences + 2) * p->groups * 384 >= (int64_t)1 << 32) return false;
   return tiles >= (p->head_dim == 128 ? 128 : 1024);
 }
 

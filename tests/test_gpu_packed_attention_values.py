@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from model_amd.attention import packed_attention_backward, packed_attention_forward
-from tests.test_gpu_packed_attention import DEV, DT, make, run_all, sums
+from tests.test_gpu_packed_attention import DEV, DT, check, definition, make, run_all, sums
 
 pytestmark = pytest.mark.gpu
 
@@ -113,3 +113,15 @@ def test_places_not_in_use_have_gradients_0(dtype, H, G, hd, n):
     for x in got[3:]:
         for i, m in enumerate(used):
             assert (x[cap * i + m:cap * (i + 1)] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_grids_of_eleven_million_tiles(dtype):
+    """1.4 million empty sequences before one of 2,048 tokens: the grid of the gradients' large tiles would pass 32 bits."""
+    n, T, H = 1_400_000, 2048, 8
+    q, k, v, g, gl = make([T], [T], H, H, 128, dtype, seed=38)
+    starts = torch.zeros(n + 1, dtype=torch.int32, device=DEV)
+    starts[-1] = T
+    want = definition(q, k, v, [T], [T], [0], 128 ** -0.5, g, gl)
+    for nm, x in zip(("out", "lse", "dq", "dk", "dv"), all_of(q, k, v, g, gl, starts)):
+        check(x, want[nm], nm)
