@@ -38,6 +38,12 @@ namespace {
 
 constexpr int kWaves = 4, kThreads = kWaves * kWave;
 
+// Tokens are at most this many elements apart, and the heads that share a key head lie
+// within 32 times that.  So the places of a stage of `rows` rows, of as many tokens where
+// a token is one row, and of its heads are offsets of 32 bits.
+constexpr int64_t kMostStride = 1 << 23;
+constexpr bool far_rows_fit(int64_t rows, int64_t size) { return (rows + 32) * kMostStride * size < (int64_t)1 << 32; }
+
 // Register r of a 32 x 32 tile holds this row of it.
 __device__ __forceinline__ int tile_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
@@ -59,6 +65,7 @@ template <int HD>
 struct Stage32 : Stage<2 * HD> {
   typedef Stage<2 * HD> Base;
   static constexpr int kBytes = 128 * HD, kLoads = kBytes / 1024;
+  static_assert(far_rows_fit(32, 4), "32-bit places");
   // The operand of the lane's row: elements 8 g + 4 (lane / 32) + [0, 4).
   __device__ __forceinline__ float4 operand(const char* lds, int g) const {
     return __builtin_bit_cast(float4, this->rows(lds, 0, g));
@@ -331,6 +338,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_forward16_kernel(const Pac
                                                                        float* __restrict__ lse) {
   typedef Stage<HD> St;
   constexpr int kBytes = kWideKeys * St::kRow, kLoads = kBytes / 1024 / kWaves;
+  static_assert(far_rows_fit(kWideKeys, 2), "32-bit places");
   __shared__ __attribute__((aligned(1024))) char lds[5 * kBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -867,6 +875,7 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
                                                                             T* __restrict__ dq) {
   typedef Stage<HD> St;
   constexpr int B = WIDE ? 2 : 1, kKeys = 32 * B, kRows = WIDE ? 128 : 32;
+  static_assert(far_rows_fit(kKeys, 2), "32-bit places");
   constexpr int kBytes = kKeys * St::kRow, kLoads = kBytes / 1024 / (WIDE ? kWaves : 1);
   constexpr int kStages = 4 * kBytes * (WIDE ? 1 : kWaves), kJoin = WIDE ? 0 : sizeof(Sums<HD, 1, kWaves>);
   __shared__ __attribute__((aligned(1024))) char lds[kStages > kJoin ? kStages : kJoin];
@@ -1028,6 +1037,7 @@ __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed
   constexpr int kKeys = 32 * KW, W = KW * RW;
   constexpr int kBytes = KW == 1 ? 32 * St::kRow : 8192, kLoads = kBytes / 1024;
   constexpr int kRows = kBytes / St::kRow, NB = kRows / 32;
+  static_assert(far_rows_fit(kRows, 2) && far_rows_fit(kKeys, 2), "32-bit places");
   // heads of 128 leave no registers for the wave's keys and values as operands: they
   // lie in LDS, behind the stages
   constexpr bool kHeld = HD < 128 || KW == 1;
@@ -1242,7 +1252,6 @@ int check_sizes(const Args* p, const char* what) {
   return MPL_OK;
 }
 
-constexpr int64_t kMostStride = 1 << 23;  // elements
 // `shared`: of k and v, whose heads lie where they like.
 int check_rows(const Args* p, const void* x, int64_t tok, int64_t head, bool shared, const char* name,
                const char* what) {
@@ -1251,7 +1260,7 @@ int check_rows(const Args* p, const void* x, int64_t tok, int64_t head, bool sha
   MPL_REQUIRE(((uintptr_t)x & 15) == 0 && tok >= 0 && head >= 0 && tok % unit == 0 && head % unit == 0, MPL_EINVAL,
               "%s: the rows of %s must be 16-byte aligned (token %lld, head %lld)", what, name, (long long)tok,
               (long long)head);
-  // places within a stage of rows are 32-bit: up to 63 tokens and a token's heads
+  // places within a stage of rows are 32-bit (far_rows_fit)
   const int64_t r = p->heads / p->groups;
   MPL_REQUIRE(tok <= kMostStride && (shared || (head <= kMostStride && head * (r < 32 ? 32 : r) <= 32 * kMostStride)),
               MPL_EUNSUPPORTED, "%s: the rows of %s lie too far apart (token %lld, head %lld)", what, name,
