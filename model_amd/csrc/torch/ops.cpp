@@ -26,6 +26,7 @@
 #include <functional>
 #include <initializer_list>
 #include <memory>
+#include <numeric>
 #include <optional>
 #include <tuple>
 #include <utility>
@@ -503,6 +504,71 @@ std::tuple<Tensor, Tensor, Tensor> packed_attention_backward(const Tensor& g_out
 }
 
 // --------------------------------------------------------------- gradient clip
+// The bytes from a tensor's first element to behind its last; `whole`: it takes them all.
+struct Span {
+  char *first, *end;
+  const Tensor* t;
+  bool whole;
+};
+
+// Whether two tensors have a byte in common.  With steps i and j along their axes and x
+// and y within an element it is one equation, sum i s - sum j t + x - y = distance; axes of
+// one stride become one unknown, and the unknowns are tried from the largest stride on as
+// far as the others' sum can still make up the rest.  Views of one matrix have one or two
+// values left for each; a search that does not end within kMostSteps finds nothing.
+struct Meeting {
+  struct Unknown {
+    int64_t stride, lo, hi;  // its steps
+    int64_t least, most;     // of the sum of the unknowns behind it
+    int64_t divisor;         // of its stride and theirs
+  };
+  std::vector<Unknown> of;
+  int64_t x_lo, x_hi;
+  int steps = 0;
+  static constexpr int kMostSteps = 100000;
+
+  void axes(const Span& s, int sign) {
+    const int64_t size = s.t->element_size();
+    auto add = [&](int64_t stride, int64_t n) {
+      if (n <= 1) return;
+      auto at = std::find_if(of.begin(), of.end(), [&](const Unknown& u) { return u.stride == stride; });
+      if (at == of.end()) at = of.insert(of.end(), Unknown{stride, 0, 0, 0, 0, 1});
+      (sign > 0 ? at->hi : at->lo) += sign * (n - 1);
+    };
+    if (s.whole) return add(size, s.t->numel());
+    for (int64_t d = 0; d < s.t->dim(); ++d) add(s.t->stride(d) * size, s.t->size(d));
+  }
+  bool from(size_t k, int64_t rest) {
+    if (++steps > kMostSteps) return false;
+    if (k == of.size()) return rest >= x_lo && rest <= x_hi;
+    const Unknown& u = of[k];
+    if (floor_div(rest - x_lo, u.divisor) * u.divisor < rest - x_hi) return false;  // no x - y leaves a multiple
+    const int64_t lo = std::max(u.lo, -floor_div(u.most - rest, u.stride));
+    const int64_t hi = std::min(u.hi, floor_div(rest - u.least, u.stride));
+    for (int64_t i = lo; i <= hi && steps <= kMostSteps; ++i)
+      if (from(k + 1, rest - i * u.stride)) return true;
+    return false;
+  }
+  static int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+  bool found(const Span& a, const Span& b) {
+    axes(a, 1);
+    axes(b, -1);
+    x_lo = 1 - (int64_t)b.t->element_size();
+    x_hi = (int64_t)a.t->element_size() - 1;
+    std::sort(of.begin(), of.end(), [](const Unknown& p, const Unknown& q) { return p.stride > q.stride; });
+    int64_t least = x_lo, most = x_hi, divisor = 0;
+    for (size_t k = of.size(); k--;) {
+      of[k].least = least;
+      of[k].most = most;
+      of[k].divisor = divisor = std::gcd(divisor, of[k].stride);
+      least += of[k].lo * of[k].stride;
+      most += of[k].hi * of[k].stride;
+    }
+    const int64_t rest = b.first - a.first;
+    return rest >= least && rest <= most && from(0, rest);
+  }
+};
+
 // `list` holds its tensors while the call runs: references, no copies of a thousand handles.
 Tensor clip_grads(const py::list& list, double grad_clip, const std::optional<Tensor>& row_sq, bool apply,
                   const char* what) {
@@ -545,7 +611,7 @@ Tensor clip_grads(const py::list& list, double grad_clip, const std::optional<Te
   std::vector<void*> x;
   std::vector<int64_t> n;
   std::vector<int> types;
-  std::vector<std::pair<char*, char*>> spans;
+  std::vector<Span> spans;
   n.reserve(grads.size());
   x.reserve(grads.size());
   types.reserve(grads.size());
@@ -553,22 +619,33 @@ Tensor clip_grads(const py::list& list, double grad_clip, const std::optional<Te
   for (const Tensor& t : grads) {
     const int64_t m = t.numel();
     if (m == 0 || t._is_zerotensor()) continue;  // add nothing, and are scaled by being what they are
-    char* at;
-    if (t.is_neg() || !t.is_non_overlapping_and_dense()) {
+    char* at = (char*)t.data_ptr();
+    const bool whole = t.is_non_overlapping_and_dense();
+    if (apply) {
+      int64_t last = m - 1;
+      if (!whole) {
+        last = 0;
+        for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+      }
+      spans.push_back({at, at + (last + 1) * t.element_size(), &t, whole});
+    }
+    if (t.is_neg() || !whole) {
       held.push_back(dense(t));
       at = (char*)held.back().data_ptr();
       if (apply) back.emplace_back(t, held.back());
-    } else {
-      at = (char*)t.data_ptr();
-      if (apply) spans.emplace_back(at, at + m * t.element_size());
     }
     x.push_back(at);
     n.push_back(m);
     types.push_back(dtype_code(t));
   }
-  std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, what, ": two of the gradients share memory");
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.first < b.first; });
+  std::vector<const Span*> open;  // those that reach to where the next begins
+  for (const Span& b : spans) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Span* a) { return a->end <= b.first; }), open.end());
+    for (const Span* a : open)
+      TORCH_CHECK_VALUE(!(a->whole && b.whole) && !Meeting().found(*a, b), what, ": two of the gradients share memory");
+    open.push_back(&b);
+  }
   const auto opt = at::TensorOptions().device(device);
   Tensor out = at::empty({2}, opt.dtype(at::kFloat));
   const Tensor r = dense(rows);
