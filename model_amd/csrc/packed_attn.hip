@@ -864,12 +864,18 @@ constexpr float kLiftP = __is_same(T, _Float16) ? 16384.f : 1.f;
 // else 32 rows, and every wave has keys and stages of its own.
 //
 // delta = g_out . out is as good as out, which was rounded to 16 bits; where a row sees
-// few keys, out is as large as v, and that error was most of dq's and dk's (3.8e-3 of
-// their norm against 2.4e-3, bf16, 10 sequences of 56 tokens together).  So tiles of up
-// to kExactKeys keys take delta = sum p dp - g_lse in a sweep of their own, which also
-// goes to memory for dk; with more keys out is an average and that error small,
-// and the sweep would cost two thirds of dq again.
-constexpr int kExactKeys = 512;
+// few keys, out is as large as v, and that error adds a tenth to dq's and dk's.  So tiles
+// of up to kExactKeys keys take delta = sum p dp - g_lse in a sweep of their own, which
+// also goes to memory for dk; with more keys out is an average and that error small, and
+// the sweep would cost two thirds of dq again.  8,192 tokens, 16 heads over 4 of 128, bf16,
+// error of dq by its norm (1e-3) and us of the backward pass, sequences of
+//   keys    64           256          512          1,024
+//   none    2.61  110    2.51  117    2.50  158    2.48  243
+//   128     2.34  116    2.34  118    2.35  159    2.36  239
+//   256     2.34  116    2.34  131    2.35  162    2.36  239
+//   512     2.34  117    2.34  132    2.35  184    2.35  250
+//   1,024   2.34  116    2.34  131    2.35  189    2.35  292
+constexpr int kExactKeys = 256;
 template <class T, int HD, bool WIDE>
 __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(const Packed a, const Grads g,
                                                                             T* __restrict__ dq) {
