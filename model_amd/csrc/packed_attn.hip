@@ -1032,10 +1032,23 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
 
 // dk and dv.  A workgroup of KW x RW waves has 32 KW keys, 32 a wave, and its rows in
 // stages (8 KB of q and of g_out, or 32 rows) that RW sets of KW waves take in turn, each set
-// with stages of its own, and join at the end.  For heads of 128 KW 2 and RW 3: KW 4 and
-// RW 2 halve the reads of rows and take 356 us where this takes 323 (24 documents), for
-// the first keys of a long document with the heads that share them are the longest way
-// through.  Of narrower heads KW 4 and RW 1 (1,129 us; KW 4, RW 2 1,414; KW 2, RW 4 1,525).
+// with stages of its own, and join at the end.  us of the backward pass, bf16 (T tokens in
+// n sequences of one length, H heads over G):
+//   KW, RW                               2, 3     4, 2     2, 2     4, 1
+//   heads of 128:  2,048, 4, 8, 8        47.1     51.1     48.5
+//                  4,096, 1, 16 over 4   416      527      455
+//                  16,384, 24, 16 over 4 346      322      361
+//                  16,384, 16, 16, 16    465      416      474
+//   of 64:         8,192, 8, 16, 16               132      129      128
+//                  16,384, 1, 16, 16              1,958    1,976    1,920
+//                  32,768, 16, 16 over 4          663      648      687
+//                  16,384, 16, 16, 16             236      225      214
+//   of 32:         16,384, 16, 8, 8               83.9     88.4     83.6
+//                  65,536, 64, 16 over 4          452      466      459
+//                  16,384, 16, 32, 32             258      297      244
+// Heads of 128 take 2, 3: documents of unlike lengths are nearer to the calls with few
+// tiles (24 of them 323 us for dk and dv, 356 with 4, 2), for the first keys of a long one
+// with the heads that share them are the longest way through.  The others take 4, 1.
 template <class T, int HD, int KW, int RW>
 __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed a, const Grads g, T* __restrict__ dk,
                                                                    T* __restrict__ dv) {
@@ -1325,9 +1338,15 @@ bool wide_of(const Args* p) {
 // us of the backward pass, tiles of 32 keys / of 64 (heads of 128) or 128:
 //   heads of 128:  2,048, 4, 8, 8 (128 tiles of 128): 53.8 / 44.7;  4,096, 16, 16 over 4 (128): 124 / 112;
 //                  2,048, 1, 16 over 4 (64): 189 / 206
+//                  16,384, 24, 16 over 4 (512): 433 / 357
 //   of 64:         4,096, 8, 8, 8 (256): 44.2 / 44.6;  8,192, 8, 8, 8 (512): 89.0 / 80.1;
-//                  8,192, 64, 32 over 8 (512): 96.8 / 106;  dk and dv of 16,384, 1, 16, 16 (2,048): 1,353 / 1,129
-//   of 32:         8,192, 8, 8, 8 (512): 51.3 / 54.4;  16,384, 16, 16 over 4 (512): 140 / 165
+//                  8,192, 64, 32 over 8 (512): 96.8 / 106;  8,192, 8, 16, 16 (1,024): 151 / 132;
+//                  32,768, 16, 16 over 4 (1,024): 682 / 702;  65,536, 64, 16 over 4 (2,048): 834 / 786;
+//                  dk and dv of 16,384, 1, 16, 16 (2,048): 1,353 / 1,129
+//   of 32:         8,192, 8, 8, 8 (512): 51.3 / 54.4;  16,384, 16, 16 over 4 (512): 140 / 165;
+//                  16,384, 1, 8, 8 (1,024): 708 / 684;  32,768, 16, 16 over 4 (1,024): 407 / 410;
+//                  16,384, 1, 16, 16 (2,048): 1,327 / 1,194;  65,536, 64, 16 over 4 (2,048): 469 / 468;
+//                  16,384, 16, 32, 32 (4,096): 294 / 252
 //
 // Heads of 128 have 384 threads a workgroup then: with more than some 11 million tiles
 // (sequences times key heads) the grid's threads would pass 32 bits, where 256 do not.
@@ -1338,21 +1357,36 @@ bool wide_keys_of(const Args* p) {
 }
 
 // Parts of the keys: where the tiles of rows do not fill the chip and the keys of
-// a sequence are many.  Only sums over the sequences are known here.  A part is worth
-// its share of the join's launch and memory from some keys on; fp32's products take
-// longer, and want more workgroups.  us by number of parts, single tokens of B streams
-// over `cap` keys each:
-//   fp32, B 1, cap 2,048, 4 heads of 64:      1: 41.9   4: 16.7   8: 14.1   16: 14.1   32: 19.3
-//   fp32, 16, 4,096, 32 over 8 of 128:        1: 170    2: 107    4: 120    8: 125     16: 150
-//   bf16, 1, 512, 4 of 64:                    1: 8.2    2: 11.1   4: 10.6
-//   bf16, 1, 8,192, 4 of 64:                  1: 42.0   4: 16.4   8: 13.3   16: 13.8   32: 18.1
-//   bf16, 1, 32,768, 32 over 8 of 128:        1: 215    8: 38.1   16: 33.9  32: 47.6   64: 64.8
-//   bf16, 16, 4,096, 32 over 8 of 128:        1: 43.7   2: 46.1   4: 48.0   8: 53.0
+// a sequence are many.  Only sums over the sequences are known here, of a cache its
+// places and not how many are in use.  A part is worth its share of the join's launch and
+// memory from some keys on; fp32's products take longer, and want more workgroups.  Of
+// heads of 128 a CU holds one of them (128 KB of LDS), and some more than 256 take twice
+// as long: there the tiles are counted from below (as for single tokens).  us by number of
+// parts, single tokens of B streams over `cap` places each, all in use / a quarter of
+// them; * what the rule takes:
+//   fp32, B 1, 4 heads of 64, cap 256:        1: 8.7 / 6.3 *   2: 8.2 / 8.3
+//     512:                                    1: 13.4 / 6.3    2: 10.7 / 8.3 *   4: 8.9 / 9.4
+//     1,024:                                  1: 23.1 / 8.6    2: 15.7 / 8.6   4: 11.3 / 8.8 *   8: 10.4 / 10.9
+//     2,048:                                  1: 42.1 / 13.4   4: 16.5 / 9.5   8: 12.7 / 10.5 *
+//   fp32, 16, 32 over 8 of 128, cap 512:      1: 26.5 / 10.5   2: 22.3 / 13.9 *   4: 29.0 / 24.3
+//     1,024:                                  1: 46.7 / 16.2   2: 32.5 / 16.7 *   3: 46.5 / 24.4   4: 39.2 / 24.8
+//     4,096:                                  1: 170 / 47.0    2: 107 / 32.5 *   3: 130 / 47.0   4: 110 / 40.0
+//   fp32, 4, 32 over 8 of 128, cap 4,096:     1: 166 / 45.6    4: 50.7 / 20.8   8: 35.9 / 18.8 *   16: 45.7 / 32.0
+//   bf16, 1, 4 of 64, cap 512:                1: 5.9 / 4.2 *   2: 7.2 / 6.2
+//     1,024:                                  1: 8.3 / 4.8    2: 8.0 / 6.2 *   4: 7.2 / 7.3
+//     2,048:                                  1: 13.1 / 6.0   4: 9.1 / 7.2 *   8: 9.0 / 8.5
+//   bf16, 1, 32 over 8 of 128, cap 4,096:     1: 31.0 / 10.8   4: 15.0 / 9.7   8: 13.9 / 11.1 *
+//     32,768, all in use:                     1: 215    8: 38.1   16: 33.9 *  32: 47.6   64: 64.8
+//   bf16, 16, 32 over 8 of 128, cap 4,096:    1: 44.3 / 15.2 *   2: 43.3 / 17.1   4: 47.1 / 20.9
+// Caches that are full at their end gain more than those that are not lose: with fp32's
+// 512 places and up to half of them in use one part would be up to 2 us shorter.
 int splits_of(const Args* p) {
   const bool f32 = p->dtype == MPL_F32;
   const int64_t r = p->heads / p->groups, n = p->sequences ? p->sequences : 1;
-  const int64_t tiles = (p->tokens * r / 32 + (p->tokens < n ? p->tokens : n)) * p->groups;
-  const int64_t want = tiles ? (f32 ? 512 : 128) / tiles : 1, most = p->keys / n / (f32 ? 256 : 512);
+  const int64_t full = p->tokens * r / 32, some = p->tokens < n ? p->tokens : n;
+  const bool single = f32 && p->head_dim == 128;  // workgroup a CU
+  const int64_t tiles = (single ? (full > some ? full : some) : full + some) * p->groups;
+  const int64_t want = tiles ? (single ? 256 : f32 ? 512 : 128) / tiles : 1, most = p->keys / n / (f32 ? 256 : 512);
   const int64_t s = want < most ? want : most;
   return s < 1 ? 1 : s > 16 ? 16 : (int)s;
 }
