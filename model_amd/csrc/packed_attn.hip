@@ -261,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void packed_forward_kernel(const Packed a
 // 2^8, exact in fp32 and of the same relative error in 16 bits, and the
 // accumulators need no scaling.
 // fp16's weights are 2^6 times as large, which the division takes out again: with
-// 2^8 that is 2^14, and those below 2^-20 of the largest keep all their bits.
+// 2^8 that is 2^14, and those down to 2^-20 of the largest keep all their bits.
 template <class T>
 constexpr float kLift = __is_same(T, _Float16) ? 6.f : 0.f;
 

@@ -27,10 +27,11 @@ def clip_global_norm(grads: Sequence[torch.Tensor], grad_clip: float, *,
 
     grads are fp32, fp16 or bf16, mixed as they come, any number and any shapes
     on one GPU; such as do not lie in one piece are scaled through a copy.  No
-    two may share memory, and none may be expanded.  row_sq (fp32, any shape)
-    are squares that join the norm: MergedRows.row_sq of the sparse rows, whose
-    update takes the scale.  Squares are summed in fp64 in a fixed order, and
-    x scale is rounded once to x's type; where scale is 1 nothing is written.
+    two may share an element, whatever their layouts, and none may be expanded.
+    row_sq (fp32, any shape) are squares that join the norm: MergedRows.row_sq of
+    the sparse rows, whose update takes the scale.  Squares are summed in fp64 in
+    a fixed order, and x scale is rounded once to x's type; where scale is 1 the
+    values stay as they are, and nothing is written but the copies' own.
     A norm that is not finite gives NaN or zero, as the formula does.  No host
     read, no atomics: it may be captured in a HIP graph."""
     return _lib.ops().clip_global_norm(list(grads), float(grad_clip), row_sq)
