@@ -587,9 +587,9 @@ struct Sums {
         *(float4*)&so[n][rw][col][32 * d + tile_row(r, half)] =
             make_float4(acc[d][r] * f, acc[d][r + 1] * f, acc[d][r + 2] * f, acc[d][r + 3] * f);
   }
-  // `place(t)`: where row t goes, null for nowhere.
+  // `place(t)`: where row t goes, null for nowhere; those from `kept` on are 0.
   template <class F>
-  __device__ __forceinline__ void write(F&& place) const {
+  __device__ __forceinline__ void write(int kept, F&& place) const {
     for (int i = threadIdx.x; i < N * 32 * HD / 4; i += 64 * N * RW) {
       const int t = i / (HD / 4), d = 4 * (i % (HD / 4));
       auto* to = place(t);
@@ -600,7 +600,7 @@ struct Sums {
         const float4 y = *(const float4*)&so[t >> 5][w][t & 31][d];
         x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
       }
-      store4(to + d, x);
+      store4(to + d, t < kept ? x : make_float4(0.f, 0.f, 0.f, 0.f));
     }
   }
 };
@@ -686,7 +686,7 @@ __global__ __launch_bounds__(kThreads) void packed_dq_kernel(const Packed a, con
   Sums<HD, 1, kWaves>& sums = *(Sums<HD, 1, kWaves>*)lds;
   sums.put(0, wave, col, half, acc, g.scale);
   __syncthreads();
-  sums.write([&](int t) -> T* {
+  sums.write(32, [&](int t) -> T* {
     if (row0 + t >= rows) return nullptr;
     const int tk = div_r(a, row0 + t);
     return dq + ((int64_t)(seg.first + tk) * a.H + group * a.R + row0 + t - tk * a.R) * HD;
@@ -798,21 +798,15 @@ __global__ __launch_bounds__(kThreads, HD <= 64 ? 2 : 1) void packed_dkv_kernel(
     }
   }
   Sums<HD, 1, kWaves>& sums = *(Sums<HD, 1, kWaves>*)lds;
-  const bool in = k0 + col < len;  // places not in use have gradients 0
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     T* to = which ? dv : dk;
     if (!to) continue;
-    f32x16 (&x)[DT] = which ? av : ak;
-    if (!in) {
-#pragma unroll
-      for (int d = 0; d < DT; ++d) x[d] = f32x16{};
-    }
     reads_done();
     __syncthreads();  // the stages become the waves' sums
-    sums.put(0, wave, col, half, x, which ? 1.f : g.scale);
+    sums.put(0, wave, col, half, which ? av : ak, which ? 1.f : g.scale);
     __syncthreads();
-    sums.write([&](int t) -> T* {
+    sums.write(len - k0, [&](int t) -> T* {  // places not in use have gradients 0
       return k0 + t < seg.len ? to + ((int64_t)(seg.first + k0 + t) * a.G + group) * HD : nullptr;
     });
   }
@@ -1022,7 +1016,7 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
     Sums<HD, 1, kWaves>& sums = *(Sums<HD, 1, kWaves>*)lds;
     sums.put(0, wave, col, half, acc, f);
     __syncthreads();
-    sums.write([&](int t) -> T* {
+    sums.write(32, [&](int t) -> T* {
       if (row0 + t >= rows) return nullptr;
       const int tk = div_r(a, row0 + t);
       return dq + ((int64_t)(seg.first + tk) * a.H + group * a.R + row0 + t - tk * a.R) * HD;
@@ -1234,7 +1228,7 @@ __global__ __launch_bounds__(64 * KW * RW) void packed_dkv16_kernel(const Packed
     __syncthreads();  // the stages become the waves' sums
     sums.put(kw, rw, col, half, x, which ? fv : fk);
     __syncthreads();
-    sums.write([&](int t) -> T* {
+    sums.write(kKeys, [&](int t) -> T* {
       return k0 + t < seg.len ? to + ((int64_t)(seg.first + k0 + t) * a.G + group) * HD : nullptr;
     });
   }
