@@ -857,19 +857,28 @@ constexpr float kLiftP = __is_same(T, _Float16) ? 16384.f : 1.f;
 // dq.  WIDE: 128 rows a workgroup, 32 a wave, 64 keys a stage that all waves read;
 // else 32 rows, and every wave has keys and stages of its own.
 //
-// delta = g_out . out is as good as out, which was rounded to 16 bits; where a row sees
-// few keys, out is as large as v, and that error adds a tenth to dq's and dk's.  So tiles
-// of up to kExactKeys keys take delta = sum p dp - g_lse in a sweep of their own, which
-// also goes to memory for dk; with more keys out is an average and that error small, and
-// the sweep would cost two thirds of dq again.  8,192 tokens, 16 heads over 4 of 128, bf16,
-// error of dq by its norm (1e-3) and us of the backward pass, sequences of
-//   keys    64           256          512          1,024
-//   none    2.61  110    2.51  117    2.50  158    2.48  243
-//   128     2.34  116    2.34  118    2.35  159    2.36  239
-//   256     2.34  116    2.34  131    2.35  162    2.36  239
-//   512     2.34  117    2.34  132    2.35  184    2.35  250
-//   1,024   2.34  116    2.34  131    2.35  189    2.35  292
-constexpr int kExactKeys = 256;
+// delta = g_out . out is as good as out, which was rounded to 16 bits; where a row's
+// weights lie on few keys, out is as large as v, and that error shows in dq and dk.  The
+// exact one is sum p dp - g_lse, known once all keys have been seen.  Tiles of up to
+// kExactKeys keys form it in a sweep of their own, two thirds of dq once more; with more
+// keys out is an average more often.  Heads of 32 are the ones that lose most, and have
+// registers left: they take g_out . out as they go, sum p k beside dz k, and add
+// (g_out . out - sum p dp) sum p k at the end, one product instead of the sweep's two and
+// its exponentials.  Either way delta goes to memory for dk.
+//
+// Error of dq by its norm, in errors of the exact value rounded once, and us of the
+// backward pass (bf16, 4,096 tokens, scores of standard deviation 1.7), sequences of
+//                                            512           1,024         4,096
+//   16 heads of 64, sweep up to 256 keys:    1.467   68    1.487   86    1.499  194
+//     512:                                   1.432   73    1.463   87    1.485  196
+//     all:                                   1.432   73    1.439  104    1.446  245
+//   16 over 4 of 128, sweep up to 256:       1.451   90    1.460  143    1.457  422
+//     512:                                   1.427  103    1.443  145    1.447  424
+//     all:                                   1.427  103    1.427  168    1.427  507
+//   16 of 32, sweep up to 512:               1.466   49    1.514   56    1.554  115
+//     beside dz k, all:                      1.463   44    1.470   55    1.480  120
+// (Two roundings, dz's and dq's own, make 1.414.)
+constexpr int kExactKeys = 512;
 template <class T, int HD, bool WIDE>
 __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(const Packed a, const Grads g,
                                                                             T* __restrict__ dq) {
@@ -962,12 +971,8 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
       }
     }
   };
-  if (most <= kExactKeys) {
-    float sum = 0.f;
-    sweep([&](const f32x16& p, const f32x16& dp, const char*, int) __attribute__((always_inline)) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sum = fmaf(p[r], dp[r], sum);
-    });
+  // The lane's sum of p dp becomes the row's exact delta, which goes to memory too.
+  auto exact = [&](float sum) __attribute__((always_inline)) {
     float other = sum;
     half_swap(sum, other);
     sum += other;
@@ -976,19 +981,34 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
       __syncthreads();
       sum = (sigma[0][col] + sigma[1][col]) + (sigma[2][col] + sigma[3][col]);
     }
-    delta = sum - (g.g_lse ? g.g_lse[(int64_t)(seg.first + tok) * a.H + head] : 0.f);
-    if (half == 0 && w0 + col < rows && (WIDE || wave == 0)) g.delta[at] = delta;
-  }
+    sum -= g.g_lse ? g.g_lse[(int64_t)(seg.first + tok) * a.H + head] : 0.f;
+    if (half == 0 && w0 + col < rows && (WIDE || wave == 0)) g.delta[at] = sum;
+    return sees <= 0 ? 0.f : sum;
+  };
+  constexpr bool kBeside = HD == 32;
   if (sees <= 0) delta = 0.f;  // a row without keys, whose weights are 0: g_lse may be anything
-  if (!dq) return;
+  if (!kBeside && most <= kExactKeys) {
+    float sum = 0.f;
+    sweep([&](const f32x16& p, const f32x16& dp, const char*, int) __attribute__((always_inline)) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum = fmaf(p[r], dp[r], sum);
+    });
+    delta = exact(sum);
+  }
+  if (!kBeside && !dq) return;
   f32x16 acc[HD / 32];
 #pragma unroll
   for (int d = 0; d < HD / 32; ++d) acc[d] = f32x16{};
   Unit<T, HD> unit;
+  f32x16 mean = f32x16{};  // sum p k
+  float sum = 0.f;
   sweep([&](const f32x16& p, const f32x16& dp, const char* k, int b) __attribute__((always_inline)) {
     f32x16 dz;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dz[r] = p[r] * (dp[r] - delta);
+    for (int r = 0; r < 16; ++r) {
+      dz[r] = p[r] * (dp[r] - delta);
+      if (kBeside) sum = fmaf(p[r], dp[r], sum);
+    }
     unit.scale(dz, acc);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -998,9 +1018,21 @@ __global__ __launch_bounds__(kThreads, WIDE ? 2 : 1) void packed_dq16_kernel(con
       const short8v w = round8<T>(x);
 #pragma unroll
       for (int d = 0; d < HD / 32; ++d) acc[d] = mma16<T>(st.cols(k, 2 * b + i, d), w, acc[d]);
+      if constexpr (kBeside) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = p[8 * i + e] * kLiftP<T>;
+        mean = mma16<T>(st.cols(k, 2 * b + i, 0), round8<T>(x), mean);
+      }
     }
   });
-  const float f = g.scale * unit.inverse();
+  float f = g.scale * unit.inverse();
+  if constexpr (kBeside) {
+    const float off = (delta - exact(sum)) * (g.scale / kLiftP<T>);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[0][r] = fmaf(mean[r], off, acc[0][r] * f);
+    f = 1.f;
+    if (!dq) return;
+  }
   if constexpr (WIDE) {
     if (w0 + col >= rows) return;
     T* to = dq + ((int64_t)(seg.first + tok) * a.H + head) * HD;

@@ -125,3 +125,22 @@ def test_grids_of_eleven_million_tiles(dtype):
     want = definition(q, k, v, [T], [T], [0], 128 ** -0.5, g, gl)
     for nm, x in zip(("out", "lse", "dq", "dk", "dv"), all_of(q, k, v, g, gl, starts)):
         check(x, want[nm], nm)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("n", [60, 300, 1100, 2500])
+def test_errors_of_16_bits(dtype, hd, n):
+    """Weights on few keys (scores of standard deviation 1.7).  Of an output's two roundings, the weights' or dz's and its
+    own, each has the error of the exact value rounded once: sqrt(2) of it together.  Up to 1.5 the rest, the most of it
+    delta from the rounded out, has half a rounding: sqrt(1.5^2 - 2)."""
+    lq = [n, n // 2]
+    q, k, v, g, _ = make(lq, lq, 8, 4, hd, dtype, seed=39)
+    q, k = q * 1.3, k * 1.3
+    starts = torch.tensor(sums(lq), dtype=torch.int32, device=DEV)
+    want = definition(q, k, v, lq, lq, sums(lq), hd ** -0.5, g)
+    for nm, x in zip(("out", "lse", "dq", "dk", "dv"), all_of(q, k, v, g, None, starts)):
+        exact = want[nm][0]
+        once = (exact.to(x.dtype).double() - exact).norm()
+        if nm != "lse":
+            assert (x.double() - exact).norm() <= 1.5 * once, nm
