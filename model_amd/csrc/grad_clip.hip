@@ -15,10 +15,11 @@
 // goes from the end on, where what was read last may still lie in the last-level
 // cache.  Bound: memory; of small sets the two launches' latency, of a thousand tensors
 // the host (65 ns each).  Measured: 1.2 G elements (bf16 matrices, fp32 vectors, 2.4 GB
-// read twice and written) 842 to 1,540 us by machine, up to 8.6 TB/s with what the cache
-// gives, against 1,497 at a large copy's 4.85 TB/s; 32 fp32 tensors of 6.3 MB 9 to 11 us, kernels 5.3 + 3.2;
-// 1,500 fp16 tensors of 22 MB below the clip 117 us, of which 27 on the GPU (eight lists
-// of 1.7, sums 9, the end 4).  A launch of each kernel for every 192 tensors instead
+// read twice and written) 1,540 us, sums 513 to 521 and the scaling 1,017, against 1,497 at
+// a large copy's 4.85 TB/s; where the scale is 1 the scaling ends at once, and the call
+// takes 522; 32 fp32 tensors of 6.3 MB 9 to 11 us, kernels 5.3 + 3.2;
+// 1,500 fp16 tensors of 65 MB below the clip 118 us, of which 39 on the GPU (eight lists
+// of 1.7, sums 21, the end 4).  A launch of each kernel for every 192 tensors instead
 // of the list took 218 us, a third launch for the norm 15.4 where two take 10.
 #include <math.h>
 

@@ -15,13 +15,15 @@
 // products instead of five, and no atomics.
 //
 // Measured (MI355X; a large bf16 product makes 1,247 TFLOP/s, an fp32 one 154), us:
-//   forward, one prompt of 16,384, 16 heads over 4 of 128, bf16      1,128   975 TFLOP/s
-//     the same of 16 heads of 64                                       670   820
-//   backward of the latter: delta 19, dq 803 (1,027), dk and dv 1,102 (998 of its four products)
-//   24 documents, 16,384 tokens, 16 heads over 4 of 128, bf16: forward 150, delta 36, dq 191,
-//     dk and dv 334: the longest document's first tiles are most of the time
-//   40 documents, 8,192 tokens, 4 heads of 64, fp32: forward 47, delta 5, dq 62, dk and dv 87
-//   4,096 tokens, 8 heads of 64, fp32: forward 169 (101 TFLOP/s), backward 557 (108 of its seven products)
+//   forward, one prompt of 16,384, 16 heads over 4 of 128, bf16      1,138   966 TFLOP/s
+//     the same of 16 heads of 64                                       673   817
+//   backward of the latter: delta 22, dq 816 (1,010), dk and dv 1,115 (986 of its four products);
+//     in fp16 2,250 for 1,945, for dz's powers of two
+//   24 documents, 16,384 tokens, 16 heads over 4 of 128, bf16: forward 148, delta 40, dq 197,
+//     dk and dv 324: the longest document's first tiles are most of the time
+//   40 documents, 8,192 tokens, 4 heads of 64, fp32: forward 47, delta 5, dq 63, dk and dv 88
+//   4,096 tokens, 8 heads of 64, fp32: forward 178 (96 TFLOP/s), backward 557 (108 of its seven products);
+//     of 128: 359 (96), 1,268 (95)
 //   64 single tokens over caches of up to 8,192, 32 heads over 8 of 128, bf16: 266, 5.2 TB/s
 // Bound: the matrix units of large 16-bit calls (half of their cycles; the vector units
 // 60 to 85 % of theirs: exponentials and conversions), memory for single tokens, for
